@@ -145,6 +145,9 @@ def prepare(case, seed):
     bt, n = _page_table(g, lens)
     s = {"case": dict(case), "pos": _i32(pos), "slot": _i32(slot), "bt": bt}
     (s["k"], s["k_scale"]), (s["v"], s["v_scale"]) = _lines(g, n, kv, hs, True), _lines(g, n, kv, hs, False)
+    if own:
+        from dllama_b200.ops import kernels as K
+        s["cache"] = K.Kv8Cache(s["k"], s["v"], s["k_scale"], s["v_scale"])
     if case["kind"] == "read":
         t = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}[case["out"]]
         s["k_out"], s["v_out"] = (torch.zeros(M, kv * hs, dtype=t, device="cuda") for _ in range(2))
@@ -160,14 +163,12 @@ def prepare(case, seed):
     if case["kind"] == "decode":
         s["y"] = torch.zeros(M, H * hs, device="cuda")
         if own:
-            from dllama_b200.ops import kernels as K
             s["splits"] = K.kv8_attention_splits(M, H, kv, bt.shape[1])
             s["scratch"] = torch.zeros(K.attention_scratch_bytes(M, H, hs, s["splits"]), dtype=torch.uint8, device="cuda")
     else:
         s["y"] = torch.zeros(M, H * hs, dtype=torch.bfloat16, device="cuda")      # what a 16-bit product reads next
         s["meta"] = _i32([1, 0, M])
         if own:
-            from dllama_b200.ops import kernels as K
             s["work"] = K.kv8_prefill_workspace(n, kv, hs, M, "cuda")
     return s
 
@@ -179,8 +180,7 @@ def _run_own(s):
     from dllama_b200.ops import kernels as K
     c = s["case"]
     M, kind = c["rows"], c["kind"]
-    cache = K.Kv8Cache(s["k"], s["v"], s["k_scale"], s["v_scale"])
-    where = (s["pos"], s["slot"], s["bt"])
+    where, cache = (s["pos"], s["slot"], s["bt"]), s["cache"]
     if kind == "read":
         K.kv8_read(M, *where, cache, s["k_out"], s["v_out"])
         return {"k": s["k_out"], "v": s["v_out"]}
