@@ -1,0 +1,263 @@
+// Writing the 8-bit token cache and reading it back (kv8.cuh has the format).
+//
+// kv8_write: the merged q|k|v rows of a layer in one pass -- rotary positions on queries and keys (pairs of neighbouring values, OP_ROPE_LLAMA,
+// ropeLlamaForward_F32_F32: nn-cpu-ops.cpp:1090-1120), keys and values to their pages (OP_SHIFT, shiftForward_F32_F32: nn-cpu-ops.cpp:1253-1275)
+// as codes and scales.
+//
+// A code is a rounding, and an input a hair beside a border lands on either side of it: so that the same rows give the same codes however they are
+// computed, keys are turned in 64 bits (angle, sine, cosine and both products) and rounded once to f32, and x * factor goes to the nearest integer in
+// one rounding, an fma with 1.5 2^23.  Queries take f32 products of the same sines and cosines.  The sines of a row are formed once for all heads.
+#include <type_traits>
+#include "epilogue.cuh"
+#include "kv8.cuh"
+
+extern void dl_set_error(const char* fmt, ...);
+extern int dl_device_sm_count();
+
+struct Kv8WriteArgs {
+    const float* qkv;          // [M][ld]: heads | kv heads | kv heads
+    long long ld;
+    const float* freqs;        // [HS / 2] or NULL: no rotation
+    float* q_out;              // [M][ldq]
+    long long ldq;
+    Kv8Rows rows;
+    DlKv8Cache c;
+    int heads;
+};
+
+#define KV8_WRITE_WARPS 8
+
+// grid (M, shares of the heads); a lane has four neighbouring values of a head
+template <int HS, bool VEC>
+__global__ void __launch_bounds__(KV8_WRITE_WARPS * 32) kv8_write_kernel(const __grid_constant__ Kv8WriteArgs a) {
+    constexpr int LPH = HS / 4, HPW = 32 / LPH;                // lanes a head, heads a warp
+    __shared__ double2 turn[HS / 2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, li = lane % LPH;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int m = blockIdx.x;
+    const int pos = a.rows.pos[m], slot = a.rows.slot[m];
+    const int T = kv8_tokens(a.rows, pos, slot);
+    if (T <= 0) return;                                        // (uniform for the CTA)
+    const int page = a.rows.block_table[(size_t)slot * a.rows.max_pages + pos / KV8_PAGE];
+    if (a.freqs != nullptr) {
+        if (tid < HS / 2) {
+            double s, c;
+            sincos((double)pos * (double)a.freqs[tid], &s, &c);
+            turn[tid] = make_double2(c, s);
+        }
+        __syncthreads();
+    }
+    const int kv = a.c.n_kv_heads, heads = a.heads + 2 * kv, units = (heads + HPW - 1) / HPW;
+    const bool there = (unsigned)page < (unsigned)a.rows.n_pages;
+    for (int u = blockIdx.y * KV8_WRITE_WARPS + warp; u < units; u += gridDim.y * KV8_WRITE_WARPS) {
+        const int h = u * HPW + lane / LPH;
+        const bool live = h < heads;
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        if (live) {
+            const float* src = a.qkv + m * a.ld + h * HS + li * 4;
+            if (VEC) {
+                const float4 v = *reinterpret_cast<const float4*>(src);
+                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = src[e];
+            }
+        }
+        const bool is_q = h < a.heads, is_k = !is_q && h < a.heads + kv;
+        if (a.freqs != nullptr && (is_q || is_k)) {
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const double2 t = turn[li * 2 + e / 2];
+                if (is_q) {
+                    const float c = (float)t.x, s = (float)t.y, x0 = x[e], x1 = x[e + 1];
+                    x[e] = x0 * c - x1 * s;
+                    x[e + 1] = x0 * s + x1 * c;
+                } else {
+                    const double x0 = x[e], x1 = x[e + 1];
+                    x[e] = (float)(x0 * t.x - x1 * t.y);
+                    x[e + 1] = (float)(x0 * t.y + x1 * t.x);
+                }
+            }
+        }
+        if (is_q) {
+            float* dst = a.q_out + m * a.ldq + h * HS + li * 4;
+            if (VEC) *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+            else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) dst[e] = x[e];
+            }
+        }
+        // the line's largest magnitude as bits: an infinity or a NaN is above every number
+        unsigned top = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (is_q || !live || !there) continue;
+        const float amax = __uint_as_float(top);
+        float scale = 0.f, factor = 0.f;
+        if (top >= 0x7f800000u) scale = __uint_as_float(0x7fffffffu);          // the line reads back as NaN
+        else if (amax >= KV8_TINY) { scale = __fdiv_rn(amax, 127.f); factor = __fdiv_rn(127.f, amax); }
+        uint32_t code = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) code |= (__float_as_uint(__fmaf_rn(top >= 0x7f800000u ? 0.f : x[e], factor, 12582912.f)) & 0xffu) << (8 * e);
+        const size_t line = ((size_t)page * kv + (h - a.heads - (is_k ? 0 : kv))) * KV8_PAGE + pos % KV8_PAGE;
+        reinterpret_cast<uint32_t*>((is_k ? a.c.k : a.c.v) + line * HS)[li] = code;
+        if (li == 0) (is_k ? a.c.k_scale : a.c.v_scale)[line] = scale;
+    }
+}
+
+struct Kv8ReadArgs {
+    void* k_out;               // [M][ld]
+    void* v_out;
+    long long ld;
+    Kv8Rows rows;
+    DlKv8Cache c;
+    int per_cta;               // rows of a CTA
+};
+
+template <typename T> DL_DEVINL T kv8_from_float(float x);
+template <> DL_DEVINL float kv8_from_float<float>(float x) { return x; }
+template <> DL_DEVINL __half kv8_from_float<__half>(float x) { return __float2half_rn(x); }
+template <> DL_DEVINL __nv_bfloat16 kv8_from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+#define KV8_READ_WARPS 8
+#define KV8_READ_ROWS 32       // most rows of a CTA
+
+// a warp takes a row at a time, a lane the codes of 16 bytes of output; rows without a token read as zeros, rows that are not in the tables as NaN
+template <int HS, typename T, bool VEC>
+__global__ void __launch_bounds__(KV8_READ_WARPS * 32) kv8_read_kernel(const __grid_constant__ Kv8ReadArgs a) {
+    constexpr int N = 16 / (int)sizeof(T), UPH = HS / N;       // values of a lane, lanes a head
+    __shared__ long long at[KV8_READ_ROWS];                    // first line of the row's token (of head 0); -1: none, -2: NaN
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int m0 = blockIdx.x * a.per_cta, n = min(a.per_cta, a.rows.M - m0), kv = a.c.n_kv_heads;
+    if (tid < n) {
+        const int pos = a.rows.pos[m0 + tid], slot = a.rows.slot[m0 + tid], t = kv8_tokens(a.rows, pos, slot);
+        long long line = t == 0 ? -1 : -2;
+        if (t > 0) {
+            const int page = a.rows.block_table[(size_t)slot * a.rows.max_pages + pos / KV8_PAGE];
+            if ((unsigned)page < (unsigned)a.rows.n_pages) line = (long long)page * kv * KV8_PAGE + pos % KV8_PAGE;
+        }
+        at[tid] = line;
+    }
+    __syncthreads();
+    const int units = 2 * kv * UPH;
+    for (int r = warp; r < n; r += KV8_READ_WARPS) {
+        const long long line0 = at[r];
+#pragma unroll 4
+        for (int u = lane; u < units; u += 32) {
+            const int g = u / UPH, part = u % UPH;
+            const bool is_k = g < kv;
+            const int h = is_k ? g : g - kv;
+            float f[N];
+            if (line0 >= 0) {
+                const long long line = line0 + (long long)h * KV8_PAGE;
+                const float s = (is_k ? a.c.k_scale : a.c.v_scale)[line];
+                const int8_t* src = (is_k ? a.c.k : a.c.v) + line * HS + part * N;
+                uint32_t w[N / 4];
+                if (N == 8) { const uint2 x = *reinterpret_cast<const uint2*>(src); w[0] = x.x; w[N / 4 - 1] = x.y; }
+                else w[0] = *reinterpret_cast<const uint32_t*>(src);
+#pragma unroll
+                for (int e = 0; e < N; e++) f[e] = (float)(int8_t)(w[e / 4] >> (8 * (e % 4))) * s;
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; e++) f[e] = line0 == -1 ? 0.f : __uint_as_float(0x7fffffffu);
+            }
+            alignas(16) T o[N];
+#pragma unroll
+            for (int e = 0; e < N; e++) o[e] = kv8_from_float<T>(f[e]);
+            T* dst = reinterpret_cast<T*>(is_k ? a.k_out : a.v_out) + (m0 + r) * a.ld + h * HS + part * N;
+            if (VEC) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(o);
+            else {
+#pragma unroll
+                for (int e = 0; e < N; e++) dst[e] = o[e];
+            }
+        }
+    }
+}
+
+int kv8_check(const char* who, const DlKv8Cache* c, const DlKv8Rows* r) {
+    if (c == nullptr || r == nullptr) { dl_set_error("%s: no cache or no rows", who); return -1; }
+    if (c->head_size != 32 && c->head_size != 64 && c->head_size != 128) { dl_set_error("%s: unsupported head_size %d (32, 64 or 128)", who, c->head_size); return -1; }
+    if (c->n_kv_heads < 1 || c->n_pages < 1) { dl_set_error("%s: %d kv heads, %d pages", who, c->n_kv_heads, c->n_pages); return -1; }
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale || !r->pos || !r->slot || !r->block_table) { dl_set_error("%s: a null pointer", who); return -1; }
+    if ((((uintptr_t)c->k | (uintptr_t)c->v | (uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 15) != 0) { dl_set_error("%s: the cache has to be aligned to 16 bytes", who); return -1; }
+    if (r->M < 0 || r->n_slots < 1 || r->max_pages < 1 || r->max_pages > 0x7fffffff / KV8_PAGE) { dl_set_error("%s: %d rows, block table [%d][%d]", who, r->M, r->n_slots, r->max_pages); return -1; }
+    return 0;
+}
+
+template <typename K, typename A>
+static int kv8_launch(const char* who, K kernel, const A& a, dim3 grid, int threads, int pdl, void* stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[1];
+    if (pdl) {
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    }
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    if (e != cudaSuccess) { dl_set_error("%s launch: %s", who, cudaGetErrorString(e)); return -(int)e; }
+    return 0;
+}
+
+static Kv8Rows kv8_rows(const DlKv8Rows& r, const DlKv8Cache& c) { return {r.pos, r.slot, r.block_table, r.M, r.n_slots, r.max_pages, c.n_pages}; }
+
+extern "C" int dl_kv8_write(const float* qkv, long long ld_qkv, int n_heads, const float* freqs, const DlKv8Rows* rows, float* q_out, long long ld_q,
+                            const DlKv8Cache* cache, int pdl, void* stream) {
+    if (const int rc = kv8_check("dl_kv8_write", cache, rows)) return rc;
+    const int hs = cache->head_size, kv = cache->n_kv_heads;
+    if (n_heads < 0 || qkv == nullptr || (n_heads > 0 && q_out == nullptr)) { dl_set_error("dl_kv8_write: %d heads, or a null pointer", n_heads); return -1; }
+    if (ld_qkv < (long long)(n_heads + 2 * kv) * hs || (n_heads > 0 && ld_q < (long long)n_heads * hs)) { dl_set_error("dl_kv8_write: rows overlap (ld %lld, %lld)", ld_qkv, ld_q); return -1; }
+    if (rows->M == 0) return 0;
+    Kv8WriteArgs a = {qkv, ld_qkv, freqs, q_out, ld_q, kv8_rows(*rows, *cache), *cache, n_heads};
+    const bool vec = ((uintptr_t)qkv & 15) == 0 && ((uintptr_t)q_out & 15) == 0 && ld_qkv % 4 == 0 && (n_heads == 0 || ld_q % 4 == 0);
+    // a row's heads go to as many CTAs as the SMs have room for, a unit for each warp at most
+    const int per_warp = 128 / hs, units = (n_heads + 2 * kv + per_warp - 1) / per_warp, most = (units + KV8_WRITE_WARPS - 1) / KV8_WRITE_WARPS;
+    const int share = 4 * dl_device_sm_count() / rows->M;
+    const dim3 grid(rows->M, share < 1 ? 1 : share < most ? share : most);
+    auto go = [&](auto hs_c) {
+        constexpr int HS = decltype(hs_c)::value;
+        return vec ? kv8_launch("dl_kv8_write", kv8_write_kernel<HS, true>, a, grid, KV8_WRITE_WARPS * 32, pdl, stream)
+                   : kv8_launch("dl_kv8_write", kv8_write_kernel<HS, false>, a, grid, KV8_WRITE_WARPS * 32, pdl, stream);
+    };
+    if (hs == 128) return go(std::integral_constant<int, 128>());
+    if (hs == 64) return go(std::integral_constant<int, 64>());
+    return go(std::integral_constant<int, 32>());
+}
+
+extern "C" int dl_kv8_read(const DlKv8Rows* rows, const DlKv8Cache* cache, void* k_out, void* v_out, long long ld, int out_type, int pdl, void* stream) {
+    if (const int rc = kv8_check("dl_kv8_read", cache, rows)) return rc;
+    const int hs = cache->head_size;
+    if (k_out == nullptr || v_out == nullptr) { dl_set_error("dl_kv8_read: a null pointer"); return -1; }
+    if (out_type != DL_KV8_F32 && out_type != DL_KV8_BF16 && out_type != DL_KV8_F16) { dl_set_error("dl_kv8_read: unsupported output type %d", out_type); return -1; }
+    if (ld < (long long)cache->n_kv_heads * hs) { dl_set_error("dl_kv8_read: rows overlap (ld %lld)", ld); return -1; }
+    if (rows->M == 0) return 0;
+    const int sms = dl_device_sm_count();
+    int per = (rows->M + 8 * sms - 1) / (8 * sms);
+    per = per < 1 ? 1 : per > KV8_READ_ROWS ? KV8_READ_ROWS : per;
+    Kv8ReadArgs a = {k_out, v_out, ld, kv8_rows(*rows, *cache), *cache, per};
+    const int size = out_type == DL_KV8_F32 ? 4 : 2;
+    const bool vec = (((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0 && ld * size % 16 == 0;
+    const dim3 grid((rows->M + per - 1) / per);
+    auto go = [&](auto hs_c, auto zero) {
+        constexpr int HS = decltype(hs_c)::value;
+        using T = decltype(zero);
+        return vec ? kv8_launch("dl_kv8_read", kv8_read_kernel<HS, T, true>, a, grid, KV8_READ_WARPS * 32, pdl, stream)
+                   : kv8_launch("dl_kv8_read", kv8_read_kernel<HS, T, false>, a, grid, KV8_READ_WARPS * 32, pdl, stream);
+    };
+    auto typed = [&](auto hs_c) {
+        if (out_type == DL_KV8_F32) return go(hs_c, float());
+        if (out_type == DL_KV8_BF16) return go(hs_c, __nv_bfloat16());
+        return go(hs_c, __half());
+    };
+    if (hs == 128) return typed(std::integral_constant<int, 128>());
+    if (hs == 64) return typed(std::integral_constant<int, 64>());
+    return typed(std::integral_constant<int, 32>());
+}

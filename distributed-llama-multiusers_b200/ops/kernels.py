@@ -12,7 +12,7 @@ from typing import List, Optional, Sequence
 import torch
 
 from . import lib
-from .lib import DlEpilogue, DlNormProlog, EPI_QKV_ROPE, EPI_SILU_MUL, EPI_STORE, check, cuda_lib
+from .lib import DlEpilogue, DlKv8Cache, DlKv8Rows, DlNormProlog, EPI_QKV_ROPE, EPI_SILU_MUL, EPI_STORE, KV8_BF16, KV8_F16, KV8_F32, check, cuda_lib
 
 Q40T_TILE_BYTES = 9216
 XQ_ROW_BYTES = 160
@@ -244,6 +244,150 @@ def attention_prefill(q, M, n_heads, n_kv_heads, head_size, k_cache, v_cache, po
         check(cuda_lib().dl_attention_prefill_tc(*args, int(k_cache.shape[0]), 1 if pdl else 0, _stream()), "dl_attention_prefill_tc")
     else:
         check(cuda_lib().dl_attention_prefill(*args, 1 if pdl else 0, _stream()), "dl_attention_prefill")
+    lib.count_launch()
+
+
+# ---- 8-bit token cache ----------------------------------------------------------------------------
+# int8 codes and one f32 scale for each token and key/value head: value = code * scale, scale = f32(amax / 127) of the token's line,
+# code = rint(x * f32(127 / amax)).  Arguments that a launch could not take raise ValueError; rows whose page is not in the tables read as NaN.
+_KV8_TYPES = {torch.float32: KV8_F32, torch.bfloat16: KV8_BF16, torch.float16: KV8_F16}
+
+
+class Kv8Cache:
+    """The pages of one layer's 8-bit token cache: k / v int8 [pages][kv heads][32][head size], k_scale / v_scale f32 [pages][kv heads][32].
+    Checked once, here; the tensors have to keep their memory."""
+    __slots__ = ("k", "v", "k_scale", "v_scale", "n_pages", "n_kv_heads", "head_size", "device", "args", "ref")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        if k.dim() != 4 or k.shape[2] != PAGE_SIZE or k.shape[3] not in (32, 64, 128) or k.shape[0] < 1 or k.shape[1] < 1:
+            raise ValueError(f"codes of shape {tuple(k.shape)}: [pages][kv heads][{PAGE_SIZE}][32, 64 or 128] is wanted")
+        if v.shape != k.shape or k_scale.shape != k.shape[:3] or v_scale.shape != k.shape[:3]:
+            raise ValueError(f"values {tuple(v.shape)}, scales {tuple(k_scale.shape)} and {tuple(v_scale.shape)} beside keys {tuple(k.shape)}")
+        if k.dtype != torch.int8 or v.dtype != torch.int8 or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+            raise ValueError(f"int8 codes and f32 scales are wanted: {k.dtype}, {v.dtype}, {k_scale.dtype}, {v_scale.dtype}")
+        for t in (k, v, k_scale, v_scale):
+            if t.device != k.device or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError("codes and scales have to be contiguous, on one device and aligned to 16 bytes")
+        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
+        self.n_pages, self.n_kv_heads, self.head_size = k.shape[0], k.shape[1], k.shape[3]
+        self.args = DlKv8Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.n_pages, self.n_kv_heads, self.head_size)
+        self.ref = C.byref(self.args)
+
+    def nbytes(self) -> int:
+        return kv8_page_bytes(self.n_kv_heads, self.head_size) * self.n_pages
+
+
+def kv8_page_bytes(n_kv_heads: int, head_size: int) -> int:
+    """Bytes of one page of one layer: codes and scales of 32 keys and values."""
+    return 2 * n_kv_heads * PAGE_SIZE * (head_size + 4)
+
+
+def alloc_kv8(n_pages: int, n_kv_heads: int, head_size: int, device) -> Kv8Cache:
+    codes = [torch.zeros(n_pages, n_kv_heads, PAGE_SIZE, head_size, dtype=torch.int8, device=device) for _ in range(2)]
+    return Kv8Cache(*codes, *(torch.zeros(n_pages, n_kv_heads, PAGE_SIZE, dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _kv8_rows(M: int, pos: torch.Tensor, slot: torch.Tensor, block_table: torch.Tensor, cache: Kv8Cache) -> DlKv8Rows:
+    dev = cache.device
+    if dev.type != "cuda" or dev.index != torch.cuda.current_device():
+        raise ValueError(f"the cache is on {dev}: the current device launches")
+    for t in (pos, slot, block_table):
+        if t.dtype is not torch.int32 or t.device != dev or not t.is_contiguous():
+            raise ValueError("pos, slot and block_table are contiguous int32 tensors on the cache's device")
+    if block_table.dim() != 2 or not 0 <= M <= pos.numel() or M > slot.numel():
+        raise ValueError(f"{M} rows of {pos.numel()} positions and {slot.numel()} sequences, block table {tuple(block_table.shape)}")
+    return DlKv8Rows(pos.data_ptr(), slot.data_ptr(), block_table.data_ptr(), M, block_table.shape[0], block_table.shape[1])
+
+
+def _kv8_matrix(t: torch.Tensor, M: int, cols: int, cache: Kv8Cache, what: str) -> int:
+    """Row stride of [>= M][cols] (neighbouring values of a row lie side by side)."""
+    if t.dim() != 2 or t.shape[0] < M or t.shape[1] != cols or t.device != cache.device or t.stride(1) != 1:
+        raise ValueError(f"{what} {tuple(t.shape)} on {t.device}: at least {M} rows of {cols} values on {cache.device} are wanted")
+    return t.stride(0) if t.shape[0] > 1 else cols
+
+
+def kv8_write(qkv: torch.Tensor, M: int, n_heads: int, freqs: Optional[torch.Tensor], pos, slot, block_table, q_out: Optional[torch.Tensor],
+              cache: Kv8Cache, pdl: bool = False):
+    """Merged rows q | k | v (f32): rotary positions on queries and keys (freqs [head size / 2], None: none), queries to q_out, keys and values
+    as codes and scales into the pages.  Rows with a negative position write nothing; rows of one place have to hold the same values."""
+    rows = _kv8_rows(M, pos, slot, block_table, cache)
+    hs = cache.head_size
+    ld = _kv8_matrix(qkv, M, (n_heads + 2 * cache.n_kv_heads) * hs, cache, "qkv")
+    ldq = _kv8_matrix(q_out, M, n_heads * hs, cache, "q_out") if n_heads else 0
+    if qkv.dtype is not torch.float32 or (n_heads and q_out.dtype is not torch.float32):
+        raise ValueError("qkv and q_out are f32")
+    if freqs is not None and (freqs.dtype is not torch.float32 or freqs.device != cache.device or freqs.numel() != hs // 2 or not freqs.is_contiguous()):
+        raise ValueError(f"{hs // 2} f32 frequencies are wanted")
+    check(cuda_lib().dl_kv8_write(qkv.data_ptr(), ld, n_heads, _p(freqs), C.byref(rows), q_out.data_ptr() if n_heads else None, ldq, cache.ref,
+                                  1 if pdl else 0, _stream()), "dl_kv8_write")
+    lib.count_launch()
+
+
+def kv8_read(M: int, pos, slot, block_table, cache: Kv8Cache, k_out: torch.Tensor, v_out: torch.Tensor, pdl: bool = False):
+    """The rows' keys and values out of their pages, [M][kv heads * head size] of f32, fp16 or bf16.  Any rows in any order: a whole conversation is
+    pos = arange(n) with its sequence in every place of slot."""
+    rows = _kv8_rows(M, pos, slot, block_table, cache)
+    cols = cache.n_kv_heads * cache.head_size
+    ld = _kv8_matrix(k_out, M, cols, cache, "k_out")
+    if _kv8_matrix(v_out, M, cols, cache, "v_out") != ld or k_out.dtype is not v_out.dtype or k_out.dtype not in _KV8_TYPES:
+        raise ValueError("k_out and v_out are f32, fp16 or bf16, alike in type and row stride")
+    check(cuda_lib().dl_kv8_read(C.byref(rows), cache.ref, k_out.data_ptr(), v_out.data_ptr(), ld, _KV8_TYPES[k_out.dtype], 1 if pdl else 0, _stream()),
+          "dl_kv8_read")
+    lib.count_launch()
+
+
+def _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out):
+    """Row strides of q and y_out, type of y_out."""
+    cols = n_heads * cache.head_size
+    ldq = _kv8_matrix(q, M, cols, cache, "q")
+    if q.dtype is not torch.float32:
+        raise ValueError("q is f32")
+    ldy, y_type = 0, KV8_F32
+    if y_out is not None:
+        ldy = _kv8_matrix(y_out, M, cols, cache, "y_out")
+        if y_out.dtype not in _KV8_TYPES:
+            raise ValueError("y_out is f32, fp16 or bf16")
+        y_type = _KV8_TYPES[y_out.dtype]
+    if xq_out is not None and xq_out.numel() < xq_bytes(cols, out_mcap) or xh_out is not None and xh_out.numel() < xh_bytes(cols, out_mcap):
+        raise ValueError(f"slabs smaller than {out_mcap} rows of {cols} values")
+    return ldq, ldy, y_type
+
+
+def kv8_attention_splits(M: int, n_heads: int, n_kv_heads: int, max_pages: int, n_sms: int = 148) -> int:
+    """Shares of the longest context that kv8_attention is given for M rows (a row takes no more than its own context is worth)."""
+    return int(max(1, min(n_sms // max(1, M * n_kv_heads), max_pages // 8, 32)))
+
+
+def kv8_attention(q, M: int, n_heads: int, pos, slot, block_table, cache: Kv8Cache, n_splits: int, scratch, xq_out=None, xh_out=None, out_mcap: int = 0,
+                  y_out=None, row_skip=None, pdl: bool = False):
+    """`attention` over an 8-bit cache.  scratch: attention_scratch_bytes() zeroed once (None with one split); launches that may run at the same time --
+    on two streams, or in two graphs -- need scratches of their own."""
+    rows = _kv8_rows(M, pos, slot, block_table, cache)
+    ldq, ldy, y_type = _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out)
+    if n_splits > 1 and (scratch is None or scratch.device != cache.device or scratch.numel() * scratch.element_size() < attention_scratch_bytes(M, n_heads, cache.head_size, n_splits)):
+        raise ValueError(f"{n_splits} splits of {M} rows need attention_scratch_bytes() of scratch on the cache's device")
+    if row_skip is not None and (row_skip.dtype is not torch.int32 or row_skip.device != cache.device or row_skip.numel() < M or not row_skip.is_contiguous()):
+        raise ValueError("row_skip is a contiguous int32 tensor of at least M values")
+    check(cuda_lib().dl_kv8_attention(q.data_ptr(), ldq, n_heads, C.byref(rows), cache.ref, n_splits, _p(scratch), _p(xq_out), _p(xh_out), out_mcap,
+                                      _p(y_out), ldy, y_type, _p(row_skip), 1 if pdl else 0, _stream()), "dl_kv8_attention")
+    lib.count_launch()
+
+
+def kv8_prefill_workspace(n_pages: int, n_kv_heads: int, head_size: int, max_rows: int, device):
+    """What kv8_attention_prefill wants beside its arguments for prompt chunks of up to max_rows rows: a pair of tensors, or None."""
+    return None
+
+
+def kv8_attention_prefill(q, M: int, n_heads: int, pos, slot, block_table, meta, cache: Kv8Cache, workspace=None, xq_out=None, xh_out=None, out_mcap: int = 0,
+                          y_out=None, pdl: bool = False):
+    """`attention_prefill` over an 8-bit cache: meta = [n_seg, begin0, end0, ...] (device int32), each range consecutive positions of one sequence; rows
+    outside are not touched.  workspace: kv8_prefill_workspace(), for one launch at a time."""
+    rows = _kv8_rows(M, pos, slot, block_table, cache)
+    ldq, ldy, y_type = _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out)
+    if meta.dtype is not torch.int32 or meta.device != cache.device or not meta.is_contiguous() or meta.numel() < 3:
+        raise ValueError("meta is a contiguous int32 tensor [n_seg, begin, end, ...]")
+    check(cuda_lib().dl_kv8_attention_prefill(q.data_ptr(), ldq, n_heads, C.byref(rows), meta.data_ptr(), cache.ref, None, None, _p(xq_out), _p(xh_out),
+                                              out_mcap, _p(y_out), ldy, y_type, 1 if pdl else 0, _stream()), "dl_kv8_attention_prefill")
     lib.count_launch()
 
 

@@ -85,6 +85,21 @@ class DlNormProlog(C.Structure):
     ]
 
 
+KV8_F32, KV8_BF16, KV8_F16 = 0, 1, 2
+
+
+class DlKv8Cache(C.Structure):
+    """Mirror of ``DlKv8Cache`` in include/dllama_b200.h."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("n_pages", C.c_int), ("n_kv_heads", C.c_int), ("head_size", C.c_int)]
+
+
+class DlKv8Rows(C.Structure):
+    """Mirror of ``DlKv8Rows``."""
+    _fields_ = [("pos", C.c_void_p), ("slot", C.c_void_p), ("block_table", C.c_void_p),
+                ("M", C.c_int), ("n_slots", C.c_int), ("max_pages", C.c_int)]
+
+
 class DlDecodeLayer(C.Structure):
     """Mirror of ``DlDecodeLayer`` (per-layer device pointers of the persistent decode kernel)."""
     _fields_ = [("qkv", C.c_void_p), ("wo", C.c_void_p), ("w13", C.c_void_p), ("w2", C.c_void_p),
@@ -190,6 +205,12 @@ def cuda_lib():
     L.dl_ipc_close.argtypes = [vp]
     L.dl_ipc_free.argtypes = [vp]
     L.dl_peer_barrier.argtypes = [C.POINTER(vp), vp, i32, i32, u32, vp]
+    L.dl_kv8_write.argtypes = [vp, i64, i32, vp, vp, vp, i64, vp, i32, vp]
+    L.dl_kv8_read.argtypes = [vp, vp, vp, vp, i64, i32, i32, vp]
+    L.dl_kv8_attention.argtypes = [vp, i64, i32, vp, vp, i32, vp, vp, vp, i32, vp, i64, i32, vp, i32, vp]
+    L.dl_kv8_attention_prefill.argtypes = [vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, i32, vp, i64, i32, i32, vp]
+    for name in ("dl_kv8_write", "dl_kv8_read", "dl_kv8_attention", "dl_kv8_attention_prefill"):
+        getattr(L, name).restype = i32
     L.dl_f32_rope_kv.argtypes = [vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp, vp, vp, i32, vp]
     L.dl_f32_silu_mul.argtypes = [vp, vp, vp, i64, i32, vp]
     L.dl_f32_push.argtypes = [vp, i32, i32, i32, C.POINTER(vp), i32, i64, i32, C.POINTER(vp), vp, u32, u32, vp, vp]

@@ -206,6 +206,42 @@ int dl_attention_prefill_tc(const float* q, int M, int n_heads, int n_kv_heads, 
                             float* y_out, int n_cache_pages /*pages in k_cache / v_cache: bounds of the TMA tensor maps*/,
                             int pdl, void* stream);
 
+/* ---- 8-bit token cache ------------------------------------------------------------------- */
+/* Keys and values as int8 codes with one f32 scale for each token and key/value head: value = code * scale, scale = f32(amax / 127) of the
+ * token's line, code = rint(x * f32(127 / amax)).  A line whose largest magnitude is below 2^-100 is held as zeros, one with an infinity or a NaN
+ * has the scale NaN.  Pages of 32 tokens, as of the fp16 cache; all four arrays aligned to 16 bytes. */
+enum { DL_KV8_F32 = 0, DL_KV8_BF16 = 1, DL_KV8_F16 = 2 };      /* types of outputs */
+typedef struct {
+    int8_t* k;                 /* [n_pages][n_kv_heads][32][head_size] */
+    int8_t* v;
+    float* k_scale;            /* [n_pages][n_kv_heads][32] */
+    float* v_scale;
+    int n_pages, n_kv_heads, head_size;      /* head_size 32, 64 or 128 */
+} DlKv8Cache;
+/* The rows of a batch: row m is position pos[m] of sequence slot[m], whose page i is block_table[slot * max_pages + i].  A row with a negative position
+ * has no token: nothing is written or read, attention gives zeros.  Sequences, positions and pages that are not in the tables are not followed: nothing
+ * is written, what is read or attended to is NaN. */
+typedef struct {
+    const int* pos;            /* device, [M] */
+    const int* slot;
+    const int* block_table;    /* device, [n_slots][max_pages] */
+    int M, n_slots, max_pages;
+} DlKv8Rows;
+/* merged rows q | k | v (row stride ld_qkv): rotary positions on the n_heads query heads and the key heads (pairs of neighbouring values; freqs NULL: none),
+ * queries to q_out (row stride ld_q), keys and values into their pages.  Keys are turned in 64 bits and rounded once, so that their codes do not depend on the
+ * order of anything.  Rows of one place (slot, position) have to hold the same values (reference: OP_ROPE_LLAMA + OP_SHIFT, nn-cpu-ops.cpp:1090-1120,1253-1275) */
+int dl_kv8_write(const float* qkv, long long ld_qkv, int n_heads, const float* freqs, const DlKv8Rows* rows /*host*/, float* q_out, long long ld_q,
+                 const DlKv8Cache* cache /*host*/, int pdl, void* stream);
+/* the rows' keys and values out of their pages: k_out / v_out [M][n_kv_heads * head_size] of DL_KV8_* (row stride ld), code * scale rounded once */
+int dl_kv8_read(const DlKv8Rows* rows /*host*/, const DlKv8Cache* cache /*host*/, void* k_out, void* v_out, long long ld, int out_type, int pdl, void* stream);
+/* dl_attention over the 8-bit cache: at most 16 query heads for each key/value head; y_out of DL_KV8_*.  scratch: dl_attention_scratch_bytes(), zeroed once; launches
+ * that may run at the same time need scratches of their own */
+int dl_kv8_attention(const float* q, long long ldq, int n_heads, const DlKv8Rows* rows /*host*/, const DlKv8Cache* cache /*host*/, int n_splits, void* scratch,
+                     uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, const int* row_skip, int pdl, void* stream);
+/* dl_attention_prefill over the 8-bit cache (meta as there) */
+int dl_kv8_attention_prefill(const float* q, long long ldq, int n_heads, const DlKv8Rows* rows /*host*/, const int* meta /*device*/, const DlKv8Cache* cache /*host*/,
+                             void* k16, void* v16, uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, int pdl, void* stream);
+
 /* Kernels that wait on copies inside a CTA (dl_attention_prefill_tc, dl_window_attention_tc's prompts, dl_attention on a ring of pages, dl_gemv_q40, dl_gemm_q40_tc,
  * dl_dense's ring for one and two rows) wait for some seconds at most.  Where one gives up, the outputs of that launch are not valid (NaN, of
  * dl_gemm_q40_tc most) and this word (in host memory; each device has its own, this is the current one's) changes: read it behind a synchronisation
