@@ -65,7 +65,8 @@ struct PtArgs {
     uint8_t* xq_out;
     uint8_t* xh_out;
     int out_mcap;
-    float* y_out;
+    void* y_out;               // [M][n_heads*128] of DL_KV8_F32 / BF16 / F16
+    int y_type;
     unsigned long long* tr;
     WaitLimit limit;
 };
@@ -657,8 +658,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
             } else {
                 inv = l > 0.0f ? 1.0f / l : 0.0f;
             }
-            float* out = nullptr;                                // this thread's row; null: none
+            float* out = nullptr;                                // this thread's row (of 16-bit values: y16); null: none
             bool vec = true;                                     // 16-byte rows
+            bool y16 = false;
             if constexpr (LINES) {
                 if (row0 >= it.rows || (it.shares == 1 && blockIdx.z > 0)) continue;
                 out = a.w.out + (size_t)m_row * a.w.ldo + h_row * PT_HS;
@@ -680,7 +682,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                 if (jb == ja) continue;
             } else {
                 if (jb == ja) continue;
-                if (a.y_out != nullptr) out = a.y_out + (size_t)(it.begin + r_live) * a.n_heads * PT_HS + head * PT_HS;
+                y16 = a.y_type != DL_KV8_F32;
+                if (a.y_out != nullptr) {
+                    const size_t at = (size_t)(it.begin + r_live) * a.n_heads * PT_HS + head * PT_HS;
+                    out = y16 ? reinterpret_cast<float*>(reinterpret_cast<uint16_t*>(a.y_out) + at) : reinterpret_cast<float*>(a.y_out) + at;
+                }
                 vec = ((uintptr_t)a.y_out & 15) == 0;
             }
             if constexpr (LINES) {                               // (the barrier's phase in the topmost bit)
@@ -714,9 +720,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
 #pragma unroll
                     for (int rr = 0; rr < 32; rr += 8) {
                         const int r = rr + (lane >> 2);
-                        float* dst = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)out, r)) + ch * 32 + h * 16 + (lane & 3) * 4;
+                        float* dst = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)out, r));
+                        const int col = ch * 32 + h * 16 + (lane & 3) * 4;
                         const float4 x = *reinterpret_cast<const float4*>(stage + r * PT_OUT_LD + (lane & 3) * 4);
                         if (r >= live) continue;
+                        if constexpr (!LINES) {
+                            if (y16) {                           // (rows of 8 bytes' alignment: dl_kv8_attention_prefill)
+                                uint2 w = make_uint2(pt_pack2<false>(x.x, x.y), pt_pack2<false>(x.z, x.w));
+                                if (a.y_type == DL_KV8_BF16) w = make_uint2(pt_pack2<true>(x.x, x.y), pt_pack2<true>(x.z, x.w));
+                                *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(dst) + col) = w;
+                                continue;
+                            }
+                        }
+                        dst += col;
                         if (vec) *reinterpret_cast<float4*>(dst) = x;
                         else { dst[0] = x.x; dst[1] = x.y; dst[2] = x.z; dst[3] = x.w; }
                     }
@@ -895,17 +911,17 @@ static int pt_make_map(CUtensorMap* m, const void* base, long long rows, int wid
     return dl_tensor_map("attention_prefill_tc", m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-extern "C" int dl_attention_prefill_tc(const float* q, int M, int n_heads, int n_kv_heads, int head_size, const void* k_cache,
-                                       const void* v_cache, const int* pos, const int* slot, const int* block_table,
-                                       int max_pages, int page_size, const int* meta, uint8_t* xq_out, uint8_t* xh_out,
-                                       int out_mcap, float* y_out, int n_cache_pages, int pdl, void* stream) {
+// y_type other than f32: y_out aligned to 8 bytes
+int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_heads, int head_size, const void* k_cache, const void* v_cache, const int* pos,
+                                  const int* slot, const int* block_table, int max_pages, int page_size, const int* meta, uint8_t* xq_out, uint8_t* xh_out,
+                                  int out_mcap, void* y_out, int y_type, int n_cache_pages, int pdl, void* stream) {
     if (page_size != 32 || head_size != PT_HS) { dl_set_error("dl_attention_prefill_tc: page size 32 and head size 128 only"); return -1; }
     if (n_heads % n_kv_heads != 0) { dl_set_error("dl_attention_prefill_tc: bad head grouping"); return -1; }
     if (n_cache_pages < 1) { dl_set_error("dl_attention_prefill_tc: n_cache_pages < 1"); return -1; }
     PtArgs a;
     a.q = q; a.k_cache = (const __half*)k_cache; a.v_cache = (const __half*)v_cache; a.pos = pos; a.slot = slot;
     a.block_table = block_table; a.meta = meta; a.M = M; a.n_heads = n_heads; a.n_kv_heads = n_kv_heads;
-    a.max_pages = max_pages; a.xq_out = xq_out; a.xh_out = xh_out; a.out_mcap = out_mcap; a.y_out = y_out;
+    a.max_pages = max_pages; a.xq_out = xq_out; a.xh_out = xh_out; a.out_mcap = out_mcap; a.y_out = y_out; a.y_type = y_type;
     if (pt_limit(&a.limit) != 0) return -1;
     a.tr = dl_trace_next(TR_ATT);
     alignas(64) CUtensorMap kmap, vmap;
@@ -930,6 +946,14 @@ extern "C" int dl_attention_prefill_tc(const float* q, int M, int n_heads, int n
     cudaError_t e = cudaLaunchKernelEx(&cfg, attention_prefill_tc_kernel<false>, a, kmap, vmap);
     if (e != cudaSuccess) { dl_set_error("attention_prefill_tc launch: %s", cudaGetErrorString(e)); return -(int)e; }
     return 0;
+}
+
+extern "C" int dl_attention_prefill_tc(const float* q, int M, int n_heads, int n_kv_heads, int head_size, const void* k_cache,
+                                       const void* v_cache, const int* pos, const int* slot, const int* block_table,
+                                       int max_pages, int page_size, const int* meta, uint8_t* xq_out, uint8_t* xh_out,
+                                       int out_mcap, float* y_out, int n_cache_pages, int pdl, void* stream) {
+    return dl_attention_prefill_tc_typed(q, M, n_heads, n_kv_heads, head_size, k_cache, v_cache, pos, slot, block_table, max_pages, page_size, meta, xq_out, xh_out,
+                                         out_mcap, y_out, DL_KV8_F32, n_cache_pages, pdl, stream);
 }
 
 // 0 if the kernel's LINES instance takes these sizes: bf16 lines of a key and a value of 128, full tiles of 64 stacked rows

@@ -13,6 +13,7 @@
 #include "smem_limit.cuh"
 
 extern void dl_set_error(const char* fmt, ...);
+extern int dl_device_sm_count();
 extern int kv8_check(const char* who, const DlKv8Cache* c, const DlKv8Rows* r);
 
 struct Kv8AttArgs {
@@ -121,8 +122,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
         n_live = min(SR, (end - begin) * G - s_lo);
         p0 = a.rows.pos[begin];
         slot = a.rows.slot[begin];
-        bad = kv8_tokens(a.rows, max(p0, 0) + (end - begin) - 1, slot) < 0;
-        T = bad ? 0 : max(0, p0 + (s_lo + n_live - 1) / G + 1);
+        bad = p0 >= 0 && (p0 > 0x7fffffff - (end - begin) || kv8_tokens(a.rows, p0 + (end - begin) - 1, slot) < 0);
+        T = bad || p0 < 0 ? 0 : p0 + (s_lo + n_live - 1) / G + 1;
     } else {
         m0 = blockIdx.z;
         if (a.row_skip != nullptr && a.row_skip[m0] != 0) return;
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
         for (int n = 0; n < NT; n++) o[mt][n][0] = o[mt][n][1] = 0.f;
     }
     int all = T;                                               // tokens that every live row of the CTA sees
-    if (PROMPT) all = max(0, p0 + s_lo / G + 1);
+    if (PROMPT) all = min(T, p0 + s_lo / G + 1);
 
     // lane's rows of the two ldmatrix forms: tokens and the pieces that they start from
     const int kt = ((lane >> 4) << 3) + (lane & 7), kc = (lane >> 3) & 1;                                   // + 16 j / 2: n-tiles j, j + 1
@@ -493,6 +494,106 @@ static int ka_prompt(const Kv8AttArgs& a, int pdl, void* stream) {
     return ka_launch<HS, MT, true, 2>("dl_kv8_attention_prefill", a, wk, dim3((unsigned)tiles, kv), pdl, stream);
 }
 
+// ------------------------------------------------------------------------------------------------
+// Long prompt chunks of heads of 128: the segments' pages widened once to fp16 (fp16(code * scale): 2^-12 of a value, the queries of that kernel are rounded alike),
+// then the tcgen05 kernel of the fp16 cache on them, under the same page numbers.  Widening inside that kernel would be done again by every CTA that meets a page
+// (rows / 128 * heads / 2 of them).  4001 rows: 12 MB in and 16 MB out, beside 131 GFLOP.
+//
+// A line with a NaN (of the key or the value) becomes a key of NaN and a value of zeros: the rows that see it give NaN, and the weights of 0 that others
+// have for it do not.  Values beyond fp16's range saturate.  What that kernel does not look at is looked at here: the segments that are in the tables are listed
+// for it, rows of the others get NaN.
+// ------------------------------------------------------------------------------------------------
+struct Kv8ExpandArgs {
+    Kv8AttArgs a;
+    __half* k16;               // [pages][kv][32][128]
+    __half* v16;
+    int* meta_out;             // [17]
+};
+
+__global__ void __launch_bounds__(256) kv8_expand_kernel(const __grid_constant__ Kv8ExpandArgs x) {
+    constexpr int HS = 128;
+    __shared__ int first[9], seg[8][3];                        // items ahead of a segment; begin, end, slot
+    __shared__ int ok[8];
+    const int tid = threadIdx.x, kv = x.a.c.n_kv_heads;
+    pdl_launch_dependents();
+    pdl_wait();
+    if (tid == 0) {
+        const int n = max(0, min(x.a.meta[0], 8));
+        int at = 0;
+        for (int i = 0; i < 8; i++) {
+            first[i] = at;
+            const int b = i < n ? x.a.meta[1 + 2 * i] : 0, e = i < n ? x.a.meta[2 + 2 * i] : 0;
+            const bool rows = b >= 0 && e <= x.a.rows.M && e > b;
+            const int p = rows ? x.a.rows.pos[b] : 0, s = rows ? x.a.rows.slot[b] : 0;
+            ok[i] = rows && p >= 0 && p <= 0x7fffffff - (e - b) && kv8_tokens(x.a.rows, p + (e - b) - 1, s) > 0;
+            seg[i][0] = b; seg[i][1] = rows ? e : b; seg[i][2] = s;
+            if (ok[i]) at += (p + (e - b) + KV8_PAGE - 1) / KV8_PAGE * kv;
+        }
+        first[8] = at;
+    }
+    __syncthreads();
+    // pages that are not there: the first CTA, which lists the segments, takes theirs as one that is not in the tables
+    for (int i = 0; i < 8; i++) {
+        if (!ok[i]) continue;
+        const int* bt = x.a.rows.block_table + (size_t)seg[i][2] * x.a.rows.max_pages;
+        const int pages = (first[i + 1] - first[i]) / kv;
+        bool bad = false;
+        if (blockIdx.x == 0)
+            for (int p = tid; p < pages; p += 256) bad |= (unsigned)bt[p] >= (unsigned)x.a.rows.n_pages;
+        if (__syncthreads_or(bad) && tid == 0) ok[i] = 0;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        if (tid == 0) {
+            int n = 0;
+            for (int i = 0; i < 8; i++)
+                if (ok[i]) { x.meta_out[1 + 2 * n] = seg[i][0]; x.meta_out[2 + 2 * n] = seg[i][1]; n++; }
+            x.meta_out[0] = n;
+        }
+        const int cols = x.a.heads * HS;
+        for (int i = 0; i < 8; i++) {
+            if (ok[i] || seg[i][1] <= seg[i][0]) continue;
+            const float none = x.a.rows.pos[seg[i][0]] < 0 ? 0.f : __uint_as_float(0x7fffffffu);      // (rows without tokens)
+            for (int m = seg[i][0] + (tid >> 5); m < seg[i][1]; m += 8)
+                for (int c = tid & 31; c < cols; c += 32) {
+                    kv8_store_y(x.a, m, c, none);
+                    if (x.a.xq_out != nullptr || x.a.xh_out != nullptr) q80_block_store(none, tid & 31, m, c >> 5, x.a.out_mcap, x.a.xq_out, x.a.xh_out);
+                }
+        }
+    }
+    for (int item = blockIdx.x; item < first[8]; item += gridDim.x) {
+        int i = 0;
+        while (item >= first[i + 1]) i++;
+        const int in = item - first[i], kvh = in % kv;
+        const int page = x.a.rows.block_table[(size_t)seg[i][2] * x.a.rows.max_pages + in / kv];
+        if ((unsigned)page >= (unsigned)x.a.rows.n_pages) continue;
+        const size_t line = ((size_t)page * kv + kvh) * KV8_PAGE + (tid >> 3);
+        const size_t at = line * HS + (tid & 7) * 16;
+        const uint4 kc = *reinterpret_cast<const uint4*>(x.a.c.k + at), vc = *reinterpret_cast<const uint4*>(x.a.c.v + at);
+        float ks = x.a.c.k_scale[line], vs = x.a.c.v_scale[line];
+        if (!(fabsf(ks) < INFINITY) || !(fabsf(vs) < INFINITY)) { ks = __uint_as_float(0x7fffffffu); vs = 0.f; }
+        auto widen = [](uint4 c, float s, __half* dst) {
+            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+            uint32_t o[8];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                float f[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    f[u] = (float)(int8_t)(w[e / 4] >> (8 * ((e + u) % 4))) * s;
+                    f[u] = f[u] != f[u] ? f[u] : fminf(fmaxf(f[u], -65504.f), 65504.f);
+                }
+                const __half2 h = __floats2half2_rn(f[0], f[1]);
+                o[e / 2] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            reinterpret_cast<uint4*>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            reinterpret_cast<uint4*>(dst)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        };
+        widen(kc, ks, x.k16 + at);
+        widen(vc, vs, x.v16 + at);
+    }
+}
+
 // what both entry points refuse
 static int kv8_att_args(const char* who, const float* q, long long ldq, int n_heads, const DlKv8Rows* rows, const DlKv8Cache* cache, uint8_t* xq_out, uint8_t* xh_out,
                         int out_mcap, void* y_out, long long ldy, int y_type, Kv8AttArgs* a) {
@@ -524,13 +625,40 @@ extern "C" int dl_kv8_attention(const float* q, long long ldq, int n_heads, cons
     return hs == 128 ? ka_decode<128>(a, n_splits, scratch, pdl, stream) : hs == 64 ? ka_decode<64>(a, n_splits, scratch, pdl, stream) : ka_decode<32>(a, n_splits, scratch, pdl, stream);
 }
 
+// Rows times heads above which heads of 128 take the tcgen05 kernel on widened pages, where there is a workspace (us on mma.sync / widened, 32 heads: 128 rows
+// behind 1000 tokens 21 / 24, behind 8000 95 / 92, 256 behind 2000 63 / 36, 512 behind 4000 208 / 60; 8 heads: 512 rows behind none 13.5 / 17.9, 1024 27 / 22)
+#define KV8_EXPAND_MIN_WORK 4096
+
+extern int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_heads, int head_size, const void* k_cache, const void* v_cache, const int* pos,
+                                         const int* slot, const int* block_table, int max_pages, int page_size, const int* meta, uint8_t* xq_out, uint8_t* xh_out,
+                                         int out_mcap, void* y_out, int y_type, int n_cache_pages, int pdl, void* stream);
+
 extern "C" int dl_kv8_attention_prefill(const float* q, long long ldq, int n_heads, const DlKv8Rows* rows, const int* meta, const DlKv8Cache* cache, void* k16, void* v16,
-                                        uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, int pdl, void* stream) {
+                                        int* meta16, uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, int pdl, void* stream) {
     Kv8AttArgs a;
     if (const int rc = kv8_att_args("dl_kv8_attention_prefill", q, ldq, n_heads, rows, cache, xq_out, xh_out, out_mcap, y_out, ldy, y_type, &a)) return rc;
-    if (meta == nullptr || (k16 == nullptr) != (v16 == nullptr)) { dl_set_error("dl_kv8_attention_prefill: a null pointer"); return -1; }
+    if (meta == nullptr || (k16 == nullptr) != (v16 == nullptr) || (k16 == nullptr) != (meta16 == nullptr)) { dl_set_error("dl_kv8_attention_prefill: a null pointer"); return -1; }
     if (rows->M == 0) return 0;
     a.meta = meta;
     const int hs = cache->head_size;
+    // (that kernel takes rows side by side, aligned)
+    const bool dense = ldq == (long long)n_heads * hs && ((uintptr_t)q & 15) == 0 && (y_out == nullptr || (ldy == ldq && ((uintptr_t)y_out & 15) == 0));
+    if (k16 != nullptr && hs == 128 && dense && (long long)rows->M * n_heads > KV8_EXPAND_MIN_WORK) {
+        if ((((uintptr_t)k16 | (uintptr_t)v16) & 15) != 0) { dl_set_error("dl_kv8_attention_prefill: the workspace has to be aligned to 16 bytes"); return -1; }
+        const Kv8ExpandArgs x = {a, (__half*)k16, (__half*)v16, meta16};
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(4 * dl_device_sm_count());
+        cfg.blockDim = dim3(256);
+        cfg.stream = (cudaStream_t)stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = pdl ? 1 : 0;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_expand_kernel, x);
+        if (e != cudaSuccess) { dl_set_error("dl_kv8_attention_prefill launch: %s", cudaGetErrorString(e)); return -(int)e; }
+        return dl_attention_prefill_tc_typed(q, rows->M, n_heads, cache->n_kv_heads, hs, k16, v16, rows->pos, rows->slot, rows->block_table, rows->max_pages, KV8_PAGE, meta16,
+                                             xq_out, xh_out, out_mcap, y_out, y_type, cache->n_pages, 1, stream);
+    }
     return hs == 128 ? ka_prompt<128>(a, pdl, stream) : hs == 64 ? ka_prompt<64>(a, pdl, stream) : ka_prompt<32>(a, pdl, stream);
 }

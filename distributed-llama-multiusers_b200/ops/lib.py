@@ -208,7 +208,7 @@ def cuda_lib():
     L.dl_kv8_write.argtypes = [vp, i64, i32, vp, vp, vp, i64, vp, i32, vp]
     L.dl_kv8_read.argtypes = [vp, vp, vp, vp, i64, i32, i32, vp]
     L.dl_kv8_attention.argtypes = [vp, i64, i32, vp, vp, i32, vp, vp, vp, i32, vp, i64, i32, vp, i32, vp]
-    L.dl_kv8_attention_prefill.argtypes = [vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, i32, vp, i64, i32, i32, vp]
+    L.dl_kv8_attention_prefill.argtypes = [vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, vp, i32, vp, i64, i32, i32, vp]
     for name in ("dl_kv8_write", "dl_kv8_read", "dl_kv8_attention", "dl_kv8_attention_prefill"):
         getattr(L, name).restype = i32
     L.dl_f32_rope_kv.argtypes = [vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp, vp, vp, i32, vp]

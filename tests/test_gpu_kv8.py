@@ -331,8 +331,8 @@ PROMPT_REL = 4e-3
 
 @pytest.mark.parametrize("heads,kv,hs,segs", [
     (4, 1, 128, [(0, 0, 16)]), (8, 2, 128, [(0, 37, 100)]), (4, 4, 64, [(3, 5, 70)]), (2, 1, 128, [(62, 200, 130)]), (2, 2, 64, [(31, 31, 33)]),
-    (4, 2, 128, [(2, 10, 40), (45, 0, 90)]), (4, 4, 128, [(0, 0, 700)]), (2, 1, 128, [(5, 900, 300)]), (8, 2, 128, [(0, 0, 257), (260, 130, 384)]),
-    (16, 1, 64, [(0, 3, 50)]), (6, 2, 32, [(1, 60, 45)]), (5, 1, 128, [(0, 100, 17), (20, 0, 1)]), (32, 8, 128, [(0, 1000, 100)]), (8, 1, 64, [(0, 2500, 31)]),
+    (4, 2, 128, [(2, 10, 40), (45, 0, 90)]), (8, 8, 128, [(0, 0, 700)]), (16, 1, 128, [(5, 900, 300)]), (8, 2, 128, [(0, 0, 257), (260, 130, 384)]),
+    (5, 1, 128, [(1, 77, 900)]), (16, 1, 64, [(0, 3, 50)]), (6, 2, 32, [(1, 60, 45)]), (5, 1, 128, [(0, 100, 17), (20, 0, 1)]), (32, 8, 128, [(0, 1000, 100)]), (8, 1, 64, [(0, 2500, 31)]),
 ])
 def test_attention_prefill(heads, kv, hs, segs):
     k = K()
@@ -363,3 +363,44 @@ def test_attention_prefill(heads, kv, hs, segs):
             k.kv8_attention_prefill(q.cuda(), M, heads, *where, meta, cache, workspace=w, y_out=y)
             _near(y[covered], ref[covered], PROMPT_REL + STEP[t])
             assert (y[~covered] == 7.0).all()                     # rows outside the segments are left alone
+
+
+@pytest.mark.parametrize("workspace", [False, True])
+def test_attention_prefill_of_unusual_lines(workspace):
+    """A line with a NaN is seen by the rows from its token on, and by no other; a segment of a sequence, a position or a page that is not there is NaN;
+    one without tokens gives zeros."""
+    k = K()
+    rng = np.random.default_rng(8)
+    heads, kv, hs = 16, 8, 128          # (more than 4096 rows times heads: the widened pages, where there is a workspace)
+    segs = [(0, 100, 60, 0), (60, 0, 40, 1), (100, 30, 20, 9), (120, 200, 30, 2), (150, -40, 20, 1), (170, 0, 33, 3), (203, 5, 50, 4)]      # begin, position, rows, sequence
+    M = 260
+    assert M * heads > 4096
+    bt, n_pages = _table(rng, [160, 40, 220, 33, 55])
+    bt = bt[:, :7]                                              # the fourth segment ends behind the table: 7 pages are 224 tokens
+    bt[3, 1] = n_pages                                          # a page that is not there
+    host = _cache(rng, n_pages, kv, hs)
+    host[2][bt[0, 4], 1, 2] = math.nan                          # token 130, keys of the second head
+    host[3][bt[1, 0], 0, 20] = math.nan                         # token 20, values of the first one
+    positions, slots, meta = [0] * M, [0] * M, [len(segs)]
+    for b, p0, n, s in segs:
+        positions[b:b + n], slots[b:b + n] = range(p0, p0 + n), [s] * n
+        meta += [b, b + n]
+    q = torch.from_numpy(rng.standard_normal((M, heads * hs)).astype(np.float32))
+    cache = k.Kv8Cache(*_dev(*host))
+    where = (_i32(positions), _i32(slots), torch.from_numpy(bt.copy()).cuda())
+    y = torch.full((M, heads * hs), 7.0, device="cuda")
+    k.kv8_attention_prefill(q.cuda(), M, heads, *where, _i32(meta), cache, workspace=k.kv8_prefill_workspace(n_pages, kv, hs, M, "cuda") if workspace else None, y_out=y)
+    y = y.cpu().view(M, heads, hs)
+    nan = torch.isnan(y)
+    assert nan[30:60, 2:4].all() and not nan[:60, :2].any() and not nan[:60, 4:].any() and not nan[:30].any()
+    assert nan[80:100, :2].all() and not nan[60:100, 2:].any() and not nan[60:80].any()
+    assert nan[100:150].all() and (y[150:170] == 0).all()
+    assert nan[202].all() and (y[253:] == 7.0).all()
+    for b, p0, n, s in (segs[0], segs[1], segs[6]):
+        kk, vv = _values(host[0], host[2], bt[s], p0 + n), _values(host[1], host[3], bt[s], p0 + n)
+        kk, vv = torch.nan_to_num(kk), torch.nan_to_num(vv)
+        for m in range(b, b + n):
+            ref = _attention(q[m].view(heads, hs), kk[:positions[m] + 1], vv[:positions[m] + 1])
+            for h in range(heads):
+                if not nan[m, h].any():
+                    _near(y[m, h], ref[h], PROMPT_REL)
