@@ -41,16 +41,21 @@ DL_DEVINL void kv8_store_y(const Kv8AttArgs& a, int m, int col, float y) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// Both products on mma.sync m16n8k32 with int8 operands: keys and values go in as they lie in the cache, nothing is widened, and sums are exact 32-bit
-// integers.  What is f32 is taken as digits of base 256 in rows of the MMA's A operand:
+// Decode rows: both products on mma.sync m16n8k32 with int8 operands: keys and values go in as they lie in the cache, nothing is widened, and sums are exact
+// 32-bit integers.  What is f32 is taken as digits of base 256 in rows of the MMA's A operand:
 //   a query   n = rint(q 8355000 / max|q|), three signed digits of a head in rows g, g + 8, g + 4 (24 bits of the head's largest value)
 //   a weight  n = rint(p s_v 2^(22 - e)), three unsigned digits; e: exponent of the largest p s_v that the row has met (held like a softmax maximum: what
-//             was summed is rescaled when it moves), s_v the value's scale.  So each weight is off by 2^-23 of the largest one at most
-// Four heads fill the 16 rows.  PROMPT: two digits (16 bits of a query, 15 of a weight), eight (row, head) pairs of one key/value head fill them; four warps
-// share a tile's pages.
+//             was summed is rescaled when it moves), s_v the value's scale.  So each weight is off by 2^-23 of the largest one at most, as a f32 sum is
+// Four heads fill the 16 rows.
 //
 // A warp takes a page (32 tokens) at a time through a private ring of cp.async stages, 16-byte pieces XOR-swizzled by the token so that both ldmatrix
 // forms are free of conflicts: no barrier between warps until the final merge.
+//
+// What bounds it: the cache's bytes for long contexts, a chain of latencies for short ones.  32 rows of 1500 to 3000 tokens (8 kv heads of 128, 152 MB) 31 us,
+// 4.9 TB/s (the same loads without the arithmetic 27); one row of 100003 tokens 40 us, 5.3 TB/s.  A page takes a warp 1240 clk from end to end (260 of them its 32 MMAs,
+// 190 the special-function unit's 24 conversions and exponentials) and an SM with three CTAs 110.  Integer sums that stay in the accumulators from page to page take
+// 3 % off that and put it back on in the end, where they are converted.  One CTA of eight warps per SM that walks an equal stretch of all
+// rows' pages evens out the SMs' loads (256 CTAs on 148 SMs: 1.5 to 1), but every change of row empties its pipeline: 45 us.
 // ------------------------------------------------------------------------------------------------
 #define KA_WARPS 4
 #define KA_MIN_SPLIT_PAGES 24        // contexts up to 768 tokens: no split
@@ -58,94 +63,175 @@ DL_DEVINL void kv8_store_y(const Kv8AttArgs& a, int m, int col, float y) {
 
 DL_DEVINL void ka_cp16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 DL_DEVINL void ka_ldm(uint32_t (&r)[4], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
 }
 // two 16 x 16 byte matrices, transposed: lane l gets rows 4 (l % 4) .. + 3 of columns l / 4 and l / 4 + 8 of the first, then of the second
 DL_DEVINL void ka_ldm_bytes(uint32_t (&r)[4], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+    asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
 }
-template <bool U8> DL_DEVINL void ka_mma(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
-    if (first) {
-        if (U8) asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
-        else asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
-    } else {
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};" : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
+DL_DEVINL void ka_mma_first(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+}
+DL_DEVINL void ka_mma(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};" : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+DL_DEVINL void ka_mma_u8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+}
+DL_DEVINL void ka_mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};" : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 DL_DEVINL float ka_exp2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 DL_DEVINL float ka_max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
-// shift of a token's 16-byte pieces: eight tokens in a row, and the eight that a phase of the byte-wise ldmatrix reads (two, then the two 8 further on, ...),
-// come to lie in eight different columns of 16 bytes
+// shift of a token's 16-byte pieces: tokens 2 j + {0, 1, 8, 9, 16, 17, 24, 25} (a column of scores for each lane) and {0 .. 3, 8 .. 11} + 4 i (a phase of the
+// byte-wise ldmatrix) come to lie in eight different columns of 16 bytes (heads of 32: in four)
 template <int HS> DL_DEVINL int ka_swizzle(int t) {
-    const int f = (t & 3) | ((((t >> 2) ^ (t >> 3)) & 1) << 2);
+    const int f = (t & 1) | (((t >> 3) & 1) << 1) | ((((t >> 4) ^ (t >> 1)) & 1) << 2);
     return HS == 128 ? f : HS == 64 ? f >> 1 : f >> 2;
 }
 
-struct Kv8Work {               // what the launch adds to the arguments
+// a page of one key/value head into a stage: codes of the keys, of the values (swizzled), scales of both
+template <int HS> struct KaStage {
+    static constexpr int CODES = KV8_PAGE * HS, BYTES = 2 * CODES + 2 * KV8_PAGE * 4;
+};
+template <int HS> DL_DEVINL void ka_load(const DlKv8Cache& c, size_t line, uint32_t dst, int lane) {
+    constexpr int CH = HS / 16, CODES = KaStage<HS>::CODES;
+    const int8_t* ks = c.k + line * HS + lane * 16;
+    const int8_t* vs = c.v + line * HS + lane * 16;
+#pragma unroll
+    for (int j = 0; j < CH; j++) {
+        const int idx = j * 32 + lane, t = idx / CH, p = idx % CH;
+        const uint32_t d = dst + t * HS + ((p ^ ka_swizzle<HS>(t)) << 4);
+        ka_cp16(d, ks + j * 512);
+        ka_cp16(d + CODES, vs + j * 512);
+    }
+    if (lane < 16) ka_cp16(dst + 2 * CODES + lane * 16, (lane < 8 ? c.k_scale : c.v_scale) + line + (lane & 7) * 4);
+}
+// the lane's share of a query: dimensions 16 k + 4 (lane % 4) .. + 3
+template <int HS> DL_DEVINL void ka_query(const float* q, bool vec, float (&x)[HS / 16][4]) {
+#pragma unroll
+    for (int k = 0; k < HS / 16; k++) {
+        if (vec) {
+            const float4 v = *reinterpret_cast<const float4*>(q + k * 16);
+            x[k][0] = v.x; x[k][1] = v.y; x[k][2] = v.z; x[k][3] = v.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[k][e] = q[k * 16 + e];
+        }
+    }
+}
+// ... as signed digits in the A fragments: THREE in rows g, g + 8 (lower) and g + 4 (the upper lanes' g), or two in rows g, g + 8.  Returns what an integer sum is
+// multiplied with, log2(e) / sqrt(HS) in it: sums are c[g] 256 + c[g + 8], of the upper lanes 2^-16 of that
+template <int HS, bool THREE> DL_DEVINL float ka_digits(const float (&x)[HS / 16][4], bool live, bool lower, uint32_t (&qf)[HS / 32][4]) {
+    unsigned top = 0;
+#pragma unroll
+    for (int k = 0; k < HS / 16; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(x[k][e]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // (queries below 2^-100: their scores are zeros)
+    const bool finite = top < 0x7f800000u, zero = !finite || __uint_as_float(top) < KV8_TINY || !live;
+    constexpr float MOST = THREE ? 8355000.f : 32600.f;
+    const float up = zero ? 0.f : MOST / __uint_as_float(top);
+#pragma unroll
+    for (int k = 0; k < HS / 16; k++) {
+        uint32_t n[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) n[e] = (uint32_t)(zero ? 0 : __float2int_rn(x[k][e] * up));
+        // signed digits: bytes of n + 0x80...80, each less 0x80
+#pragma unroll
+        for (int e = 0; e < 4; e++) n[e] = THREE ? (n[e] + 0x808080u) ^ 0x808080u : (n[e] + 0x8080u) ^ 0x8080u;
+        const uint32_t sel = !THREE ? 0x4051u : lower ? 0x5162u : 0x5140u;
+        const uint32_t u = __byte_perm(n[0], n[1], sel), v = __byte_perm(n[2], n[3], sel);
+        qf[k / 2][(k & 1) * 2] = __byte_perm(u, v, 0x5410);
+        qf[k / 2][(k & 1) * 2 + 1] = !THREE || lower ? __byte_perm(u, v, 0x7632) : 0u;
+    }
+    if (!finite && live) return __uint_as_float(0x7fffffffu);
+    return zero ? 0.f : __uint_as_float(top) / MOST * (rsqrtf((float)HS) * 1.44269504088896341f) * (!THREE ? 1.f : lower ? 256.f : 1.f / 256.f);
+}
+// integer scores of a page.  Column n of score tile j is token 8 (n / 2) + 2 j + n % 2, so that a lane has the eight tokens 8 (lane % 4) .. + 7
+template <int HS, int MT> DL_DEVINL void ka_scores(uint32_t kb, int lane, const uint32_t (&qf)[MT][HS / 32][4], int (&c)[MT][4][4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+        const int t = (((lane & 7) >> 1) << 3) + ((lane >> 4) << 1) + (lane & 1) + j * 2, piece = (lane >> 3) & 1;
+        const uint32_t base = kb + t * HS, sw = ka_swizzle<HS>(t);
+#pragma unroll
+        for (int k = 0; k < HS / 32; k++) {
+            uint32_t b[4];
+            ka_ldm(b, base + (((2 * k + piece) ^ sw) << 4));
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                if (k == 0) {
+                    ka_mma_first(c[mt][j], qf[mt][k], b[0], b[1]);
+                    ka_mma_first(c[mt][j + 1], qf[mt][k], b[2], b[3]);
+                } else {
+                    ka_mma(c[mt][j], qf[mt][k], b[0], b[1]);
+                    ka_mma(c[mt][j + 1], qf[mt][k], b[2], b[3]);
+                }
+            }
+        }
+    }
+}
+// the lane's row of the values' ldmatrix: k index 4 a + i of a product is token 8 a + i, k index 16 + 4 a + i token 8 a + 4 + i
+DL_DEVINL int ka_value_row(int lane) { return (((lane & 15) >> 2) << 3) + (lane & 3) + ((lane >> 4) << 2); }
+// scales of the lane's eight tokens
+DL_DEVINL void ka_scales(const float* at, float (&s)[8]) {
+    const float4 x = *reinterpret_cast<const float4*>(at), y = *reinterpret_cast<const float4*>(at + 4);
+    s[0] = x.x; s[1] = x.y; s[2] = x.z; s[3] = x.w; s[4] = y.x; s[5] = y.y; s[6] = y.z; s[7] = y.w;
+}
+// four warps' sums of a stacked row and dimension: the largest reference, the sum of weights, the weighted sum (references in units of log2)
+template <int HS, int SR> DL_DEVINL void ka_merge(const float* w_acc, const float* w_ml, int s, int d, float& Mx, float& L, float& O) {
+    Mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < KA_WARPS; w++) Mx = fmaxf(Mx, w_ml[(w * SR + s) * 2]);
+    const float Mu = Mx == -INFINITY ? 0.f : Mx;
+    L = O = 0.f;
+#pragma unroll
+    for (int w = 0; w < KA_WARPS; w++) {
+        const float e = ka_exp2(w_ml[(w * SR + s) * 2] - Mu);
+        L += w_ml[(w * SR + s) * 2 + 1] * e;
+        O += w_acc[(w * SR + s) * HS + d] * e;
+    }
+}
+
+struct Kv8Work {               // what the launch adds to the arguments of decode rows
     int n_splits, groups;      // groups: CTAs that share a key/value head's query heads
-    unsigned* counters;
+    unsigned* counters;        // [M][kv heads * groups]
     float* part_o;             // [M][heads][n_splits][HS]
     float* part_ml;            // [M][heads][n_splits][2]
 };
 
-template <int HS, int MT, bool PROMPT, int ST>
+// grid (kv heads * groups, M, splits): the splits that short rows do not take come last, when the others have their SMs
+template <int HS, int MT, int ST>
 __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __grid_constant__ Kv8AttArgs a, const __grid_constant__ Kv8Work wk) {
-    constexpr int CH = HS / 16, KS = HS / 32, NT = HS / 8;
-    constexpr int CODES = KV8_PAGE * HS, STAGE = 2 * CODES + 2 * KV8_PAGE * 4;
-    constexpr int SPT = PROMPT ? 8 : 4, SR = MT * SPT;                     // stacked rows of an MMA, of the CTA
-    constexpr int TOP = PROMPT ? 14 : 22;                                  // a weight's integer is below 2^(TOP + 1)
+    constexpr int CH = HS / 16, KS = HS / 32, NT = HS / 8, STAGE = KaStage<HS>::BYTES, CODES = KaStage<HS>::CODES;
+    constexpr int SR = MT * 4;                                             // heads of the CTA
+    constexpr int TOP = 22;                                                // a weight's integer is at most 2^(TOP + 1)
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, qd = lane & 3;
-    const int kvh = blockIdx.y / wk.groups;
-    const int G = a.heads / a.c.n_kv_heads;
+    const int kvh = blockIdx.x / wk.groups, m0 = blockIdx.y, sp = blockIdx.z;
+    const int G = a.heads / a.c.n_kv_heads, per = (G + wk.groups - 1) / wk.groups, h_lo = (blockIdx.x % wk.groups) * per, n_live = min(per, G - h_lo);
+    const bool lower = g < 4;
     pdl_launch_dependents();
     pdl_wait();
-
-    // which rows and heads: m0 the first row, p0 its position; stacked row s is head h_lo + s (decode), or pair s_lo + s = row * G + head of the group
-    int m0, slot, T, h_lo = 0, s_lo = 0, n_live, sp = 0, n_eff = 1, p0 = 0;
-    bool bad;
-    if constexpr (PROMPT) {
-        int tile = gridDim.x - 1 - blockIdx.x, begin = 0, end = 0, i = 0;  // late tiles (long histories) first
-        const int n_seg = min(a.meta[0], 8);
-        for (; i < n_seg; i++) {
-            begin = a.meta[1 + 2 * i];
-            end = a.meta[2 + 2 * i];
-            if (begin < 0 || end > a.rows.M || end <= begin) continue;
-            const int nt = ((end - begin) * G + SR - 1) / SR;
-            if (tile < nt) break;
-            tile -= nt;
-        }
-        if (i >= n_seg) return;
-        m0 = begin;
-        s_lo = tile * SR;
-        n_live = min(SR, (end - begin) * G - s_lo);
-        p0 = a.rows.pos[begin];
-        slot = a.rows.slot[begin];
-        bad = p0 >= 0 && (p0 > 0x7fffffff - (end - begin) || kv8_tokens(a.rows, p0 + (end - begin) - 1, slot) < 0);
-        T = bad || p0 < 0 ? 0 : p0 + (s_lo + n_live - 1) / G + 1;
-    } else {
-        m0 = blockIdx.z;
-        if (a.row_skip != nullptr && a.row_skip[m0] != 0) return;
-        sp = blockIdx.x;
-        slot = a.rows.slot[m0];
-        T = kv8_tokens(a.rows, a.rows.pos[m0], slot);
-        bad = T < 0;
-        T = max(T, 0);
-        const int per = (G + wk.groups - 1) / wk.groups;
-        h_lo = (blockIdx.y % wk.groups) * per;
-        n_live = min(per, G - h_lo);
+    if (a.row_skip != nullptr && a.row_skip[m0] != 0) return;
+    const int pos = a.rows.pos[m0], slot = a.rows.slot[m0];
+    float x[MT][2 * KS][4];                                                // (asked for ahead of what hangs on pos)
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        const int h = mt * 4 + (g & 3);
+        ka_query<HS>(a.q + (size_t)m0 * a.ldq + (kvh * G + h_lo + (h < n_live ? h : 0)) * HS + qd * 4, ((uintptr_t)a.q & 15) == 0 && (a.ldq & 3) == 0, x[mt]);
     }
+    const int T0 = kv8_tokens(a.rows, pos, slot), T = max(T0, 0);
+    bool bad = T0 < 0;
     const int n_pages = (T + KV8_PAGE - 1) / KV8_PAGE;
-    if (!PROMPT) {
-        n_eff = n_pages <= KA_MIN_SPLIT_PAGES ? 1 : min(wk.n_splits, (n_pages + 7) / 8);
-        if (sp >= n_eff) return;
-    }
+    const int n_eff = n_pages <= KA_MIN_SPLIT_PAGES ? 1 : min(wk.n_splits, (n_pages + 7) / 8);
+    if (sp >= n_eff) return;
     const int pps = (n_pages + n_eff - 1) / n_eff, pg0 = sp * pps, pg1 = min(n_pages, pg0 + pps);
     const int n_my = max(0, (pg1 - pg0 - warp + KA_WARPS - 1) / KA_WARPS);             // this warp's pages: pg0 + warp + 4 i
     const int* bt = a.rows.block_table + (size_t)(bad ? 0 : slot) * a.rows.max_pages;
-    auto row_of = [&](int s) { return PROMPT ? m0 + (s_lo + s) / G : m0; };
-    auto head_of = [&](int s) { return kvh * G + (PROMPT ? (s_lo + s) % G : h_lo + s); };
 
     const uint32_t ring = smem_u32(smem) + warp * (ST * STAGE);
     auto page_at = [&](int i) {
@@ -154,20 +240,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
         return p;
     };
     int my_page = page_at(lane);                               // the lanes hold the next 32 page numbers
-    auto load = [&](int st, int page) {
-        const size_t line = ((size_t)page * a.c.n_kv_heads + kvh) * KV8_PAGE;
-        const uint32_t dst = ring + st * STAGE;
-        const int8_t* ks = a.c.k + line * HS + lane * 16;
-        const int8_t* vs = a.c.v + line * HS + lane * 16;
-#pragma unroll
-        for (int j = 0; j < CH; j++) {
-            const int idx = j * 32 + lane, t = idx / CH, c = idx % CH;
-            const uint32_t d = dst + t * HS + ((c ^ ka_swizzle<HS>(t)) << 4);
-            ka_cp16(d, ks + j * 512);
-            ka_cp16(d + CODES, vs + j * 512);
-        }
-        if (lane < 16) ka_cp16(dst + 2 * CODES + lane * 16, (lane < 8 ? a.c.k_scale : a.c.v_scale) + line + (lane & 7) * 4);
-    };
+    auto load = [&](int st, int page) { ka_load<HS>(a.c, ((size_t)page * a.c.n_kv_heads + kvh) * KV8_PAGE, ring + st * STAGE, lane); };
 #pragma unroll
     for (int i = 0; i < ST - 1; i++) {
         const int page = __shfl_sync(0xffffffffu, my_page, i);
@@ -175,72 +248,21 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
 
-    // queries: digits in the A fragments; fl: what an integer sum is multiplied with, log2(e) / sqrt(HS) in it
-    const bool lower = PROMPT || g < 4;
     uint32_t qf[MT][KS][4];
     float fl[MT];
-    int lim[MT];                                               // tokens that the lane's stacked row sees
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        const int s = mt * SPT + (PROMPT ? g : g & 3);
-        const bool live = s < n_live;
-        lim[mt] = !live ? 0 : PROMPT ? max(0, min(T, p0 + (s_lo + s) / G + 1)) : T;
-        const float* q = a.q + (size_t)row_of(live ? s : 0) * a.ldq + head_of(live ? s : 0) * HS + qd * 4;
-        float x[2 * KS][4];
-        unsigned top = 0;
-        const bool vec = ((uintptr_t)a.q & 15) == 0 && (a.ldq & 3) == 0;
-#pragma unroll
-        for (int k = 0; k < 2 * KS; k++) {
-            if (vec) {
-                const float4 v = *reinterpret_cast<const float4*>(q + k * 16);
-                x[k][0] = v.x; x[k][1] = v.y; x[k][2] = v.z; x[k][3] = v.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[k][e] = q[k * 16 + e];
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(x[k][e]) & 0x7fffffffu);
-        }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // (queries below 2^-100: their scores are zeros)
-        const bool finite = top < 0x7f800000u, zero = !finite || __uint_as_float(top) < KV8_TINY || !live;
-        constexpr float MOST = PROMPT ? 32600.f : 8355000.f;
-        const float up = zero ? 0.f : MOST / __uint_as_float(top);
-        fl[mt] = !finite && live ? __uint_as_float(0x7fffffffu) : zero ? 0.f : __uint_as_float(top) / MOST * (rsqrtf((float)HS) * 1.44269504088896341f) * (PROMPT ? 1.f : lower ? 256.f : 1.f / 256.f);
-#pragma unroll
-        for (int k = 0; k < 2 * KS; k++) {
-            uint32_t n[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) n[e] = (uint32_t)(zero ? 0 : __float2int_rn(x[k][e] * up));
-            // signed digits: bytes of n + 0x80...80, each less 0x80
-#pragma unroll
-            for (int e = 0; e < 4; e++) n[e] = PROMPT ? (n[e] + 0x8080u) ^ 0x8080u : (n[e] + 0x808080u) ^ 0x808080u;
-            const uint32_t sel = PROMPT ? 0x4051u : lower ? 0x5162u : 0x5140u;
-            const uint32_t u = __byte_perm(n[0], n[1], sel), v = __byte_perm(n[2], n[3], sel);
-            qf[mt][k / 2][(k & 1) * 2] = __byte_perm(u, v, 0x5410);
-            qf[mt][k / 2][(k & 1) * 2 + 1] = lower ? __byte_perm(u, v, 0x7632) : 0u;
-        }
-    }
-
     float o[MT][NT][2];
     float run_m[MT], run_l[MT], run_w[MT];                     // maximum of scores, sum of weights (this lane's tokens), largest weight * scale
     int ex[MT];                                                // exponent field of run_w: the unit of o
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
+        fl[mt] = ka_digits<HS, true>(x[mt], mt * 4 + (g & 3) < n_live, lower, qf[mt]);
         run_m[mt] = -INFINITY;
         run_l[mt] = run_w[mt] = 0.f;
         ex[mt] = 24;
 #pragma unroll
         for (int n = 0; n < NT; n++) o[mt][n][0] = o[mt][n][1] = 0.f;
     }
-    int all = T;                                               // tokens that every live row of the CTA sees
-    if (PROMPT) all = min(T, p0 + s_lo / G + 1);
-
-    // lane's rows of the two ldmatrix forms: tokens and the pieces that they start from
-    const int kt = ((lane >> 4) << 3) + (lane & 7), kc = (lane >> 3) & 1;                                   // + 16 j / 2: n-tiles j, j + 1
-    const int vr = lane & 15, vt = ((lane >> 4) << 4) + ((vr & 2) << 2) + ((vr >> 2) << 1) + (vr & 1);      // k index 4 a + i is token 8 (i / 2) + 2 a + i % 2
-    const uint32_t v_at = vt * HS, v_sw = ka_swizzle<HS>(vt);
+    const uint32_t v_at = ka_value_row(lane) * HS, v_sw = ka_swizzle<HS>(ka_value_row(lane));
 
     int st = 0;
     for (int i = 0; i < n_my; i++) {
@@ -254,31 +276,16 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
         asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
         __syncwarp();
         const uint32_t kb = ring + st * STAGE, vb = kb + CODES;
-        const float* scales = reinterpret_cast<const float*>(smem + (size_t)warp * ST * STAGE + st * STAGE + 2 * CODES);
-        const int tok0 = (pg0 + warp + KA_WARPS * i) * KV8_PAGE;
+        const float* scales = reinterpret_cast<const float*>(smem + (size_t)(warp * ST + st) * STAGE + 2 * CODES) + qd * 8;
+        const int left = T - (pg0 + warp + KA_WARPS * i) * KV8_PAGE;
+        float sk[8], sv[8];
+        ka_scales(scales, sk);
+        ka_scales(scales + KV8_PAGE, sv);
         int c[MT][4][4];
+        ka_scores<HS, MT>(kb, lane, qf, c);
+        uint32_t vf[CH][4];                                    // (asked for ahead of the weights)
 #pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-            const int t = kt + j * 8;
-            const uint32_t base = kb + t * HS, sw = ka_swizzle<HS>(t);
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
-                uint32_t b[4];
-                ka_ldm(b, base + (((2 * k + kc) ^ sw) << 4));
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    ka_mma<false>(c[mt][j], qf[mt][k], b[0], b[1], k == 0);
-                    ka_mma<false>(c[mt][j + 1], qf[mt][k], b[2], b[3], k == 0);
-                }
-            }
-        }
-        float2 sk[4], sv[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            sk[j] = *reinterpret_cast<const float2*>(scales + j * 8 + qd * 2);
-            sv[j] = *reinterpret_cast<const float2*>(scales + KV8_PAGE + j * 8 + qd * 2);
-        }
-        const bool part = tok0 + KV8_PAGE > all;
+        for (int ch = 0; ch < CH; ch++) ka_ldm_bytes(vf[ch], vb + v_at + ((ch ^ v_sw) << 4));
         uint32_t pa[MT][4];
         float f[MT];
 #pragma unroll
@@ -286,16 +293,15 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
             float s[8], w[8], mx = -INFINITY;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const int j = e >> 1;
-                s[e] = (float)(c[mt][j][e & 1] * 256 + c[mt][j][(e & 1) + 2]) * fl[mt];
-                if (!PROMPT) s[e] += __shfl_xor_sync(0xffffffffu, s[e], 16);
-                s[e] *= (e & 1) ? sk[j].y : sk[j].x;
-                w[e] = (e & 1) ? sv[j].y : sv[j].x;
+                s[e] = (float)(c[mt][e >> 1][e & 1] * 256 + c[mt][e >> 1][(e & 1) + 2]) * fl[mt];
+                s[e] += __shfl_xor_sync(0xffffffffu, s[e], 16);
+                s[e] *= sk[e];
+                w[e] = sv[e];
             }
-            if (part) {
+            if (left < KV8_PAGE) {
 #pragma unroll
                 for (int e = 0; e < 8; e++)
-                    if (tok0 + (e >> 1) * 8 + qd * 2 + (e & 1) >= lim[mt]) { s[e] = -INFINITY; w[e] = 0.f; }
+                    if (qd * 8 + e >= left) { s[e] = -INFINITY; w[e] = 0.f; }
             }
 #pragma unroll
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, s[e]);
@@ -325,27 +331,25 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
             uint32_t n[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) n[e] = __float_as_uint(fmaf(w[e], up, 8388608.f));     // the integer in the low 23 bits (and 2^23 itself as its top byte)
-            const uint32_t sel = PROMPT ? 0x4051u : lower ? 0x5162u : 0x5140u;
+            const uint32_t sel = lower ? 0x5162u : 0x5140u;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const uint32_t x = __byte_perm(n[4 * u], n[4 * u + 1], sel), y = __byte_perm(n[4 * u + 2], n[4 * u + 3], sel);
-                pa[mt][2 * u] = __byte_perm(x, y, 0x5410);
-                pa[mt][2 * u + 1] = lower ? __byte_perm(x, y, 0x7632) : 0u;
+                const uint32_t y = __byte_perm(n[4 * u], n[4 * u + 1], sel), z = __byte_perm(n[4 * u + 2], n[4 * u + 3], sel);
+                pa[mt][2 * u] = __byte_perm(y, z, 0x5410);
+                pa[mt][2 * u + 1] = lower ? __byte_perm(y, z, 0x7632) : 0u;
             }
         }
 #pragma unroll
         for (int ch = 0; ch < CH; ch++) {
-            uint32_t b[4];
-            ka_ldm_bytes(b, vb + v_at + ((ch ^ v_sw) << 4));
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) {
-                int x[4], y[4];
-                ka_mma<true>(x, pa[mt], b[0], b[2], true);
-                ka_mma<true>(y, pa[mt], b[1], b[3], true);
+                int y[4], z[4];
+                ka_mma_u8(y, pa[mt], vf[ch][0], vf[ch][2]);
+                ka_mma_u8(z, pa[mt], vf[ch][1], vf[ch][3]);
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    o[mt][2 * ch][e] = fmaf(o[mt][2 * ch][e], f[mt], (float)(x[e] * 256 + x[e + 2]));
-                    o[mt][2 * ch + 1][e] = fmaf(o[mt][2 * ch + 1][e], f[mt], (float)(y[e] * 256 + y[e + 2]));
+                    o[mt][2 * ch][e] = fmaf(o[mt][2 * ch][e], f[mt], (float)(y[e] * 256 + y[e + 2]));
+                    o[mt][2 * ch + 1][e] = fmaf(o[mt][2 * ch + 1][e], f[mt], (float)(z[e] * 256 + z[e + 2]));
                 }
             }
         }
@@ -363,98 +367,318 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
         run_l[mt] += __shfl_xor_sync(0xffffffffu, run_l[mt], 1);
         run_l[mt] += __shfl_xor_sync(0xffffffffu, run_l[mt], 2);
         if (bad) run_l[mt] = __uint_as_float(0x7fffffffu);
-        const float unit = __uint_as_float((uint32_t)(ex[mt] - TOP) << 23) * (PROMPT ? 1.f : lower ? 256.f : 1.f / 256.f);
-        const int s = mt * SPT + (PROMPT ? g : g & 3);
-        float* w = w_acc + (warp * SR + s) * HS + qd * 2;
+        const float unit = __uint_as_float((uint32_t)(ex[mt] - TOP) << 23) * (lower ? 256.f : 1.f / 256.f);
+        const int s = warp * SR + mt * 4 + (g & 3);
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             float v[2];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 v[e] = o[mt][n][e] * unit;
-                if (!PROMPT) v[e] += __shfl_xor_sync(0xffffffffu, v[e], 16);
+                v[e] += __shfl_xor_sync(0xffffffffu, v[e], 16);
             }
-            if (lower) *reinterpret_cast<float2*>(w + n * 8) = make_float2(v[0], v[1]);
+            if (lower) *reinterpret_cast<float2*>(w_acc + s * HS + qd * 2 + n * 8) = make_float2(v[0], v[1]);
         }
-        if (lower && qd == 0) { w_ml[(warp * SR + s) * 2] = run_m[mt]; w_ml[(warp * SR + s) * 2 + 1] = run_l[mt]; }
+        if (lower && qd == 0) { w_ml[s * 2] = run_m[mt]; w_ml[s * 2 + 1] = run_l[mt]; }
     }
     __syncthreads();
-
-    // the four warps' shares: a warp takes 32 dimensions of a stacked row at a time (maxima are in units of log2)
     const bool single = n_eff == 1;
-    for (int idx = tid; idx < n_live * HS; idx += KA_WARPS * 32) {
-        const int s = idx / HS, d = idx % HS;
-        float Mx = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < KA_WARPS; w++) Mx = fmaxf(Mx, w_ml[(w * SR + s) * 2]);
-        const float Mu = Mx == -INFINITY ? 0.f : Mx;
-        float L = 0.f, O = 0.f;
-#pragma unroll
-        for (int w = 0; w < KA_WARPS; w++) {
-            const float e = ka_exp2(w_ml[(w * SR + s) * 2] - Mu);
-            L += w_ml[(w * SR + s) * 2 + 1] * e;
-            O += w_acc[(w * SR + s) * HS + d] * e;
-        }
-        const int m = row_of(s), hd = head_of(s);
+    for (int idx = tid; idx < n_live * HS; idx += KA_WARPS * 32) {         // a warp takes 32 dimensions of a head at a time
+        const int s = idx / HS, d = idx % HS, hd = kvh * G + h_lo + s;
+        float Mx, L, O;
+        ka_merge<HS, SR>(w_acc, w_ml, s, d, Mx, L, O);
         if (single) {
             const float y = L == 0.f ? 0.f : O / L;
-            kv8_store_y(a, m, hd * HS + d, y);
-            if (a.xq_out != nullptr || a.xh_out != nullptr) q80_block_store(y, lane, m, (hd * HS + d) >> 5, a.out_mcap, a.xq_out, a.xh_out);
+            kv8_store_y(a, m0, hd * HS + d, y);
+            if (a.xq_out != nullptr || a.xh_out != nullptr) q80_block_store(y, lane, m0, (hd * HS + d) >> 5, a.out_mcap, a.xq_out, a.xh_out);
         } else {
-            const size_t pidx = ((size_t)m * a.heads + hd) * wk.n_splits + sp;
+            const size_t pidx = ((size_t)m0 * a.heads + hd) * wk.n_splits + sp;
             wk.part_o[pidx * HS + d] = O;
             if (d == 0) { wk.part_ml[pidx * 2] = Mx; wk.part_ml[pidx * 2 + 1] = L; }
         }
     }
-    if (PROMPT || single) return;
-    __threadfence();
+    if (single) return;
     __syncthreads();
-    if (tid == 0) {
-        unsigned* counter = &wk.counters[m0 * gridDim.y + blockIdx.y];
-        const unsigned prev = atomicAdd(counter, 1u);
+    if (tid == 0) {                                            // the CTA's sums, ahead of the barrier, are released with its count
+        unsigned* counter = &wk.counters[m0 * gridDim.x + blockIdx.x];
+        unsigned prev;
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(prev) : "l"(counter) : "memory");
         *s_last = prev == (unsigned)n_eff - 1u ? 1 : 0;
         if (*s_last) *counter = 0u;
     }
     __syncthreads();
     if (!*s_last) return;
-    __threadfence();
-    // a warp merges a head: lane s holds split s's (max, sum), every lane sums its dims over the splits in their order
+    // a warp merges a head: the lanes hold the splits' (max, sum); then HS / 4 lanes take a split's sums, 32 / (HS / 4) splits side by side, eight of each in flight
+    constexpr int LPH = HS / 4, ZP = 32 / LPH;
+    float* y_s = w_acc + warp * HS;                            // (the four warps' sums are done with)
     for (int s = warp; s < n_live; s += KA_WARPS) {
-        constexpr int DPL = HS / 32;
-        const int hd = head_of(s);
+        const int hd = kvh * G + h_lo + s;
         const size_t base = ((size_t)m0 * a.heads + hd) * wk.n_splits;
-        float ms = -INFINITY, ls = 0.f;
-        if (lane < n_eff) { ms = __ldcg(&wk.part_ml[(base + lane) * 2]); ls = __ldcg(&wk.part_ml[(base + lane) * 2 + 1]); }
-        const float Mx = warp_max(ms), Mu = Mx == -INFINITY ? 0.f : Mx;
-        const float e = lane < n_eff ? ka_exp2(ms - Mu) : 0.f;
-        const float L = warp_sum(ls * e);
-        float O[DPL];
+        float mz[2], lz[2];
 #pragma unroll
-        for (int d = 0; d < DPL; d++) O[d] = 0.f;
-#pragma unroll 4
-        for (int z = 0; z < n_eff; z++) {
-            const float ez = __shfl_sync(0xffffffffu, e, z);
+        for (int u = 0; u < 2; u++) {
+            const int z = u * 32 + lane;
+            mz[u] = z < n_eff ? __ldcg(&wk.part_ml[(base + z) * 2]) : -INFINITY;
+            lz[u] = z < n_eff ? __ldcg(&wk.part_ml[(base + z) * 2 + 1]) : 0.f;
+        }
+        const float Mx = warp_max(fmaxf(mz[0], mz[1])), Mu = Mx == -INFINITY ? 0.f : Mx;
 #pragma unroll
-            for (int d = 0; d < DPL; d++) O[d] += __ldcg(&wk.part_o[(base + z) * HS + d * 32 + lane]) * ez;
+        for (int u = 0; u < 2; u++) mz[u] = ka_exp2(mz[u] - Mu);
+        const float L = warp_sum(fmaf(lz[0], mz[0], lz[1] * mz[1]));
+        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float* src = wk.part_o + base * HS + lane % LPH * 4;
+        for (int z0 = 0; z0 < n_eff; z0 += 8 * ZP) {
+            float4 x[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int z = z0 + u * ZP + lane / LPH;
+                x[u] = z < n_eff ? __ldcg(reinterpret_cast<const float4*>(src + (size_t)z * HS)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int z = z0 + u * ZP + lane / LPH;
+                const float e0 = __shfl_sync(0xffffffffu, mz[0], z & 31), e1 = __shfl_sync(0xffffffffu, mz[1], z & 31), e = z < 32 ? e0 : e1;
+                O.x = fmaf(x[u].x, e, O.x); O.y = fmaf(x[u].y, e, O.y); O.z = fmaf(x[u].z, e, O.z); O.w = fmaf(x[u].w, e, O.w);
+            }
         }
 #pragma unroll
-        for (int d = 0; d < DPL; d++) {                        // 32 dims at a time: one Q80 block
-            const float y = L == 0.f ? 0.f : O[d] / L;
+        for (int w = LPH; w < 32; w <<= 1) {
+            O.x += __shfl_xor_sync(0xffffffffu, O.x, w); O.y += __shfl_xor_sync(0xffffffffu, O.y, w);
+            O.z += __shfl_xor_sync(0xffffffffu, O.z, w); O.w += __shfl_xor_sync(0xffffffffu, O.w, w);
+        }
+        __syncwarp();
+        if (lane < LPH) *reinterpret_cast<float4*>(y_s + lane * 4) = O;
+        __syncwarp();
+#pragma unroll
+        for (int d = 0; d < HS / 32; d++) {                    // 32 dims at a time: one Q80 block
+            const float y = L == 0.f ? 0.f : y_s[d * 32 + lane] / L;
             kv8_store_y(a, m0, hd * HS + d * 32 + lane, y);
-            if (a.xq_out != nullptr || a.xh_out != nullptr) q80_block_store(y, lane, m0, hd * DPL + d, a.out_mcap, a.xq_out, a.xh_out);
+            if (a.xq_out != nullptr || a.xh_out != nullptr) q80_block_store(y, lane, m0, hd * (HS / 32) + d, a.out_mcap, a.xq_out, a.xh_out);
         }
     }
 }
 
-template <int HS, int MT, bool PROMPT, int ST>
-static int ka_launch(const char* who, const Kv8AttArgs& a, const Kv8Work& wk, dim3 grid, int pdl, void* stream) {
-    constexpr int SR = MT * (PROMPT ? 8 : 4), STAGE = 2 * KV8_PAGE * HS + 2 * KV8_PAGE * 4;
-    constexpr int ring = KA_WARPS * ST * STAGE, merge = KA_WARPS * SR * (HS + 2) * 4 + 16, smem = ring > merge ? ring : merge;
-    static SmemLimit given;
-    if (const int rc = dl_smem_limit(who, kv8_attention_kernel<HS, MT, PROMPT, ST>, smem, given)) return rc;
+// ------------------------------------------------------------------------------------------------
+// Prompt chunks: eight (row, head) pairs of one key/value head, of two digits a query (16 bits), fill an int8 MMA, two of them make the 16 rows of a tile, whose
+// pages four warps share.  Two digits of a weight would not do: what is below 2^-16 of the largest weight is lost, however many tokens there are.  So
+// weights are fp16 here (2^-12 of themselves), values are widened in registers -- codes are exact in fp16 -- and sums are the f32 accumulators of m16n8k16.
+// p = 2^(s - ref) goes by a reference that moves only when a score is more than 2^8 above it, or a weight outgrows fp16: a vote of the warp, so that a page in the
+// steady state takes no exchange for a running maximum and no rescaling.
+// ------------------------------------------------------------------------------------------------
+template <int HS, int ST>
+__global__ void __launch_bounds__(KA_WARPS * 32) kv8_prompt_kernel(const __grid_constant__ Kv8AttArgs a) {
+    constexpr int CH = HS / 16, KS = HS / 32, NT = HS / 8, STAGE = KaStage<HS>::BYTES, CODES = KaStage<HS>::CODES;
+    constexpr int SR = 16;                                                 // stacked rows of the CTA
+    constexpr int TOP = 6;                                                 // the largest weight is below 2^(TOP + 1) units when the unit is chosen,
+    constexpr float MOST_W = 0x1p15f, AHEAD = 8.f;                         // and below this always; scores may pass the reference by so much (log2)
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, qd = lane & 3;
+    const int kvh = blockIdx.y, G = a.heads / a.c.n_kv_heads;
+    pdl_launch_dependents();
+    pdl_wait();
+    // stacked row s of the tile is pair s_lo + s = row * G + head of the group, row 0 (batch row m0) at position p0
+    int tile = gridDim.x - 1 - blockIdx.x, m0 = 0, end = 0, i0 = 0;        // late tiles (long histories) first
+    const int n_seg = min(a.meta[0], 8);
+    for (; i0 < n_seg; i0++) {
+        m0 = a.meta[1 + 2 * i0];
+        end = a.meta[2 + 2 * i0];
+        if (m0 < 0 || end > a.rows.M || end <= m0) continue;
+        const int nt = ((end - m0) * G + SR - 1) / SR;
+        if (tile < nt) break;
+        tile -= nt;
+    }
+    if (i0 >= n_seg) return;
+    const int s_lo = tile * SR, n_live = min(SR, (end - m0) * G - s_lo), p0 = a.rows.pos[m0], slot = a.rows.slot[m0];
+    auto row_of = [&](int s) { return m0 + (s_lo + s) / G; };
+    auto head_of = [&](int s) { return kvh * G + (s_lo + s) % G; };
+    float x[2][2 * KS][4];
+#pragma unroll
+    for (int mt = 0; mt < 2; mt++) {
+        const int s = mt * 8 + g < n_live ? mt * 8 + g : 0;
+        ka_query<HS>(a.q + (size_t)row_of(s) * a.ldq + head_of(s) * HS + qd * 4, ((uintptr_t)a.q & 15) == 0 && (a.ldq & 3) == 0, x[mt]);
+    }
+    bool bad = p0 >= 0 && (p0 > 0x7fffffff - (end - m0) || kv8_tokens(a.rows, p0 + (end - m0) - 1, slot) < 0);
+    const int T = bad || p0 < 0 ? 0 : p0 + (s_lo + n_live - 1) / G + 1, all = min(T, p0 + s_lo / G + 1);       // tokens that the last, that every row of the tile sees
+    const int n_pages = (T + KV8_PAGE - 1) / KV8_PAGE, n_my = max(0, (n_pages - warp + KA_WARPS - 1) / KA_WARPS);       // this warp's pages: warp + 4 i
+    const int* bt = a.rows.block_table + (size_t)(bad ? 0 : slot) * a.rows.max_pages;
+
+    const uint32_t ring = smem_u32(smem) + warp * (ST * STAGE);
+    auto page_at = [&](int i) {
+        int p = i < n_my ? bt[warp + KA_WARPS * i] : 0;
+        if ((unsigned)p >= (unsigned)a.rows.n_pages) { bad = true; p = 0; }
+        return p;
+    };
+    int my_page = page_at(lane);                               // the lanes hold the next 32 page numbers
+    auto load = [&](int st, int page) { ka_load<HS>(a.c, ((size_t)page * a.c.n_kv_heads + kvh) * KV8_PAGE, ring + st * STAGE, lane); };
+#pragma unroll
+    for (int i = 0; i < ST - 1; i++) {
+        const int page = __shfl_sync(0xffffffffu, my_page, i);
+        if (i < n_my) load(i, page);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    uint32_t qf[2][KS][4];
+    float fl[2], ref[2], run_l[2], up[2];                      // reference of the weights, their sum (this lane's tokens), their unit's inverse
+    int lim[2];                                                // tokens that the lane's rows see
+#pragma unroll
+    for (int mt = 0; mt < 2; mt++) {
+        const int s = mt * 8 + g;
+        fl[mt] = ka_digits<HS, false>(x[mt], s < n_live, true, qf[mt]);
+        lim[mt] = s < n_live ? min(T, p0 + (s_lo + s) / G + 1) : 0;
+        ref[mt] = -INFINITY;
+        run_l[mt] = 0.f;
+        up[mt] = 0x1p125f;
+    }
+    float o[NT][4];                                            // rows g (0, 1) and g + 8 (2, 3)
+#pragma unroll
+    for (int n = 0; n < NT; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    auto rescale = [&](float c0, float c1) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) { o[n][0] *= c0; o[n][1] *= c0; o[n][2] *= c1; o[n][3] *= c1; }
+    };
+    const uint32_t v_at = ka_value_row(lane) * HS, v_sw = ka_swizzle<HS>(ka_value_row(lane));
+
+    int st = 0;
+    for (int i = 0; i < n_my; i++) {
+        {
+            const int nx = i + ST - 1;
+            if ((nx & 31) == 0) my_page = page_at(nx + lane);
+            const int page = __shfl_sync(0xffffffffu, my_page, nx & 31);
+            if (nx < n_my) load(st == 0 ? ST - 1 : st - 1, page);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+        __syncwarp();
+        const uint32_t kb = ring + st * STAGE, vb = kb + CODES;
+        const float* scales = reinterpret_cast<const float*>(smem + (size_t)(warp * ST + st) * STAGE + 2 * CODES) + qd * 8;
+        const int tok0 = (warp + KA_WARPS * i) * KV8_PAGE;
+        float sk[8], sv[8], s[2][8], w[2][8], top[2];
+        ka_scales(scales, sk);
+        ka_scales(scales + KV8_PAGE, sv);
+        int c[2][4][4];
+        ka_scores<HS, 2>(kb, lane, qf, c);
+        bool move = false;
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                s[mt][e] = (float)(c[mt][e >> 1][e & 1] * 256 + c[mt][e >> 1][(e & 1) + 2]) * fl[mt] * sk[e];
+                w[mt][e] = sv[e];
+            }
+            if (tok0 + KV8_PAGE > all) {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (tok0 + qd * 8 + e >= lim[mt]) { s[mt][e] = -INFINITY; w[mt][e] = 0.f; }
+            }
+            top[mt] = s[mt][0];
+#pragma unroll
+            for (int e = 1; e < 8; e++) top[mt] = fmaxf(top[mt], s[mt][e]);
+            move |= top[mt] > ref[mt] + AHEAD;
+        }
+        if (__any_sync(0xffffffffu, move)) {                   // the references move to the maxima
+            float corr[2];
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+                top[mt] = fmaxf(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 1));
+                top[mt] = fmaxf(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 2));
+                top[mt] = fmaxf(top[mt], ref[mt]);
+                corr[mt] = ref[mt] == -INFINITY ? 0.f : ka_exp2(ref[mt] - top[mt]);
+                ref[mt] = top[mt];
+                run_l[mt] *= corr[mt];
+            }
+            rescale(corr[0], corr[1]);
+        }
+        bool grow = false;
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++) {
+            const float m = ref[mt] == -INFINITY ? 0.f : ref[mt];
+            float sum = 0.f;
+            top[mt] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float p = ka_exp2(s[mt][e] - m);
+                sum += p;
+                w[mt][e] *= p;
+                top[mt] = ka_max_nan(top[mt], w[mt][e]);
+            }
+            run_l[mt] += sum;
+            grow |= !(top[mt] * up[mt] < MOST_W);
+        }
+        if (__any_sync(0xffffffffu, grow)) {                   // a larger unit (or a NaN)
+            float wider[2] = {1.f, 1.f};
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+                top[mt] = ka_max_nan(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 1));
+                top[mt] = ka_max_nan(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 2));
+                if (!(top[mt] < INFINITY)) run_l[mt] = __uint_as_float(0x7fffffffu);
+                else if (top[mt] * up[mt] >= MOST_W) {
+                    const float unit = __uint_as_float((uint32_t)(TOP + 254 - min(max((int)(__float_as_uint(top[mt]) >> 23), 24), 254)) << 23);
+                    wider[mt] = unit / up[mt];
+                    up[mt] = unit;
+                }
+            }
+            rescale(wider[0], wider[1]);
+        }
+        // values of 8 tokens for each lane: k index 2 a, 2 a + 1, 8 + 2 a, 9 + 2 a of an MMA are tokens 8 a .. + 3, of the next one 8 a + 4 .. + 7
+        uint32_t pa[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) {                      // row g, row g + 8, then the same of the next two tokens
+                const int e = h * 4 + (u >> 1) * 2;
+                const __half2 y = __floats2half2_rn(w[u & 1][e] * up[u & 1], w[u & 1][e + 1] * up[u & 1]);
+                pa[h][u] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+#pragma unroll
+        for (int ch = 0; ch < CH; ch++) {
+            uint32_t b[4];
+            ka_ldm_bytes(b, vb + v_at + ((ch ^ v_sw) << 4));
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {                  // 1024 + 128 + code as fp16, less 1152
+                    const uint32_t y = b[h * 2 + u] ^ 0x80808080u;
+                    uint32_t lo = __byte_perm(y, 0x64646464u, 0x4140), hi = __byte_perm(y, 0x64646464u, 0x4342);
+                    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(0x64806480u));
+                    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(hi) : "r"(0x64806480u));
+                    ka_mma_f16(o[2 * ch + u], pa[h], lo, hi);
+                }
+        }
+        __syncwarp();
+        st = st == ST - 1 ? 0 : st + 1;
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();                                           // the ring is done with
+    float* w_acc = reinterpret_cast<float*>(smem);             // [WARPS][SR][HS]
+    float* w_ml = w_acc + KA_WARPS * SR * HS;                  // [WARPS][SR][2]
+    rescale(1.f / up[0], 1.f / up[1]);
+#pragma unroll
+    for (int mt = 0; mt < 2; mt++) {
+        run_l[mt] += __shfl_xor_sync(0xffffffffu, run_l[mt], 1);
+        run_l[mt] += __shfl_xor_sync(0xffffffffu, run_l[mt], 2);
+        if (bad) run_l[mt] = __uint_as_float(0x7fffffffu);
+        const int s = warp * SR + mt * 8 + g;
+#pragma unroll
+        for (int n = 0; n < NT; n++) *reinterpret_cast<float2*>(w_acc + s * HS + qd * 2 + n * 8) = make_float2(o[n][2 * mt], o[n][2 * mt + 1]);
+        if (qd == 0) { w_ml[s * 2] = ref[mt]; w_ml[s * 2 + 1] = run_l[mt]; }
+    }
+    __syncthreads();
+    for (int idx = tid; idx < n_live * HS; idx += KA_WARPS * 32) {         // a warp takes 32 dimensions of a stacked row at a time
+        const int s = idx / HS, d = idx % HS, m = row_of(s), hd = head_of(s);
+        float Mx, L, O;
+        ka_merge<HS, SR>(w_acc, w_ml, s, d, Mx, L, O);
+        const float y = L == 0.f ? 0.f : O / L;
+        kv8_store_y(a, m, hd * HS + d, y);
+        if (a.xq_out != nullptr || a.xh_out != nullptr) q80_block_store(y, lane, m, (hd * HS + d) >> 5, a.out_mcap, a.xq_out, a.xh_out);
+    }
+}
+
+template <typename K, typename... A>
+static int ka_launch(const char* who, K kernel, SmemLimit& given, dim3 grid, int threads, int smem, int pdl, void* stream, const A&... args) {
+    if (const int rc = smem > 0 ? dl_smem_limit(who, kernel, smem, given) : 0) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(KA_WARPS * 32);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attr[1];
@@ -464,11 +688,18 @@ static int ka_launch(const char* who, const Kv8AttArgs& a, const Kv8Work& wk, di
         cfg.attrs = attr;
         cfg.numAttrs = 1;
     }
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_attention_kernel<HS, MT, PROMPT, ST>, a, wk);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e != cudaSuccess) { dl_set_error("%s launch: %s", who, cudaGetErrorString(e)); return -(int)e; }
     return 0;
 }
 
+template <int HS, int MT>
+static int ka_decode_mt(const Kv8AttArgs& a, const Kv8Work& wk, dim3 grid, int pdl, void* stream) {
+    constexpr int ST = 256 / HS, smem = KA_WARPS * ST * KaStage<HS>::BYTES;
+    static_assert(KA_WARPS * MT * 4 * (HS + 2) * 4 + 4 <= smem, "the merge fits the ring");
+    static SmemLimit given;
+    return ka_launch("dl_kv8_attention", kv8_attention_kernel<HS, MT, ST>, given, grid, KA_WARPS * 32, smem, pdl, stream, a, wk);
+}
 template <int HS>
 static int ka_decode(const Kv8AttArgs& a, int n_splits, void* scratch, int pdl, void* stream) {
     const int kv = a.c.n_kv_heads, G = a.heads / kv, M = a.rows.M;
@@ -480,18 +711,16 @@ static int ka_decode(const Kv8AttArgs& a, int n_splits, void* scratch, int pdl, 
         wk.part_o = reinterpret_cast<float*>(at + KA_COUNTER_BYTES);
         wk.part_ml = reinterpret_cast<float*>(at + KA_COUNTER_BYTES + ((long long)M * a.heads * n_splits * HS * 4 + 255) / 256 * 256);
     }
-    const dim3 grid(n_splits, kv * wk.groups, M);
-    constexpr int ST = 2;
-    if (G <= 4) return ka_launch<HS, 1, false, ST>("dl_kv8_attention", a, wk, grid, pdl, stream);
-    return ka_launch<HS, 2, false, ST>("dl_kv8_attention", a, wk, grid, pdl, stream);
+    const dim3 grid(kv * wk.groups, M, n_splits);
+    return G <= 4 ? ka_decode_mt<HS, 1>(a, wk, grid, pdl, stream) : ka_decode_mt<HS, 2>(a, wk, grid, pdl, stream);
 }
 template <int HS>
 static int ka_prompt(const Kv8AttArgs& a, int pdl, void* stream) {
-    constexpr int MT = 2;
-    const int kv = a.c.n_kv_heads, G = a.heads / kv;
-    const Kv8Work wk = {1, 1, nullptr, nullptr, nullptr};
-    const long long tiles = ((long long)a.rows.M * G + MT * 8 - 1) / (MT * 8) + 8;        // upper bound of the tiles of all segments
-    return ka_launch<HS, MT, true, 2>("dl_kv8_attention_prefill", a, wk, dim3((unsigned)tiles, kv), pdl, stream);
+    constexpr int ST = 256 / HS, smem = KA_WARPS * ST * KaStage<HS>::BYTES;
+    static_assert(KA_WARPS * 16 * (HS + 2) * 4 <= smem, "the merge fits the ring");
+    const long long tiles = ((long long)a.rows.M * (a.heads / a.c.n_kv_heads) + 15) / 16 + 8;        // upper bound of the tiles of all segments
+    static SmemLimit given;
+    return ka_launch("dl_kv8_attention_prefill", kv8_prompt_kernel<HS, ST>, given, dim3((unsigned)tiles, a.c.n_kv_heads), KA_WARPS * 32, smem, pdl, stream, a);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -618,7 +847,7 @@ extern "C" int dl_kv8_attention(const float* q, long long ldq, int n_heads, cons
     if (const int rc = kv8_att_args("dl_kv8_attention", q, ldq, n_heads, rows, cache, xq_out, xh_out, out_mcap, y_out, ldy, y_type, &a)) return rc;
     if (n_splits > 1 && scratch == nullptr) { dl_set_error("dl_kv8_attention: n_splits>1 needs scratch"); return -1; }
     if (rows->M == 0) return 0;
-    if (n_splits > 32) { dl_set_error("dl_kv8_attention: %d splits (32 at most)", n_splits); return -1; }
+    if (n_splits > 64) { dl_set_error("dl_kv8_attention: %d splits (64 at most)", n_splits); return -1; }
     if (n_splits < 1) n_splits = 1;
     a.row_skip = row_skip;
     const int hs = cache->head_size;
@@ -646,17 +875,8 @@ extern "C" int dl_kv8_attention_prefill(const float* q, long long ldq, int n_hea
     if (k16 != nullptr && hs == 128 && dense && (long long)rows->M * n_heads > KV8_EXPAND_MIN_WORK) {
         if ((((uintptr_t)k16 | (uintptr_t)v16) & 15) != 0) { dl_set_error("dl_kv8_attention_prefill: the workspace has to be aligned to 16 bytes"); return -1; }
         const Kv8ExpandArgs x = {a, (__half*)k16, (__half*)v16, meta16};
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(4 * dl_device_sm_count());
-        cfg.blockDim = dim3(256);
-        cfg.stream = (cudaStream_t)stream;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = pdl ? 1 : 0;
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_expand_kernel, x);
-        if (e != cudaSuccess) { dl_set_error("dl_kv8_attention_prefill launch: %s", cudaGetErrorString(e)); return -(int)e; }
+        static SmemLimit none;
+        if (const int rc = ka_launch("dl_kv8_attention_prefill", kv8_expand_kernel, none, dim3(4 * dl_device_sm_count()), 256, 0, pdl, stream, x)) return rc;
         return dl_attention_prefill_tc_typed(q, rows->M, n_heads, cache->n_kv_heads, hs, k16, v16, rows->pos, rows->slot, rows->block_table, rows->max_pages, KV8_PAGE, meta16,
                                              xq_out, xh_out, out_mcap, y_out, y_type, cache->n_pages, 1, stream);
     }
