@@ -14,7 +14,7 @@
 
 extern void dl_set_error(const char* fmt, ...);
 extern int dl_device_sm_count();
-extern int kv8_check(const char* who, const DlKv8Cache* c, const DlKv8Rows* r);
+extern int kv8_check(const char* who, const DlKv8Cache* c, const Kv8Rows* r);
 
 struct Kv8AttArgs {
     const float* q;            // [M][ldq]
@@ -30,6 +30,7 @@ struct Kv8AttArgs {
     void* y_out;               // [M][ldy] or NULL
     long long ldy;
     int y_type;
+    bool y_vec;                // rows of y_out take four values at once
 };
 
 DL_DEVINL void kv8_store_y(const Kv8AttArgs& a, int m, int col, float y) {
@@ -38,6 +39,59 @@ DL_DEVINL void kv8_store_y(const Kv8AttArgs& a, int m, int col, float y) {
     if (a.y_type == DL_KV8_F32) reinterpret_cast<float*>(a.y_out)[at] = y;
     else if (a.y_type == DL_KV8_BF16) reinterpret_cast<__nv_bfloat16*>(a.y_out)[at] = __float2bfloat16_rn(y);
     else reinterpret_cast<__half*>(a.y_out)[at] = __float2half_rn(y);
+}
+
+// four neighbouring values of a row from column col on, eight lanes side by side a Q80 block of 32 (by whole warps; live: the lane has any)
+DL_DEVINL void kv8_store4(const Kv8AttArgs& a, int m, int col, float4 y, bool live, int lane) {
+    if (a.y_out != nullptr && live) {
+        const size_t at = (size_t)m * a.ldy + col;
+        if (a.y_type == DL_KV8_F32) {
+            float* d = reinterpret_cast<float*>(a.y_out) + at;
+            if (a.y_vec) *reinterpret_cast<float4*>(d) = y;
+            else { d[0] = y.x; d[1] = y.y; d[2] = y.z; d[3] = y.w; }
+        } else {
+            uint32_t lo, hi;
+            if (a.y_type == DL_KV8_BF16) {
+                const __nv_bfloat162 u = __floats2bfloat162_rn(y.x, y.y), v = __floats2bfloat162_rn(y.z, y.w);
+                lo = *reinterpret_cast<const uint32_t*>(&u);
+                hi = *reinterpret_cast<const uint32_t*>(&v);
+            } else {
+                const __half2 u = __floats2half2_rn(y.x, y.y), v = __floats2half2_rn(y.z, y.w);
+                lo = *reinterpret_cast<const uint32_t*>(&u);
+                hi = *reinterpret_cast<const uint32_t*>(&v);
+            }
+            uint16_t* d = reinterpret_cast<uint16_t*>(a.y_out) + at;
+            if (a.y_vec) *reinterpret_cast<uint2*>(d) = make_uint2(lo, hi);
+            else { d[0] = (uint16_t)lo; d[1] = (uint16_t)(lo >> 16); d[2] = (uint16_t)hi; d[3] = (uint16_t)(hi >> 16); }
+        }
+    }
+    if (a.xq_out == nullptr && a.xh_out == nullptr) return;
+    // as q80_block_store: scale from the block's largest magnitude, codes by its reciprocal
+    float amax = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
+#pragma unroll
+    for (int w = 1; w < 8; w <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, w));
+    const float d = amax / 127.0f, id = d != 0.0f ? 1.0f / d : 0.0f, df = __half2float(__float2half_rn(d));
+    const int q[4] = {__float2int_rn(y.x * id), __float2int_rn(y.y * id), __float2int_rn(y.z * id), __float2int_rn(y.w * id)};
+    const int kt = col >> 7, kb = (col >> 5) & 3, j = (col & 31) >> 2;
+    if (a.xq_out != nullptr) {
+        int sum = q[0] + q[1] + q[2] + q[3];
+#pragma unroll
+        for (int w = 1; w < 8; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        if (live) {
+            uint8_t* row = a.xq_out + ((size_t)kt * a.out_mcap + m) * XQ_ROW_BYTES;
+            *reinterpret_cast<uint32_t*>(row + kb * 32 + j * 4) = (uint32_t)(q[0] & 0xff) | ((uint32_t)(q[1] & 0xff) << 8) | ((uint32_t)(q[2] & 0xff) << 16) | ((uint32_t)(q[3] & 0xff) << 24);
+            if (j == 0) {
+                reinterpret_cast<float*>(row + 128)[kb] = df;
+                reinterpret_cast<int*>(row + 144)[kb] = 8 * sum;
+            }
+        }
+    }
+    if (a.xh_out != nullptr && live) {
+        const float dfh = fminf(df, 515.0f);
+        const __half2 u = __floats2half2_rn((float)q[0] * dfh, (float)q[2] * dfh), v = __floats2half2_rn((float)q[1] * dfh, (float)q[3] * dfh);      // (K order of xh_slot)
+        uint8_t* at = a.xh_out + ((size_t)kt * (a.out_mcap >> 3) + (m >> 3)) * XH_ROWGROUP_BYTES + (size_t)(kb * 4 + (j & 3)) * 128 + (m & 7) * 16 + (j >> 2) * 8;
+        *reinterpret_cast<uint2*>(at) = make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -59,6 +113,7 @@ DL_DEVINL void kv8_store_y(const Kv8AttArgs& a, int m, int col, float y) {
 // ------------------------------------------------------------------------------------------------
 #define KA_WARPS 4
 #define KA_MIN_SPLIT_PAGES 24        // contexts up to 768 tokens: no split
+#define KA_MOST_CTAS 8               // of a cluster that shares a prompt tile's pages
 #define KA_COUNTER_BYTES 65536       // completion counters at scratch offset 0 (dl_attention_scratch_bytes)
 
 DL_DEVINL void ka_cp16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
@@ -181,20 +236,8 @@ DL_DEVINL void ka_scales(const float* at, float (&s)[8]) {
     const float4 x = *reinterpret_cast<const float4*>(at), y = *reinterpret_cast<const float4*>(at + 4);
     s[0] = x.x; s[1] = x.y; s[2] = x.z; s[3] = x.w; s[4] = y.x; s[5] = y.y; s[6] = y.z; s[7] = y.w;
 }
-// four warps' sums of a stacked row and dimension: the largest reference, the sum of weights, the weighted sum (references in units of log2)
-template <int HS, int SR> DL_DEVINL void ka_merge(const float* w_acc, const float* w_ml, int s, int d, float& Mx, float& L, float& O) {
-    Mx = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < KA_WARPS; w++) Mx = fmaxf(Mx, w_ml[(w * SR + s) * 2]);
-    const float Mu = Mx == -INFINITY ? 0.f : Mx;
-    L = O = 0.f;
-#pragma unroll
-    for (int w = 0; w < KA_WARPS; w++) {
-        const float e = ka_exp2(w_ml[(w * SR + s) * 2] - Mu);
-        L += w_ml[(w * SR + s) * 2 + 1] * e;
-        O += w_acc[(w * SR + s) * HS + d] * e;
-    }
-}
+// The warps' sums in shared memory, rows 8 floats apart beyond their length: the eight rows that a warp's lanes store at once lie in different banks
+template <int HS> struct KaSums { static constexpr int LD = HS + 8; };
 
 struct Kv8Work {               // what the launch adds to the arguments of decode rows
     int n_splits, groups;      // groups: CTAs that share a key/value head's query heads
@@ -359,8 +402,9 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
     bad = __any_sync(0xffffffffu, bad);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();                                           // the ring is done with
-    float* w_acc = reinterpret_cast<float*>(smem);             // [WARPS][SR][HS]
-    float* w_ml = w_acc + KA_WARPS * SR * HS;                  // [WARPS][SR][2]
+    constexpr int LD = KaSums<HS>::LD, LPH = HS / 4, ZP = 32 / LPH;        // LPH lanes take a head
+    float* w_acc = reinterpret_cast<float*>(smem);             // [WARPS][SR][LD]
+    float* w_ml = w_acc + KA_WARPS * SR * LD;                  // [WARPS][SR][2]
     int* s_last = reinterpret_cast<int*>(w_ml + KA_WARPS * SR * 2);
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
@@ -369,31 +413,42 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
         if (bad) run_l[mt] = __uint_as_float(0x7fffffffu);
         const float unit = __uint_as_float((uint32_t)(ex[mt] - TOP) << 23) * (lower ? 256.f : 1.f / 256.f);
         const int s = warp * SR + mt * 4 + (g & 3);
+        // the upper lanes' digits go to the lower ones, which take the even n-tiles; and the other way round
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
+        for (int n = 0; n < NT; n += 2) {
             float v[2];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                v[e] = o[mt][n][e] * unit;
-                v[e] += __shfl_xor_sync(0xffffffffu, v[e], 16);
+                const float x0 = o[mt][n][e] * unit, x1 = o[mt][n + 1][e] * unit;
+                v[e] = (lower ? x0 : x1) + __shfl_xor_sync(0xffffffffu, lower ? x1 : x0, 16);
             }
-            if (lower) *reinterpret_cast<float2*>(w_acc + s * HS + qd * 2 + n * 8) = make_float2(v[0], v[1]);
+            *reinterpret_cast<float2*>(w_acc + s * LD + qd * 2 + (lower ? n : n + 1) * 8) = make_float2(v[0], v[1]);
         }
         if (lower && qd == 0) { w_ml[s * 2] = run_m[mt]; w_ml[s * 2 + 1] = run_l[mt]; }
     }
     __syncthreads();
     const bool single = n_eff == 1;
-    for (int idx = tid; idx < n_live * HS; idx += KA_WARPS * 32) {         // a warp takes 32 dimensions of a head at a time
-        const int s = idx / HS, d = idx % HS, hd = kvh * G + h_lo + s;
-        float Mx, L, O;
-        ka_merge<HS, SR>(w_acc, w_ml, s, d, Mx, L, O);
+    for (int base = warp * 32; base < n_live * LPH; base += KA_WARPS * 32) {       // a lane takes four dimensions of a head
+        const int s = min((base + lane) / LPH, n_live - 1), d = lane % LPH * 4, hd = kvh * G + h_lo + s;
+        const bool live = base + lane < n_live * LPH;
+        float mw[KA_WARPS], Mx = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < KA_WARPS; w++) { mw[w] = w_ml[(w * SR + s) * 2]; Mx = fmaxf(Mx, mw[w]); }
+        const float Mu = Mx == -INFINITY ? 0.f : Mx;
+        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < KA_WARPS; w++) {
+            const float e = ka_exp2(mw[w] - Mu);
+            const float4 x = *reinterpret_cast<const float4*>(w_acc + (w * SR + s) * LD + d);
+            L = fmaf(w_ml[(w * SR + s) * 2 + 1], e, L);
+            O.x = fmaf(x.x, e, O.x); O.y = fmaf(x.y, e, O.y); O.z = fmaf(x.z, e, O.z); O.w = fmaf(x.w, e, O.w);
+        }
         if (single) {
-            const float y = L == 0.f ? 0.f : O / L;
-            kv8_store_y(a, m0, hd * HS + d, y);
-            if (a.xq_out != nullptr || a.xh_out != nullptr) q80_block_store(y, lane, m0, (hd * HS + d) >> 5, a.out_mcap, a.xq_out, a.xh_out);
-        } else {
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            kv8_store4(a, m0, hd * HS + d, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv), live, lane);
+        } else if (live) {
             const size_t pidx = ((size_t)m0 * a.heads + hd) * wk.n_splits + sp;
-            wk.part_o[pidx * HS + d] = O;
+            *reinterpret_cast<float4*>(wk.part_o + pidx * HS + d) = O;
             if (d == 0) { wk.part_ml[pidx * 2] = Mx; wk.part_ml[pidx * 2 + 1] = L; }
         }
     }
@@ -409,8 +464,6 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
     __syncthreads();
     if (!*s_last) return;
     // a warp merges a head: the lanes hold the splits' (max, sum); then HS / 4 lanes take a split's sums, 32 / (HS / 4) splits side by side, eight of each in flight
-    constexpr int LPH = HS / 4, ZP = 32 / LPH;
-    float* y_s = w_acc + warp * HS;                            // (the four warps' sums are done with)
     for (int s = warp; s < n_live; s += KA_WARPS) {
         const int hd = kvh * G + h_lo + s;
         const size_t base = ((size_t)m0 * a.heads + hd) * wk.n_splits;
@@ -446,15 +499,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
             O.x += __shfl_xor_sync(0xffffffffu, O.x, w); O.y += __shfl_xor_sync(0xffffffffu, O.y, w);
             O.z += __shfl_xor_sync(0xffffffffu, O.z, w); O.w += __shfl_xor_sync(0xffffffffu, O.w, w);
         }
-        __syncwarp();
-        if (lane < LPH) *reinterpret_cast<float4*>(y_s + lane * 4) = O;
-        __syncwarp();
-#pragma unroll
-        for (int d = 0; d < HS / 32; d++) {                    // 32 dims at a time: one Q80 block
-            const float y = L == 0.f ? 0.f : y_s[d * 32 + lane] / L;
-            kv8_store_y(a, m0, hd * HS + d * 32 + lane, y);
-            if (a.xq_out != nullptr || a.xh_out != nullptr) q80_block_store(y, lane, m0, hd * (HS / 32) + d, a.out_mcap, a.xq_out, a.xh_out);
-        }
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        kv8_store4(a, m0, hd * HS + lane % LPH * 4, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv), lane < LPH, lane);
     }
 }
 
@@ -466,7 +512,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
 // steady state takes no exchange for a running maximum and no rescaling.
 // ------------------------------------------------------------------------------------------------
 template <int HS, int ST>
-__global__ void __launch_bounds__(KA_WARPS * 32) kv8_prompt_kernel(const __grid_constant__ Kv8AttArgs a) {
+__global__ void __launch_bounds__(KA_WARPS * 32, HS == 128 ? 3 : 4) kv8_prompt_kernel(const __grid_constant__ Kv8AttArgs a) {
     constexpr int CH = HS / 16, KS = HS / 32, NT = HS / 8, STAGE = KaStage<HS>::BYTES, CODES = KaStage<HS>::CODES;
     constexpr int SR = 16;                                                 // stacked rows of the CTA
     constexpr int TOP = 6;                                                 // the largest weight is below 2^(TOP + 1) units when the unit is chosen,
@@ -474,20 +520,27 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_prompt_kernel(const __grid_
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, qd = lane & 3;
     const int kvh = blockIdx.y, G = a.heads / a.c.n_kv_heads;
+    uint32_t n_cta, rank;                                      // CTAs of the cluster: they share the tile's pages
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n_cta));
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     pdl_launch_dependents();
     pdl_wait();
     // stacked row s of the tile is pair s_lo + s = row * G + head of the group, row 0 (batch row m0) at position p0
-    int tile = gridDim.x - 1 - blockIdx.x, m0 = 0, end = 0, i0 = 0;        // late tiles (long histories) first
-    const int n_seg = min(a.meta[0], 8);
-    for (; i0 < n_seg; i0++) {
-        m0 = a.meta[1 + 2 * i0];
-        end = a.meta[2 + 2 * i0];
-        if (m0 < 0 || end > a.rows.M || end <= m0) continue;
-        const int nt = ((end - m0) * G + SR - 1) / SR;
-        if (tile < nt) break;
-        tile -= nt;
+    int tile = (gridDim.x - 1 - blockIdx.x) / n_cta, m0 = 0, end = 0;      // late tiles (long histories) first
+    {
+        const int mine = lane < 17 ? a.meta[min(lane, 2 * min(max(a.meta[0], 0), 8))] : 0;      // (what lies behind the last segment is not read)
+        const int n_seg = min(__shfl_sync(0xffffffffu, mine, 0), 8);
+        int i = 0;
+        for (; i < n_seg; i++) {
+            m0 = __shfl_sync(0xffffffffu, mine, 1 + 2 * i);
+            end = __shfl_sync(0xffffffffu, mine, 2 + 2 * i);
+            if (m0 < 0 || end > a.rows.M || end <= m0) continue;
+            const int nt = ((end - m0) * G + SR - 1) / SR;
+            if (tile < nt) break;
+            tile -= nt;
+        }
+        if (i >= n_seg) return;
     }
-    if (i0 >= n_seg) return;
     const int s_lo = tile * SR, n_live = min(SR, (end - m0) * G - s_lo), p0 = a.rows.pos[m0], slot = a.rows.slot[m0];
     auto row_of = [&](int s) { return m0 + (s_lo + s) / G; };
     auto head_of = [&](int s) { return kvh * G + (s_lo + s) % G; };
@@ -499,12 +552,16 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_prompt_kernel(const __grid_
     }
     bool bad = p0 >= 0 && (p0 > 0x7fffffff - (end - m0) || kv8_tokens(a.rows, p0 + (end - m0) - 1, slot) < 0);
     const int T = bad || p0 < 0 ? 0 : p0 + (s_lo + n_live - 1) / G + 1, all = min(T, p0 + s_lo / G + 1);       // tokens that the last, that every row of the tile sees
-    const int n_pages = (T + KV8_PAGE - 1) / KV8_PAGE, n_my = max(0, (n_pages - warp + KA_WARPS - 1) / KA_WARPS);       // this warp's pages: warp + 4 i
+    if ((T + KV8_PAGE - 1) / KV8_PAGE < 8 * (int)n_cta) {      // too few pages to share: the first CTA's
+        if (rank > 0) return;
+        n_cta = 1;
+    }
+    const int step = KA_WARPS * n_cta, w0 = rank * KA_WARPS + warp, n_pages = (T + KV8_PAGE - 1) / KV8_PAGE, n_my = max(0, (n_pages - w0 + step - 1) / step);      // this warp's pages: w0 + step i
     const int* bt = a.rows.block_table + (size_t)(bad ? 0 : slot) * a.rows.max_pages;
 
     const uint32_t ring = smem_u32(smem) + warp * (ST * STAGE);
     auto page_at = [&](int i) {
-        int p = i < n_my ? bt[warp + KA_WARPS * i] : 0;
+        int p = i < n_my ? bt[w0 + step * i] : 0;
         if ((unsigned)p >= (unsigned)a.rows.n_pages) { bad = true; p = 0; }
         return p;
     };
@@ -550,7 +607,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_prompt_kernel(const __grid_
         __syncwarp();
         const uint32_t kb = ring + st * STAGE, vb = kb + CODES;
         const float* scales = reinterpret_cast<const float*>(smem + (size_t)(warp * ST + st) * STAGE + 2 * CODES) + qd * 8;
-        const int tok0 = (warp + KA_WARPS * i) * KV8_PAGE;
+        const int tok0 = (w0 + step * i) * KV8_PAGE;
         float sk[8], sv[8], s[2][8], w[2][8], top[2];
         ka_scales(scales, sk);
         ka_scales(scales + KV8_PAGE, sv);
@@ -649,8 +706,11 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_prompt_kernel(const __grid_
     bad = __any_sync(0xffffffffu, bad);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();                                           // the ring is done with
-    float* w_acc = reinterpret_cast<float*>(smem);             // [WARPS][SR][HS]
-    float* w_ml = w_acc + KA_WARPS * SR * HS;                  // [WARPS][SR][2]
+    constexpr int LD = KaSums<HS>::LD, LPH = HS / 4;           // LPH lanes take a row
+    float* w_acc = reinterpret_cast<float*>(smem);             // [WARPS][SR][LD]
+    float* w_ml = w_acc + KA_WARPS * SR * LD;                  // [WARPS][SR][2]
+    float* share = w_ml + KA_WARPS * SR * 2;                   // [SR][WARPS * CTAs]: what a row's sums count
+    int* place = reinterpret_cast<int*>(share + SR * KA_WARPS * KA_MOST_CTAS);     // [SR][2]: batch row, first column
     rescale(1.f / up[0], 1.f / up[1]);
 #pragma unroll
     for (int mt = 0; mt < 2; mt++) {
@@ -659,34 +719,71 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_prompt_kernel(const __grid_
         if (bad) run_l[mt] = __uint_as_float(0x7fffffffu);
         const int s = warp * SR + mt * 8 + g;
 #pragma unroll
-        for (int n = 0; n < NT; n++) *reinterpret_cast<float2*>(w_acc + s * HS + qd * 2 + n * 8) = make_float2(o[n][2 * mt], o[n][2 * mt + 1]);
+        for (int n = 0; n < NT; n++) *reinterpret_cast<float2*>(w_acc + s * LD + qd * 2 + n * 8) = make_float2(o[n][2 * mt], o[n][2 * mt + 1]);
         if (qd == 0) { w_ml[s * 2] = ref[mt]; w_ml[s * 2 + 1] = run_l[mt]; }
     }
-    __syncthreads();
-    for (int idx = tid; idx < n_live * HS; idx += KA_WARPS * 32) {         // a warp takes 32 dimensions of a stacked row at a time
-        const int s = idx / HS, d = idx % HS, m = row_of(s), hd = head_of(s);
-        float Mx, L, O;
-        ka_merge<HS, SR>(w_acc, w_ml, s, d, Mx, L, O);
-        const float y = L == 0.f ? 0.f : O / L;
-        kv8_store_y(a, m, hd * HS + d, y);
-        if (a.xq_out != nullptr || a.xh_out != nullptr) q80_block_store(y, lane, m, (hd * HS + d) >> 5, a.out_mcap, a.xq_out, a.xh_out);
+    // every CTA of the cluster sums its share of the tile's rows over all of them
+    cg::cluster_group cluster = cg::this_cluster();
+    if (n_cta > 1) cluster.sync();
+    else __syncthreads();
+    const int mine = n_live > (int)rank ? (n_live - 1 - (int)rank) / (int)n_cta + 1 : 0;       // rows rank, rank + n_cta, ...
+    const int parts = KA_WARPS * n_cta;                        // (a power of two, 32 at most: a row's lanes lie in one warp)
+    if (warp < 2) {
+        const int j = tid / parts, z = tid % parts, s = rank + j * n_cta;
+        float m = -INFINITY, l = 0.f;
+        if (j < mine) {
+            const float* ml = cluster.map_shared_rank(w_ml, z / KA_WARPS) + ((z % KA_WARPS) * SR + s) * 2;
+            m = ml[0];
+            l = ml[1];
+        }
+        float Mx = m;
+        for (int w = 1; w < parts; w <<= 1) Mx = fmaxf(Mx, __shfl_xor_sync(0xffffffffu, Mx, w));
+        const float e = ka_exp2(m - (Mx == -INFINITY ? 0.f : Mx));
+        float L = l * e;
+        for (int w = 1; w < parts; w <<= 1) L += __shfl_xor_sync(0xffffffffu, L, w);
+        if (j < mine) {
+            share[tid] = L == 0.f ? 0.f : e / L;
+            if (z == 0) { place[j * 2] = row_of(s); place[j * 2 + 1] = head_of(s) * HS; }
+        }
     }
+    __syncthreads();
+    for (int base = warp * 32; base < mine * LPH; base += KA_WARPS * 32) {         // a lane takes four dimensions of a row
+        const int j = min((base + lane) / LPH, mine - 1), s = rank + j * n_cta, d = lane % LPH * 4;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t r = 0; r < n_cta; r++) {
+            const float* from = cluster.map_shared_rank(w_acc, r) + s * LD + d;
+            const float4 e4 = *reinterpret_cast<const float4*>(share + j * parts + r * KA_WARPS);
+            const float e[4] = {e4.x, e4.y, e4.z, e4.w};
+#pragma unroll
+            for (int w = 0; w < KA_WARPS; w++) {
+                const float4 x = *reinterpret_cast<const float4*>(from + w * SR * LD);
+                y.x = fmaf(x.x, e[w], y.x); y.y = fmaf(x.y, e[w], y.y); y.z = fmaf(x.z, e[w], y.z); y.w = fmaf(x.w, e[w], y.w);
+            }
+        }
+        kv8_store4(a, place[j * 2], place[j * 2 + 1] + d, y, base + lane < mine * LPH, lane);
+    }
+    if (n_cta > 1) cluster.sync();                             // (no CTA leaves while its sums are read)
 }
 
 template <typename K, typename... A>
-static int ka_launch(const char* who, K kernel, SmemLimit& given, dim3 grid, int threads, int smem, int pdl, void* stream, const A&... args) {
+static int ka_launch(const char* who, K kernel, SmemLimit& given, dim3 grid, int cluster, int threads, int smem, int pdl, void* stream, const A&... args) {
     if (const int rc = smem > 0 ? dl_smem_limit(who, kernel, smem, given) : 0) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        cfg.numAttrs++;
+    }
     if (pdl) {
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     }
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e != cudaSuccess) { dl_set_error("%s launch: %s", who, cudaGetErrorString(e)); return -(int)e; }
@@ -696,9 +793,9 @@ static int ka_launch(const char* who, K kernel, SmemLimit& given, dim3 grid, int
 template <int HS, int MT>
 static int ka_decode_mt(const Kv8AttArgs& a, const Kv8Work& wk, dim3 grid, int pdl, void* stream) {
     constexpr int ST = 256 / HS, smem = KA_WARPS * ST * KaStage<HS>::BYTES;
-    static_assert(KA_WARPS * MT * 4 * (HS + 2) * 4 + 4 <= smem, "the merge fits the ring");
+    static_assert(KA_WARPS * MT * 4 * (KaSums<HS>::LD + 2) * 4 + 4 <= smem, "the merge fits the ring");
     static SmemLimit given;
-    return ka_launch("dl_kv8_attention", kv8_attention_kernel<HS, MT, ST>, given, grid, KA_WARPS * 32, smem, pdl, stream, a, wk);
+    return ka_launch("dl_kv8_attention", kv8_attention_kernel<HS, MT, ST>, given, grid, 1, KA_WARPS * 32, smem, pdl, stream, a, wk);
 }
 template <int HS>
 static int ka_decode(const Kv8AttArgs& a, int n_splits, void* scratch, int pdl, void* stream) {
@@ -716,11 +813,14 @@ static int ka_decode(const Kv8AttArgs& a, int n_splits, void* scratch, int pdl, 
 }
 template <int HS>
 static int ka_prompt(const Kv8AttArgs& a, int pdl, void* stream) {
-    constexpr int ST = 256 / HS, smem = KA_WARPS * ST * KaStage<HS>::BYTES;
-    static_assert(KA_WARPS * 16 * (HS + 2) * 4 <= smem, "the merge fits the ring");
+    constexpr int ST = HS == 32 ? 4 : 2, ring = KA_WARPS * ST * KaStage<HS>::BYTES, merge = 16 * (KA_WARPS * (KaSums<HS>::LD + 2 + KA_MOST_CTAS) + 2) * 4, smem = ring > merge ? ring : merge;
     const long long tiles = ((long long)a.rows.M * (a.heads / a.c.n_kv_heads) + 15) / 16 + 8;        // upper bound of the tiles of all segments
     static SmemLimit given;
-    return ka_launch("dl_kv8_attention_prefill", kv8_prompt_kernel<HS, ST>, given, dim3((unsigned)tiles, a.c.n_kv_heads), KA_WARPS * 32, smem, pdl, stream, a);
+    // CTAs of a tile where tiles leave SMs idle (us with one / two / four: 32 tiles behind 3000 tokens 31 / 25 / 23, behind none 8.1 / 8.6 / 9.2; 64 behind 1000 15.7 /
+    // 14.7 / 15.6; 128 behind 2000 30.2 / 25.6 / 31.3, behind 500 14.4 / 14.9 / 24; 200 behind 1000 20.1 / 19.2 / 31, behind none 9.1 / 10.6 / 16)
+    const long long ctas = (tiles - 8) * a.c.n_kv_heads;
+    const int cluster = ctas <= 40 ? 4 : ctas <= 160 ? 2 : 1;
+    return ka_launch("dl_kv8_attention_prefill", kv8_prompt_kernel<HS, ST>, given, dim3((unsigned)tiles * cluster, a.c.n_kv_heads), cluster, KA_WARPS * 32, smem, pdl, stream, a);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -824,29 +924,31 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const __grid_constant__
 }
 
 // what both entry points refuse
-static int kv8_att_args(const char* who, const float* q, long long ldq, int n_heads, const DlKv8Rows* rows, const DlKv8Cache* cache, uint8_t* xq_out, uint8_t* xh_out,
+static int kv8_att_args(const char* who, const float* q, long long ldq, int n_heads, const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const DlKv8Cache* cache, uint8_t* xq_out, uint8_t* xh_out,
                         int out_mcap, void* y_out, long long ldy, int y_type, Kv8AttArgs* a) {
-    if (const int rc = kv8_check(who, cache, rows)) return rc;
+    const Kv8Rows rows = {pos, slot, block_table, M, n_slots, max_pages, cache ? cache->n_pages : 0};
+    if (const int rc = kv8_check(who, cache, &rows)) return rc;
     const int hs = cache->head_size, kv = cache->n_kv_heads;
     if (n_heads < kv || n_heads % kv != 0 || n_heads / kv > 16) { dl_set_error("%s: unsupported head grouping %d/%d", who, n_heads, kv); return -1; }
     if (q == nullptr || (xq_out == nullptr && xh_out == nullptr && y_out == nullptr)) { dl_set_error("%s: no queries or no output", who); return -1; }
     if (ldq < (long long)n_heads * hs || (y_out != nullptr && ldy < (long long)n_heads * hs)) { dl_set_error("%s: rows overlap (ld %lld, %lld)", who, ldq, ldy); return -1; }
     if (y_type != DL_KV8_F32 && y_type != DL_KV8_BF16 && y_type != DL_KV8_F16) { dl_set_error("%s: unsupported output type %d", who, y_type); return -1; }
-    if ((xq_out != nullptr || xh_out != nullptr) && ((long long)n_heads * hs % 128 != 0 || out_mcap < rows->M || (xh_out != nullptr && out_mcap % 8 != 0))) {
+    if ((xq_out != nullptr || xh_out != nullptr) && ((long long)n_heads * hs % 128 != 0 || out_mcap < M || (xh_out != nullptr && out_mcap % 8 != 0))) {
         dl_set_error("%s: slabs of %d rows, %d columns", who, out_mcap, n_heads * hs);
         return -1;
     }
-    *a = {q, ldq, {rows->pos, rows->slot, rows->block_table, rows->M, rows->n_slots, rows->max_pages, cache->n_pages}, *cache, n_heads, nullptr, nullptr, xq_out, xh_out, out_mcap, y_out, ldy, y_type};
-    if (rows->M > 65535) { dl_set_error("%s: %d rows (65535 at most)", who, rows->M); return -1; }
+    *a = {q, ldq, rows, *cache, n_heads, nullptr, nullptr, xq_out, xh_out, out_mcap, y_out, ldy, y_type,
+          ((uintptr_t)y_out & (y_type == DL_KV8_F32 ? 15 : 7)) == 0 && ldy % 4 == 0};
+    if (M > 65535) { dl_set_error("%s: %d rows (65535 at most)", who, M); return -1; }
     return 0;
 }
 
-extern "C" int dl_kv8_attention(const float* q, long long ldq, int n_heads, const DlKv8Rows* rows, const DlKv8Cache* cache, int n_splits, void* scratch, uint8_t* xq_out,
+extern "C" int dl_kv8_attention(const float* q, long long ldq, int n_heads, const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const DlKv8Cache* cache, int n_splits, void* scratch, uint8_t* xq_out,
                                 uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, const int* row_skip, int pdl, void* stream) {
     Kv8AttArgs a;
-    if (const int rc = kv8_att_args("dl_kv8_attention", q, ldq, n_heads, rows, cache, xq_out, xh_out, out_mcap, y_out, ldy, y_type, &a)) return rc;
-    if (n_splits > 1 && scratch == nullptr) { dl_set_error("dl_kv8_attention: n_splits>1 needs scratch"); return -1; }
-    if (rows->M == 0) return 0;
+    if (const int rc = kv8_att_args("dl_kv8_attention", q, ldq, n_heads, pos, slot, block_table, M, n_slots, max_pages, cache, xq_out, xh_out, out_mcap, y_out, ldy, y_type, &a)) return rc;
+    if (n_splits > 1 && (scratch == nullptr || ((uintptr_t)scratch & 15) != 0)) { dl_set_error("dl_kv8_attention: n_splits>1 needs scratch, aligned to 16 bytes"); return -1; }
+    if (M == 0) return 0;
     if (n_splits > 64) { dl_set_error("dl_kv8_attention: %d splits (64 at most)", n_splits); return -1; }
     if (n_splits < 1) n_splits = 1;
     a.row_skip = row_skip;
@@ -862,22 +964,22 @@ extern int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int
                                          const int* slot, const int* block_table, int max_pages, int page_size, const int* meta, uint8_t* xq_out, uint8_t* xh_out,
                                          int out_mcap, void* y_out, int y_type, int n_cache_pages, int pdl, void* stream);
 
-extern "C" int dl_kv8_attention_prefill(const float* q, long long ldq, int n_heads, const DlKv8Rows* rows, const int* meta, const DlKv8Cache* cache, void* k16, void* v16,
+extern "C" int dl_kv8_attention_prefill(const float* q, long long ldq, int n_heads, const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const int* meta, const DlKv8Cache* cache, void* k16, void* v16,
                                         int* meta16, uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, int pdl, void* stream) {
     Kv8AttArgs a;
-    if (const int rc = kv8_att_args("dl_kv8_attention_prefill", q, ldq, n_heads, rows, cache, xq_out, xh_out, out_mcap, y_out, ldy, y_type, &a)) return rc;
+    if (const int rc = kv8_att_args("dl_kv8_attention_prefill", q, ldq, n_heads, pos, slot, block_table, M, n_slots, max_pages, cache, xq_out, xh_out, out_mcap, y_out, ldy, y_type, &a)) return rc;
     if (meta == nullptr || (k16 == nullptr) != (v16 == nullptr) || (k16 == nullptr) != (meta16 == nullptr)) { dl_set_error("dl_kv8_attention_prefill: a null pointer"); return -1; }
-    if (rows->M == 0) return 0;
+    if (M == 0) return 0;
     a.meta = meta;
     const int hs = cache->head_size;
     // (that kernel takes rows side by side, aligned)
     const bool dense = ldq == (long long)n_heads * hs && ((uintptr_t)q & 15) == 0 && (y_out == nullptr || (ldy == ldq && ((uintptr_t)y_out & 15) == 0));
-    if (k16 != nullptr && hs == 128 && dense && (long long)rows->M * n_heads > KV8_EXPAND_MIN_WORK) {
+    if (k16 != nullptr && hs == 128 && dense && (long long)M * n_heads > KV8_EXPAND_MIN_WORK) {
         if ((((uintptr_t)k16 | (uintptr_t)v16) & 15) != 0) { dl_set_error("dl_kv8_attention_prefill: the workspace has to be aligned to 16 bytes"); return -1; }
         const Kv8ExpandArgs x = {a, (__half*)k16, (__half*)v16, meta16};
         static SmemLimit none;
-        if (const int rc = ka_launch("dl_kv8_attention_prefill", kv8_expand_kernel, none, dim3(4 * dl_device_sm_count()), 256, 0, pdl, stream, x)) return rc;
-        return dl_attention_prefill_tc_typed(q, rows->M, n_heads, cache->n_kv_heads, hs, k16, v16, rows->pos, rows->slot, rows->block_table, rows->max_pages, KV8_PAGE, meta16,
+        if (const int rc = ka_launch("dl_kv8_attention_prefill", kv8_expand_kernel, none, dim3(4 * dl_device_sm_count()), 1, 256, 0, pdl, stream, x)) return rc;
+        return dl_attention_prefill_tc_typed(q, M, n_heads, cache->n_kv_heads, hs, k16, v16, pos, slot, block_table, max_pages, KV8_PAGE, meta16,
                                              xq_out, xh_out, out_mcap, y_out, y_type, cache->n_pages, 1, stream);
     }
     return hs == 128 ? ka_prompt<128>(a, pdl, stream) : hs == 64 ? ka_prompt<64>(a, pdl, stream) : ka_prompt<32>(a, pdl, stream);

@@ -12,7 +12,7 @@ from typing import List, NamedTuple, Optional, Sequence
 import torch
 
 from . import lib
-from .lib import DlEpilogue, DlKv8Cache, DlKv8Rows, DlNormProlog, EPI_QKV_ROPE, EPI_SILU_MUL, EPI_STORE, KV8_BF16, KV8_F16, KV8_F32, check, cuda_lib
+from .lib import DlEpilogue, DlKv8Cache, DlNormProlog, EPI_QKV_ROPE, EPI_SILU_MUL, EPI_STORE, KV8_BF16, KV8_F16, KV8_F32, check, cuda_lib
 
 Q40T_TILE_BYTES = 9216
 XQ_ROW_BYTES = 160
@@ -256,7 +256,7 @@ _KV8_TYPES = {torch.float32: KV8_F32, torch.bfloat16: KV8_BF16, torch.float16: K
 class Kv8Cache:
     """The pages of one layer's 8-bit token cache: k / v int8 [pages][kv heads][32][head size], k_scale / v_scale f32 [pages][kv heads][32].
     Checked once, here; the tensors have to keep their memory."""
-    __slots__ = ("k", "v", "k_scale", "v_scale", "n_pages", "n_kv_heads", "head_size", "device", "args", "ref")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "n_pages", "n_kv_heads", "head_size", "device", "index", "args", "ref")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dim() != 4 or k.shape[2] != PAGE_SIZE or k.shape[3] not in (32, 64, 128) or k.shape[0] < 1 or k.shape[1] < 1:
@@ -270,6 +270,7 @@ class Kv8Cache:
                 raise ValueError("codes and scales have to be contiguous, on one device and aligned to 16 bytes")
         self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
         self.n_pages, self.n_kv_heads, self.head_size = k.shape[0], k.shape[1], k.shape[3]
+        self.index = k.get_device()
         self.args = DlKv8Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.n_pages, self.n_kv_heads, self.head_size)
         self.ref = C.byref(self.args)
 
@@ -287,23 +288,24 @@ def alloc_kv8(n_pages: int, n_kv_heads: int, head_size: int, device) -> Kv8Cache
     return Kv8Cache(*codes, *(torch.zeros(n_pages, n_kv_heads, PAGE_SIZE, dtype=torch.float32, device=device) for _ in range(2)))
 
 
-def _kv8_rows(M: int, pos: torch.Tensor, slot: torch.Tensor, block_table: torch.Tensor, cache: Kv8Cache) -> DlKv8Rows:
-    dev = cache.device
-    if dev.type != "cuda" or dev.index != torch.cuda.current_device():
-        raise ValueError(f"the cache is on {dev}: the current device launches")
-    for t in (pos, slot, block_table):
-        if t.dtype is not torch.int32 or t.device != dev or not t.is_contiguous():
-            raise ValueError("pos, slot and block_table are contiguous int32 tensors on the cache's device")
+def _kv8_rows(M: int, pos: torch.Tensor, slot: torch.Tensor, block_table: torch.Tensor, cache: Kv8Cache):
+    """The rows' arguments of the C functions."""
+    d = cache.index
+    if d < 0 or d != torch._C._cuda_getDevice():
+        raise ValueError(f"the cache is on {cache.device}: the current device launches")
+    if not (pos.dtype is slot.dtype is block_table.dtype is torch.int32 and pos.get_device() == slot.get_device() == block_table.get_device() == d
+            and pos.is_contiguous() and slot.is_contiguous() and block_table.is_contiguous()):
+        raise ValueError("pos, slot and block_table are contiguous int32 tensors on the cache's device")
     if block_table.dim() != 2 or not 0 <= M <= pos.numel() or M > slot.numel():
         raise ValueError(f"{M} rows of {pos.numel()} positions and {slot.numel()} sequences, block table {tuple(block_table.shape)}")
-    return DlKv8Rows(pos.data_ptr(), slot.data_ptr(), block_table.data_ptr(), M, block_table.shape[0], block_table.shape[1])
+    return pos.data_ptr(), slot.data_ptr(), block_table.data_ptr(), M, *block_table.shape
 
 
 def _kv8_matrix(t: torch.Tensor, M: int, cols: int, cache: Kv8Cache, what: str) -> int:
     """Row stride of [>= M][cols] (neighbouring values of a row lie side by side)."""
-    if t.dim() != 2 or t.shape[0] < M or t.shape[1] != cols or t.device != cache.device or t.stride(1) != 1:
+    if t.dim() != 2 or t.size(0) < M or t.size(1) != cols or t.get_device() != cache.index or t.stride(1) != 1:
         raise ValueError(f"{what} {tuple(t.shape)} on {t.device}: at least {M} rows of {cols} values on {cache.device} are wanted")
-    return t.stride(0) if t.shape[0] > 1 else cols
+    return t.stride(0) if t.size(0) > 1 else cols
 
 
 def kv8_write(qkv: torch.Tensor, M: int, n_heads: int, freqs: Optional[torch.Tensor], pos, slot, block_table, q_out: Optional[torch.Tensor],
@@ -316,9 +318,9 @@ def kv8_write(qkv: torch.Tensor, M: int, n_heads: int, freqs: Optional[torch.Ten
     ldq = _kv8_matrix(q_out, M, n_heads * hs, cache, "q_out") if n_heads else 0
     if qkv.dtype is not torch.float32 or (n_heads and q_out.dtype is not torch.float32):
         raise ValueError("qkv and q_out are f32")
-    if freqs is not None and (freqs.dtype is not torch.float32 or freqs.device != cache.device or freqs.numel() != hs // 2 or not freqs.is_contiguous()):
+    if freqs is not None and (freqs.dtype is not torch.float32 or freqs.get_device() != cache.index or freqs.numel() != hs // 2 or not freqs.is_contiguous()):
         raise ValueError(f"{hs // 2} f32 frequencies are wanted")
-    check(cuda_lib().dl_kv8_write(qkv.data_ptr(), ld, n_heads, _p(freqs), C.byref(rows), q_out.data_ptr() if n_heads else None, ldq, cache.ref,
+    check(cuda_lib().dl_kv8_write(qkv.data_ptr(), ld, n_heads, _p(freqs), *rows, q_out.data_ptr() if n_heads else None, ldq, cache.ref,
                                   1 if pdl else 0, _stream()), "dl_kv8_write")
     lib.count_launch()
 
@@ -331,7 +333,7 @@ def kv8_read(M: int, pos, slot, block_table, cache: Kv8Cache, k_out: torch.Tenso
     ld = _kv8_matrix(k_out, M, cols, cache, "k_out")
     if _kv8_matrix(v_out, M, cols, cache, "v_out") != ld or k_out.dtype is not v_out.dtype or k_out.dtype not in _KV8_TYPES:
         raise ValueError("k_out and v_out are f32, fp16 or bf16, alike in type and row stride")
-    check(cuda_lib().dl_kv8_read(C.byref(rows), cache.ref, k_out.data_ptr(), v_out.data_ptr(), ld, _KV8_TYPES[k_out.dtype], 1 if pdl else 0, _stream()),
+    check(cuda_lib().dl_kv8_read(*rows, cache.ref, k_out.data_ptr(), v_out.data_ptr(), ld, _KV8_TYPES[k_out.dtype], 1 if pdl else 0, _stream()),
           "dl_kv8_read")
     lib.count_launch()
 
@@ -348,14 +350,23 @@ def _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out):
         if y_out.dtype not in _KV8_TYPES:
             raise ValueError("y_out is f32, fp16 or bf16")
         y_type = _KV8_TYPES[y_out.dtype]
-    if xq_out is not None and xq_out.numel() < xq_bytes(cols, out_mcap) or xh_out is not None and xh_out.numel() < xh_bytes(cols, out_mcap):
-        raise ValueError(f"slabs smaller than {out_mcap} rows of {cols} values")
+    for slab, need in ((xq_out, xq_bytes), (xh_out, xh_bytes)):
+        if slab is not None and (out_mcap < M or slab.get_device() != cache.index or not slab.is_contiguous() or slab.numel() * slab.element_size() < need(cols, out_mcap)):
+            raise ValueError(f"slabs of {out_mcap} rows of {cols} values on {cache.device} are wanted")
     return ldq, ldy, y_type
 
 
-def kv8_attention_splits(M: int, n_heads: int, n_kv_heads: int, max_pages: int, n_sms: int = 148) -> int:
-    """Shares of the longest context that kv8_attention is given for M rows (a row takes no more than its own context is worth)."""
-    return int(max(1, min(n_sms // max(1, M * n_kv_heads), max_pages // 8, 32)))
+def kv8_attention_splits(M: int, n_heads: int, n_kv_heads: int, max_pages: int) -> int:
+    """Shares of the longest context that kv8_attention is given for M rows: some 256 CTAs, eight pages each or more (a row takes no more than its own
+    context is worth; 8 kv heads, us with one split / this many / twice as many: one row of 100003 tokens 620 / 40 / 54, 8 rows of 2000 15.0 / 10.4 / 10.5,
+    32 rows of 3000 31.3 / 31.3 / 38.8)."""
+    groups = 2 if n_heads > 8 * n_kv_heads else 1
+    return max(1, min(256 // max(1, M * n_kv_heads * groups), max_pages // 8, 48))
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(M: int, n_heads: int, head_size: int, n_splits: int) -> int:
+    return attention_scratch_bytes(M, n_heads, head_size, n_splits)
 
 
 def kv8_attention(q, M: int, n_heads: int, pos, slot, block_table, cache: Kv8Cache, n_splits: int, scratch, xq_out=None, xh_out=None, out_mcap: int = 0,
@@ -364,11 +375,11 @@ def kv8_attention(q, M: int, n_heads: int, pos, slot, block_table, cache: Kv8Cac
     on two streams, or in two graphs -- need scratches of their own."""
     rows = _kv8_rows(M, pos, slot, block_table, cache)
     ldq, ldy, y_type = _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out)
-    if n_splits > 1 and (scratch is None or scratch.device != cache.device or scratch.numel() * scratch.element_size() < attention_scratch_bytes(M, n_heads, cache.head_size, n_splits)):
+    if n_splits > 1 and (scratch is None or scratch.get_device() != cache.index or not scratch.is_contiguous() or scratch.numel() * scratch.element_size() < _scratch_bytes(M, n_heads, cache.head_size, n_splits)):
         raise ValueError(f"{n_splits} splits of {M} rows need attention_scratch_bytes() of scratch on the cache's device")
-    if row_skip is not None and (row_skip.dtype is not torch.int32 or row_skip.device != cache.device or row_skip.numel() < M or not row_skip.is_contiguous()):
+    if row_skip is not None and (row_skip.dtype is not torch.int32 or row_skip.get_device() != cache.index or row_skip.numel() < M or not row_skip.is_contiguous()):
         raise ValueError("row_skip is a contiguous int32 tensor of at least M values")
-    check(cuda_lib().dl_kv8_attention(q.data_ptr(), ldq, n_heads, C.byref(rows), cache.ref, n_splits, _p(scratch), _p(xq_out), _p(xh_out), out_mcap,
+    check(cuda_lib().dl_kv8_attention(q.data_ptr(), ldq, n_heads, *rows, cache.ref, n_splits, _p(scratch), _p(xq_out), _p(xh_out), out_mcap,
                                       _p(y_out), ldy, y_type, _p(row_skip), 1 if pdl else 0, _stream()), "dl_kv8_attention")
     lib.count_launch()
 
@@ -394,17 +405,17 @@ def kv8_attention_prefill(q, M: int, n_heads: int, pos, slot, block_table, meta,
     outside are not touched.  workspace: kv8_prefill_workspace(), for one launch at a time."""
     rows = _kv8_rows(M, pos, slot, block_table, cache)
     ldq, ldy, y_type = _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out)
-    if meta.dtype is not torch.int32 or meta.device != cache.device or not meta.is_contiguous() or meta.numel() < 3:
+    if meta.dtype is not torch.int32 or meta.get_device() != cache.index or not meta.is_contiguous() or meta.numel() < 3:
         raise ValueError("meta is a contiguous int32 tensor [n_seg, begin, end, ...]")
     k16 = v16 = meta16 = None
     if workspace is not None:
         k16, v16, meta16 = workspace
         if k16.shape != cache.k.shape or v16.shape != cache.k.shape or k16.dtype is not torch.float16 or v16.dtype is not torch.float16 \
-                or k16.device != cache.device or v16.device != cache.device or meta16.device != cache.device \
+                or not k16.get_device() == v16.get_device() == meta16.get_device() == cache.index \
                 or not k16.is_contiguous() or not v16.is_contiguous() or meta16.dtype is not torch.int32 or meta16.numel() < 17 or not meta16.is_contiguous():
             raise ValueError("the workspace is not one of kv8_prefill_workspace() for this cache")
         k16, v16, meta16 = k16.data_ptr(), v16.data_ptr(), meta16.data_ptr()
-    check(cuda_lib().dl_kv8_attention_prefill(q.data_ptr(), ldq, n_heads, C.byref(rows), meta.data_ptr(), cache.ref, k16, v16, meta16, _p(xq_out), _p(xh_out),
+    check(cuda_lib().dl_kv8_attention_prefill(q.data_ptr(), ldq, n_heads, *rows, meta.data_ptr(), cache.ref, k16, v16, meta16, _p(xq_out), _p(xh_out),
                                               out_mcap, _p(y_out), ldy, y_type, 1 if pdl else 0, _stream()), "dl_kv8_attention_prefill")
     lib.count_launch()
 

@@ -94,12 +94,6 @@ class DlKv8Cache(C.Structure):
                 ("n_pages", C.c_int), ("n_kv_heads", C.c_int), ("head_size", C.c_int)]
 
 
-class DlKv8Rows(C.Structure):
-    """Mirror of ``DlKv8Rows``."""
-    _fields_ = [("pos", C.c_void_p), ("slot", C.c_void_p), ("block_table", C.c_void_p),
-                ("M", C.c_int), ("n_slots", C.c_int), ("max_pages", C.c_int)]
-
-
 class DlDecodeLayer(C.Structure):
     """Mirror of ``DlDecodeLayer`` (per-layer device pointers of the persistent decode kernel)."""
     _fields_ = [("qkv", C.c_void_p), ("wo", C.c_void_p), ("w13", C.c_void_p), ("w2", C.c_void_p),
@@ -205,10 +199,11 @@ def cuda_lib():
     L.dl_ipc_close.argtypes = [vp]
     L.dl_ipc_free.argtypes = [vp]
     L.dl_peer_barrier.argtypes = [C.POINTER(vp), vp, i32, i32, u32, vp]
-    L.dl_kv8_write.argtypes = [vp, i64, i32, vp, vp, vp, i64, vp, i32, vp]
-    L.dl_kv8_read.argtypes = [vp, vp, vp, vp, i64, i32, i32, vp]
-    L.dl_kv8_attention.argtypes = [vp, i64, i32, vp, vp, i32, vp, vp, vp, i32, vp, i64, i32, vp, i32, vp]
-    L.dl_kv8_attention_prefill.argtypes = [vp, i64, i32, vp, vp, vp, vp, vp, vp, vp, vp, i32, vp, i64, i32, i32, vp]
+    rows = [vp, vp, vp, i32, i32, i32]
+    L.dl_kv8_write.argtypes = [vp, i64, i32, vp, *rows, vp, i64, vp, i32, vp]
+    L.dl_kv8_read.argtypes = [*rows, vp, vp, vp, i64, i32, i32, vp]
+    L.dl_kv8_attention.argtypes = [vp, i64, i32, *rows, vp, i32, vp, vp, vp, i32, vp, i64, i32, vp, i32, vp]
+    L.dl_kv8_attention_prefill.argtypes = [vp, i64, i32, *rows, vp, vp, vp, vp, vp, vp, vp, i32, vp, i64, i32, i32, vp]
     for name in ("dl_kv8_write", "dl_kv8_read", "dl_kv8_attention", "dl_kv8_attention_prefill"):
         getattr(L, name).restype = i32
     L.dl_f32_rope_kv.argtypes = [vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp, vp, vp, i32, vp]

@@ -218,30 +218,24 @@ typedef struct {
     float* v_scale;
     int n_pages, n_kv_heads, head_size;      /* head_size 32, 64 or 128 */
 } DlKv8Cache;
-/* The rows of a batch: row m is position pos[m] of sequence slot[m], whose page i is block_table[slot * max_pages + i].  A row with a negative position
- * has no token: nothing is written or read, attention gives zeros.  Sequences, positions and pages that are not in the tables are not followed: nothing
- * is written, what is read or attended to is NaN. */
-typedef struct {
-    const int* pos;            /* device, [M] */
-    const int* slot;
-    const int* block_table;    /* device, [n_slots][max_pages] */
-    int M, n_slots, max_pages;
-} DlKv8Rows;
+/* The rows of a batch (device arrays): row m is position pos[m] of sequence slot[m], whose page i is block_table[slot * max_pages + i], of n_slots sequences.  A row
+ * with a negative position has no token: nothing is written or read, attention gives zeros.  Sequences, positions and pages that are not in the tables are not
+ * followed: nothing is written, what is read or attended to is NaN. */
 /* merged rows q | k | v (row stride ld_qkv): rotary positions on the n_heads query heads and the key heads (pairs of neighbouring values; freqs NULL: none),
  * queries to q_out (row stride ld_q), keys and values into their pages.  Keys are turned in 64 bits and rounded once, so that their codes do not depend on the
  * order of anything.  Rows of one place (slot, position) have to hold the same values (reference: OP_ROPE_LLAMA + OP_SHIFT, nn-cpu-ops.cpp:1090-1120,1253-1275) */
-int dl_kv8_write(const float* qkv, long long ld_qkv, int n_heads, const float* freqs, const DlKv8Rows* rows /*host*/, float* q_out, long long ld_q,
+int dl_kv8_write(const float* qkv, long long ld_qkv, int n_heads, const float* freqs, const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, float* q_out, long long ld_q,
                  const DlKv8Cache* cache /*host*/, int pdl, void* stream);
 /* the rows' keys and values out of their pages: k_out / v_out [M][n_kv_heads * head_size] of DL_KV8_* (row stride ld), code * scale rounded once */
-int dl_kv8_read(const DlKv8Rows* rows /*host*/, const DlKv8Cache* cache /*host*/, void* k_out, void* v_out, long long ld, int out_type, int pdl, void* stream);
+int dl_kv8_read(const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const DlKv8Cache* cache /*host*/, void* k_out, void* v_out, long long ld, int out_type, int pdl, void* stream);
 /* dl_attention over the 8-bit cache: at most 16 query heads for each key/value head; y_out of DL_KV8_*.  scratch: dl_attention_scratch_bytes(), zeroed once; launches
  * that may run at the same time need scratches of their own */
-int dl_kv8_attention(const float* q, long long ldq, int n_heads, const DlKv8Rows* rows /*host*/, const DlKv8Cache* cache /*host*/, int n_splits, void* scratch,
+int dl_kv8_attention(const float* q, long long ldq, int n_heads, const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const DlKv8Cache* cache /*host*/, int n_splits, void* scratch,
                      uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, const int* row_skip, int pdl, void* stream);
 /* dl_attention_prefill over the 8-bit cache (meta as there; a segment of which a sequence, position or page is not in the tables: NaN in the rows that see it, or in
  * all of its rows).  k16 / v16 / meta16: NULL, or a workspace for one launch at a time, fp16 [n_pages][n_kv_heads][32][128] twice and int[17]: heads of 128
  * with more than 4096 rows times heads are then widened once, and multiplied on tcgen05 (keys and values beyond fp16's range saturate) */
-int dl_kv8_attention_prefill(const float* q, long long ldq, int n_heads, const DlKv8Rows* rows /*host*/, const int* meta /*device*/, const DlKv8Cache* cache /*host*/,
+int dl_kv8_attention_prefill(const float* q, long long ldq, int n_heads, const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const int* meta /*device*/, const DlKv8Cache* cache /*host*/,
                              void* k16, void* v16, int* meta16, uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, int pdl,
                              void* stream);
 
