@@ -13,7 +13,8 @@ Options: --buffer-float-type {f32,f16,q40,q80}, --workers host:port ..., --port,
 --gpu-index, --gpu-segments a:b, --net-turbo {0,1}; unknown options raise (src/app.cpp:131-133).
 New here: --max-batch (rows per forward / concurrent users), --n-slots, --device {auto,cuda,cpu},
 --api-backend {native,python} (dllama-api front end: the C++ epoll server or the Python one),
---dtype {bfloat16,float32} (model directories, i.e. config.json + model.safetensors, chosen by models/registry.py).
+--dtype {bfloat16,float32} (model directories, i.e. config.json + model.safetensors, chosen by models/registry.py),
+--kv-cache {f16,q8} (Q40 models on a GPU: keys and values as fp16, or as int8 with a scale for each token and head in half the memory).
 
 Multi-GPU: every node is one process on one GPU of the same NVSwitch box.  Two equivalent ways to
 start them: (a) the reference's way -- ``dllama worker --port P`` per extra GPU, then the root with
@@ -63,6 +64,7 @@ class AppArgs:
     n_slots: int = 0
     device: str = "auto"
     api_backend: str = "native"
+    kv_cache: str = "f16"       # Q40 models on a GPU: f16, or q8 (int8 with a scale for each token and key/value head)
     dtype: str = "bfloat16"     # model directories: bfloat16 (weights, caches, matmul operands) or float32
     benchmark: bool = False
 
@@ -120,6 +122,10 @@ class AppArgs:
                 if value not in ("bfloat16", "float32"):
                     raise ValueError(f"Invalid dtype: {value}")
                 a.dtype = value
+            elif name == "--kv-cache":
+                if value not in ("f16", "q8"):
+                    raise ValueError(f"Invalid KV cache type: {value}")
+                a.kv_cache = value
             elif name == "--api-backend":
                 if value not in ("native", "python"):
                     raise ValueError(f"Invalid API backend: {value}")
@@ -142,6 +148,7 @@ Options:
   --dtype {bfloat16,float32}   (model directories: config.json + model.safetensors)
   --buffer-float-type {f32,f16,q40,q80}   --max-seq-len <n>   --temperature <f> --topp <f> --seed <n>
   --workers <host:port> ...   --port <n>   --chat-template {llama2,llama3,deepSeek3}
+  --kv-cache {f16,q8}   (Q40 models on a GPU: tokens of a conversation in 16 or 8 bits)
   --max-batch <rows>  --n-slots <sequences>  --gpu-index <i>  --device {auto,cuda,cpu,cpu-oracle}
   --api-backend {native,python}   (dllama-api: C++ epoll front end, or the Python one)
   --nthreads <n>  threads of the CPU backend (no GPU); --gpu-segments / --net-turbo are accepted for compatibility."""
@@ -184,7 +191,7 @@ def dial_workers(args: AppArgs, master_port: int) -> int:
         with socket.create_connection((host, port), timeout=60) as s:
             _send_msg(s, {"rank": i + 1, "world": world, "master_addr": "127.0.0.1", "master_port": master_port,
                           "model": os.path.abspath(args.model_path), "max_seq_len": args.max_seq_len,
-                          "max_batch": args.max_batch, "n_slots": args.n_slots, "sync_type": args.sync_type,
+                          "max_batch": args.max_batch, "n_slots": args.n_slots, "sync_type": args.sync_type, "kv_cache": args.kv_cache,
                           "ctl": f"{os.getpid()}"})
             ack = _recv_msg(s)
             if not ack.get("ok"):
@@ -219,9 +226,11 @@ def use_cuda_device(device: str) -> bool:
 
 def build_engine(model_path: str, rank: int, world: int, max_batch: int, n_slots: int, max_seq_len: int,
                  sync_type: int, device: str = "auto", gpu_index: int = -1, workers=(), n_threads: int = 0,
-                 dtype: str = "bfloat16"):
+                 dtype: str = "bfloat16", kv_cache: str = "f16"):
     import torch
     from ..models import registry
+    if kv_cache != "f16" and (registry.is_model_dir(model_path) or not use_cuda_device(device)):
+        raise ValueError("--kv-cache q8 is for Q40 models on a GPU")
     if registry.is_model_dir(model_path):
         # a model directory (config.json + model.safetensors): the engine its architecture names, in --dtype
         if not use_cuda_device(device):
@@ -248,7 +257,9 @@ def build_engine(model_path: str, rank: int, world: int, max_batch: int, n_slots
         # bucket_rows: the CLI and the API server run arbitrary batch shapes (prompt chunks, changing user
         # counts); padding them to powers of two bounds the number of CUDA graphs (same flag on every rank)
         return LlamaEngine(model_path, rank=rank, world=world, max_rows=max_batch, n_slots=slots,
-                           max_seq_len=seq_len, sync_q80=True, bucket_rows=True)
+                           max_seq_len=seq_len, sync_q80=True, bucket_rows=True, kv_dtype=torch.int8 if kv_cache == "q8" else torch.float16)
+    if use_cuda and kv_cache != "f16":
+        raise ValueError("--kv-cache q8 is for Q40 models on a GPU")
     if use_cuda:
         # f32 / f16 weights with an f32 buffer: the library path (cuBLAS + NCCL), same engine surface
         from ..models.f32_engine import F32Engine
@@ -313,7 +324,7 @@ def run_worker_app(args: AppArgs):
                           MASTER_ADDR=cfg["master_addr"], MASTER_PORT=str(cfg["master_port"]))
         rank, world, _ = init_distributed()
         engine = build_engine(cfg["model"], rank, world, cfg["max_batch"], cfg["n_slots"], cfg["max_seq_len"],
-                              cfg["sync_type"], "cuda", -1)
+                              cfg["sync_type"], "cuda", -1, kv_cache=cfg.get("kv_cache", "f16"))
         ctl = ControlChannel(cfg["ctl"], rank, world, cfg["max_batch"])
         print("🚁 Worker is ready", flush=True)
         worker_loop(engine, ctl)
@@ -342,14 +353,14 @@ class InferenceContext:
         print(f"📄 SpecialVocabSize: {self.tokenizer.special_vocab_size}")
         self.engine = build_engine(args.model_path, self.rank, self.world, args.max_batch, args.n_slots,
                                    args.max_seq_len, args.sync_type, args.device, args.gpu_index, args.workers,
-                                   args.n_threads, args.dtype)
+                                   args.n_threads, args.dtype, args.kv_cache)
         self.header = self.engine.h
         print(self.header.describe(), flush=True)
         try:
             from ..models.memory import describe, required_memory
             print(describe(required_memory(self.header, max(1, getattr(self.engine, "world", 1)), self.engine.max_rows,
                                            self.engine.n_slots, self.engine.seq_len,
-                                           "cuda" if self.engine.device.type == "cuda" else "cpu")), flush=True)
+                                           "cuda" if self.engine.device.type == "cuda" else "cpu", args.kv_cache)), flush=True)
         except Exception as e:                 # the estimate is informational: never let it stop a run
             print(f"📀 RequiredMemory: n/a ({e})", flush=True)
         if self.tokenizer.vocab_size != self.header.vocab_size:

@@ -116,10 +116,14 @@ class LlamaEngine:
         self.tokens, self.pos, self.slot, self.row_skip, self.meta = (self.desc[i] for i in range(5))
         self._hd = self.h_desc.numpy()                                   # host view, filled by set_batch
         self._desc3, self._h_desc3 = self.desc[:3], self.h_desc[:3]      # tokens | pos | slot: all a batch without prompt chunks needs
-        self.prefill_attention = kv_dtype == torch.float16 and self.hs in (64, 128)
+        # kv_dtype int8: codes with an f32 scale for each token and key/value head (ops.kernels.Kv8Cache), half the bytes of fp16.  The scales want
+        # whole lines, so q|k|v leave the matmul as f32 rows and kv8_write turns, quantises and stores them: one launch more per layer
+        self.kv8 = kv_dtype == torch.int8
+        self.prefill_attention = self.kv8 or (kv_dtype == torch.float16 and self.hs in (64, 128))
         self._chunk = False
         self.x = [torch.zeros(R, h.dim, dtype=torch.float32, device=dev) for _ in range(2)]
         self.q = torch.zeros(R, self.q_loc, dtype=torch.float32, device=dev)
+        self.qkv = torch.zeros(R, self.qkv_d, dtype=torch.float32, device=dev) if self.kv8 else None
         self.xq_dim = K.alloc_xq(h.dim, GEMV_MAX_M, dev)
         self.xq_att = K.alloc_xq(self.q_loc, GEMV_MAX_M, dev)
         self.xq_hid = K.alloc_xq(self.hid_loc, GEMV_MAX_M, dev)
@@ -188,6 +192,9 @@ class LlamaEngine:
         # the page pool is shared by all sequences and grows on demand, so it does not have to cover
         # n_slots x max_seq_len (Llama-3.1 headers say 131072): cap it at 85 % of the free HBM
         page_bytes = 2 * h.n_layers * self.n_kv_loc * PAGE * self.hs * torch.empty((), dtype=kv_dtype).element_size()
+        widen = self.kv8 and self.hs == 128 and R * self.n_heads_loc > K.KV8_WIDEN_MIN_WORK       # long prompt chunks: fp16 pages of one layer
+        if self.kv8:
+            page_bytes = h.n_layers * K.kv8_page_bytes(self.n_kv_loc, self.hs) + (4 * self.n_kv_loc * PAGE * self.hs if widen else 0)
         if n_pages is None and dev.type == "cuda":
             free_b, _ = torch.cuda.mem_get_info(dev)
             fit = int(0.85 * free_b) // page_bytes
@@ -208,8 +215,13 @@ class LlamaEngine:
         self.block_table = torch.zeros(n_slots, self.max_pages, dtype=torch.int32, device=dev)
         self.h_block_table = torch.zeros(n_slots, self.max_pages, dtype=torch.int32).pin_memory()
         kv_shape = (self.n_pages, self.n_kv_loc, PAGE, self.hs)
-        self.k_cache = [torch.zeros(kv_shape, dtype=kv_dtype, device=dev) for _ in range(h.n_layers)]
-        self.v_cache = [torch.zeros(kv_shape, dtype=kv_dtype, device=dev) for _ in range(h.n_layers)]
+        if self.kv8:
+            self.kv8_cache = [K.alloc_kv8(self.n_pages, self.n_kv_loc, self.hs, dev) for _ in range(h.n_layers)]
+            self.kv8_work = K.kv8_prefill_workspace(self.n_pages, self.n_kv_loc, self.hs, R, dev) if widen else None
+            self.k_cache, self.v_cache = [c.k for c in self.kv8_cache], [c.v for c in self.kv8_cache]
+        else:
+            self.k_cache = [torch.zeros(kv_shape, dtype=kv_dtype, device=dev) for _ in range(h.n_layers)]
+            self.v_cache = [torch.zeros(kv_shape, dtype=kv_dtype, device=dev) for _ in range(h.n_layers)]
         self._pad_slot, self._Mp = -1, 0
         if bucket_rows:
             self._pad_slot = n_slots - 1
@@ -538,14 +550,24 @@ class LlamaEngine:
         pending = None
         for l, W in enumerate(self.layers):
             # --- attention block ---
-            epi = K.epi_qkv_rope(self.q, self.q_loc, self.kv_loc, self.hs, self.rope_freqs, self.pos, self.slot,
-                                 self.block_table, self.max_pages, self.n_kv_loc, self.k_cache[l], self.v_cache[l])
-            norm_then(W["rms_att"], pending, l, W["qkv"], self.qkv_d, EPI_QKV_ROPE, epi)
-            if chunk != 2:
+            if self.kv8:
+                norm_then(W["rms_att"], pending, l, W["qkv"], self.qkv_d, EPI_STORE, K.epi_store([self.qkv.data_ptr()], self.qkv_d))
+                where, cache = (self.pos, self.slot, self.block_table), self.kv8_cache[l]
+                K.kv8_write(self.qkv, M, self.n_heads_loc, self.rope_freqs, *where, self.q, cache, pdl=pdl)
+                if chunk != 2:
+                    K.kv8_attention(self.q, M, self.n_heads_loc, *where, cache, n_splits, self.att_scratch, xq(self.xq_att), xh(self.xh_att), mcap,
+                                    row_skip=self.row_skip if chunk else None, pdl=pdl)
+                if chunk:
+                    K.kv8_attention_prefill(self.q, M, self.n_heads_loc, *where, self.meta, cache, self.kv8_work, xq(self.xq_att), xh(self.xh_att), mcap, pdl=pdl)
+            else:
+                epi = K.epi_qkv_rope(self.q, self.q_loc, self.kv_loc, self.hs, self.rope_freqs, self.pos, self.slot,
+                                     self.block_table, self.max_pages, self.n_kv_loc, self.k_cache[l], self.v_cache[l])
+                norm_then(W["rms_att"], pending, l, W["qkv"], self.qkv_d, EPI_QKV_ROPE, epi)
+            if chunk != 2 and not self.kv8:
                 K.attention(self.q, M, self.n_heads_loc, self.n_kv_loc, self.hs, self.k_cache[l], self.v_cache[l], self.pos,
                             self.slot, self.block_table, self.max_pages, n_splits, self.att_scratch, xq(self.xq_att),
                             xh(self.xh_att), mcap, pdl=pdl, row_skip=self.row_skip if chunk else None)
-            if chunk:        # prompt-chunk rows (skipped above) on the tensor cores
+            if chunk and not self.kv8:        # prompt-chunk rows (skipped above) on the tensor cores
                 K.attention_prefill(self.q, M, self.n_heads_loc, self.n_kv_loc, self.hs, self.k_cache[l], self.v_cache[l],
                                     self.pos, self.slot, self.block_table, self.max_pages, self.meta, xq(self.xq_att),
                                     xh(self.xh_att), mcap, pdl=pdl, tc=self.hs == 128 and M >= PREFILL_TC_MIN_ROWS)
@@ -575,6 +597,8 @@ class LlamaEngine:
             K.wait_flags(self.flags_log_local, N, sc, 1, 0)
 
     def _attention_splits(self, M: int) -> int:
+        if self.kv8:
+            return K.kv8_attention_splits(M, self.n_heads_loc, self.n_kv_loc, self.max_pages)
         ctas = M * self.n_kv_loc
         want = max(1, self.n_sms // max(1, ctas))
         max_by_ctx = max(1, self.max_pages // 8)           # >= 8 pages per split; the kernel uses fewer splits for short rows
@@ -801,6 +825,18 @@ class LlamaEngine:
             idx = (first_step + i) % self.history_cap
             out[i] = raw[idx * M: idx * M + M]
         return out
+
+    def read_cache(self, layer: int, slot: int, n_tokens: int, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values of a sequence's first n_tokens, [n_tokens][this rank's key/value heads * head size]: to keep a conversation outside of its pages."""
+        assert 0 < n_tokens <= int(self.pages.n_used[slot]) * PAGE
+        if not self.kv8:
+            pages = torch.from_numpy(self.pages.table[slot, :(n_tokens + PAGE - 1) // PAGE].astype(np.int64)).to(self.device)
+            return tuple(c[layer][pages].transpose(1, 2).reshape(-1, self.kv_loc)[:n_tokens].to(dtype) for c in (self.k_cache, self.v_cache))
+        self._sync_block_table()
+        k, v = (torch.empty(n_tokens, self.kv_loc, dtype=dtype, device=self.device) for _ in range(2))
+        pos = torch.arange(n_tokens, dtype=torch.int32, device=self.device)
+        K.kv8_read(n_tokens, pos, torch.full_like(pos, slot), self.block_table, self.kv8_cache[layer], k, v)
+        return k, v
 
     def current_step(self) -> int:
         t = self.symm.tensor(self._off_flags + 96, (1,), torch.int32)

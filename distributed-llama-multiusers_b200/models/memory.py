@@ -14,9 +14,9 @@ B200_HBM_BYTES = 180 * 10 ** 9
 
 
 def required_memory(h: LlmHeader, n_nodes: int = 1, max_rows: int = 32, n_slots: int = 4, seq_len: int = 0,
-                    backend: str = "cuda") -> Dict[str, int]:
+                    backend: str = "cuda", kv_cache: str = "f16") -> Dict[str, int]:
     """Bytes one node needs.  backend "cuda": Q40T tiles (same 4.5 bits/weight as the file, row count padded to 128),
-    replicated f32 embedding, fp16 paged KV; backend "cpu": file-layout slices, embedding on the root only, f32 KV."""
+    replicated f32 embedding, fp16 paged KV (kv_cache "q8": int8 codes and an f32 scale for each token and head); backend "cpu": file-layout slices, embedding on the root only, f32 KV."""
     N = n_nodes
     seq = seq_len or h.seq_len
     wt = h.weight_type
@@ -34,10 +34,12 @@ def required_memory(h: LlmHeader, n_nodes: int = 1, max_rows: int = 32, n_slots:
     weights = L * per_layer + dim * 4 + mat(vocab // N, dim)
     embedding = vocab * dim * 4
     kv_elem = 2 if backend == "cuda" else 4
-    kv_cache = 2 * L * n_slots * seq * (kv // N) * kv_elem
+    kv_bytes = 2 * L * n_slots * seq * (kv // N) * kv_elem
+    if backend == "cuda" and kv_cache == "q8":
+        kv_bytes = 2 * L * n_slots * seq * (kv // N + h.n_kv_heads // N * 4)
     # residual stream, normalised / quantised activations, q/k/v, hidden, logits, exchange area (N slices per sync)
     act = max_rows * (4 * dim * 4 + (dim + 2 * kv) // N * 4 + 3 * (hid // N) * 4 + vocab * 4 + 2 * N * dim * 8)
-    out = {"weights": weights, "embedding": embedding, "kv_cache": kv_cache, "activations": act}
+    out = {"weights": weights, "embedding": embedding, "kv_cache": kv_bytes, "activations": act}
     # fp16 copy of the layer matrices for prompt-sized batches (LlamaEngine prefill_wh="resident": 2 bytes per weight,
     # rows padded to 128); only engines that can see >= 768-row batches build it, and "auto" declines it when it would
     # take more than a quarter of the free memory

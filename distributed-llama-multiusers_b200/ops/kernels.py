@@ -250,6 +250,7 @@ def attention_prefill(q, M, n_heads, n_kv_heads, head_size, k_cache, v_cache, po
 # ---- 8-bit token cache ----------------------------------------------------------------------------
 # int8 codes and one f32 scale for each token and key/value head: value = code * scale, scale = f32(amax / 127) of the token's line,
 # code = rint(x * f32(127 / amax)).  Arguments that a launch could not take raise ValueError; rows whose page is not in the tables read as NaN.
+_I32, _F32, _current_device = torch.int32, torch.float32, torch._C._cuda_getDevice
 _KV8_TYPES = {torch.float32: KV8_F32, torch.bfloat16: KV8_BF16, torch.float16: KV8_F16}
 
 
@@ -278,6 +279,9 @@ class Kv8Cache:
         return kv8_page_bytes(self.n_kv_heads, self.head_size) * self.n_pages
 
 
+KV8_WIDEN_MIN_WORK = 4096          # rows times heads above which kv8_attention_prefill uses a workspace (KV8_EXPAND_MIN_WORK in csrc/cuda/kv8_attention.cu)
+
+
 def kv8_page_bytes(n_kv_heads: int, head_size: int) -> int:
     """Bytes of one page of one layer: codes and scales of 32 keys and values."""
     return 2 * n_kv_heads * PAGE_SIZE * (head_size + 4)
@@ -291,21 +295,21 @@ def alloc_kv8(n_pages: int, n_kv_heads: int, head_size: int, device) -> Kv8Cache
 def _kv8_rows(M: int, pos: torch.Tensor, slot: torch.Tensor, block_table: torch.Tensor, cache: Kv8Cache):
     """The rows' arguments of the C functions."""
     d = cache.index
-    if d < 0 or d != torch._C._cuda_getDevice():
+    if d < 0 or d != _current_device():
         raise ValueError(f"the cache is on {cache.device}: the current device launches")
-    if not (pos.dtype is slot.dtype is block_table.dtype is torch.int32 and pos.get_device() == slot.get_device() == block_table.get_device() == d
+    if not (pos.dtype is slot.dtype is block_table.dtype is _I32 and pos.get_device() == slot.get_device() == block_table.get_device() == d
             and pos.is_contiguous() and slot.is_contiguous() and block_table.is_contiguous()):
         raise ValueError("pos, slot and block_table are contiguous int32 tensors on the cache's device")
     if block_table.dim() != 2 or not 0 <= M <= pos.numel() or M > slot.numel():
         raise ValueError(f"{M} rows of {pos.numel()} positions and {slot.numel()} sequences, block table {tuple(block_table.shape)}")
-    return pos.data_ptr(), slot.data_ptr(), block_table.data_ptr(), M, *block_table.shape
+    return pos.data_ptr(), slot.data_ptr(), block_table.data_ptr(), M, block_table.size(0), block_table.size(1)
 
 
 def _kv8_matrix(t: torch.Tensor, M: int, cols: int, cache: Kv8Cache, what: str) -> int:
     """Row stride of [>= M][cols] (neighbouring values of a row lie side by side)."""
     if t.dim() != 2 or t.size(0) < M or t.size(1) != cols or t.get_device() != cache.index or t.stride(1) != 1:
         raise ValueError(f"{what} {tuple(t.shape)} on {t.device}: at least {M} rows of {cols} values on {cache.device} are wanted")
-    return t.stride(0) if t.size(0) > 1 else cols
+    return t.stride(0) if M > 1 else cols
 
 
 def kv8_write(qkv: torch.Tensor, M: int, n_heads: int, freqs: Optional[torch.Tensor], pos, slot, block_table, q_out: Optional[torch.Tensor],
@@ -342,17 +346,17 @@ def _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out):
     """Row strides of q and y_out, type of y_out."""
     cols = n_heads * cache.head_size
     ldq = _kv8_matrix(q, M, cols, cache, "q")
-    if q.dtype is not torch.float32:
+    if q.dtype is not _F32:
         raise ValueError("q is f32")
     ldy, y_type = 0, KV8_F32
     if y_out is not None:
-        ldy = _kv8_matrix(y_out, M, cols, cache, "y_out")
-        if y_out.dtype not in _KV8_TYPES:
+        ldy, y_type = _kv8_matrix(y_out, M, cols, cache, "y_out"), _KV8_TYPES.get(y_out.dtype)
+        if y_type is None:
             raise ValueError("y_out is f32, fp16 or bf16")
-        y_type = _KV8_TYPES[y_out.dtype]
-    for slab, need in ((xq_out, xq_bytes), (xh_out, xh_bytes)):
-        if slab is not None and (out_mcap < M or slab.get_device() != cache.index or not slab.is_contiguous() or slab.numel() * slab.element_size() < need(cols, out_mcap)):
-            raise ValueError(f"slabs of {out_mcap} rows of {cols} values on {cache.device} are wanted")
+    if xq_out is not None or xh_out is not None:
+        for slab, need in ((xq_out, xq_bytes), (xh_out, xh_bytes)):
+            if slab is not None and (out_mcap < M or slab.get_device() != cache.index or not slab.is_contiguous() or slab.numel() * slab.element_size() < need(cols, out_mcap)):
+                raise ValueError(f"slabs of {out_mcap} rows of {cols} values on {cache.device} are wanted")
     return ldq, ldy, y_type
 
 
@@ -379,8 +383,12 @@ def kv8_attention(q, M: int, n_heads: int, pos, slot, block_table, cache: Kv8Cac
         raise ValueError(f"{n_splits} splits of {M} rows need attention_scratch_bytes() of scratch on the cache's device")
     if row_skip is not None and (row_skip.dtype is not torch.int32 or row_skip.get_device() != cache.index or row_skip.numel() < M or not row_skip.is_contiguous()):
         raise ValueError("row_skip is a contiguous int32 tensor of at least M values")
-    check(cuda_lib().dl_kv8_attention(q.data_ptr(), ldq, n_heads, *rows, cache.ref, n_splits, _p(scratch), _p(xq_out), _p(xh_out), out_mcap,
-                                      _p(y_out), ldy, y_type, _p(row_skip), 1 if pdl else 0, _stream()), "dl_kv8_attention")
+    rc = cuda_lib().dl_kv8_attention(q.data_ptr(), ldq, n_heads, *rows, cache.ref, n_splits, scratch if scratch is None else scratch.data_ptr(),
+                                     xq_out if xq_out is None else xq_out.data_ptr(), xh_out if xh_out is None else xh_out.data_ptr(), out_mcap,
+                                     y_out if y_out is None else y_out.data_ptr(), ldy, y_type, row_skip if row_skip is None else row_skip.data_ptr(),
+                                     1 if pdl else 0, torch._C._cuda_getCurrentRawStream(cache.index))
+    if rc:
+        check(rc, "dl_kv8_attention")
     lib.count_launch()
 
 

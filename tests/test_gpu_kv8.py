@@ -74,8 +74,9 @@ def _code(x):
     amax = x.abs().amax(-1)
     live = amax >= 2.0 ** -100
     bad = ~torch.isfinite(x).all(-1)
-    factor = torch.where(live & ~bad, 127.0 / amax, torch.zeros_like(amax))
-    scale = torch.where(live, amax / 127.0, torch.zeros_like(amax))
+    most = torch.full_like(amax, 127.0)                         # (number / tensor is a reciprocal and a product: two roundings)
+    factor = torch.where(live & ~bad, most / amax, torch.zeros_like(amax))
+    scale = torch.where(live, amax / most, torch.zeros_like(amax))
     codes = torch.round(torch.nan_to_num(x.double(), 0.0, 0.0, 0.0) * factor.double()[..., None]).to(torch.int8)
     return torch.where(bad[..., None], torch.zeros_like(codes), codes), torch.where(bad, torch.full_like(scale, math.nan), scale)
 
@@ -319,6 +320,19 @@ def test_attention_into_the_slabs(heads, hs):
     dq = _decode_xq(xq, heads * hs, 8, M)[0]
     got = y.cpu().numpy()
     np.testing.assert_allclose(dq, quant.q80_roundtrip(got), rtol=0, atol=np.abs(got).max() / 127 * 1.01)      # a code beside a border
+    from test_gpu_kernels import _decode_xh
+    xh = k.alloc_xh(heads * hs, 16, "cuda")
+    k.kv8_attention(q.cuda(), M, heads, *where, cache, 3, scratch, None, xh, 16)
+    np.testing.assert_allclose(_decode_xh(xh, heads * hs, 16, M), dq, rtol=2e-3, atol=1e-7)                      # the same codes, times the scale in fp16
+    # a prompt chunk's rows take the same places
+    n = 20
+    bt2 = torch.from_numpy(bt[1:2].copy()).cuda()
+    pos, slot, meta = torch.arange(700, 700 + n, dtype=torch.int32, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda"), _i32([1, 0, n])
+    qp = torch.randn(n, heads * hs, device="cuda")
+    xh, y = k.alloc_xh(heads * hs, 32, "cuda"), torch.zeros(n, heads * hs, device="cuda")
+    k.kv8_attention_prefill(qp, n, heads, pos, slot, bt2, meta, cache, xh_out=xh, out_mcap=32, y_out=y)
+    got = y.cpu().numpy()
+    np.testing.assert_allclose(_decode_xh(xh, heads * hs, 32, n), quant.q80_roundtrip(got), rtol=2e-3, atol=np.abs(got).max() / 127 * 1.01)
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -404,3 +418,120 @@ def test_attention_prefill_of_unusual_lines(workspace):
             for h in range(heads):
                 if not nan[m, h].any():
                     _near(y[m, h], ref[h], PROMPT_REL)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# together, as they are used
+# ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("heads,kv,hs", [(8, 2, 128), (16, 8, 64), (4, 2, 32)])
+def test_a_conversation(heads, kv, hs):
+    """A prompt in two chunks, tokens one by one beside another user's: what attention gives is the formula on what the cache reads back."""
+    k = K()
+    g = torch.Generator(device="cuda")
+    g.manual_seed(hs)
+    rng = np.random.default_rng(hs)
+    n, n_pages = 90, 12
+    bt = torch.from_numpy(rng.permutation(n_pages).astype(np.int32).reshape(2, 6)).cuda()
+    cache, freqs = k.alloc_kv8(n_pages, kv, hs, "cuda"), torch.from_numpy((10000.0 ** (-np.arange(0, hs, 2) / hs)).astype(np.float32)).cuda()
+    scratch = torch.zeros(k.attention_scratch_bytes(2, heads, hs, 2), dtype=torch.uint8, device="cuda")
+    seen = {}                                                    # rotated queries and outputs by (sequence, position)
+
+    def step(positions, slots, chunk):
+        M = len(positions)
+        qkv = torch.randn(M, (heads + 2 * kv) * hs, generator=g, device="cuda")
+        q, y = torch.zeros(M, heads * hs, device="cuda"), torch.zeros(M, heads * hs, device="cuda")
+        where = (_i32(positions), _i32(slots), bt)
+        k.kv8_write(qkv, M, heads, freqs, *where, q, cache)
+        if chunk:
+            k.kv8_attention_prefill(q, M, heads, *where, _i32([1, 0, M]), cache, y_out=y)
+        else:
+            k.kv8_attention(q, M, heads, *where, cache, 2, scratch, y_out=y)
+        for m, at in enumerate(zip(slots, positions)):
+            seen[at] = (q[m].cpu(), y[m].cpu(), chunk)
+
+    step(list(range(50)), [0] * 50, True)
+    step(list(range(50, n)), [0] * (n - 50), True)
+    step(list(range(17)), [1] * 17, True)
+    for i in range(40):
+        step([n + i, 17 + i], [0, 1], False)
+    lens = [n + 40, 57]
+    for s, T in enumerate(lens):
+        pos, slot = torch.arange(T, dtype=torch.int32, device="cuda"), torch.full((T,), s, dtype=torch.int32, device="cuda")
+        kk, vv = (torch.zeros(T, kv * hs, device="cuda") for _ in range(2))
+        k.kv8_read(T, pos, slot, bt, cache, kk, vv)
+        kk, vv = (x.double().cpu().view(T, kv, hs) for x in (kk, vv))
+        for p in range(T):
+            q, y, chunk = seen[s, p]
+            _near(y[None], _attention(q.view(heads, hs), kk[:p + 1], vv[:p + 1]).reshape(1, -1), PROMPT_REL if chunk else ATT_REL)
+
+
+def test_captured_replayed_and_on_other_streams():
+    """Two graphs with scratches of their own, replayed side by side on two streams, then again on new inputs; and eager calls on a side stream."""
+    k = K()
+    heads, kv, hs, positions, splits = 16, 2, 128, [1500, 40, 901], 6
+    M = len(positions)
+    bt, host, q, ref = _decode_case(heads, kv, hs, positions)
+    cache = k.Kv8Cache(*_dev(*host))
+    where = (_i32(positions), _i32(list(range(M))), torch.from_numpy(bt).cuda())
+    streams, graphs, qs, ys = [torch.cuda.Stream() for _ in range(2)], [], [], []
+    torch.cuda.synchronize()
+    for st in streams:
+        qs.append(torch.zeros(M, heads * hs, device="cuda"))
+        ys.append(torch.zeros(M, heads * hs, device="cuda"))
+        scratch = torch.zeros(k.attention_scratch_bytes(M, heads, hs, splits), dtype=torch.uint8, device="cuda")
+        with torch.cuda.stream(st):
+            st.wait_stream(torch.cuda.default_stream())
+            k.kv8_attention(qs[-1], M, heads, *where, cache, splits, scratch, y_out=ys[-1])       # (functions are loaded ahead of the capture)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            for _ in range(4):
+                k.kv8_attention(qs[-1], M, heads, *where, cache, splits, scratch, y_out=ys[-1])
+        graphs.append(graph)
+    for f in (1.0, -0.5):
+        for t in qs:
+            t.copy_(q.cuda() * f)
+        want = ref if f == 1.0 else torch.stack([_attention(f * q[m].view(heads, hs), _values(host[0], host[2], bt[m], p + 1), _values(host[1], host[3], bt[m], p + 1)).reshape(-1) for m, p in enumerate(positions)])
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for st, graph in zip(streams, graphs):
+                with torch.cuda.stream(st):
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(ys[0], ys[1])
+        _near(ys[0], want, ATT_REL)
+    st = streams[0]
+    with torch.cuda.stream(st):
+        kk, vv = (torch.zeros(M, kv * hs, dtype=torch.float16, device="cuda") for _ in range(2))
+        k.kv8_read(M, *where, cache, kk, vv)
+    st.synchronize()
+    for m, p in enumerate(positions):
+        assert torch.equal(kk[m].cpu().view(kv, hs), _values(host[0], host[2], bt[m], p + 1)[p].half())
+
+
+def test_far_pages_of_a_large_cache():
+    """Lines beyond 2^31 bytes of codes."""
+    k = K()
+    free, _ = torch.cuda.mem_get_info()
+    n_pages, kv, hs = 70000, 8, 128                              # 2.3 GB of codes of the keys, as many of the values
+    if free < 8 << 30:
+        pytest.skip("8 GB of device memory")
+    heads, T = 8, 100
+    cache = k.alloc_kv8(n_pages, kv, hs, "cuda")
+    bt = torch.tensor([[n_pages - 1, 5, n_pages - 2, n_pages - 7]], dtype=torch.int32, device="cuda")
+    pos, slot = torch.arange(T, dtype=torch.int32, device="cuda"), torch.zeros(T, dtype=torch.int32, device="cuda")
+    qkv = torch.randn(T, (heads + 2 * kv) * hs, device="cuda")
+    q, y = torch.zeros(T, heads * hs, device="cuda"), torch.zeros(1, heads * hs, device="cuda")
+    k.kv8_write(qkv, T, heads, None, pos, slot, bt, q, cache)
+    codes, scales = _code(qkv.cpu().view(T, -1, hs)[:, heads:])
+    held = (codes.double() * scales.double()[..., None])
+    kk, vv = (torch.zeros(T, kv * hs, device="cuda") for _ in range(2))
+    k.kv8_read(T, pos, slot, bt, cache, kk, vv)
+    assert torch.equal(kk.cpu().view(T, kv, hs), held[:, :kv].float()) and torch.equal(vv.cpu().view(T, kv, hs), held[:, kv:].float())
+    k.kv8_attention(q[T - 1:], 1, heads, pos[T - 1:], slot[:1], bt, cache, 1, None, y_out=y)
+    _near(y, _attention(q[T - 1].cpu().view(heads, hs), held[:, :kv], held[:, kv:]).reshape(1, -1), ATT_REL)
+    n = 20
+    yp = torch.zeros(n, heads * hs, device="cuda")
+    k.kv8_attention_prefill(q[T - n:], n, heads, pos[T - n:], slot[:n], bt, _i32([1, 0, n]), cache, y_out=yp)
+    for m in range(n):
+        _near(yp[m:m + 1], _attention(q[T - n + m].cpu().view(heads, hs), held[:T - n + m + 1, :kv], held[:T - n + m + 1, kv:]).reshape(1, -1), PROMPT_REL)
