@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
 // steady state takes no exchange for a running maximum and no rescaling.
 // ------------------------------------------------------------------------------------------------
 template <int HS, int ST>
-__global__ void __launch_bounds__(KA_WARPS * 32, HS == 128 ? 3 : 4) kv8_prompt_kernel(const __grid_constant__ Kv8AttArgs a) {
+__global__ void __launch_bounds__(KA_WARPS * 32, HS == 128 ? 2 : 4) kv8_prompt_kernel(const __grid_constant__ Kv8AttArgs a) {
     constexpr int CH = HS / 16, KS = HS / 32, NT = HS / 8, STAGE = KaStage<HS>::BYTES, CODES = KaStage<HS>::CODES;
     constexpr int SR = 16;                                                 // stacked rows of the CTA
     constexpr int TOP = 6;                                                 // the largest weight is below 2^(TOP + 1) units when the unit is chosen,
