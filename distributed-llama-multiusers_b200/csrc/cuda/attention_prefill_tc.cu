@@ -1,4 +1,4 @@
-// Causal attention for long prompt chunks on the 5th-gen tensor cores (head size 128): the same job as
+// Causal attention for long prompt chunks on the 5th-gen tensor cores (head size 128, over the widened 8-bit cache 64 too): the same job as
 // attention_prefill.cu (segments of consecutive positions of one sequence, listed in `meta`), with both products
 // as tcgen05.mma and the score / probability / output tiles in TENSOR MEMORY instead of registers.
 //
@@ -239,6 +239,18 @@ DL_DEVINL void pt_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t desc
         ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// ... of heads of 64: the first half tiles alone
+DL_DEVINL void pt_mma_ss4(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q, r;\n\t.reg .b32 x, y;\n\t.reg .b64 a, b;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.eq.b32 r, 0, 0;\n\t"
+        "add.u32 x, %1, 0; add.u32 y, %2, 0; mov.b64 a, {x, %3}; mov.b64 b, {y, %3}; @p tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, q;\n\t"
+        "add.u32 x, %1, 2; add.u32 y, %2, 2; mov.b64 a, {x, %3}; mov.b64 b, {y, %3}; @p tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, r;\n\t"
+        "add.u32 x, %1, 4; add.u32 y, %2, 4; mov.b64 a, {x, %3}; mov.b64 b, {y, %3}; @p tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, r;\n\t"
+        "add.u32 x, %1, 6; add.u32 y, %2, 6; mov.b64 a, {x, %3}; mov.b64 b, {y, %3}; @p tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, r;\n\t}"
+        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 // D += A B, A in tensor memory (8 columns per MMA), B MN-major (two 8-token groups of 1024 B per MMA)
 DL_DEVINL void pt_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -403,22 +415,25 @@ DL_DEVINL void pt_run_item(const PtLineArgs& a, const int (&run)[4], PtItem& it)
     it.first_page = max(it.first_page, it.j0 * (PT_KV / 32));
 }
 
-// Queries of 32 rows into the tile's K-major, swizzled image: lane i holds the address of row r0 + i; all in flight, a row a load
-template <bool LINES, typename Ready>
+// Queries of 32 rows into the tile's K-major, swizzled image: lane i holds the address of row r0 + i; all in flight, a row (two of heads of 64) a load
+template <bool LINES, int HS, typename Ready>
 DL_DEVINL void pt_load_rows(const float* mine, uint8_t* tile, int r0, Ready ready) {
-    const int lane = threadIdx.x & 31;
-    uint8_t* qd = tile + r0 * 128 + (lane >> 4) * 16384 + (lane & 1) * 8;
-    float4 x[32];
+    constexpr int PER = PT_HS / HS;
+    const int lane = threadIdx.x & 31, in = lane * 4 / HS, col = lane * 4 % HS;
+    uint8_t* qd = tile + (r0 + in) * 128 + (col >> 6) * 16384 + (lane & 1) * 8;
+    float4 x[32 / PER];
 #pragma unroll
-    for (int u = 0; u < 32; u++) x[u] = reinterpret_cast<const float4*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)mine, u))[lane];
+    for (int u = 0; u < 32; u += PER) x[u / PER] = reinterpret_cast<const float4*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)mine, u + in))[col >> 2];
     ready();
 #pragma unroll
-    for (int u = 0; u < 32; u++)                 // 16-byte piece c of a half row -> swizzled slot c ^ (row & 7)
-        *reinterpret_cast<uint2*>(qd + u * 128 + ((((lane >> 1) & 7) ^ (u & 7)) << 4)) = make_uint2(pt_pack2<LINES>(x[u].x, x[u].y), pt_pack2<LINES>(x[u].z, x[u].w));
+    for (int u = 0; u < 32; u += PER)            // 16-byte piece c of a half row -> swizzled slot c ^ (row & 7)
+        *reinterpret_cast<uint2*>(qd + u * 128 + ((((lane >> 1) & 7) ^ ((u + in) & 7)) << 4)) =
+            make_uint2(pt_pack2<LINES>(x[u / PER].x, x[u / PER].y), pt_pack2<LINES>(x[u / PER].z, x[u / PER].w));
     fence_proxy_async_smem();
 }
 
-template <bool LINES>
+// HS: head size; 64 (LINES: not) takes the first half of every tile and accumulator
+template <bool LINES, int HS = PT_HS>
 __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(const __grid_constant__ typename PtKernelArgs<LINES>::T a,
                                                                              const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -512,7 +527,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
     auto row_of = [&](const PtItem& it, int t, int row) -> const float* {      // the queries of a tile's row (rows that are not there: of the last one)
         const int r = min((t ? it.row0[1] : it.row0[0]) + row, it.rows - 1);
         if constexpr (LINES) return a.w.q + (size_t)a.tile_rows[it.begin + r / a.rep] * a.w.ldq + (it.kvh * a.rep + r % a.rep) * PT_HS;
-        else return a.q + (size_t)(it.begin + r) * a.n_heads * PT_HS + (t ? it.head[1] : it.head[0]) * PT_HS;
+        else return a.q + (size_t)(it.begin + r) * a.n_heads * HS + (t ? it.head[1] : it.head[0]) * HS;
     };
 
     // 128-byte-swizzled operands: rows of 128 B (64 halfs), 8-row groups 1024 B apart; the head dimension is split in
@@ -529,7 +544,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
         // the queries of the tile's next item: all rows in flight at once, ahead of this item's outputs
         auto load_queries = [&](const PtItem& of) {
             if (!(t ? of.jb[1] > of.ja[1] : of.jb[0] > of.ja[0])) return;
-            pt_load_rows<LINES>(row_of(of, t, row), q_s + t * PT_TILE_BYTES, quarter * 32, [&] {
+            pt_load_rows<LINES, HS>(row_of(of, t, row), q_s + t * PT_TILE_BYTES, quarter * 32, [&] {
                 if (nq > 0) wait(&q_empty[t], (nq - 1) & 1);      // the tile's last scores have read the queries before
             });
             nq++;
@@ -558,7 +573,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                 if (shaped) sc = 1.f;
             } else {
                 pos_r = it.p0 + r_abs;
-                sc = 1.4426950408889634f * rsqrtf((float)PT_HS);     // scores in the log2 domain
+                sc = 1.4426950408889634f * rsqrtf((float)HS);        // scores in the log2 domain
             }
             float m_used = -INFINITY, l = 0.0f;
             for (int j = ja; j < jb; j++, ns++) {
@@ -629,7 +644,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                 if (moved && j > ja) {      // the accumulated output moves to the new reference (rare after the first steps)
                     uint32_t w[32];
 #pragma unroll 1
-                    for (int ch = 0; ch < 4; ch++) {
+                    for (int ch = 0; ch < HS / 32; ch++) {
                         tmem_ld_32x32b_x32(T_O + ch * 32, w);
                         tmem_ld_wait();
 #pragma unroll
@@ -684,7 +699,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                 if (jb == ja) continue;
                 y16 = a.y_type != DL_KV8_F32;
                 if (a.y_out != nullptr) {
-                    const size_t at = (size_t)(it.begin + r_live) * a.n_heads * PT_HS + head * PT_HS;
+                    const size_t at = (size_t)(it.begin + r_live) * a.n_heads * HS + head * HS;
                     out = y16 ? reinterpret_cast<float*>(reinterpret_cast<uint16_t*>(a.y_out) + at) : reinterpret_cast<float*>(a.y_out) + at;
                 }
                 vec = ((uintptr_t)a.y_out & 15) == 0;
@@ -699,7 +714,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
             if (gave_up_s) inv = __int_as_float(0x7fffffff);
             const int live = it.rows - (row0 + quarter * 32);      // rows of this warp that are there
 #pragma unroll 1
-            for (int ch = 0; ch < 4; ch++) {
+            for (int ch = 0; ch < HS / 32; ch++) {
                 uint32_t o[32];
                 float f[32];
                 tmem_ld_32x32b_x32(T_O + ch * 32, o);
@@ -708,7 +723,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                 for (int e = 0; e < 32; e++) f[e] = __uint_as_float(o[e]) * inv;
                 if constexpr (!LINES) {
                     if (r_abs < it.rows && (a.xq_out != nullptr || a.xh_out != nullptr))
-                        pt_q80_block(f, it.begin + r_abs, head * (PT_HS / 32) + ch, a.out_mcap, a.xq_out, a.xh_out);
+                        pt_q80_block(f, it.begin + r_abs, head * (HS / 32) + ch, a.out_mcap, a.xq_out, a.xh_out);
                     if (out == nullptr) continue;
                 }
 #pragma unroll
@@ -745,7 +760,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
         const uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
         if (warp == 8) {
             // ---------------- MMAs, all by one thread: what it issues runs in that order ----------------
-            const uint32_t idesc_s = pt_idesc(PT_ROWS, PT_KV, 0, LINES), idesc_pv = pt_idesc(PT_ROWS, PT_HS, 1, LINES);
+            const uint32_t idesc_s = pt_idesc(PT_ROWS, PT_KV, 0, LINES), idesc_pv = pt_idesc(PT_ROWS, HS, 1, LINES);
             const uint32_t q_lo = ((smem_u32(q_s) & 0x3FFFFu) >> 4) | (1u << 16), k_lo = ((smem_u32(k_s) & 0x3FFFFu) >> 4) | (1u << 16);
             const uint32_t v_lo = ((smem_u32(v_s) & 0x3FFFFu) >> 4) | ((16384u >> 4) << 16);
             uint32_t g = 0, n_s = 0, ns[2] = {0, 0}, nq[2] = {0, 0};      // steps, scores, steps of a tile, items of a tile so far
@@ -761,7 +776,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                     n_s++;
                     tc_fence_after();
                     __syncwarp();
-                    pt_mma_ss(tmem_base, q_lo + t * (PT_TILE_BYTES >> 4), k_lo + st * (PT_TILE_BYTES >> 4), desc_hi, idesc_s, 0);
+                    if constexpr (HS == 128) pt_mma_ss(tmem_base, q_lo + t * (PT_TILE_BYTES >> 4), k_lo + st * (PT_TILE_BYTES >> 4), desc_hi, idesc_s, 0);
+                    else pt_mma_ss4(tmem_base, q_lo + t * (PT_TILE_BYTES >> 4), k_lo + st * (PT_TILE_BYTES >> 4), desc_hi, idesc_s, 0);
                     pt_commit(&s_full[t]);
                     if (t == 1 || !on(1, j)) pt_commit(&k_empty[st]);
                     if (j + 1 == it.jb[t]) pt_commit(&q_empty[t]);
@@ -807,8 +823,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                     if ((LINES && it.first_page * 32 > tok0) || tok0 + PT_KV > it.seq_end) {
                         uint8_t* vz = v_s + st * PT_TILE_BYTES;
                         const int z0 = LINES ? max(0, it.first_page * 32 - tok0) : 0, z1 = min(PT_KV, it.seq_end - tok0);
-                        for (int idx = lane; idx < PT_KV * 16; idx += 32) {      // 16 pieces of 16 B per token row (two halves)
-                            const int r = idx >> 4, c = idx & 15;
+                        for (int idx = lane; idx < PT_KV * (HS / 8); idx += 32) {      // 16 pieces of 16 B per token row (two halves)
+                            const int r = idx / (HS / 8), c = idx % (HS / 8);
                             if (r < z0 || r >= z1) *reinterpret_cast<uint4*>(vz + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
                         }
                         fence_proxy_async_smem();
@@ -856,7 +872,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                         if (gave_up_s) break;                    // no more copies into a CTA that ends
                         const int n_pg = min(4, total_pages - 4 * (it.j0 + j));                          // pages of this step that exist
                         const int p_lo = LINES ? max(0, it.first_page - 4 * (it.j0 + j)) : 0;            // ... and are looked at (at most the first step starts later)
-                        mbar_arrive_expect_tx(&full[st], (uint32_t)max(0, n_pg - p_lo) * 2u * 4096u);
+                        mbar_arrive_expect_tx(&full[st], (uint32_t)max(0, n_pg - p_lo) * (HS / 64) * 4096u);
                         const uint32_t dst = smem_u32(ring + st * PT_TILE_BYTES), bar = smem_u32(&full[st]);
 #pragma unroll
                         for (int p4 = 0; p4 < 4; p4++) {
@@ -864,7 +880,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                             if (LINES && p4 < p_lo) continue;
                             const int y = (pg[p4] * n_kv + it.kvh) * 32;      // first row of the page in the [rows][128] view
 #pragma unroll
-                            for (int h = 0; h < 2; h++)
+                            for (int h = 0; h < HS / 64; h++)
                                 asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
                                                  dst + h * 16384 + p4 * 4096),
                                              "l"(map), "r"((LINES && !is_k ? PT_HS : 0) + h * 64), "r"(y), "r"(bar)
@@ -911,11 +927,11 @@ static int pt_make_map(CUtensorMap* m, const void* base, long long rows, int wid
     return dl_tensor_map("attention_prefill_tc", m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// y_type other than f32: y_out aligned to 8 bytes
+// heads of 64 too; y_type other than f32: y_out aligned to 8 bytes
 int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_heads, int head_size, const void* k_cache, const void* v_cache, const int* pos,
                                   const int* slot, const int* block_table, int max_pages, int page_size, const int* meta, uint8_t* xq_out, uint8_t* xh_out,
                                   int out_mcap, void* y_out, int y_type, int n_cache_pages, int pdl, void* stream) {
-    if (page_size != 32 || head_size != PT_HS) { dl_set_error("dl_attention_prefill_tc: page size 32 and head size 128 only"); return -1; }
+    if (page_size != 32 || (head_size != 128 && head_size != 64)) { dl_set_error("dl_attention_prefill_tc: page size 32 and head size 64 or 128 only"); return -1; }
     if (n_heads % n_kv_heads != 0) { dl_set_error("dl_attention_prefill_tc: bad head grouping"); return -1; }
     if (n_cache_pages < 1) { dl_set_error("dl_attention_prefill_tc: n_cache_pages < 1"); return -1; }
     PtArgs a;
@@ -926,10 +942,10 @@ int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_h
     a.tr = dl_trace_next(TR_ATT);
     alignas(64) CUtensorMap kmap, vmap;
     const long long rows = (long long)n_cache_pages * n_kv_heads * 32;
-    if (pt_make_map(&kmap, k_cache, rows, PT_HS, false) != 0 || pt_make_map(&vmap, v_cache, rows, PT_HS, false) != 0) return -1;
+    if (pt_make_map(&kmap, k_cache, rows, head_size, false) != 0 || pt_make_map(&vmap, v_cache, rows, head_size, false) != 0) return -1;
     const size_t smem = PT_SMEM;
-    static SmemLimit given;
-    if (const int rc = dl_smem_limit("attention_prefill_tc", attention_prefill_tc_kernel<false>, smem, given)) return rc;
+    static SmemLimit given, given_64;
+    if (const int rc = head_size == 64 ? dl_smem_limit("attention_prefill_tc", attention_prefill_tc_kernel<false, 64>, smem, given_64) : dl_smem_limit("attention_prefill_tc", attention_prefill_tc_kernel<false>, smem, given)) return rc;
     cudaLaunchConfig_t cfg = {};
     const long long most = ((long long)(M + PT_ROWS - 1) / PT_ROWS + PT_MAX_SEG - 1) * n_heads;        // upper bound of the tiles of all segments
     cfg.gridDim = dim3((unsigned)(most < dl_device_sm_count() ? most : dl_device_sm_count()));
@@ -943,7 +959,7 @@ int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_h
         cfg.attrs = attr;
         cfg.numAttrs = 1;
     }
-    cudaError_t e = cudaLaunchKernelEx(&cfg, attention_prefill_tc_kernel<false>, a, kmap, vmap);
+    cudaError_t e = head_size == 64 ? cudaLaunchKernelEx(&cfg, attention_prefill_tc_kernel<false, 64>, a, kmap, vmap) : cudaLaunchKernelEx(&cfg, attention_prefill_tc_kernel<false>, a, kmap, vmap);
     if (e != cudaSuccess) { dl_set_error("attention_prefill_tc launch: %s", cudaGetErrorString(e)); return -(int)e; }
     return 0;
 }
@@ -952,6 +968,7 @@ extern "C" int dl_attention_prefill_tc(const float* q, int M, int n_heads, int n
                                        const void* v_cache, const int* pos, const int* slot, const int* block_table,
                                        int max_pages, int page_size, const int* meta, uint8_t* xq_out, uint8_t* xh_out,
                                        int out_mcap, float* y_out, int n_cache_pages, int pdl, void* stream) {
+    if (head_size != PT_HS) { dl_set_error("dl_attention_prefill_tc: page size 32 and head size 128 only"); return -1; }
     return dl_attention_prefill_tc_typed(q, M, n_heads, n_kv_heads, head_size, k_cache, v_cache, pos, slot, block_table, max_pages, page_size, meta, xq_out, xh_out,
                                          out_mcap, y_out, DL_KV8_F32, n_cache_pages, pdl, stream);
 }

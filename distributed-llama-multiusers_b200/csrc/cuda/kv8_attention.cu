@@ -824,7 +824,7 @@ static int ka_prompt(const Kv8AttArgs& a, int pdl, void* stream) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// Long prompt chunks of heads of 128: the segments' pages widened once to fp16 (fp16(code * scale): 2^-12 of a value, the queries of that kernel are rounded alike),
+// Long prompt chunks of heads of 64 and 128: the segments' pages widened once to fp16 (fp16(code * scale): 2^-12 of a value, the queries of that kernel are rounded alike),
 // then the tcgen05 kernel of the fp16 cache on them, under the same page numbers.  Widening inside that kernel would be done again by every CTA that meets a page
 // (rows / 128 * heads / 2 of them).  4001 rows: 12 MB in and 16 MB out, beside 131 GFLOP.
 //
@@ -834,13 +834,13 @@ static int ka_prompt(const Kv8AttArgs& a, int pdl, void* stream) {
 // ------------------------------------------------------------------------------------------------
 struct Kv8ExpandArgs {
     Kv8AttArgs a;
-    __half* k16;               // [pages][kv][32][128]
+    __half* k16;               // [pages][kv][32][HS]
     __half* v16;
     int* meta_out;             // [17]
 };
 
+template <int HS>
 __global__ void __launch_bounds__(256) kv8_expand_kernel(const __grid_constant__ Kv8ExpandArgs x) {
-    constexpr int HS = 128;
     __shared__ int first[9], seg[8][3];                        // items ahead of a segment; begin, end, slot
     __shared__ int ok[8];
     const int tid = threadIdx.x, kv = x.a.c.n_kv_heads;
@@ -896,11 +896,6 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const __grid_constant__
         const int in = item - first[i], kvh = in % kv;
         const int page = x.a.rows.block_table[(size_t)seg[i][2] * x.a.rows.max_pages + in / kv];
         if ((unsigned)page >= (unsigned)x.a.rows.n_pages) continue;
-        const size_t line = ((size_t)page * kv + kvh) * KV8_PAGE + (tid >> 3);
-        const size_t at = line * HS + (tid & 7) * 16;
-        const uint4 kc = *reinterpret_cast<const uint4*>(x.a.c.k + at), vc = *reinterpret_cast<const uint4*>(x.a.c.v + at);
-        float ks = x.a.c.k_scale[line], vs = x.a.c.v_scale[line];
-        if (!(fabsf(ks) < INFINITY) || !(fabsf(vs) < INFINITY)) { ks = __uint_as_float(0x7fffffffu); vs = 0.f; }
         auto widen = [](uint4 c, float s, __half* dst) {
             const uint32_t w[4] = {c.x, c.y, c.z, c.w};
             uint32_t o[8];
@@ -918,8 +913,16 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const __grid_constant__
             reinterpret_cast<uint4*>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
             reinterpret_cast<uint4*>(dst)[1] = make_uint4(o[4], o[5], o[6], o[7]);
         };
-        widen(kc, ks, x.k16 + at);
-        widen(vc, vs, x.v16 + at);
+#pragma unroll
+        for (int v = tid; v < 2 * KV8_PAGE * (HS / 16); v += 256) {          // pieces of 16 codes: the keys', then the values'
+            const bool is_k = v < KV8_PAGE * (HS / 16);
+            const int piece = v % (KV8_PAGE * (HS / 16));
+            const size_t line = ((size_t)page * kv + kvh) * KV8_PAGE + piece / (HS / 16), at = line * HS + piece % (HS / 16) * 16;
+            const uint4 codes = *reinterpret_cast<const uint4*>((is_k ? x.a.c.k : x.a.c.v) + at);
+            float ks = x.a.c.k_scale[line], vs = x.a.c.v_scale[line];
+            if (!(fabsf(ks) < INFINITY) || !(fabsf(vs) < INFINITY)) { ks = __uint_as_float(0x7fffffffu); vs = 0.f; }
+            widen(codes, is_k ? ks : vs, (is_k ? x.k16 : x.v16) + at);
+        }
     }
 }
 
@@ -956,9 +959,11 @@ extern "C" int dl_kv8_attention(const float* q, long long ldq, int n_heads, cons
     return hs == 128 ? ka_decode<128>(a, n_splits, scratch, pdl, stream) : hs == 64 ? ka_decode<64>(a, n_splits, scratch, pdl, stream) : ka_decode<32>(a, n_splits, scratch, pdl, stream);
 }
 
-// Rows times heads above which heads of 128 take the tcgen05 kernel on widened pages, where there is a workspace (us on mma.sync / widened, 32 heads: 128 rows
-// behind 1000 tokens 21 / 24, behind 8000 95 / 92, 256 behind 2000 63 / 36, 512 behind 4000 208 / 60; 8 heads: 512 rows behind none 13.5 / 17.9, 1024 27 / 22)
-#define KV8_EXPAND_MIN_WORK 4096
+// Rows times heads above which a prompt takes the tcgen05 kernel on widened pages, where there is a workspace (us on mma.sync / widened.  Heads of 128, 32
+// of them: 128 rows behind 1000 tokens 21 / 24, behind 8000 95 / 92, 256 behind 2000 63 / 36, 512 behind 4000 208 / 60; 8 heads: 512 rows behind none
+// 13.5 / 17.9, 1024 27 / 22.  Heads of 64, 32 of them: 200 rows behind 1000 21 / 22, 256 behind 2000 36 / 31, 512 behind 4000 103 / 52, 4001 behind none
+// 382 / 108; 8 heads: 520 behind none 10.4 / 16.6, 1024 19.1 / 19.9)
+static bool ka_widens(long long rows, int n_heads, int hs) { return (hs == 128 && rows * n_heads > 4096) || (hs == 64 && rows * n_heads > 7168); }
 
 extern int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_heads, int head_size, const void* k_cache, const void* v_cache, const int* pos,
                                          const int* slot, const int* block_table, int max_pages, int page_size, const int* meta, uint8_t* xq_out, uint8_t* xh_out,
@@ -974,11 +979,13 @@ extern "C" int dl_kv8_attention_prefill(const float* q, long long ldq, int n_hea
     const int hs = cache->head_size;
     // (that kernel takes rows side by side, aligned)
     const bool dense = ldq == (long long)n_heads * hs && ((uintptr_t)q & 15) == 0 && (y_out == nullptr || (ldy == ldq && ((uintptr_t)y_out & 15) == 0));
-    if (k16 != nullptr && hs == 128 && dense && (long long)M * n_heads > KV8_EXPAND_MIN_WORK) {
+    if (k16 != nullptr && dense && ka_widens(M, n_heads, hs)) {
         if ((((uintptr_t)k16 | (uintptr_t)v16) & 15) != 0) { dl_set_error("dl_kv8_attention_prefill: the workspace has to be aligned to 16 bytes"); return -1; }
         const Kv8ExpandArgs x = {a, (__half*)k16, (__half*)v16, meta16};
         static SmemLimit none;
-        if (const int rc = ka_launch("dl_kv8_attention_prefill", kv8_expand_kernel, none, dim3(4 * dl_device_sm_count()), 1, 256, 0, pdl, stream, x)) return rc;
+        const dim3 grid(4 * dl_device_sm_count());
+        if (const int rc = hs == 128 ? ka_launch("dl_kv8_attention_prefill", kv8_expand_kernel<128>, none, grid, 1, 256, 0, pdl, stream, x)
+                                     : ka_launch("dl_kv8_attention_prefill", kv8_expand_kernel<64>, none, grid, 1, 256, 0, pdl, stream, x)) return rc;
         return dl_attention_prefill_tc_typed(q, M, n_heads, cache->n_kv_heads, hs, k16, v16, pos, slot, block_table, max_pages, KV8_PAGE, meta16,
                                              xq_out, xh_out, out_mcap, y_out, y_type, cache->n_pages, 1, stream);
     }

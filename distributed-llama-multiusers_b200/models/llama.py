@@ -192,7 +192,7 @@ class LlamaEngine:
         # the page pool is shared by all sequences and grows on demand, so it does not have to cover
         # n_slots x max_seq_len (Llama-3.1 headers say 131072): cap it at 85 % of the free HBM
         page_bytes = 2 * h.n_layers * self.n_kv_loc * PAGE * self.hs * torch.empty((), dtype=kv_dtype).element_size()
-        widen = self.kv8 and self.hs == 128 and R * self.n_heads_loc > K.KV8_WIDEN_MIN_WORK       # long prompt chunks: fp16 pages of one layer
+        widen = self.kv8 and K.kv8_widens(R, self.n_heads_loc, self.hs)       # long prompt chunks: fp16 pages of one layer
         if self.kv8:
             page_bytes = h.n_layers * K.kv8_page_bytes(self.n_kv_loc, self.hs) + (4 * self.n_kv_loc * PAGE * self.hs if widen else 0)
         if n_pages is None and dev.type == "cuda":

@@ -37,6 +37,9 @@ def required_memory(h: LlmHeader, n_nodes: int = 1, max_rows: int = 32, n_slots:
     kv_bytes = 2 * L * n_slots * seq * (kv // N) * kv_elem
     if backend == "cuda" and kv_cache == "q8":
         kv_bytes = 2 * L * n_slots * seq * (kv // N + h.n_kv_heads // N * 4)
+        from ..ops.kernels import kv8_widens
+        if kv8_widens(max_rows, h.n_heads // N, kv // h.n_kv_heads):          # fp16 pages of one layer
+            kv_bytes += 4 * n_slots * seq * (kv // N)
     # residual stream, normalised / quantised activations, q/k/v, hidden, logits, exchange area (N slices per sync)
     act = max_rows * (4 * dim * 4 + (dim + 2 * kv) // N * 4 + 3 * (hid // N) * 4 + vocab * 4 + 2 * N * dim * 8)
     out = {"weights": weights, "embedding": embedding, "kv_cache": kv_bytes, "activations": act}

@@ -279,7 +279,7 @@ class Kv8Cache:
         return kv8_page_bytes(self.n_kv_heads, self.head_size) * self.n_pages
 
 
-KV8_WIDEN_MIN_WORK = 4096          # rows times heads above which kv8_attention_prefill uses a workspace (KV8_EXPAND_MIN_WORK in csrc/cuda/kv8_attention.cu)
+KV8_WIDEN_MIN_WORK = {128: 4096, 64: 7168}         # kv8_widens()
 
 
 def kv8_page_bytes(n_kv_heads: int, head_size: int) -> int:
@@ -410,10 +410,15 @@ class Kv8Workspace(NamedTuple):
     meta: torch.Tensor
 
 
+def kv8_widens(rows: int, n_heads: int, head_size: int) -> bool:
+    """Whether kv8_attention_prefill uses a workspace for this many rows (ka_widens in csrc/cuda/kv8_attention.cu)."""
+    return rows * n_heads > KV8_WIDEN_MIN_WORK.get(head_size, rows * n_heads)
+
+
 def kv8_prefill_workspace(n_pages: int, n_kv_heads: int, head_size: int, max_rows: int, device) -> Optional[Kv8Workspace]:
     """What kv8_attention_prefill wants beside its arguments for prompt chunks of up to max_rows rows over a cache of these pages, or None: fp16 pages under
     the cache's page numbers (one workspace serves all layers of a model, one launch at a time)."""
-    if head_size != 128 or max_rows < 16:
+    if head_size < 64 or max_rows < 16:
         return None
     pages = [torch.zeros(n_pages, n_kv_heads, PAGE_SIZE, head_size, dtype=torch.float16, device=device) for _ in range(2)]
     return Kv8Workspace(*pages, torch.zeros(17, dtype=torch.int32, device=device))

@@ -243,7 +243,7 @@ def _near(got, ref, rel):
     (32, 8, 128, [0], 1), (32, 8, 128, [191], 2), (4, 1, 128, [0, 1, 15, 16, 30, 31, 32, 33, 63, 64, 65, -1], 1),
     (8, 4, 32, [0, 5, 31, 32, 100], 1), (8, 8, 64, [63, 64, 65, 700], 2), (16, 2, 128, [300], 8), (16, 1, 128, [129, 1000], 32),
     (64, 8, 64, [1200, 3, 900], 6), (5, 1, 128, [777, 40], 4), (12, 2, 64, [2000], 5), (7, 7, 32, [900, 45], 3), (9, 1, 32, [801], 4),
-    (3, 1, 128, [1000 - 1] * 3, 2), (24, 2, 128, [767, 768, 769], 7), (4, 1, 64, [20000], 32),
+    (3, 1, 128, [1000 - 1] * 3, 2), (20, 2, 128, [767, 768, 769], 7), (4, 1, 64, [20000], 32),
 ])
 def test_attention(heads, kv, hs, positions, splits):
     k = K()
@@ -347,6 +347,7 @@ PROMPT_REL = 4e-3
     (4, 1, 128, [(0, 0, 16)]), (8, 2, 128, [(0, 37, 100)]), (4, 4, 64, [(3, 5, 70)]), (2, 1, 128, [(62, 200, 130)]), (2, 2, 64, [(31, 31, 33)]),
     (4, 2, 128, [(2, 10, 40), (45, 0, 90)]), (8, 8, 128, [(0, 0, 700)]), (16, 1, 128, [(5, 900, 300)]), (8, 2, 128, [(0, 0, 257), (260, 130, 384)]),
     (5, 1, 128, [(1, 77, 900)]), (16, 1, 64, [(0, 3, 50)]), (6, 2, 32, [(1, 60, 45)]), (5, 1, 128, [(0, 100, 17), (20, 0, 1)]), (32, 8, 128, [(0, 1000, 100)]), (8, 1, 64, [(0, 2500, 31)]),
+    (32, 8, 64, [(0, 10, 230)]), (5, 1, 64, [(1, 77, 1450)]), (8, 8, 64, [(0, 100, 930)]), (16, 2, 64, [(0, 0, 257), (260, 130, 200)]),
 ])
 def test_attention_prefill(heads, kv, hs, segs):
     k = K()
@@ -379,16 +380,16 @@ def test_attention_prefill(heads, kv, hs, segs):
             assert (y[~covered] == 7.0).all()                     # rows outside the segments are left alone
 
 
-@pytest.mark.parametrize("workspace", [False, True])
-def test_attention_prefill_of_unusual_lines(workspace):
+@pytest.mark.parametrize("workspace,hs", [(False, 128), (True, 128), (False, 64), (True, 64)])
+def test_attention_prefill_of_unusual_lines(workspace, hs):
     """A line with a NaN is seen by the rows from its token on, and by no other; a segment of a sequence, a position or a page that is not there is NaN;
     one without tokens gives zeros."""
     k = K()
     rng = np.random.default_rng(8)
-    heads, kv, hs = 16, 8, 128          # (more than 4096 rows times heads: the widened pages, where there is a workspace)
+    heads, kv = (16, 8) if hs == 128 else (32, 16)
     segs = [(0, 100, 60, 0), (60, 0, 40, 1), (100, 30, 20, 9), (120, 200, 30, 2), (150, -40, 20, 1), (170, 0, 33, 3), (203, 5, 50, 4)]      # begin, position, rows, sequence
     M = 260
-    assert M * heads > 4096
+    assert k.kv8_widens(M, heads, hs)                           # the widened pages, where there is a workspace
     bt, n_pages = _table(rng, [160, 40, 220, 33, 55])
     bt = bt[:, :7]                                              # the fourth segment ends behind the table: 7 pages are 224 tokens
     bt[3, 1] = n_pages                                          # a page that is not there

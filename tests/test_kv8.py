@@ -1,5 +1,6 @@
 """The 8-bit token cache without a GPU: what its entry points refuse, sizes, and the command line."""
 import ctypes as C
+import dataclasses
 
 import pytest
 import torch
@@ -103,7 +104,9 @@ def test_splits(M, heads, kv, pages, want):
 def test_workspace():
     w = K.kv8_prefill_workspace(3, 2, 128, 512, "cpu")
     assert w.k16.shape == w.v16.shape == (3, 2, 32, 128) and w.k16.dtype == torch.float16 and w.meta.numel() == 17
-    assert K.kv8_prefill_workspace(3, 2, 64, 512, "cpu") is None and K.kv8_prefill_workspace(3, 2, 128, 1, "cpu") is None
+    assert K.kv8_prefill_workspace(3, 2, 64, 512, "cpu").v16.shape == (3, 2, 32, 64)
+    assert K.kv8_prefill_workspace(3, 2, 32, 512, "cpu") is None and K.kv8_prefill_workspace(3, 2, 128, 1, "cpu") is None
+    assert [K.kv8_widens(128, 32, 128), K.kv8_widens(129, 32, 128), K.kv8_widens(129, 32, 64), K.kv8_widens(256, 32, 64), K.kv8_widens(4096, 32, 32)] == [False, True, False, True, False]
 
 
 def test_command_line(tiny_model_path):
@@ -123,3 +126,6 @@ def test_required_memory_of_the_cache(tiny_model_path):
     h = read_header(tiny_model_path, 0)
     f16, q8 = (required_memory(h, 1, n_slots=3, seq_len=64, kv_cache=t)["kv_cache"] for t in ("f16", "q8"))
     assert f16 == 2 * 2 * 3 * 64 * 4 * 32 * 2 and q8 == 2 * 3 * 2 * K.kv8_page_bytes(4, 32)
+    wide = dataclasses.replace(h, dim=2048, n_heads=32, n_kv_heads=8)
+    few, many = (required_memory(wide, 1, rows, n_slots=3, seq_len=64, kv_cache="q8")["kv_cache"] for rows in (64, 512))
+    assert few == 2 * 3 * 2 * K.kv8_page_bytes(8, 64) and many == few + 3 * 64 * 2 * 512 * 2        # and fp16 pages of one layer
