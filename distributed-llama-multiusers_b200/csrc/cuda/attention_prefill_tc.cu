@@ -38,6 +38,7 @@
 #include <atomic>
 #include "epilogue.cuh"
 #include "f32_pairs.cuh"
+#include "prefill_shares.cuh"
 #include "smem_limit.cuh"
 #include "tensor_map.cuh"
 #include "waits.cuh"
@@ -52,6 +53,7 @@
 #define PT_STAGES 2                    // K tiles and V tiles in flight
 #define PT_OUT_LD 20
 #define PT_SHARE_STEPS 4
+#define PT_LEAST_STEPS 4               // of a share of the Llama path; of an item that goes to two CTAs: 32
 
 struct PtArgs {
     const float* q;            // [M][n_heads*128]
@@ -67,6 +69,7 @@ struct PtArgs {
     int out_mcap;
     void* y_out;               // [M][n_heads*128] of DL_KV8_F32 / BF16 / F16
     int y_type;
+    PtShares part;
     unsigned long long* tr;
     WaitLimit limit;
 };
@@ -295,7 +298,8 @@ struct PtItem {
     int ja[2], jb[2];                      // steps [ja, jb) of these are tile t's (none: the tile is not there)
     int row0[2], rows, head[2];            // first row of tile t, rows of the segment (or run), the tile's head
     int seen_from[2], seen_to[2];          // LINES: tokens that rows of tile t see, from the start of the first one's page
-    int shares;                            // LINES: into how many shares (grid.z) the steps of the run go
+    int shares;                            // into how many shares the steps go: LINES: of the run (grid.z), else of the item, whose this is `share`
+    int share;
     int begin;                             // batch row of the segment's first row; LINES: entry of tile_rows where the run starts
 };
 
@@ -316,14 +320,26 @@ struct PtWaits {
 };
 
 // Llama path: the items of a batch are (128-row tile of a segment, query head), late tiles (long histories) first: two heads of one key/value head
-// side by side, or two tiles of one head where the heads come alone; single tiles while there are SMs for all of them.  Item `idx` of the
-// order that all roles of all CTAs walk; false behind the last one.
+// side by side, or two tiles of one head where the heads come alone; single tiles while there are SMs for all of them.  With a place for shares the steps of
+// a long item go to as many CTAs as there are for each.  Two tiles in one CTA take 1.75 us a step, a single one 1.03, and the join 5 us more: 130 rows of 32 heads
+// behind 2000 tokens 37 us alike, behind 8000 92 without shares and 63 with them; 512 rows (two shares) behind none 21 / 27, behind 4000 62 / 61, behind 16000 182 / 159
+// (those of heads of 64 behind 16000 156 / 122).  Item `idx` of the order that all roles of all CTAs walk; false behind the last one.
 DL_DEVINL bool pt_item(const PtArgs& a, const int (*seg)[4], int n_seg, int idx, PtItem& it) {
     const int rep = a.n_heads / a.n_kv_heads;
-    int tiles = 0;
-    for (int i = 0; i < n_seg; i++) tiles += (seg[i][1] + PT_ROWS - 1) / PT_ROWS;
-    const bool single = tiles * a.n_heads <= (int)gridDim.x, by_heads = !single && rep % 2 == 0, by_rows = !single && !by_heads;
-    const int cols = by_heads ? a.n_heads / 2 : a.n_heads;
+    const bool even = rep % 2 == 0;
+    int tiles = 0, pairs = 0, last = 0, spread = 1;
+    for (int i = 0; i < n_seg; i++) {
+        const int nt = (seg[i][1] + PT_ROWS - 1) / PT_ROWS;
+        tiles += nt;
+        pairs += even ? nt : (nt + 1) / 2;
+        last = max(last, seg[i][2] + seg[i][1]);
+    }
+    if (a.part.arrived != nullptr && pairs > 0)
+        spread = max(1, min((int)gridDim.x / (pairs * (even ? a.n_heads / 2 : a.n_heads)), last / (PT_KV * PT_LEAST_STEPS)));
+    if (spread == 2 && last < PT_KV * 32) spread = 1;
+    const bool single = spread == 1 && tiles * a.n_heads <= (int)gridDim.x, by_heads = !single && even, by_rows = !single && !by_heads;
+    const int cols = by_heads ? a.n_heads / 2 : a.n_heads, share = idx % spread;
+    idx /= spread;
     for (int i = 0; i < n_seg; i++) {
         const int nt = (seg[i][1] + PT_ROWS - 1) / PT_ROWS, groups = by_rows ? (nt + 1) / 2 : nt;
         if (idx >= groups * cols) { idx -= groups * cols; continue; }
@@ -341,6 +357,15 @@ DL_DEVINL bool pt_item(const PtArgs& a, const int (*seg)[4], int n_seg, int idx,
             it.J = max(it.J, it.jb[t]);
         }
         it.kvh = it.head[0] / rep;
+        it.shares = min(spread, max(1, it.J / PT_LEAST_STEPS));
+        it.share = share;
+        if (spread > 1) {
+            const int per = (it.J + it.shares - 1) / it.shares, z0 = min(it.J, share * per), z1 = min(it.J, z0 + per);
+#pragma unroll
+            for (int t = 0; t < 2; t++) it.jb[t] = max(0, min(it.jb[t], z1) - z0);
+            it.j0 = z0;
+            it.J = z1 - z0;
+        }
         return true;
     }
     return false;
@@ -675,7 +700,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
             }
             float* out = nullptr;                                // this thread's row (of 16-bit values: y16); null: none
             bool vec = true;                                     // 16-byte rows
-            bool y16 = false;
+            bool y16 = false, part = false;                      // part: of several shares' rows
             if constexpr (LINES) {
                 if (row0 >= it.rows || (it.shares == 1 && blockIdx.z > 0)) continue;
                 out = a.w.out + (size_t)m_row * a.w.ldo + h_row * PT_HS;
@@ -696,7 +721,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                 }
                 if (jb == ja) continue;
             } else {
-                if (jb == ja) continue;
+                part = it.shares > 1 && it.share < it.shares && row0 < it.rows;
+                if (jb == ja && !part) continue;
                 y16 = a.y_type != DL_KV8_F32;
                 if (a.y_out != nullptr) {
                     const size_t at = (size_t)(it.begin + r_live) * a.n_heads * HS + head * HS;
@@ -707,20 +733,85 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
             if constexpr (LINES) {                               // (the barrier's phase in the topmost bit)
                 wait(&o_full[t], ns >> 31);
                 ns ^= 1u << 31;
-            } else {
+            } else if (jb > ja) {
                 wait(&o_full[t], (ns - 1) & 1);
             }
             tc_fence_after();
             if (gave_up_s) inv = __int_as_float(0x7fffffff);
+            const float4* sums = nullptr;                        // of the first share's
+            const float2* norms = nullptr;
+            float top = 0.f;                                     // the shares' common reference
+            if constexpr (!LINES) {
+                if (part) {
+                    const size_t slot = (size_t)blockIdx.x * PT_SHARE_WARPS + warp, first = slot - it.share * PT_SHARE_WARPS;
+                    a.part.norms[slot * 32 + lane] = make_float2(m_used, gave_up_s ? inv : jb > ja ? l : -1.f);
+#pragma unroll 1
+                    for (int ch = 0; ch < HS / 32 && jb > ja; ch++) {
+                        uint32_t o[32];
+                        tmem_ld_32x32b_x32(T_O + ch * 32, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            a.part.sums[(slot * (HS / 4) + ch * 8 + e / 4) * 32 + lane] = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                    }
+                    tc_fence_before();
+                    __threadfence();
+                    __syncwarp();
+                    unsigned before = 0;
+                    if (lane == 0) before = atomicAdd(&a.part.arrived[first], 1u);
+                    if (__shfl_sync(0xffffffffu, before, 0) != (unsigned)it.shares - 1) continue;
+                    __threadfence();
+                    if (lane == 0) a.part.arrived[first] = 0;
+                    sums = a.part.sums + first * (HS / 4) * 32 + lane;
+                    norms = a.part.norms + first * 32 + lane;
+                    top = -INFINITY;
+                    l = 0.f;
+                    for (int z = 0; z < it.shares; z++) {
+                        const float2 n = __ldcg(norms + z * PT_SHARE_WARPS * 32);
+                        if (!(n.y < 0.f)) top = fmaxf(top, n.x);
+                    }
+                    if (top == -INFINITY) top = 0.f;
+                    for (int z = 0; z < it.shares; z++) {
+                        const float2 n = __ldcg(norms + z * PT_SHARE_WARPS * 32);
+                        if (!(n.y < 0.f)) l = fmaf(n.y, pt_ex2(n.x - top), l);
+                    }
+                    inv = l > 0.f ? 1.f / l : l != l ? l : 0.f;
+                }
+            }
             const int live = it.rows - (row0 + quarter * 32);      // rows of this warp that are there
 #pragma unroll 1
             for (int ch = 0; ch < HS / 32; ch++) {
                 uint32_t o[32];
                 float f[32];
-                tmem_ld_32x32b_x32(T_O + ch * 32, o);
-                tmem_ld_wait();
+                if (LINES || !part) {
+                    tmem_ld_32x32b_x32(T_O + ch * 32, o);
+                    tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; e++) f[e] = __uint_as_float(o[e]) * inv;
+                    for (int e = 0; e < 32; e++) f[e] = __uint_as_float(o[e]) * inv;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) f[e] = 0.f;
+#pragma unroll 1
+                    for (int z = 0; z < it.shares; z += 2) {     // two shares' in flight
+                        float4 x[2][8];
+                        float w[2];
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const float2 n = z + u < it.shares ? __ldcg(norms + (z + u) * PT_SHARE_WARPS * 32) : make_float2(0.f, -1.f);
+                            const bool has = !(n.y < 0.f);
+                            w[u] = has ? pt_ex2(n.x - top) * inv : 0.f;
+#pragma unroll
+                            for (int e = 0; e < 8; e++) x[u][e] = has ? __ldcg(sums + ((size_t)(z + u) * PT_SHARE_WARPS * (HS / 4) + ch * 8 + e) * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
+#pragma unroll
+                        for (int u = 0; u < 2; u++)
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                f[e * 4] = fmaf(x[u][e].x, w[u], f[e * 4]); f[e * 4 + 1] = fmaf(x[u][e].y, w[u], f[e * 4 + 1]);
+                                f[e * 4 + 2] = fmaf(x[u][e].z, w[u], f[e * 4 + 2]); f[e * 4 + 3] = fmaf(x[u][e].w, w[u], f[e * 4 + 3]);
+                            }
+                    }
+                }
                 if constexpr (!LINES) {
                     if (r_abs < it.rows && (a.xq_out != nullptr || a.xh_out != nullptr))
                         pt_q80_block(f, it.begin + r_abs, head * (HS / 32) + ch, a.out_mcap, a.xq_out, a.xh_out);
@@ -927,10 +1018,13 @@ static int pt_make_map(CUtensorMap* m, const void* base, long long rows, int wid
     return dl_tensor_map("attention_prefill_tc", m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// heads of 64 too; y_type other than f32: y_out aligned to 8 bytes
+// CTAs of a launch that may leave shares
+int pt_share_ctas() { return dl_device_sm_count() < PT_SHARE_SLOTS ? dl_device_sm_count() : PT_SHARE_SLOTS; }
+
+// heads of 64 too; y_type other than f32: y_out aligned to 8 bytes; shares: NULL, or where a launch may leave shares of items to be joined
 int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_heads, int head_size, const void* k_cache, const void* v_cache, const int* pos,
                                   const int* slot, const int* block_table, int max_pages, int page_size, const int* meta, uint8_t* xq_out, uint8_t* xh_out,
-                                  int out_mcap, void* y_out, int y_type, int n_cache_pages, int pdl, void* stream) {
+                                  int out_mcap, void* y_out, int y_type, const PtShares* shares, int n_cache_pages, int pdl, void* stream) {
     if (page_size != 32 || (head_size != 128 && head_size != 64)) { dl_set_error("dl_attention_prefill_tc: page size 32 and head size 64 or 128 only"); return -1; }
     if (n_heads % n_kv_heads != 0) { dl_set_error("dl_attention_prefill_tc: bad head grouping"); return -1; }
     if (n_cache_pages < 1) { dl_set_error("dl_attention_prefill_tc: n_cache_pages < 1"); return -1; }
@@ -938,6 +1032,7 @@ int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_h
     a.q = q; a.k_cache = (const __half*)k_cache; a.v_cache = (const __half*)v_cache; a.pos = pos; a.slot = slot;
     a.block_table = block_table; a.meta = meta; a.M = M; a.n_heads = n_heads; a.n_kv_heads = n_kv_heads;
     a.max_pages = max_pages; a.xq_out = xq_out; a.xh_out = xh_out; a.out_mcap = out_mcap; a.y_out = y_out; a.y_type = y_type;
+    a.part = shares != nullptr ? *shares : PtShares{};
     if (pt_limit(&a.limit) != 0) return -1;
     a.tr = dl_trace_next(TR_ATT);
     alignas(64) CUtensorMap kmap, vmap;
@@ -948,7 +1043,7 @@ int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_h
     if (const int rc = head_size == 64 ? dl_smem_limit("attention_prefill_tc", attention_prefill_tc_kernel<false, 64>, smem, given_64) : dl_smem_limit("attention_prefill_tc", attention_prefill_tc_kernel<false>, smem, given)) return rc;
     cudaLaunchConfig_t cfg = {};
     const long long most = ((long long)(M + PT_ROWS - 1) / PT_ROWS + PT_MAX_SEG - 1) * n_heads;        // upper bound of the tiles of all segments
-    cfg.gridDim = dim3((unsigned)(most < dl_device_sm_count() ? most : dl_device_sm_count()));
+    cfg.gridDim = dim3((unsigned)(shares != nullptr ? pt_share_ctas() : most < dl_device_sm_count() ? most : dl_device_sm_count()));
     cfg.blockDim = dim3(PT_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t)stream;
@@ -970,7 +1065,7 @@ extern "C" int dl_attention_prefill_tc(const float* q, int M, int n_heads, int n
                                        int out_mcap, float* y_out, int n_cache_pages, int pdl, void* stream) {
     if (head_size != PT_HS) { dl_set_error("dl_attention_prefill_tc: page size 32 and head size 128 only"); return -1; }
     return dl_attention_prefill_tc_typed(q, M, n_heads, n_kv_heads, head_size, k_cache, v_cache, pos, slot, block_table, max_pages, page_size, meta, xq_out, xh_out,
-                                         out_mcap, y_out, DL_KV8_F32, n_cache_pages, pdl, stream);
+                                         out_mcap, y_out, DL_KV8_F32, nullptr, n_cache_pages, pdl, stream);
 }
 
 // 0 if the kernel's LINES instance takes these sizes: bf16 lines of a key and a value of 128, full tiles of 64 stacked rows

@@ -10,6 +10,7 @@
 #include <type_traits>
 #include "epilogue.cuh"
 #include "kv8.cuh"
+#include "prefill_shares.cuh"
 #include "smem_limit.cuh"
 
 extern void dl_set_error(const char* fmt, ...);
@@ -967,27 +968,43 @@ static bool ka_widens(long long rows, int n_heads, int hs) { return (hs == 128 &
 
 extern int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_heads, int head_size, const void* k_cache, const void* v_cache, const int* pos,
                                          const int* slot, const int* block_table, int max_pages, int page_size, const int* meta, uint8_t* xq_out, uint8_t* xh_out,
-                                         int out_mcap, void* y_out, int y_type, int n_cache_pages, int pdl, void* stream);
+                                         int out_mcap, void* y_out, int y_type, const PtShares* shares, int n_cache_pages, int pdl, void* stream);
+extern int pt_share_ctas();
+
+#define KV8_META_BYTES 128             // of a workspace's scratch: the segments of the launch, then its shares
+extern "C" long long dl_kv8_prefill_scratch_bytes(int head_size) {
+    return KV8_META_BYTES + pt_share_bytes(head_size);
+}
 
 extern "C" int dl_kv8_attention_prefill(const float* q, long long ldq, int n_heads, const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const int* meta, const DlKv8Cache* cache, void* k16, void* v16,
-                                        int* meta16, uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, int pdl, void* stream) {
+                                        void* scratch16, uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, int pdl, void* stream) {
+    const char* who = "dl_kv8_attention_prefill";
     Kv8AttArgs a;
-    if (const int rc = kv8_att_args("dl_kv8_attention_prefill", q, ldq, n_heads, pos, slot, block_table, M, n_slots, max_pages, cache, xq_out, xh_out, out_mcap, y_out, ldy, y_type, &a)) return rc;
-    if (meta == nullptr || (k16 == nullptr) != (v16 == nullptr) || (k16 == nullptr) != (meta16 == nullptr)) { dl_set_error("dl_kv8_attention_prefill: a null pointer"); return -1; }
+    if (const int rc = kv8_att_args(who, q, ldq, n_heads, pos, slot, block_table, M, n_slots, max_pages, cache, xq_out, xh_out, out_mcap, y_out, ldy, y_type, &a)) return rc;
+    if (meta == nullptr || (k16 == nullptr) != (v16 == nullptr) || (k16 == nullptr) != (scratch16 == nullptr)) { dl_set_error("dl_kv8_attention_prefill: a null pointer"); return -1; }
     if (M == 0) return 0;
     a.meta = meta;
     const int hs = cache->head_size;
     // (that kernel takes rows side by side, aligned)
     const bool dense = ldq == (long long)n_heads * hs && ((uintptr_t)q & 15) == 0 && (y_out == nullptr || (ldy == ldq && ((uintptr_t)y_out & 15) == 0));
     if (k16 != nullptr && dense && ka_widens(M, n_heads, hs)) {
-        if ((((uintptr_t)k16 | (uintptr_t)v16) & 15) != 0) { dl_set_error("dl_kv8_attention_prefill: the workspace has to be aligned to 16 bytes"); return -1; }
+        if ((((uintptr_t)k16 | (uintptr_t)v16 | (uintptr_t)scratch16) & 15) != 0) { dl_set_error("dl_kv8_attention_prefill: the workspace has to be aligned to 16 bytes"); return -1; }
+        uint8_t* scratch = reinterpret_cast<uint8_t*>(scratch16);
+        int* meta16 = reinterpret_cast<int*>(scratch);
         const Kv8ExpandArgs x = {a, (__half*)k16, (__half*)v16, meta16};
         static SmemLimit none;
         const dim3 grid(4 * dl_device_sm_count());
-        if (const int rc = hs == 128 ? ka_launch("dl_kv8_attention_prefill", kv8_expand_kernel<128>, none, grid, 1, 256, 0, pdl, stream, x)
-                                     : ka_launch("dl_kv8_attention_prefill", kv8_expand_kernel<64>, none, grid, 1, 256, 0, pdl, stream, x)) return rc;
-        return dl_attention_prefill_tc_typed(q, M, n_heads, cache->n_kv_heads, hs, k16, v16, pos, slot, block_table, max_pages, KV8_PAGE, meta16,
-                                             xq_out, xh_out, out_mcap, y_out, y_type, cache->n_pages, 1, stream);
+        if (const int rc = hs == 128 ? ka_launch(who, kv8_expand_kernel<128>, none, grid, 1, 256, 0, pdl, stream, x) : ka_launch(who, kv8_expand_kernel<64>, none, grid, 1, 256, 0, pdl, stream, x)) return rc;
+        // items that leave half of the SMs without one go to several CTAs each
+        const int tiles = (M + 127) / 128, items = n_heads / cache->n_kv_heads % 2 == 0 ? tiles * (n_heads / 2) : (tiles + 1) / 2 * n_heads;
+        PtShares part = {};
+        if (2 * items <= pt_share_ctas()) {
+            part.arrived = reinterpret_cast<unsigned*>(scratch + KV8_META_BYTES);
+            part.norms = reinterpret_cast<float2*>(part.arrived + PT_SHARE_SLOTS * PT_SHARE_WARPS);
+            part.sums = reinterpret_cast<float4*>(part.norms + PT_SHARE_SLOTS * PT_SHARE_WARPS * 32);
+        }
+        return dl_attention_prefill_tc_typed(q, M, n_heads, cache->n_kv_heads, hs, k16, v16, pos, slot, block_table, max_pages, KV8_PAGE, meta16, xq_out, xh_out,
+                                             out_mcap, y_out, y_type, part.arrived != nullptr ? &part : nullptr, cache->n_pages, 1, stream);
     }
     return hs == 128 ? ka_prompt<128>(a, pdl, stream) : hs == 64 ? ka_prompt<64>(a, pdl, stream) : ka_prompt<32>(a, pdl, stream);
 }

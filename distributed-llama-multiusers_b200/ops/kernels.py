@@ -407,7 +407,7 @@ def kv8_attention(q, M: int, n_heads: int, pos, slot, block_table, cache: Kv8Cac
 class Kv8Workspace(NamedTuple):
     k16: torch.Tensor          # fp16, shaped like the cache's codes
     v16: torch.Tensor
-    meta: torch.Tensor
+    scratch: torch.Tensor      # dl_kv8_prefill_scratch_bytes()
 
 
 def kv8_widens(rows: int, n_heads: int, head_size: int) -> bool:
@@ -421,7 +421,7 @@ def kv8_prefill_workspace(n_pages: int, n_kv_heads: int, head_size: int, max_row
     if head_size < 64 or max_rows < 16:
         return None
     pages = [torch.zeros(n_pages, n_kv_heads, PAGE_SIZE, head_size, dtype=torch.float16, device=device) for _ in range(2)]
-    return Kv8Workspace(*pages, torch.zeros(17, dtype=torch.int32, device=device))
+    return Kv8Workspace(*pages, torch.zeros(cuda_lib().dl_kv8_prefill_scratch_bytes(head_size), dtype=torch.uint8, device=device))
 
 
 def kv8_attention_prefill(q, M: int, n_heads: int, pos, slot, block_table, meta, cache: Kv8Cache, workspace=None, xq_out=None, xh_out=None, out_mcap: int = 0,
@@ -432,15 +432,16 @@ def kv8_attention_prefill(q, M: int, n_heads: int, pos, slot, block_table, meta,
     ldq, ldy, y_type = _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out)
     if meta.dtype is not torch.int32 or meta.get_device() != cache.index or not meta.is_contiguous() or meta.numel() < 3:
         raise ValueError("meta is a contiguous int32 tensor [n_seg, begin, end, ...]")
-    k16 = v16 = meta16 = None
+    k16 = v16 = scratch = None
     if workspace is not None:
-        k16, v16, meta16 = workspace
+        k16, v16, scratch = workspace
         if k16.shape != cache.k.shape or v16.shape != cache.k.shape or k16.dtype is not torch.float16 or v16.dtype is not torch.float16 \
-                or not k16.get_device() == v16.get_device() == meta16.get_device() == cache.index \
-                or not k16.is_contiguous() or not v16.is_contiguous() or meta16.dtype is not torch.int32 or meta16.numel() < 17 or not meta16.is_contiguous():
+                or not k16.get_device() == v16.get_device() == scratch.get_device() == cache.index \
+                or not k16.is_contiguous() or not v16.is_contiguous() or not scratch.is_contiguous() \
+                or scratch.nbytes < cuda_lib().dl_kv8_prefill_scratch_bytes(cache.head_size):
             raise ValueError("the workspace is not one of kv8_prefill_workspace() for this cache")
-        k16, v16, meta16 = k16.data_ptr(), v16.data_ptr(), meta16.data_ptr()
-    check(cuda_lib().dl_kv8_attention_prefill(q.data_ptr(), ldq, n_heads, *rows, meta.data_ptr(), cache.ref, k16, v16, meta16, _p(xq_out), _p(xh_out),
+        k16, v16, scratch = k16.data_ptr(), v16.data_ptr(), scratch.data_ptr()
+    check(cuda_lib().dl_kv8_attention_prefill(q.data_ptr(), ldq, n_heads, *rows, meta.data_ptr(), cache.ref, k16, v16, scratch, _p(xq_out), _p(xh_out),
                                               out_mcap, _p(y_out), ldy, y_type, 1 if pdl else 0, _stream()), "dl_kv8_attention_prefill")
     lib.count_launch()
 

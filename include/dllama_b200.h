@@ -233,10 +233,12 @@ int dl_kv8_read(const int* pos, const int* slot, const int* block_table, int M, 
 int dl_kv8_attention(const float* q, long long ldq, int n_heads, const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const DlKv8Cache* cache /*host*/, int n_splits, void* scratch,
                      uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, const int* row_skip, int pdl, void* stream);
 /* dl_attention_prefill over the 8-bit cache (meta as there; a segment of which a sequence, position or page is not in the tables: NaN in the rows that see it, or in
- * all of its rows).  k16 / v16 / meta16: NULL, or a workspace for one launch at a time, fp16 [n_pages][n_kv_heads][32][head_size] twice and int[17]: pages of heads
- * of 128 with more than 4096 rows times heads, of 64 with more than 7168, are then widened once, and multiplied on tcgen05 (keys and values beyond fp16's range saturate) */
+ * all of its rows).  k16 / v16 / scratch16: NULL, or a workspace for one launch at a time, fp16 [n_pages][n_kv_heads][32][head_size] twice and dl_kv8_prefill_scratch_bytes()
+ * zeroed once (all aligned to 16 bytes): pages of heads of 128 with more than 4096 rows times heads, of 64 with more than 7168, are then widened once, and multiplied on
+ * tcgen05 (keys and values beyond fp16's range saturate) */
+long long dl_kv8_prefill_scratch_bytes(int head_size);
 int dl_kv8_attention_prefill(const float* q, long long ldq, int n_heads, const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const int* meta /*device*/, const DlKv8Cache* cache /*host*/,
-                             void* k16, void* v16, int* meta16, uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, int pdl,
+                             void* k16, void* v16, void* scratch16, uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, int pdl,
                              void* stream);
 
 /* Kernels that wait on copies inside a CTA (dl_attention_prefill_tc, dl_window_attention_tc's prompts, dl_attention on a ring of pages, dl_gemv_q40, dl_gemm_q40_tc,

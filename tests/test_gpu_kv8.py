@@ -348,6 +348,8 @@ PROMPT_REL = 4e-3
     (4, 2, 128, [(2, 10, 40), (45, 0, 90)]), (8, 8, 128, [(0, 0, 700)]), (16, 1, 128, [(5, 900, 300)]), (8, 2, 128, [(0, 0, 257), (260, 130, 384)]),
     (5, 1, 128, [(1, 77, 900)]), (16, 1, 64, [(0, 3, 50)]), (6, 2, 32, [(1, 60, 45)]), (5, 1, 128, [(0, 100, 17), (20, 0, 1)]), (32, 8, 128, [(0, 1000, 100)]), (8, 1, 64, [(0, 2500, 31)]),
     (32, 8, 64, [(0, 10, 230)]), (5, 1, 64, [(1, 77, 1450)]), (8, 8, 64, [(0, 100, 930)]), (16, 2, 64, [(0, 0, 257), (260, 130, 200)]),
+    # (few rows behind many tokens: several CTAs for an item)
+    (16, 2, 128, [(0, 2500, 260), (300, 40, 100)]), (8, 8, 128, [(3, 2600, 530)]), (5, 1, 64, [(0, 3000, 1440)]), (4, 1, 128, [(1, 9000, 1100)]), (32, 8, 64, [(0, 5000, 129), (130, 2100, 120)]),
 ])
 def test_attention_prefill(heads, kv, hs, segs):
     k = K()
@@ -378,6 +380,28 @@ def test_attention_prefill(heads, kv, hs, segs):
             k.kv8_attention_prefill(q.cuda(), M, heads, *where, meta, cache, workspace=w, y_out=y)
             _near(y[covered], ref[covered], PROMPT_REL + STEP[t])
             assert (y[~covered] == 7.0).all()                     # rows outside the segments are left alone
+
+
+@pytest.mark.parametrize("heads,kv,hs,rows,context", [(16, 4, 128, 300, 700), (5, 5, 128, 830, 2600), (40, 8, 64, 200, 1500), (32, 8, 64, 250, 2500)])
+def test_attention_prefill_into_the_cast_for_the_next_matmul(heads, kv, hs, rows, context):
+    from dllama_b200.ops import quant
+    from test_gpu_kernels import _decode_xh, _decode_xq
+    k = K()
+    rng = np.random.default_rng(rows)
+    M, mcap = rows + 1, (rows + 8) // 8 * 8
+    bt, n_pages = _table(rng, [context + rows])
+    cache = k.Kv8Cache(*_dev(*_cache(rng, n_pages, kv, hs)))
+    where = (_i32([0] + list(range(context, context + rows))), _i32([0] * M), torch.from_numpy(bt).cuda())
+    q = torch.from_numpy(rng.standard_normal((M, heads * hs)).astype(np.float32)).cuda()
+    assert k.kv8_widens(M, heads, hs)
+    work = k.kv8_prefill_workspace(n_pages, kv, hs, M, "cuda")
+    xq, xh, y = k.alloc_xq(heads * hs, mcap, "cuda"), k.alloc_xh(heads * hs, mcap, "cuda"), torch.zeros(M, heads * hs, device="cuda")
+    k.kv8_attention_prefill(q, M, heads, *where, _i32([1, 1, M]), cache, work, xq, xh, mcap, y)
+    got = y.cpu().numpy()[1:]
+    dq = _decode_xq(xq, heads * hs, mcap, M)[0][1:]
+    np.testing.assert_allclose(dq, quant.q80_roundtrip(got), rtol=0, atol=np.abs(got).max() / 127 * 1.01)          # a code beside a border
+    np.testing.assert_allclose(_decode_xh(xh, heads * hs, mcap, M)[1:], dq, rtol=2e-3, atol=1e-7)
+    assert not _decode_xq(xq, heads * hs, mcap, M)[0][0].any()                                                      # the row outside the segment
 
 
 @pytest.mark.parametrize("workspace,hs", [(False, 128), (True, 128), (False, 64), (True, 64)])
