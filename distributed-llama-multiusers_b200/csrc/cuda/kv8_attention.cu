@@ -847,32 +847,36 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const __grid_constant__
     const int tid = threadIdx.x, kv = x.a.c.n_kv_heads;
     pdl_launch_dependents();
     pdl_wait();
-    if (tid == 0) {
+    if (tid < 8) {                                             // a lane for each segment
         const int n = max(0, min(x.a.meta[0], 8));
-        int at = 0;
-        for (int i = 0; i < 8; i++) {
-            first[i] = at;
-            const int b = i < n ? x.a.meta[1 + 2 * i] : 0, e = i < n ? x.a.meta[2 + 2 * i] : 0;
-            const bool rows = b >= 0 && e <= x.a.rows.M && e > b;
-            const int p = rows ? x.a.rows.pos[b] : 0, s = rows ? x.a.rows.slot[b] : 0;
-            ok[i] = rows && p >= 0 && p <= 0x7fffffff - (e - b) && kv8_tokens(x.a.rows, p + (e - b) - 1, s) > 0;
-            seg[i][0] = b; seg[i][1] = rows ? e : b; seg[i][2] = s;
-            if (ok[i]) at += (p + (e - b) + KV8_PAGE - 1) / KV8_PAGE * kv;
+        const int b = tid < n ? x.a.meta[1 + 2 * tid] : 0, e = tid < n ? x.a.meta[2 + 2 * tid] : 0;
+        const bool rows = b >= 0 && e <= x.a.rows.M && e > b;
+        const int p = rows ? x.a.rows.pos[b] : 0, s = rows ? x.a.rows.slot[b] : 0;
+        const bool there = rows && p >= 0 && p <= 0x7fffffff - (e - b) && kv8_tokens(x.a.rows, p + (e - b) - 1, s) > 0;
+        int upto = there ? (p + (e - b) + KV8_PAGE - 1) / KV8_PAGE * kv : 0;
+#pragma unroll
+        for (int w = 1; w < 8; w <<= 1) {
+            const int ahead = __shfl_up_sync(0xffu, upto, w);
+            if (tid >= w) upto += ahead;
         }
-        first[8] = at;
+        if (tid == 0) first[0] = 0;
+        first[tid + 1] = upto;
+        seg[tid][0] = b; seg[tid][1] = rows ? e : b; seg[tid][2] = s;
+        ok[tid] = there;
     }
     __syncthreads();
-    // pages that are not there: the first CTA, which lists the segments, takes theirs as one that is not in the tables
-    for (int i = 0; i < 8; i++) {
-        if (!ok[i]) continue;
-        const int* bt = x.a.rows.block_table + (size_t)seg[i][2] * x.a.rows.max_pages;
-        const int pages = (first[i + 1] - first[i]) / kv;
-        bool bad = false;
-        if (blockIdx.x == 0)
+    if (blockIdx.x == 0) {
+        // pages that are not there: this CTA, which lists the segments, takes theirs as one that is not in the tables
+        for (int i = 0; i < 8; i++) {
+            if (first[i + 1] == first[i]) continue;
+            const int* bt = x.a.rows.block_table + (size_t)seg[i][2] * x.a.rows.max_pages;
+            const int pages = (first[i + 1] - first[i]) / kv;
+            bool bad = false;
             for (int p = tid; p < pages; p += 256) bad |= (unsigned)bt[p] >= (unsigned)x.a.rows.n_pages;
-        if (__syncthreads_or(bad) && tid == 0) ok[i] = 0;
+            if (__syncthreads_or(bad) && tid == 0) ok[i] = 0;
+        }
+        __syncthreads();
     }
-    __syncthreads();
     if (blockIdx.x == 0) {
         if (tid == 0) {
             int n = 0;
