@@ -7,6 +7,9 @@
 // A code is a rounding, and an input a hair beside a border lands on either side of it: so that the same rows give the same codes however they are
 // computed, keys are turned in 64 bits (angle, sine, cosine and both products) and rounded once to f32, and x * factor goes to the nearest integer in
 // one rounding, an fma with 1.5 2^23.  Queries take f32 products of the same sines and cosines.  The sines of a row are formed once for all heads.
+//
+// What bounds both: the bytes, for many rows, else one chain of latencies.  Written, 32 query heads and 8 key/value heads of 128: one row 3.1 us, 32 3.3, 4001 (172 MB) 37.6,
+// 4.6 TB/s; read as fp16: 4001 rows 8.3 us, 100003 (621 MB) 101.9, 6.1 TB/s, of which a copy reaches 6.45.
 #include <type_traits>
 #include "epilogue.cuh"
 #include "kv8.cuh"
@@ -33,7 +36,7 @@ template <bool VEC> DL_DEVINL float4 kv8_fetch(const float* src, bool live) {
 }
 
 // grid (M, shares of a row's heads).  A warp takes a "unit" of 32 / (HS / 4) heads of one kind at a time, a lane four neighbouring values of the same place in
-// every head, so that it reads its sines once a row
+// every head, so that it reads its sines once a row; six units in flight (4001 rows of 48 heads of 128 37 us, 38.5 with one)
 template <int HS, bool VEC>
 __global__ void __launch_bounds__(KV8_WRITE_WARPS * 32) kv8_write_kernel(const __grid_constant__ Kv8WriteArgs a) {
     constexpr int LPH = HS / 4, HPW = 32 / LPH, AHEAD = 6;     // lanes a head, heads a unit, units in flight
@@ -125,7 +128,7 @@ template <> DL_DEVINL __nv_bfloat16 kv8_from_float<__nv_bfloat16>(float x) { ret
 
 #define KV8_READ_WARPS 8
 #define KV8_READ_ROWS 32       // most rows of a CTA
-#define KV8_READ_AHEAD 8       // pieces of a lane in flight
+#define KV8_READ_AHEAD 8       // pieces of a lane in flight (100003 tokens of 8 heads of 128 into fp16: 102 us, 165 with one)
 
 // a warp takes a row at a time, a lane the codes of 16 bytes of output; rows without a token read as zeros, rows that are not in the tables as NaN
 template <int HS, typename T, bool VEC>

@@ -106,8 +106,8 @@ DL_DEVINL void kv8_store4(const Kv8AttArgs& a, int m, int col, float4 y, bool li
 // A warp takes a page (32 tokens) at a time through a private ring of cp.async stages, 16-byte pieces XOR-swizzled by the token so that both ldmatrix
 // forms are free of conflicts: no barrier between warps until the final merge.
 //
-// What bounds it: the cache's bytes for long contexts, a chain of latencies for short ones.  32 rows of 1500 to 3000 tokens (8 kv heads of 128, 152 MB) 31 us,
-// 4.9 TB/s (the same loads without the arithmetic 27); one row of 100003 tokens 40 us, 5.3 TB/s.  A page takes a warp 1240 clk from end to end (260 of them its 32 MMAs,
+// What bounds it: the cache's bytes for long contexts, a chain of latencies for short ones.  32 rows of 1500 to 3000 tokens (8 kv heads of 128, 152 MB) 29.6
+// us, 5.1 TB/s (the same loads without the arithmetic 27.3); one row of 100003 tokens 38.5 us, 5.5 TB/s; one of 192 tokens 4.5 us.  A page takes a warp 1240 clk from end to end (260 of them its 32 MMAs,
 // 190 the special-function unit's 24 conversions and exponentials) and an SM with three CTAs 110.  Integer sums that stay in the accumulators from page to page take
 // 3 % off that and put it back on in the end, where they are converted.  One CTA of eight warps per SM that walks an equal stretch of all
 // rows' pages evens out the SMs' loads (256 CTAs on 148 SMs: 1.5 to 1), but every change of row empties its pipeline: 45 us.
@@ -511,6 +511,11 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
 // weights are fp16 here (2^-12 of themselves), values are widened in registers -- codes are exact in fp16 -- and sums are the f32 accumulators of m16n8k16.
 // p = 2^(s - ref) goes by a reference that moves only when a score is more than 2^8 above it, or a weight outgrows fp16: a vote of the warp, so that a page in the
 // steady state takes no exchange for a running maximum and no rescaling.
+//
+// What bounds it: a warp's chain of latencies through a page, with two warps of 218 registers on each scheduler (64 MMAs a page, the tensor pipe is 14 % busy, a
+// third of the clocks issue).  100 rows of 32 heads on 8 of 128 behind 1000 tokens 18.8 us, 500 of 64 behind none 21.  32 stacked rows a CTA, which halves the
+// widening, takes 34 % more for 30 rows of heads of 64 behind 1000 tokens (there are half the CTAs) and as much for 200; the next page's scores ahead of this one's
+// products spill.
 // ------------------------------------------------------------------------------------------------
 template <int HS, int ST>
 __global__ void __launch_bounds__(KA_WARPS * 32, HS == 128 ? 2 : 4) kv8_prompt_kernel(const __grid_constant__ Kv8AttArgs a) {
@@ -827,7 +832,8 @@ static int ka_prompt(const Kv8AttArgs& a, int pdl, void* stream) {
 // ------------------------------------------------------------------------------------------------
 // Long prompt chunks of heads of 64 and 128: the segments' pages widened once to fp16 (fp16(code * scale): 2^-12 of a value, the queries of that kernel are rounded alike),
 // then the tcgen05 kernel of the fp16 cache on them, under the same page numbers.  Widening inside that kernel would be done again by every CTA that meets a page
-// (rows / 128 * heads / 2 of them).  4001 rows: 12 MB in and 16 MB out, beside 131 GFLOP.
+// (rows / 128 * heads / 2 of them).  4001 rows behind 77 tokens: 8 MB in and 17 MB out, beside 136 GFLOP; both kernels 150 us, 908 TFLOP/s (174 with inputs in turn).
+// Eight lanes list a segment each: one thread after the other, and every CTA for pages that are not there, took 0.8 us more.
 //
 // A line with a NaN (of the key or the value) becomes a key of NaN and a value of zeros: the rows that see it give NaN, and the weights of 0 that others
 // have for it do not.  Values beyond fp16's range saturate.  What that kernel does not look at is looked at here: the segments that are in the tables are listed
