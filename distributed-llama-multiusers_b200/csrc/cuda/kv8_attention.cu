@@ -25,6 +25,7 @@ struct Kv8AttArgs {
     int heads;
     const int* row_skip;       // NULL, or row_skip[m] != 0: not this launch's row
     const int* meta;           // NULL, or rows outside its segments are not this launch's
+    int n_seg;                 // segments that are looked at, at most
     uint8_t* xq_out;
     uint8_t* xh_out;
     int out_mcap;
@@ -534,8 +535,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, HS == 128 ? 2 : 4) kv8_prompt_k
     // stacked row s of the tile is pair s_lo + s = row * G + head of the group, row 0 (batch row m0) at position p0
     int tile = (gridDim.x - 1 - blockIdx.x) / n_cta, m0 = 0, end = 0;      // late tiles (long histories) first
     {
-        const int mine = lane < 17 ? a.meta[min(lane, 2 * min(max(a.meta[0], 0), 8))] : 0;      // (what lies behind the last segment is not read)
-        const int n_seg = min(__shfl_sync(0xffffffffu, mine, 0), 8);
+        const int mine = lane < 17 ? a.meta[min(lane, 2 * min(max(a.meta[0], 0), a.n_seg))] : 0;      // (what lies behind the last segment is not read)
+        const int n_seg = min(__shfl_sync(0xffffffffu, mine, 0), a.n_seg);
         int i = 0;
         for (; i < n_seg; i++) {
             m0 = __shfl_sync(0xffffffffu, mine, 1 + 2 * i);
@@ -854,7 +855,7 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const __grid_constant__
     pdl_launch_dependents();
     pdl_wait();
     if (tid < 8) {                                             // a lane for each segment
-        const int n = max(0, min(x.a.meta[0], 8));
+        const int n = max(0, min(x.a.meta[0], x.a.n_seg));
         const int b = tid < n ? x.a.meta[1 + 2 * tid] : 0, e = tid < n ? x.a.meta[2 + 2 * tid] : 0;
         const bool rows = b >= 0 && e <= x.a.rows.M && e > b;
         const int p = rows ? x.a.rows.pos[b] : 0, s = rows ? x.a.rows.slot[b] : 0;
@@ -951,7 +952,7 @@ static int kv8_att_args(const char* who, const float* q, long long ldq, int n_he
         dl_set_error("%s: slabs of %d rows, %d columns", who, out_mcap, n_heads * hs);
         return -1;
     }
-    *a = {q, ldq, rows, *cache, n_heads, nullptr, nullptr, xq_out, xh_out, out_mcap, y_out, ldy, y_type,
+    *a = {q, ldq, rows, *cache, n_heads, nullptr, nullptr, 0, xq_out, xh_out, out_mcap, y_out, ldy, y_type,
           ((uintptr_t)y_out & (y_type == DL_KV8_F32 ? 15 : 7)) == 0 && ldy % 4 == 0};
     if (M > 65535) { dl_set_error("%s: %d rows (65535 at most)", who, M); return -1; }
     return 0;
@@ -986,14 +987,15 @@ extern "C" long long dl_kv8_prefill_scratch_bytes(int head_size) {
     return KV8_META_BYTES + pt_share_bytes(head_size);
 }
 
-extern "C" int dl_kv8_attention_prefill(const float* q, long long ldq, int n_heads, const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const int* meta, const DlKv8Cache* cache, void* k16, void* v16,
+extern "C" int dl_kv8_attention_prefill(const float* q, long long ldq, int n_heads, const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const int* meta, int max_seg, const DlKv8Cache* cache, void* k16, void* v16,
                                         void* scratch16, uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, int pdl, void* stream) {
     const char* who = "dl_kv8_attention_prefill";
     Kv8AttArgs a;
     if (const int rc = kv8_att_args(who, q, ldq, n_heads, pos, slot, block_table, M, n_slots, max_pages, cache, xq_out, xh_out, out_mcap, y_out, ldy, y_type, &a)) return rc;
-    if (meta == nullptr || (k16 == nullptr) != (v16 == nullptr) || (k16 == nullptr) != (scratch16 == nullptr)) { dl_set_error("dl_kv8_attention_prefill: a null pointer"); return -1; }
+    if (meta == nullptr || max_seg < 1 || (k16 == nullptr) != (v16 == nullptr) || (k16 == nullptr) != (scratch16 == nullptr)) { dl_set_error("dl_kv8_attention_prefill: a null pointer, or no place for a segment"); return -1; }
     if (M == 0) return 0;
     a.meta = meta;
+    a.n_seg = max_seg < 8 ? max_seg : 8;
     const int hs = cache->head_size;
     // (that kernel takes rows side by side, aligned)
     const bool dense = ldq == (long long)n_heads * hs && ((uintptr_t)q & 15) == 0 && (y_out == nullptr || (ldy == ldq && ((uintptr_t)y_out & 15) == 0));

@@ -426,8 +426,9 @@ def kv8_prefill_workspace(n_pages: int, n_kv_heads: int, head_size: int, max_row
 
 def kv8_attention_prefill(q, M: int, n_heads: int, pos, slot, block_table, meta, cache: Kv8Cache, workspace=None, xq_out=None, xh_out=None, out_mcap: int = 0,
                           y_out=None, pdl: bool = False):
-    """`attention_prefill` over an 8-bit cache: meta = [n_seg, begin0, end0, ...] (device int32), each range consecutive positions of one sequence; rows
-    outside are not touched.  workspace: kv8_prefill_workspace(), for one launch at a time."""
+    """`attention_prefill` over an 8-bit cache: meta = [n_seg, begin0, end0, ...] (device int32), each range consecutive positions of one sequence, no row
+    in two, eight at most (what is listed beyond that, or beyond the tensor's end, is not looked at); rows outside are not touched.  workspace: kv8_prefill_workspace(), for one launch at a time; with
+    it long prompts are multiplied in fp16 (queries, keys and values in its range)."""
     rows = _kv8_rows(M, pos, slot, block_table, cache)
     ldq, ldy, y_type = _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out)
     if meta.dtype is not torch.int32 or meta.get_device() != cache.index or not meta.is_contiguous() or meta.numel() < 3:
@@ -441,7 +442,7 @@ def kv8_attention_prefill(q, M: int, n_heads: int, pos, slot, block_table, meta,
                 or scratch.nbytes < cuda_lib().dl_kv8_prefill_scratch_bytes(cache.head_size):
             raise ValueError("the workspace is not one of kv8_prefill_workspace() for this cache")
         k16, v16, scratch = k16.data_ptr(), v16.data_ptr(), scratch.data_ptr()
-    check(cuda_lib().dl_kv8_attention_prefill(q.data_ptr(), ldq, n_heads, *rows, meta.data_ptr(), cache.ref, k16, v16, scratch, _p(xq_out), _p(xh_out),
+    check(cuda_lib().dl_kv8_attention_prefill(q.data_ptr(), ldq, n_heads, *rows, meta.data_ptr(), (meta.numel() - 1) // 2, cache.ref, k16, v16, scratch, _p(xq_out), _p(xh_out),
                                               out_mcap, _p(y_out), ldy, y_type, 1 if pdl else 0, _stream()), "dl_kv8_attention_prefill")
     lib.count_launch()
 

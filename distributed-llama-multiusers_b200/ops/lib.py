@@ -203,7 +203,7 @@ def cuda_lib():
     L.dl_kv8_write.argtypes = [vp, i64, i32, vp, *rows, vp, i64, vp, i32, vp]
     L.dl_kv8_read.argtypes = [*rows, vp, vp, vp, i64, i32, i32, vp]
     L.dl_kv8_attention.argtypes = [vp, i64, i32, *rows, vp, i32, vp, vp, vp, i32, vp, i64, i32, vp, i32, vp]
-    L.dl_kv8_attention_prefill.argtypes = [vp, i64, i32, *rows, vp, vp, vp, vp, vp, vp, vp, i32, vp, i64, i32, i32, vp]
+    L.dl_kv8_attention_prefill.argtypes = [vp, i64, i32, *rows, vp, i32, vp, vp, vp, vp, vp, vp, i32, vp, i64, i32, i32, vp]
     L.dl_kv8_prefill_scratch_bytes.argtypes, L.dl_kv8_prefill_scratch_bytes.restype = [i32], i64
     for name in ("dl_kv8_write", "dl_kv8_read", "dl_kv8_attention", "dl_kv8_attention_prefill"):
         getattr(L, name).restype = i32

@@ -404,6 +404,24 @@ def test_attention_prefill_into_the_cast_for_the_next_matmul(heads, kv, hs, rows
     assert not _decode_xq(xq, heads * hs, mcap, M)[0][0].any()                                                      # the row outside the segment
 
 
+@pytest.mark.parametrize("workspace", [False, True])
+def test_attention_prefill_looks_at_the_segments_that_are_there(workspace):
+    """meta that promises more than its tensor holds: the segments that it holds are taken, what lies behind is not read."""
+    k = K()
+    rng = np.random.default_rng(3)
+    heads, kv, hs, M = 32, 8, 128, 150
+    bt, n_pages = _table(rng, [M])
+    cache = k.Kv8Cache(*_dev(*_cache(rng, n_pages, kv, hs)))
+    where = (_i32(list(range(M))), _i32([0] * M), torch.from_numpy(bt).cuda())
+    q = torch.from_numpy(rng.standard_normal((M, heads * hs)).astype(np.float32)).cuda()
+    work = k.kv8_prefill_workspace(n_pages, kv, hs, M, "cuda") if workspace else None
+    holds = _i32([8, 0, 100, 100, 140, 140, 150])
+    y, ref = torch.full((M, heads * hs), 7.0, device="cuda"), torch.full((M, heads * hs), 7.0, device="cuda")
+    k.kv8_attention_prefill(q, M, heads, *where, holds[:5], cache, work, y_out=y)
+    k.kv8_attention_prefill(q, M, heads, *where, _i32([2, 0, 100, 100, 140]), cache, work, y_out=ref)
+    assert torch.equal(y, ref) and (y[140:] == 7.0).all() and not (y[:140] == 7.0).any()
+
+
 @pytest.mark.parametrize("workspace,hs", [(False, 128), (True, 128), (False, 64), (True, 64)])
 def test_attention_prefill_of_unusual_lines(workspace, hs):
     """A line with a NaN is seen by the rows from its token on, and by no other; a segment of a sequence, a position or a page that is not there is NaN;

@@ -68,7 +68,7 @@ def test_library_refuses_caches_and_rows(cache, rows):
     c, r = _cache(**cache), _rows(**rows)
     for rc in (L.dl_kv8_write(A, 512, 4, None, *r, A, 256, c, 0, None), L.dl_kv8_read(*r, c, A, A, 128, 0, 0, None),
                L.dl_kv8_attention(A, 256, 4, *r, c, 1, None, None, None, 0, A, 256, 0, None, 0, None),
-               L.dl_kv8_attention_prefill(A, 256, 4, *r, A, c, None, None, None, None, None, 0, A, 256, 0, 0, None)):
+               L.dl_kv8_attention_prefill(A, 256, 4, *r, A, 1, c, None, None, None, None, None, 0, A, 256, 0, 0, None)):
         with pytest.raises(NativeLibraryError):
             check(rc, "dl_kv8")
 
@@ -85,15 +85,16 @@ def test_library_refuses_arguments():
         bad.append(L.dl_kv8_attention(A, ldq, heads, *r, c, splits, scratch, xq, None, mcap, y, ldy, t, None, 0, None))
     bad.append(L.dl_kv8_attention(A, 256, 4, *_rows(M=65536), c, 1, None, None, None, 0, A, 256, 0, None, 0, None))
     bad.append(L.dl_kv8_attention(A, 256, 4, *_rows(M=10000), c, 2, A, None, None, 0, A, 256, 0, None, 0, None))       # more units than there are counters
-    bad.append(L.dl_kv8_attention_prefill(A, 256, 4, *r, None, c, None, None, None, None, None, 0, A, 256, 0, 0, None))
-    bad.append(L.dl_kv8_attention_prefill(A, 256, 4, *r, A, c, A, None, None, None, None, 0, A, 256, 0, 0, None))
-    bad.append(L.dl_kv8_attention_prefill(A, 256, 4, *r, A, c, None, None, A, None, None, 0, A, 256, 0, 0, None))
+    bad.append(L.dl_kv8_attention_prefill(A, 256, 4, *r, A, 0, c, None, None, None, None, None, 0, A, 256, 0, 0, None))
+    bad.append(L.dl_kv8_attention_prefill(A, 256, 4, *r, None, 1, c, None, None, None, None, None, 0, A, 256, 0, 0, None))
+    bad.append(L.dl_kv8_attention_prefill(A, 256, 4, *r, A, 1, c, A, None, None, None, None, 0, A, 256, 0, 0, None))
+    bad.append(L.dl_kv8_attention_prefill(A, 256, 4, *r, A, 1, c, None, None, A, None, None, 0, A, 256, 0, 0, None))
     assert all(rc != 0 for rc in bad), bad
     # nothing to do: no launch
     none = _rows(M=0)
     assert L.dl_kv8_write(A, 512, 4, None, *none, A, 256, c, 0, None) == 0 and L.dl_kv8_read(*none, c, A, A, 128, 0, 0, None) == 0
     assert L.dl_kv8_attention(A, 256, 4, *none, c, 1, None, None, None, 0, A, 256, 0, None, 0, None) == 0
-    assert L.dl_kv8_attention_prefill(A, 256, 4, *none, A, c, None, None, None, None, None, 0, A, 256, 0, 0, None) == 0
+    assert L.dl_kv8_attention_prefill(A, 256, 4, *none, A, 1, c, None, None, None, None, None, 0, A, 256, 0, 0, None) == 0
 
 
 @pytest.mark.parametrize("M,heads,kv,pages,want", [(1, 32, 8, 6, 1), (1, 32, 8, 125, 15), (1, 32, 8, 4000, 32), (8, 32, 8, 4000, 5), (32, 32, 8, 4000, 1), (1, 16, 1, 4000, 32), (4, 128, 8, 4000, 4), (7, 64, 8, 157, 5), (500, 32, 8, 100, 1)])
