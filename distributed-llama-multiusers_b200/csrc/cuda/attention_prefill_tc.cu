@@ -324,22 +324,24 @@ struct PtWaits {
 // a long item go to as many CTAs as there are for each.  Two tiles in one CTA take 1.75 us a step, a single one 1.03, and the join 5 us more: 130 rows of 32 heads
 // behind 2000 tokens 37 us alike, behind 8000 92 without shares and 63 with them; 512 rows (two shares) behind none 21 / 27, behind 4000 62 / 61, behind 16000 182 / 159
 // (those of heads of 64 behind 16000 156 / 122).  Item `idx` of the order that all roles of all CTAs walk; false behind the last one.
-DL_DEVINL bool pt_item(const PtArgs& a, const int (*seg)[4], int n_seg, int idx, PtItem& it) {
+template <bool SHARES> DL_DEVINL bool pt_item(const PtArgs& a, const int (*seg)[4], int n_seg, int idx, PtItem& it) {
     const int rep = a.n_heads / a.n_kv_heads;
     const bool even = rep % 2 == 0;
-    int tiles = 0, pairs = 0, last = 0, spread = 1;
-    for (int i = 0; i < n_seg; i++) {
-        const int nt = (seg[i][1] + PT_ROWS - 1) / PT_ROWS;
-        tiles += nt;
-        pairs += even ? nt : (nt + 1) / 2;
-        last = max(last, seg[i][2] + seg[i][1]);
+    int tiles = 0, spread = 1;
+    for (int i = 0; i < n_seg; i++) tiles += (seg[i][1] + PT_ROWS - 1) / PT_ROWS;
+    if (SHARES) {
+        int pairs = 0, last = 0;
+        for (int i = 0; i < n_seg; i++) {
+            const int nt = (seg[i][1] + PT_ROWS - 1) / PT_ROWS;
+            pairs += even ? nt : (nt + 1) / 2;
+            last = max(last, seg[i][2] + seg[i][1]);
+        }
+        if (pairs > 0) spread = max(1, min((int)gridDim.x / (pairs * (even ? a.n_heads / 2 : a.n_heads)), last / (PT_KV * PT_LEAST_STEPS)));
+        if (spread == 2 && last < PT_KV * 32) spread = 1;
     }
-    if (a.part.arrived != nullptr && pairs > 0)
-        spread = max(1, min((int)gridDim.x / (pairs * (even ? a.n_heads / 2 : a.n_heads)), last / (PT_KV * PT_LEAST_STEPS)));
-    if (spread == 2 && last < PT_KV * 32) spread = 1;
     const bool single = spread == 1 && tiles * a.n_heads <= (int)gridDim.x, by_heads = !single && even, by_rows = !single && !by_heads;
-    const int cols = by_heads ? a.n_heads / 2 : a.n_heads, share = idx % spread;
-    idx /= spread;
+    const int cols = by_heads ? a.n_heads / 2 : a.n_heads, share = SHARES ? idx % spread : 0;
+    if (SHARES) idx /= spread;
     for (int i = 0; i < n_seg; i++) {
         const int nt = (seg[i][1] + PT_ROWS - 1) / PT_ROWS, groups = by_rows ? (nt + 1) / 2 : nt;
         if (idx >= groups * cols) { idx -= groups * cols; continue; }
@@ -359,7 +361,7 @@ DL_DEVINL bool pt_item(const PtArgs& a, const int (*seg)[4], int n_seg, int idx,
         it.kvh = it.head[0] / rep;
         it.shares = min(spread, max(1, it.J / PT_LEAST_STEPS));
         it.share = share;
-        if (spread > 1) {
+        if (SHARES && spread > 1) {
             const int per = (it.J + it.shares - 1) / it.shares, z0 = min(it.J, share * per), z1 = min(it.J, z0 + per);
 #pragma unroll
             for (int t = 0; t < 2; t++) it.jb[t] = max(0, min(it.jb[t], z1) - z0);
@@ -457,8 +459,9 @@ DL_DEVINL void pt_load_rows(const float* mine, uint8_t* tile, int r0, Ready read
     fence_proxy_async_smem();
 }
 
-// HS: head size; 64 (LINES: not) takes the first half of every tile and accumulator
-template <bool LINES, int HS = PT_HS>
+// HS: head size; 64 (LINES: not) takes the first half of every tile and accumulator.  SHARES (LINES: not): items may go to several CTAs (4001 rows, whose
+// items do not, take 1.2 % longer with it)
+template <bool LINES, int HS = PT_HS, bool SHARES = false>
 __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(const __grid_constant__ typename PtKernelArgs<LINES>::T a,
                                                                              const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -542,7 +545,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
             return round < n_seg;
         } else {
             const int G = gridDim.x, b = blockIdx.x;
-            return pt_item(a, seg, n_seg, round * G + ((round & 1) ? G - 1 - b : b), it);
+            return pt_item<SHARES>(a, seg, n_seg, round * G + ((round & 1) ? G - 1 - b : b), it);
         }
     };
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
@@ -721,7 +724,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                 }
                 if (jb == ja) continue;
             } else {
-                part = it.shares > 1 && it.share < it.shares && row0 < it.rows;
+                part = SHARES && it.shares > 1 && it.share < it.shares && row0 < it.rows;
                 if (jb == ja && !part) continue;
                 y16 = a.y_type != DL_KV8_F32;
                 if (a.y_out != nullptr) {
@@ -741,7 +744,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
             const float4* sums = nullptr;                        // of the first share's
             const float2* norms = nullptr;
             float top = 0.f;                                     // the shares' common reference
-            if constexpr (!LINES) {
+            if constexpr (SHARES) {
                 if (part) {
                     const size_t slot = (size_t)blockIdx.x * PT_SHARE_WARPS + warp, first = slot - it.share * PT_SHARE_WARPS;
                     a.part.norms[slot * 32 + lane] = make_float2(m_used, gave_up_s ? inv : jb > ja ? l : -1.f);
@@ -783,7 +786,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
             for (int ch = 0; ch < HS / 32; ch++) {
                 uint32_t o[32];
                 float f[32];
-                if (LINES || !part) {
+                if (!SHARES || !part) {
                     tmem_ld_32x32b_x32(T_O + ch * 32, o);
                     tmem_ld_wait();
 #pragma unroll
@@ -1039,8 +1042,10 @@ int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_h
     const long long rows = (long long)n_cache_pages * n_kv_heads * 32;
     if (pt_make_map(&kmap, k_cache, rows, head_size, false) != 0 || pt_make_map(&vmap, v_cache, rows, head_size, false) != 0) return -1;
     const size_t smem = PT_SMEM;
-    static SmemLimit given, given_64;
-    if (const int rc = head_size == 64 ? dl_smem_limit("attention_prefill_tc", attention_prefill_tc_kernel<false, 64>, smem, given_64) : dl_smem_limit("attention_prefill_tc", attention_prefill_tc_kernel<false>, smem, given)) return rc;
+    static SmemLimit given[4];
+    const int which = (head_size == 64) + 2 * (shares != nullptr);
+    auto* kernel = which == 0 ? attention_prefill_tc_kernel<false> : which == 1 ? attention_prefill_tc_kernel<false, 64> : which == 2 ? attention_prefill_tc_kernel<false, 128, true> : attention_prefill_tc_kernel<false, 64, true>;
+    if (const int rc = dl_smem_limit("attention_prefill_tc", kernel, smem, given[which])) return rc;
     cudaLaunchConfig_t cfg = {};
     const long long most = ((long long)(M + PT_ROWS - 1) / PT_ROWS + PT_MAX_SEG - 1) * n_heads;        // upper bound of the tiles of all segments
     cfg.gridDim = dim3((unsigned)(shares != nullptr ? pt_share_ctas() : most < dl_device_sm_count() ? most : dl_device_sm_count()));
@@ -1054,7 +1059,7 @@ int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_h
         cfg.attrs = attr;
         cfg.numAttrs = 1;
     }
-    cudaError_t e = head_size == 64 ? cudaLaunchKernelEx(&cfg, attention_prefill_tc_kernel<false, 64>, a, kmap, vmap) : cudaLaunchKernelEx(&cfg, attention_prefill_tc_kernel<false>, a, kmap, vmap);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, kmap, vmap);
     if (e != cudaSuccess) { dl_set_error("attention_prefill_tc launch: %s", cudaGetErrorString(e)); return -(int)e; }
     return 0;
 }
