@@ -102,7 +102,8 @@ DL_DEVINL void kv8_store4(const Kv8AttArgs& a, int m, int col, float4 y, bool li
 //   a query   n = rint(q 8355000 / max|q|), three signed digits of a head in rows g, g + 8, g + 4 (24 bits of the head's largest value)
 //   a weight  n = rint(p s_v 2^(22 - e)), three unsigned digits; e: exponent of the largest p s_v that the row has met (held like a softmax maximum: what
 //             was summed is rescaled when it moves), s_v the value's scale.  So each weight is off by 2^-23 of the largest one at most, as a f32 sum is
-// Four heads fill the 16 rows.
+// Four heads fill the 16 rows; more heads of a key/value head go to CTAs of their own, which find its pages in L2 (eight in two tiles of one CTA, 255 registers: one
+// row of 30000 tokens 22.4 us for 19.7, 6 rows of 3000 13.9 for 12.6, 40 rows 53 for 47, with heads of 64 31 for 34).
 //
 // A warp takes a page (32 tokens) at a time through a private ring of cp.async stages, 16-byte pieces XOR-swizzled by the token so that both ldmatrix
 // forms are free of conflicts: no barrier between warps until the final merge.
@@ -249,10 +250,10 @@ struct Kv8Work {               // what the launch adds to the arguments of decod
 };
 
 // grid (kv heads * groups, M, splits): the splits that short rows do not take come last, when the others have their SMs
-template <int HS, int MT, int ST>
+template <int HS, int ST>
 __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __grid_constant__ Kv8AttArgs a, const __grid_constant__ Kv8Work wk) {
     constexpr int CH = HS / 16, KS = HS / 32, NT = HS / 8, STAGE = KaStage<HS>::BYTES, CODES = KaStage<HS>::CODES;
-    constexpr int SR = MT * 4;                                             // heads of the CTA
+    constexpr int SR = 4;                                                  // heads of the CTA
     constexpr int TOP = 22;                                                // a weight's integer is at most 2^(TOP + 1)
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, qd = lane & 3;
@@ -263,12 +264,9 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
     pdl_wait();
     if (a.row_skip != nullptr && a.row_skip[m0] != 0) return;
     const int pos = a.rows.pos[m0], slot = a.rows.slot[m0];
-    float x[MT][2 * KS][4];                                                // (asked for ahead of what hangs on pos)
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        const int h = mt * 4 + (g & 3);
-        ka_query<HS>(a.q + (size_t)m0 * a.ldq + (kvh * G + h_lo + (h < n_live ? h : 0)) * HS + qd * 4, ((uintptr_t)a.q & 15) == 0 && (a.ldq & 3) == 0, x[mt]);
-    }
+    const int my_head = g & 3;
+    float x[2 * KS][4];                                                    // (asked for ahead of what hangs on pos)
+    ka_query<HS>(a.q + (size_t)m0 * a.ldq + (kvh * G + h_lo + (my_head < n_live ? my_head : 0)) * HS + qd * 4, ((uintptr_t)a.q & 15) == 0 && (a.ldq & 3) == 0, x);
     const int T0 = kv8_tokens(a.rows, pos, slot), T = max(T0, 0);
     bool bad = T0 < 0;
     const int n_pages = (T + KV8_PAGE - 1) / KV8_PAGE;
@@ -293,20 +291,13 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
 
-    uint32_t qf[MT][KS][4];
-    float fl[MT];
-    float o[MT][NT][2];
-    float run_m[MT], run_l[MT], run_w[MT];                     // maximum of scores, sum of weights (this lane's tokens), largest weight * scale
-    int ex[MT];                                                // exponent field of run_w: the unit of o
+    uint32_t qf[1][KS][4];
+    const float fl = ka_digits<HS, true>(x, my_head < n_live, lower, qf[0]);
+    float o[NT][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        fl[mt] = ka_digits<HS, true>(x[mt], mt * 4 + (g & 3) < n_live, lower, qf[mt]);
-        run_m[mt] = -INFINITY;
-        run_l[mt] = run_w[mt] = 0.f;
-        ex[mt] = 24;
-#pragma unroll
-        for (int n = 0; n < NT; n++) o[mt][n][0] = o[mt][n][1] = 0.f;
-    }
+    for (int n = 0; n < NT; n++) o[n][0] = o[n][1] = 0.f;
+    float run_m = -INFINITY, run_l = 0.f, run_w = 0.f;         // maximum of scores, sum of weights (this lane's tokens), largest weight * scale
+    int ex = 24;                                               // exponent field of run_w: the unit of o
     const uint32_t v_at = ka_value_row(lane) * HS, v_sw = ka_swizzle<HS>(ka_value_row(lane));
 
     int st = 0;
@@ -326,76 +317,69 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
         float sk[8], sv[8];
         ka_scales(scales, sk);
         ka_scales(scales + KV8_PAGE, sv);
-        int c[MT][4][4];
-        ka_scores<HS, MT>(kb, lane, qf, c);
+        int c[1][4][4];
+        ka_scores<HS, 1>(kb, lane, qf, c);
         uint32_t vf[CH][4];                                    // (asked for ahead of the weights)
 #pragma unroll
         for (int ch = 0; ch < CH; ch++) ka_ldm_bytes(vf[ch], vb + v_at + ((ch ^ v_sw) << 4));
-        uint32_t pa[MT][4];
-        float f[MT];
+        uint32_t pa[4];
+        float s[8], w[8], mx = -INFINITY;
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            float s[8], w[8], mx = -INFINITY;
+        for (int e = 0; e < 8; e++) {
+            s[e] = (float)(c[0][e >> 1][e & 1] * 256 + c[0][e >> 1][(e & 1) + 2]) * fl;
+            s[e] += __shfl_xor_sync(0xffffffffu, s[e], 16);
+            s[e] *= sk[e];
+            w[e] = sv[e];
+        }
+        if (left < KV8_PAGE) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                s[e] = (float)(c[mt][e >> 1][e & 1] * 256 + c[mt][e >> 1][(e & 1) + 2]) * fl[mt];
-                s[e] += __shfl_xor_sync(0xffffffffu, s[e], 16);
-                s[e] *= sk[e];
-                w[e] = sv[e];
-            }
-            if (left < KV8_PAGE) {
+            for (int e = 0; e < 8; e++)
+                if (qd * 8 + e >= left) { s[e] = -INFINITY; w[e] = 0.f; }
+        }
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (qd * 8 + e >= left) { s[e] = -INFINITY; w[e] = 0.f; }
-            }
+        for (int e = 0; e < 8; e++) mx = fmaxf(mx, s[e]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(run_m, mx), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float corr = ka_exp2(run_m - m_use);
+        run_m = m_new;
+        float sum = 0.f, big = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) mx = fmaxf(mx, s[e]);
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float m_new = fmaxf(run_m[mt], mx), m_use = m_new == -INFINITY ? 0.f : m_new;
-            const float corr = ka_exp2(run_m[mt] - m_use);
-            run_m[mt] = m_new;
-            float sum = 0.f, big = 0.f;
+        for (int e = 0; e < 8; e++) {
+            const float p = ka_exp2(s[e] - m_use);
+            sum += p;
+            w[e] *= p;
+            big = ka_max_nan(big, w[e]);
+        }
+        run_l = fmaf(run_l, corr, sum);
+        big = ka_max_nan(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = ka_max_nan(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        big = ka_max_nan(big, run_w * corr);
+        run_w = big;
+        const int e_new = min(max((int)(__float_as_uint(big) >> 23), 24), 254);
+        const float up = __uint_as_float((uint32_t)(TOP + 254 - e_new) << 23);
+        float f = corr * __uint_as_float((uint32_t)(ex - TOP) << 23) * up;
+        if (big != big) f = big;
+        ex = e_new;
+        uint32_t n[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float p = ka_exp2(s[e] - m_use);
-                sum += p;
-                w[e] *= p;
-                big = ka_max_nan(big, w[e]);
-            }
-            run_l[mt] = fmaf(run_l[mt], corr, sum);
-            big = ka_max_nan(big, __shfl_xor_sync(0xffffffffu, big, 1));
-            big = ka_max_nan(big, __shfl_xor_sync(0xffffffffu, big, 2));
-            big = ka_max_nan(big, run_w[mt] * corr);
-            run_w[mt] = big;
-            const int e_new = min(max((int)(__float_as_uint(big) >> 23), 24), 254);
-            const float up = __uint_as_float((uint32_t)(TOP + 254 - e_new) << 23);
-            f[mt] = corr * __uint_as_float((uint32_t)(ex[mt] - TOP) << 23) * up;
-            if (big != big) f[mt] = big;
-            ex[mt] = e_new;
-            uint32_t n[8];
+        for (int e = 0; e < 8; e++) n[e] = __float_as_uint(fmaf(w[e], up, 8388608.f));     // the integer in the low 23 bits (and 2^23 itself as its top byte)
+        const uint32_t sel = lower ? 0x5162u : 0x5140u;
 #pragma unroll
-            for (int e = 0; e < 8; e++) n[e] = __float_as_uint(fmaf(w[e], up, 8388608.f));     // the integer in the low 23 bits (and 2^23 itself as its top byte)
-            const uint32_t sel = lower ? 0x5162u : 0x5140u;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const uint32_t y = __byte_perm(n[4 * u], n[4 * u + 1], sel), z = __byte_perm(n[4 * u + 2], n[4 * u + 3], sel);
-                pa[mt][2 * u] = __byte_perm(y, z, 0x5410);
-                pa[mt][2 * u + 1] = lower ? __byte_perm(y, z, 0x7632) : 0u;
-            }
+        for (int u = 0; u < 2; u++) {
+            const uint32_t y = __byte_perm(n[4 * u], n[4 * u + 1], sel), z = __byte_perm(n[4 * u + 2], n[4 * u + 3], sel);
+            pa[2 * u] = __byte_perm(y, z, 0x5410);
+            pa[2 * u + 1] = lower ? __byte_perm(y, z, 0x7632) : 0u;
         }
 #pragma unroll
         for (int ch = 0; ch < CH; ch++) {
+            int y[4], z[4];
+            ka_mma_u8(y, pa, vf[ch][0], vf[ch][2]);
+            ka_mma_u8(z, pa, vf[ch][1], vf[ch][3]);
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                int y[4], z[4];
-                ka_mma_u8(y, pa[mt], vf[ch][0], vf[ch][2]);
-                ka_mma_u8(z, pa[mt], vf[ch][1], vf[ch][3]);
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    o[mt][2 * ch][e] = fmaf(o[mt][2 * ch][e], f[mt], (float)(y[e] * 256 + y[e + 2]));
-                    o[mt][2 * ch + 1][e] = fmaf(o[mt][2 * ch + 1][e], f[mt], (float)(z[e] * 256 + z[e + 2]));
-                }
+            for (int e = 0; e < 2; e++) {
+                o[2 * ch][e] = fmaf(o[2 * ch][e], f, (float)(y[e] * 256 + y[e + 2]));
+                o[2 * ch + 1][e] = fmaf(o[2 * ch + 1][e], f, (float)(z[e] * 256 + z[e + 2]));
             }
         }
         __syncwarp();
@@ -408,26 +392,23 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
     float* w_acc = reinterpret_cast<float*>(smem);             // [WARPS][SR][LD]
     float* w_ml = w_acc + KA_WARPS * SR * LD;                  // [WARPS][SR][2]
     int* s_last = reinterpret_cast<int*>(w_ml + KA_WARPS * SR * 2);
+    run_l += __shfl_xor_sync(0xffffffffu, run_l, 1);
+    run_l += __shfl_xor_sync(0xffffffffu, run_l, 2);
+    if (bad) run_l = __uint_as_float(0x7fffffffu);
+    const float unit = __uint_as_float((uint32_t)(ex - TOP) << 23) * (lower ? 256.f : 1.f / 256.f);
+    const int s = warp * SR + my_head;
+    // the upper lanes' digits go to the lower ones, which take the even n-tiles; and the other way round
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-        run_l[mt] += __shfl_xor_sync(0xffffffffu, run_l[mt], 1);
-        run_l[mt] += __shfl_xor_sync(0xffffffffu, run_l[mt], 2);
-        if (bad) run_l[mt] = __uint_as_float(0x7fffffffu);
-        const float unit = __uint_as_float((uint32_t)(ex[mt] - TOP) << 23) * (lower ? 256.f : 1.f / 256.f);
-        const int s = warp * SR + mt * 4 + (g & 3);
-        // the upper lanes' digits go to the lower ones, which take the even n-tiles; and the other way round
+    for (int n = 0; n < NT; n += 2) {
+        float v[2];
 #pragma unroll
-        for (int n = 0; n < NT; n += 2) {
-            float v[2];
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const float x0 = o[mt][n][e] * unit, x1 = o[mt][n + 1][e] * unit;
-                v[e] = (lower ? x0 : x1) + __shfl_xor_sync(0xffffffffu, lower ? x1 : x0, 16);
-            }
-            *reinterpret_cast<float2*>(w_acc + s * LD + qd * 2 + (lower ? n : n + 1) * 8) = make_float2(v[0], v[1]);
+        for (int e = 0; e < 2; e++) {
+            const float x0 = o[n][e] * unit, x1 = o[n + 1][e] * unit;
+            v[e] = (lower ? x0 : x1) + __shfl_xor_sync(0xffffffffu, lower ? x1 : x0, 16);
         }
-        if (lower && qd == 0) { w_ml[s * 2] = run_m[mt]; w_ml[s * 2 + 1] = run_l[mt]; }
+        *reinterpret_cast<float2*>(w_acc + s * LD + qd * 2 + (lower ? n : n + 1) * 8) = make_float2(v[0], v[1]);
     }
+    if (lower && qd == 0) { w_ml[s * 2] = run_m; w_ml[s * 2 + 1] = run_l; }
     __syncthreads();
     const bool single = n_eff == 1;
     for (int base = warp * 32; base < n_live * LPH; base += KA_WARPS * 32) {       // a lane takes four dimensions of a head
@@ -797,17 +778,13 @@ static int ka_launch(const char* who, K kernel, SmemLimit& given, dim3 grid, int
     return 0;
 }
 
-template <int HS, int MT>
-static int ka_decode_mt(const Kv8AttArgs& a, const Kv8Work& wk, dim3 grid, int pdl, void* stream) {
-    constexpr int ST = 256 / HS, smem = KA_WARPS * ST * KaStage<HS>::BYTES;
-    static_assert(KA_WARPS * MT * 4 * (KaSums<HS>::LD + 2) * 4 + 4 <= smem, "the merge fits the ring");
-    static SmemLimit given;
-    return ka_launch("dl_kv8_attention", kv8_attention_kernel<HS, MT, ST>, given, grid, 1, KA_WARPS * 32, smem, pdl, stream, a, wk);
-}
 template <int HS>
 static int ka_decode(const Kv8AttArgs& a, int n_splits, void* scratch, int pdl, void* stream) {
+    constexpr int ST = 256 / HS, smem = KA_WARPS * ST * KaStage<HS>::BYTES;
+    static_assert(KA_WARPS * 4 * (KaSums<HS>::LD + 2) * 4 + 4 <= smem, "the merge fits the ring");
+    static SmemLimit given;
     const int kv = a.c.n_kv_heads, G = a.heads / kv, M = a.rows.M;
-    Kv8Work wk = {n_splits, G > 8 ? 2 : 1, nullptr, nullptr, nullptr};
+    Kv8Work wk = {n_splits, (G + 3) / 4, nullptr, nullptr, nullptr};
     if (n_splits > 1) {
         if ((long long)M * kv * wk.groups * 4 > KA_COUNTER_BYTES) { dl_set_error("dl_kv8_attention: M*n_kv_heads too large for splits"); return -1; }
         uint8_t* at = reinterpret_cast<uint8_t*>(scratch);
@@ -815,8 +792,7 @@ static int ka_decode(const Kv8AttArgs& a, int n_splits, void* scratch, int pdl, 
         wk.part_o = reinterpret_cast<float*>(at + KA_COUNTER_BYTES);
         wk.part_ml = reinterpret_cast<float*>(at + KA_COUNTER_BYTES + ((long long)M * a.heads * n_splits * HS * 4 + 255) / 256 * 256);
     }
-    const dim3 grid(kv * wk.groups, M, n_splits);
-    return G <= 4 ? ka_decode_mt<HS, 1>(a, wk, grid, pdl, stream) : ka_decode_mt<HS, 2>(a, wk, grid, pdl, stream);
+    return ka_launch("dl_kv8_attention", kv8_attention_kernel<HS, ST>, given, dim3(kv * wk.groups, M, n_splits), 1, KA_WARPS * 32, smem, pdl, stream, a, wk);
 }
 template <int HS>
 static int ka_prompt(const Kv8AttArgs& a, int pdl, void* stream) {

@@ -371,13 +371,14 @@ def _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out):
 
 
 def kv8_attention_splits(M: int, n_heads: int, n_kv_heads: int, max_pages: int) -> int:
-    """Shares of the longest context that kv8_attention is given for M rows: as many CTAs as the SMs hold with some to spare (two an SM with more than
-    four query heads for each of 128, three otherwise), eight pages each or more; a row takes no more than its own context is worth.  8 kv heads of 128, us
-    with one split / this many / about twice as many: one row of 100003 tokens 528 / 38.5 / 54, 6 rows of 3000 20 / 10.1 / 13.3, 12 rows of 3000 19.7 / 15.8 / 20,
-    20 rows of 4000 30.8 / 28.1 / 30.3, 32 rows of 3000 29.7 / 29.7 / 37; eight heads for each: 4 rows of 5000 42 / 15.5 / 21, 10 of 3000 30 / 19.6 / 24."""
-    group = n_heads // n_kv_heads
-    units = max(1, M * n_kv_heads * (2 if group > 8 else 1))
-    return max(1, min((320 if group <= 4 else 288) // units, max_pages // 8, 32))
+    """Shares of the longest context that kv8_attention is given for M rows: as many CTAs as the SMs hold with some to spare (a CTA for four query heads at
+    most; more of them where those of one key/value head read the same pages), eight pages each or more; a row takes no more than its own context is worth.  8 kv
+    heads of 128, us with one split / this many / about twice as many: one row of 100003 tokens 528 / 38.5 / 54, 6 rows of 3000 20 / 10.1 / 13.3, 12 rows of 3000
+    19.7 / 15.8 / 20, 20 rows of 4000 30.8 / 28.1 / 30.3, 32 rows of 3000 29.7 / 29.7 / 37; eight heads for each: one row of 30000 165 / 20 / 23.5, 7 of 5000
+    24 / 17.5 / 20, of heads of 64 18 / 13.1 / 15.6."""
+    group = (n_heads // n_kv_heads + 3) // 4
+    units = max(1, M * n_kv_heads * group)
+    return max(1, min((320 if group == 1 else 400) // units, max_pages // 8, 32))
 
 
 @functools.lru_cache(maxsize=4096)
