@@ -243,13 +243,53 @@ DL_DEVINL void ka_scales(const float* at, float (&s)[8]) {
 template <int HS> struct KaSums { static constexpr int LD = HS + 8; };
 
 struct Kv8Work {               // what the launch adds to the arguments of decode rows
-    int n_splits, groups;      // groups: CTAs that share a key/value head's query heads
+    int n_splits, groups;      // shares of a row at most; CTAs that share a key/value head's query heads
+    int shares;                // shares of rows beyond the first that the launch has room for
+    float part;                // 1 / shares
     unsigned* counters;        // [M][kv heads * groups]
     float* part_o;             // [M][heads][n_splits][HS]
     float* part_ml;            // [M][heads][n_splits][2]
 };
 
-// grid (kv heads * groups, M, splits): the splits that short rows do not take come last, when the others have their SMs
+// Rows share the launch's CTAs by their lengths: of all pages a share has P = pages / wk.shares, a row as many shares as it has P, whole ones, one at least.  So one
+// user deep in a document beside many others is not one CTA's per head (32 rows of 32 heads, one of 30000 tokens, the others of 300: 119 us with shares by the number
+// of rows, 17.4 so), and rows of like lengths get what they would get by their number (us by their number / so: 2 rows of 3000 8.5 / 9.2, 12 12.9 / 13.0, 20 of 4000 28.2 /
+// 26.9, 32 of 3000 30.1 / 29.9, 64 of 1500 33.3 / 35.1).
+DL_DEVINL int ka_pages(const Kv8AttArgs& a, int m) {           // < 0: not this launch's row
+    if (m >= a.rows.M || (a.row_skip != nullptr && a.row_skip[m] != 0)) return -1;
+    const int t = kv8_tokens(a.rows, a.rows.pos[m], a.rows.slot[m]);
+    return t > 0 ? (t - 1) / KV8_PAGE + 1 : 0;
+}
+// 1 / P, from all rows' pages
+DL_DEVINL float ka_part(const Kv8Work& wk, unsigned total) { return __fdividef(1.f, fmaxf(8.f, (float)total * wk.part)); }
+// whole parts, of eight pages begun ones (one less is below the quotient, so those beyond the rows' first are wk.shares at most, even if it is off a little: every
+// warp finds the same numbers)
+DL_DEVINL int ka_shares(const Kv8Work& wk, int pages, float part) {
+    return pages <= KA_MIN_SPLIT_PAGES ? 1 : min(max((int)fmaf((float)pages, part, part == 0.125f ? 0.95f : 0.05f), 1), wk.n_splits);
+}
+// Of number idx among the shares that are not their row's first, in 32 rows whose shares the lanes have: row * 4096 + share * 64 + shares - 1, or -1 and idx less theirs
+DL_DEVINL int ka_find(int n, int lane, int& idx) {
+    int upto = n - 1;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+        const int ahead = __shfl_up_sync(0xffffffffu, upto, w);
+        if (lane >= w) upto += ahead;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, upto > idx);
+    const int l = hit != 0 ? __ffs(hit) - 1 : 31, found = l * 4096 + (idx - (upto - n + 1) + 1) * 64 + n - 1;
+    idx -= __shfl_sync(0xffffffffu, upto, 31);
+    return hit != 0 ? __shfl_sync(0xffffffffu, found, l) : -1;
+}
+// ... in more than 32 rows.  (Not inlined: what a launch of few rows does not run it does not fetch)
+__device__ __noinline__ int ka_find_in_many(const Kv8AttArgs& a, const Kv8Work& wk, int idx, float part, int lane) {
+    for (int base = 0; base < a.rows.M; base += 32) {
+        const int found = ka_find(ka_shares(wk, ka_pages(a, base + lane), part), lane, idx);
+        if (found >= 0) return base * 4096 + found;
+    }
+    return -1;
+}
+
+// grid (kv heads * groups, M + wk.shares): the rows' first shares, then the others
 template <int HS, int ST>
 __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __grid_constant__ Kv8AttArgs a, const __grid_constant__ Kv8Work wk) {
     constexpr int CH = HS / 16, KS = HS / 32, NT = HS / 8, STAGE = KaStage<HS>::BYTES, CODES = KaStage<HS>::CODES;
@@ -257,39 +297,67 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
     constexpr int TOP = 22;                                                // a weight's integer is at most 2^(TOP + 1)
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, qd = lane & 3;
-    const int kvh = blockIdx.x / wk.groups, m0 = blockIdx.y, sp = blockIdx.z;
+    const int kvh = blockIdx.x / wk.groups;
     const int G = a.heads / a.c.n_kv_heads, per = (G + wk.groups - 1) / wk.groups, h_lo = (blockIdx.x % wk.groups) * per, n_live = min(per, G - h_lo);
     const bool lower = g < 4;
     pdl_launch_dependents();
     pdl_wait();
-    if (a.row_skip != nullptr && a.row_skip[m0] != 0) return;
-    const int pos = a.rows.pos[m0], slot = a.rows.slot[m0];
+    const int further = (int)blockIdx.y - a.rows.M;            // < 0: a row's first share
+    const bool many = a.rows.M > 32, one = a.rows.M == 1;      // (one row: its number of shares hangs on nothing else; 0.7 us less than by the others' way)
+    int m0 = further < 0 ? blockIdx.y : 0, sp = one ? blockIdx.y : 0, n_eff = 1;
+    int mine = 0;                                              // pages of row `lane`, and of all rows that come to the lane (asked for with this CTA's own position)
+    unsigned ours = 0;
+    if (wk.n_splits > 1 && !one) {
+        mine = ka_pages(a, lane);
+        ours = max(mine, 0);
+        if (many) {
+#pragma unroll 4
+            for (int base = 32; base < a.rows.M; base += 32) ours += max(ka_pages(a, base + lane), 0);
+        }
+    }
     const int my_head = g & 3;
-    float x[2 * KS][4];                                                    // (asked for ahead of what hangs on pos)
-    ka_query<HS>(a.q + (size_t)m0 * a.ldq + (kvh * G + h_lo + (my_head < n_live ? my_head : 0)) * HS + qd * 4, ((uintptr_t)a.q & 15) == 0 && (a.ldq & 3) == 0, x);
+    float x[2 * KS][4];
+    auto ask = [&] { ka_query<HS>(a.q + (size_t)m0 * a.ldq + (kvh * G + h_lo + (my_head < n_live ? my_head : 0)) * HS + qd * 4, ((uintptr_t)a.q & 15) == 0 && (a.ldq & 3) == 0, x); };
+    if (further < 0 || one) {
+        ask();                                                 // (ahead of what hangs on positions)
+        if (a.row_skip != nullptr && a.row_skip[m0] != 0) return;
+    } else {
+        int idx = further;
+        const float part = ka_part(wk, __reduce_add_sync(0xffffffffu, ours));
+        const int found = many ? ka_find_in_many(a, wk, idx, part, lane) : ka_find(ka_shares(wk, mine, part), lane, idx);
+        if (found < 0) return;
+        m0 = found >> 12;
+        sp = (found >> 6) & 63;
+        n_eff = (found & 63) + 1;
+        ask();
+    }
+    const int pos = a.rows.pos[m0], slot = a.rows.slot[m0];
     const int T0 = kv8_tokens(a.rows, pos, slot), T = max(T0, 0);
     bool bad = T0 < 0;
     const int n_pages = (T + KV8_PAGE - 1) / KV8_PAGE;
-    const int n_eff = n_pages <= KA_MIN_SPLIT_PAGES ? 1 : min(wk.n_splits, (n_pages + 7) / 8);
-    if (sp >= n_eff) return;
-    const int pps = (n_pages + n_eff - 1) / n_eff, pg0 = sp * pps, pg1 = min(n_pages, pg0 + pps);
-    const int n_my = max(0, (pg1 - pg0 - warp + KA_WARPS - 1) / KA_WARPS);             // this warp's pages: pg0 + warp + 4 i
+    if (one) {
+        if (n_pages > KA_MIN_SPLIT_PAGES) n_eff = min(wk.n_splits, (n_pages + 7) / 8);
+        if (sp >= n_eff) return;
+    }
+    const int pg0 = sp * ((n_pages + n_eff - 1) / n_eff);
     const int* bt = a.rows.block_table + (size_t)(bad ? 0 : slot) * a.rows.max_pages;
-
-    const uint32_t ring = smem_u32(smem) + warp * (ST * STAGE);
-    auto page_at = [&](int i) {
-        int p = i < n_my ? bt[pg0 + warp + KA_WARPS * i] : 0;
+    auto page_at = [&](int i) {                                // page i of this warp: pg0 + warp + 4 i
+        int p = pg0 + warp + KA_WARPS * i < n_pages ? bt[pg0 + warp + KA_WARPS * i] : 0;
         if ((unsigned)p >= (unsigned)a.rows.n_pages) { bad = true; p = 0; }
         return p;
     };
     int my_page = page_at(lane);                               // the lanes hold the next 32 page numbers
+    const uint32_t ring = smem_u32(smem) + warp * (ST * STAGE);
     auto load = [&](int st, int page) { ka_load<HS>(a.c, ((size_t)page * a.c.n_kv_heads + kvh) * KV8_PAGE, ring + st * STAGE, lane); };
 #pragma unroll
     for (int i = 0; i < ST - 1; i++) {
         const int page = __shfl_sync(0xffffffffu, my_page, i);
-        if (i < n_my) load(i, page);
+        if (pg0 + warp + KA_WARPS * i < n_pages) load(i, page);            // (those of another share, where this one ends ahead of them, are not looked at)
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    if (further < 0 && !one && wk.n_splits > 1 && n_pages > KA_MIN_SPLIT_PAGES)
+        n_eff = ka_shares(wk, n_pages, ka_part(wk, __reduce_add_sync(0xffffffffu, ours)));
+    const int pps = (n_pages + n_eff - 1) / n_eff, pg1 = min(n_pages, pg0 + pps), n_my = max(0, (pg1 - pg0 - warp + KA_WARPS - 1) / KA_WARPS);
 
     uint32_t qf[1][KS][4];
     const float fl = ka_digits<HS, true>(x, my_head < n_live, lower, qf[0]);
@@ -784,7 +852,15 @@ static int ka_decode(const Kv8AttArgs& a, int n_splits, void* scratch, int pdl, 
     static_assert(KA_WARPS * 4 * (KaSums<HS>::LD + 2) * 4 + 4 <= smem, "the merge fits the ring");
     static SmemLimit given;
     const int kv = a.c.n_kv_heads, G = a.heads / kv, M = a.rows.M;
-    Kv8Work wk = {n_splits, (G + 3) / 4, nullptr, nullptr, nullptr};
+    Kv8Work wk = {n_splits, (G + 3) / 4, 0, 0.f, nullptr, nullptr, nullptr};
+    // CTAs: as many as the SMs hold with some to spare, more where those of one key/value head read the same pages.  8 kv heads of 128, rows of one length, us with
+    // one share each / these / about twice as many: one row of 100003 tokens 528 / 38.5 / 54, 6 rows of 3000 20 / 10.1 / 13.3, 12 rows of 3000 19.7 / 15.8 / 20, 20 rows of
+    // 4000 30.8 / 28.1 / 30.3, 32 rows of 3000 29.7 / 29.7 / 37; eight heads for each: one row of 30000 165 / 20 / 23.5, 7 of 5000 24 / 17.5 / 20, of heads of 64 18 /
+    // 13.1 / 15.6
+    // Where the rows alone take as many, 128 more, for rows that are much longer than the others
+    const int unit = kv * wk.groups, ctas = wk.groups == 1 ? 320 : 400;
+    wk.shares = max(1, ((long long)M * unit < ctas ? ctas : 128) / unit);
+    wk.part = 1.f / wk.shares;
     if (n_splits > 1) {
         if ((long long)M * kv * wk.groups * 4 > KA_COUNTER_BYTES) { dl_set_error("dl_kv8_attention: M*n_kv_heads too large for splits"); return -1; }
         uint8_t* at = reinterpret_cast<uint8_t*>(scratch);
@@ -792,7 +868,9 @@ static int ka_decode(const Kv8AttArgs& a, int n_splits, void* scratch, int pdl, 
         wk.part_o = reinterpret_cast<float*>(at + KA_COUNTER_BYTES);
         wk.part_ml = reinterpret_cast<float*>(at + KA_COUNTER_BYTES + ((long long)M * a.heads * n_splits * HS * 4 + 255) / 256 * 256);
     }
-    return ka_launch("dl_kv8_attention", kv8_attention_kernel<HS, ST>, given, dim3(kv * wk.groups, M, n_splits), 1, KA_WARPS * 32, smem, pdl, stream, a, wk);
+    if (M == 1 && wk.n_splits > wk.shares) wk.n_splits = wk.shares;
+    const unsigned rows = wk.n_splits == 1 ? M : min((long long)M + wk.shares, (long long)M * wk.n_splits);
+    return ka_launch("dl_kv8_attention", kv8_attention_kernel<HS, ST>, given, dim3(kv * wk.groups, rows), 1, KA_WARPS * 32, smem, pdl, stream, a, wk);
 }
 template <int HS>
 static int ka_prompt(const Kv8AttArgs& a, int pdl, void* stream) {

@@ -371,14 +371,10 @@ def _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out):
 
 
 def kv8_attention_splits(M: int, n_heads: int, n_kv_heads: int, max_pages: int) -> int:
-    """Shares of the longest context that kv8_attention is given for M rows: as many CTAs as the SMs hold with some to spare (a CTA for four query heads at
-    most; more of them where those of one key/value head read the same pages), eight pages each or more; a row takes no more than its own context is worth.  8 kv
-    heads of 128, us with one split / this many / about twice as many: one row of 100003 tokens 528 / 38.5 / 54, 6 rows of 3000 20 / 10.1 / 13.3, 12 rows of 3000
-    19.7 / 15.8 / 20, 20 rows of 4000 30.8 / 28.1 / 30.3, 32 rows of 3000 29.7 / 29.7 / 37; eight heads for each: one row of 30000 165 / 20 / 23.5, 7 of 5000
-    24 / 17.5 / 20, of heads of 64 18 / 13.1 / 15.6."""
-    group = (n_heads // n_kv_heads + 3) // 4
-    units = max(1, M * n_kv_heads * group)
-    return max(1, min((320 if group == 1 else 400) // units, max_pages // 8, 32))
+    """Shares of a row's context that kv8_attention is given room for: for few rows 32, each of eight pages or more, for more rows fewer, so that the
+    scratch stays small, beyond 64 rows one (128 rows of 500 tokens take 23.4 us, and 28.1 where shares are looked for).  How many a row takes goes by its part of
+    all rows' pages (ka_shares in csrc/cuda/kv8_attention.cu)."""
+    return max(1, min(512 // max(1, M) if M <= 64 else 1, max_pages // 8, 32))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -388,7 +384,8 @@ def _scratch_bytes(M: int, n_heads: int, head_size: int, n_splits: int) -> int:
 
 def kv8_attention(q, M: int, n_heads: int, pos, slot, block_table, cache: Kv8Cache, n_splits: int, scratch, xq_out=None, xh_out=None, out_mcap: int = 0,
                   y_out=None, row_skip=None, pdl: bool = False):
-    """`attention` over an 8-bit cache.  scratch: attention_scratch_bytes() zeroed once (None with one split); launches that may run at the same time --
+    """`attention` over an 8-bit cache.  scratch: attention_scratch_bytes() zeroed once (None with one split); n_splits: shares of
+    a row at most, kv8_attention_splits(); launches that may run at the same time --
     on two streams, or in two graphs -- need scratches of their own."""
     rows = _kv8_rows(M, pos, slot, block_table, cache)
     ldq, ldy, y_type = _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out)

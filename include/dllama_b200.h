@@ -228,7 +228,8 @@ int dl_kv8_write(const float* qkv, long long ld_qkv, int n_heads, const float* f
                  const DlKv8Cache* cache /*host*/, int pdl, void* stream);
 /* the rows' keys and values out of their pages: k_out / v_out [M][n_kv_heads * head_size] of DL_KV8_* (row stride ld), code * scale rounded once */
 int dl_kv8_read(const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const DlKv8Cache* cache /*host*/, void* k_out, void* v_out, long long ld, int out_type, int pdl, void* stream);
-/* dl_attention over the 8-bit cache: at most 16 query heads for each key/value head; y_out of DL_KV8_*.  scratch: dl_attention_scratch_bytes(), zeroed once; launches
+/* dl_attention over the 8-bit cache: at most 16 query heads for each key/value head; y_out of DL_KV8_*.  n_splits: shares of a row at most, of 64; how many a row
+ * takes goes by its part of all rows' pages.  scratch: dl_attention_scratch_bytes(), zeroed once; launches
  * that may run at the same time need scratches of their own */
 int dl_kv8_attention(const float* q, long long ldq, int n_heads, const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const DlKv8Cache* cache /*host*/, int n_splits, void* scratch,
                      uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, const int* row_skip, int pdl, void* stream);

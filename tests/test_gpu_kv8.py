@@ -259,6 +259,38 @@ def test_attention(heads, kv, hs, positions, splits):
         assert (y[M] == 3.0).all()
 
 
+@pytest.mark.parametrize("heads,kv,hs,M,long,splits", [
+    (4, 2, 64, 2, {1: 5000}, 32), (8, 2, 32, 5, {0: 9000, 4: 2600}, 64), (4, 1, 128, 32, {31: 6000}, 8), (16, 2, 64, 33, {32: 5000, 3: 900}, 16), (2, 1, 32, 70, {5: 12000, 40: 1000, 69: 3000}, 7),
+    (4, 4, 32, 100, {7: 4000}, 2), (4, 4, 32, 3, {0: 800, 1: 800, 2: 800}, 16), (8, 8, 64, 3, {0: 16 * 32 * 8 - 1, 1: 255, 2: 768}, 32),
+])
+def test_attention_of_rows_of_unlike_lengths(heads, kv, hs, M, long, splits):
+    """Rows take shares by their part of all pages; some are skipped, one has no token, one is in no table."""
+    k = K()
+    rng = np.random.default_rng(M)
+    positions = [long.get(m, int(rng.integers(0, 70))) for m in range(M)]
+    skip = [int(m not in long and rng.random() < 0.3) for m in range(M)]
+    if M > 5:
+        positions[2], skip[2] = -1, 0
+    bt, host, q, ref = _decode_case(heads, kv, hs, positions)
+    cache = k.Kv8Cache(*_dev(*host))
+    slots = list(range(M))
+    nowhere = [m for m in range(M) if M > 5 and m == 6]
+    for m in nowhere:
+        slots[m], skip[m] = M + 5, 0
+    where = (_i32(positions), _i32(slots), torch.from_numpy(bt).cuda())
+    scratch = torch.zeros(k.attention_scratch_bytes(M, heads, hs, splits), dtype=torch.uint8, device="cuda")
+    live = [m for m in range(M) if not skip[m] and m not in nowhere]
+    first = None
+    for _ in range(2):                                          # twice: the counters of the splits go back to zero, and the sums' order is always the same
+        y = torch.full((M, heads * hs), 3.0, device="cuda")
+        k.kv8_attention(q.cuda(), M, heads, *where, cache, splits, scratch, y_out=y, row_skip=_i32(skip))
+        _near(y[live], ref[live], ATT_REL)
+        assert (y[[m for m in range(M) if skip[m]]] == 3.0).all() and torch.isnan(y[nowhere]).all()
+        assert first is None or torch.equal(first[live], y[live])
+        first = y
+    assert not scratch[:65536].any()
+
+
 def test_attention_strides_alignment_and_skipped_rows():
     k = K()
     heads, kv, hs, positions = 8, 2, 128, [100, 37, 900, 0]

@@ -97,7 +97,7 @@ def test_library_refuses_arguments():
     assert L.dl_kv8_attention_prefill(A, 256, 4, *none, A, 1, c, None, None, None, None, None, 0, A, 256, 0, 0, None) == 0
 
 
-@pytest.mark.parametrize("M,heads,kv,pages,want", [(1, 32, 8, 6, 1), (1, 32, 8, 125, 15), (1, 32, 8, 4000, 32), (8, 32, 8, 4000, 5), (32, 32, 8, 4000, 1), (1, 16, 1, 4000, 32), (4, 128, 8, 4000, 3), (7, 64, 8, 157, 3), (500, 32, 8, 100, 1)])
+@pytest.mark.parametrize("M,heads,kv,pages,want", [(0, 32, 8, 6, 1), (1, 32, 8, 6, 1), (1, 32, 8, 125, 15), (1, 32, 8, 4000, 32), (16, 32, 8, 4000, 32), (32, 32, 8, 4000, 16), (7, 64, 8, 157, 19), (64, 32, 8, 100, 8), (65, 32, 8, 100, 1)])
 def test_splits(M, heads, kv, pages, want):
     assert K.kv8_attention_splits(M, heads, kv, pages) == want
 
