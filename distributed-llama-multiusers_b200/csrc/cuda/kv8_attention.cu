@@ -246,22 +246,30 @@ struct Kv8Work {               // what the launch adds to the arguments of decod
     int n_splits, groups;      // shares of a row at most; CTAs that share a key/value head's query heads
     int shares;                // shares of rows beyond the first that the launch has room for
     float part;                // 1 / shares
+    int least;                 // pages of a share at least
     unsigned* counters;        // [M][kv heads * groups]
     float* part_o;             // [M][heads][n_splits][HS]
     float* part_ml;            // [M][heads][n_splits][2]
 };
 
-// Rows share the launch's CTAs by their lengths: of all pages a share has P = pages / wk.shares, a row as many shares as it has P, whole ones, one at least.  So one
-// user deep in a document beside many others is not one CTA's per head (32 rows of 32 heads, one of 30000 tokens, the others of 300: 119 us with shares by the number
-// of rows, 17.4 so), and rows of like lengths get what they would get by their number (us by their number / so: 2 rows of 3000 8.5 / 9.2, 12 12.9 / 13.0, 20 of 4000 28.2 /
-// 26.9, 32 of 3000 30.1 / 29.9, 64 of 1500 33.3 / 35.1).
+// Rows share the launch's CTAs by their lengths: of all pages a share has P = pages / wk.shares, at least wk.least, and a row as many shares as it has P, whole ones,
+// one at least.  So one user deep in a document beside others is not one CTA's per head (us with shares by the number of rows / so: 8 rows of 32 heads, one of 30000
+// tokens, the others of 300: 29 / 15, 32 such rows 119 / 38), and rows of like lengths get about what they would get by their number (2 rows of 3000 8.5 / 9.4, 6 9.9 / 10.7,
+// 12 12.9 / 13.2, 20 of 4000 28.2 / 27.3, 32 of 3000 29.9 / 29.2, 64 of 1500 33.3 / 33.3).
 DL_DEVINL int ka_pages(const Kv8AttArgs& a, int m) {           // < 0: not this launch's row
     if (m >= a.rows.M || (a.row_skip != nullptr && a.row_skip[m] != 0)) return -1;
     const int t = kv8_tokens(a.rows, a.rows.pos[m], a.rows.slot[m]);
     return t > 0 ? (t - 1) / KV8_PAGE + 1 : 0;
 }
 // 1 / P, from all rows' pages
-DL_DEVINL float ka_part(const Kv8Work& wk, unsigned total) { return __fdividef(1.f, fmaxf(8.f, (float)total * wk.part)); }
+DL_DEVINL float ka_part(const Kv8Work& wk, unsigned total) { return __fdividef(1.f, fmaxf((float)wk.least, (float)total * wk.part)); }
+// pages of all rows behind the first 32 that come to a lane
+DL_DEVINL unsigned ka_rest(const Kv8AttArgs& a, int lane) {
+    unsigned ours = 0;
+#pragma unroll 4
+    for (int base = 32; base < a.rows.M; base += 32) ours += max(ka_pages(a, base + lane), 0);
+    return ours;
+}
 // whole parts, of eight pages begun ones (one less is below the quotient, so those beyond the rows' first are wk.shares at most, even if it is off a little: every
 // warp finds the same numbers)
 DL_DEVINL int ka_shares(const Kv8Work& wk, int pages, float part) {
@@ -305,16 +313,15 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
     const int further = (int)blockIdx.y - a.rows.M;            // < 0: a row's first share
     const bool many = a.rows.M > 32, one = a.rows.M == 1;      // (one row: its number of shares hangs on nothing else; 0.7 us less than by the others' way)
     int m0 = further < 0 ? blockIdx.y : 0, sp = one ? blockIdx.y : 0, n_eff = 1;
-    int mine = 0;                                              // pages of row `lane`, and of all rows that come to the lane (asked for with this CTA's own position)
+    int mine = 0;                                              // pages of row `lane`, and of all rows that come to the lane
     unsigned ours = 0;
-    if (wk.n_splits > 1 && !one) {
+    auto all_rows = [&] {
         mine = ka_pages(a, lane);
         ours = max(mine, 0);
-        if (many) {
-#pragma unroll 4
-            for (int base = 32; base < a.rows.M; base += 32) ours += max(ka_pages(a, base + lane), 0);
-        }
-    }
+        if (many) ours += ka_rest(a, lane);
+    };
+    const bool at_once = wk.least == 8;                        // most rows will have several shares: asked for with this CTA's own position
+    if (wk.n_splits > 1 && !one && (at_once || further >= 0)) all_rows();
     const int my_head = g & 3;
     float x[2 * KS][4];
     auto ask = [&] { ka_query<HS>(a.q + (size_t)m0 * a.ldq + (kvh * G + h_lo + (my_head < n_live ? my_head : 0)) * HS + qd * 4, ((uintptr_t)a.q & 15) == 0 && (a.ldq & 3) == 0, x); };
@@ -355,8 +362,10 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
         if (pg0 + warp + KA_WARPS * i < n_pages) load(i, page);            // (those of another share, where this one ends ahead of them, are not looked at)
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    if (further < 0 && !one && wk.n_splits > 1 && n_pages > KA_MIN_SPLIT_PAGES)
+    if (further < 0 && !one && wk.n_splits > 1 && n_pages > max(KA_MIN_SPLIT_PAGES, wk.least)) {
+        if (!at_once) all_rows();
         n_eff = ka_shares(wk, n_pages, ka_part(wk, __reduce_add_sync(0xffffffffu, ours)));
+    }
     const int pps = (n_pages + n_eff - 1) / n_eff, pg1 = min(n_pages, pg0 + pps), n_my = max(0, (pg1 - pg0 - warp + KA_WARPS - 1) / KA_WARPS);
 
     uint32_t qf[1][KS][4];
@@ -852,14 +861,17 @@ static int ka_decode(const Kv8AttArgs& a, int n_splits, void* scratch, int pdl, 
     static_assert(KA_WARPS * 4 * (KaSums<HS>::LD + 2) * 4 + 4 <= smem, "the merge fits the ring");
     static SmemLimit given;
     const int kv = a.c.n_kv_heads, G = a.heads / kv, M = a.rows.M;
-    Kv8Work wk = {n_splits, (G + 3) / 4, 0, 0.f, nullptr, nullptr, nullptr};
+    Kv8Work wk = {n_splits, (G + 3) / 4, 0, 0.f, 8, nullptr, nullptr, nullptr};
     // CTAs: as many as the SMs hold with some to spare, more where those of one key/value head read the same pages.  8 kv heads of 128, rows of one length, us with
     // one share each / these / about twice as many: one row of 100003 tokens 528 / 38.5 / 54, 6 rows of 3000 20 / 10.1 / 13.3, 12 rows of 3000 19.7 / 15.8 / 20, 20 rows of
     // 4000 30.8 / 28.1 / 30.3, 32 rows of 3000 29.7 / 29.7 / 37; eight heads for each: one row of 30000 165 / 20 / 23.5, 7 of 5000 24 / 17.5 / 20, of heads of 64 18 /
     // 13.1 / 15.6
-    // Where the rows alone take as many, 128 more, for rows that are much longer than the others
+    // Where the rows alone take three quarters of them, 64 more, for rows that are much longer than the others, of 64 pages each or more: 128 cost 32 rows of 3000 that
+    // have no use for them 0.4 us more, and summing up all rows' pages in every CTA 0.8 more
     const int unit = kv * wk.groups, ctas = wk.groups == 1 ? 320 : 400;
-    wk.shares = max(1, ((long long)M * unit < ctas ? ctas : 128) / unit);
+    const bool full = 4LL * M * unit >= 3 * ctas;
+    wk.shares = max(1, (full ? 64 : ctas) / unit);
+    if (full) wk.least = 64;
     wk.part = 1.f / wk.shares;
     if (n_splits > 1) {
         if ((long long)M * kv * wk.groups * 4 > KA_COUNTER_BYTES) { dl_set_error("dl_kv8_attention: M*n_kv_heads too large for splits"); return -1; }
