@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
         if (n_pages > KA_MIN_SPLIT_PAGES) n_eff = min(wk.n_splits, (n_pages + 7) / 8);
         if (sp >= n_eff) return;
     }
-    const int pg0 = sp * ((n_pages + n_eff - 1) / n_eff);
+    const int pg0 = sp == 0 ? 0 : sp * ((n_pages + n_eff - 1) / n_eff);
     const int* bt = a.rows.block_table + (size_t)(bad ? 0 : slot) * a.rows.max_pages;
     auto page_at = [&](int i) {                                // page i of this warp: pg0 + warp + 4 i
         int p = pg0 + warp + KA_WARPS * i < n_pages ? bt[pg0 + warp + KA_WARPS * i] : 0;
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
         if (!at_once) all_rows();
         n_eff = ka_shares(wk, n_pages, ka_part(wk, __reduce_add_sync(0xffffffffu, ours)));
     }
-    const int pps = (n_pages + n_eff - 1) / n_eff, pg1 = min(n_pages, pg0 + pps), n_my = max(0, (pg1 - pg0 - warp + KA_WARPS - 1) / KA_WARPS);
+    const int pps = n_eff == 1 ? n_pages : (n_pages + n_eff - 1) / n_eff, pg1 = min(n_pages, pg0 + pps), n_my = max(0, (pg1 - pg0 - warp + KA_WARPS - 1) / KA_WARPS);
 
     uint32_t qf[1][KS][4];
     const float fl = ka_digits<HS, true>(x, my_head < n_live, lower, qf[0]);
