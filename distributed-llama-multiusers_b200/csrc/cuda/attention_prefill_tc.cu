@@ -53,7 +53,6 @@
 #define PT_STAGES 2                    // K tiles and V tiles in flight
 #define PT_OUT_LD 20
 #define PT_SHARE_STEPS 4
-#define PT_LEAST_STEPS 4               // of a share of the Llama path; of an item that goes to two CTAs: 32
 
 struct PtArgs {
     const float* q;            // [M][n_heads*128]
@@ -324,24 +323,14 @@ struct PtWaits {
 // a long item go to as many CTAs as there are for each.  Two tiles in one CTA take 1.75 us a step, a single one 1.03, and the join 5 us more: 130 rows of 32 heads
 // behind 2000 tokens 37 us alike, behind 8000 92 without shares and 63 with them; 512 rows (two shares) behind none 21 / 27, behind 4000 62 / 61, behind 16000 182 / 159
 // (those of heads of 64 behind 16000 156 / 122).  Item `idx` of the order that all roles of all CTAs walk; false behind the last one.
-template <bool SHARES> DL_DEVINL bool pt_item(const PtArgs& a, const int (*seg)[4], int n_seg, int idx, PtItem& it) {
+template <bool SHARES> DL_DEVINL bool pt_item(const PtArgs& a, const int (*seg)[4], int n_seg, int spread, int idx, PtItem& it) {
     const int rep = a.n_heads / a.n_kv_heads;
     const bool even = rep % 2 == 0;
-    int tiles = 0, spread = 1;
+    int tiles = 0;
     for (int i = 0; i < n_seg; i++) tiles += (seg[i][1] + PT_ROWS - 1) / PT_ROWS;
-    if (SHARES) {
-        int pairs = 0, last = 0;
-        for (int i = 0; i < n_seg; i++) {
-            const int nt = (seg[i][1] + PT_ROWS - 1) / PT_ROWS;
-            pairs += even ? nt : (nt + 1) / 2;
-            last = max(last, seg[i][2] + seg[i][1]);
-        }
-        if (pairs > 0) spread = max(1, min((int)gridDim.x / (pairs * (even ? a.n_heads / 2 : a.n_heads)), last / (PT_KV * PT_LEAST_STEPS)));
-        if (spread == 2 && last < PT_KV * 32) spread = 1;
-    }
     const bool single = spread == 1 && tiles * a.n_heads <= (int)gridDim.x, by_heads = !single && even, by_rows = !single && !by_heads;
-    const int cols = by_heads ? a.n_heads / 2 : a.n_heads, share = SHARES ? idx % spread : 0;
-    if (SHARES) idx /= spread;
+    const int cols = by_heads ? a.n_heads / 2 : a.n_heads, share = SHARES && spread > 1 ? idx % spread : 0;
+    if (SHARES && spread > 1) idx /= spread;
     for (int i = 0; i < n_seg; i++) {
         const int nt = (seg[i][1] + PT_ROWS - 1) / PT_ROWS, groups = by_rows ? (nt + 1) / 2 : nt;
         if (idx >= groups * cols) { idx -= groups * cols; continue; }
@@ -465,7 +454,7 @@ template <bool LINES, int HS = PT_HS, bool SHARES = false>
 __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(const __grid_constant__ typename PtKernelArgs<LINES>::T a,
                                                                              const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ int seg[PT_MAX_SEG][4], n_seg_s, gave_up_s;
+    __shared__ int seg[PT_MAX_SEG][4], n_seg_s, spread_s, gave_up_s;
     if constexpr (!LINES) trace_begin(a.tr);
     uint8_t* q_s = smem;                                        // [2] query tiles
     uint8_t* k_s = q_s + 2 * PT_TILE_BYTES;                     // [2] K tiles (tokens x head dim, K-major)
@@ -516,6 +505,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                 seg[lane][2] = e > b ? a.pos[b] : 0;
                 seg[lane][3] = e > b ? a.slot[b] : 0;
             }
+            if constexpr (SHARES) {                               // CTAs of an item at most
+                __syncwarp();
+                const bool even = a.n_heads / a.n_kv_heads % 2 == 0;
+                const int nt = lane < ns ? (seg[lane][1] + PT_ROWS - 1) / PT_ROWS : 0, last = __reduce_max_sync(0xffffffffu, lane < ns ? seg[lane][2] + seg[lane][1] : 0);
+                const int items = __reduce_add_sync(0xffffffffu, even ? nt : (nt + 1) / 2) * (even ? a.n_heads / 2 : a.n_heads);
+                int spread = last >= PT_SHARE_TOKENS && items > 0 ? max(1, min((int)gridDim.x / items, last / (PT_KV * PT_LEAST_STEPS))) : 1;
+                if (spread == 2 && last < PT_KV * 32) spread = 1;
+                if (lane == 0) spread_s = spread;
+            }
         }
     } else {
         // (launched behind a kernel that writes the rows of other tiles and reads the same inputs: nothing to wait for here.  What
@@ -537,7 +535,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
     __syncthreads();
     tc_fence_after();
     const PtWaits wait = {&gave_up_s, globaltimer_ns(), a.limit.ns};
-    const int n_seg = n_seg_s;
+    const int n_seg = n_seg_s, spread = SHARES ? spread_s : 1;
     // the items of this CTA, in the same order for every role; rounds run back and forth over the CTAs, so that a long item goes with a short one
     auto item_at = [&](int round, PtItem& it) {
         if constexpr (LINES) {
@@ -545,7 +543,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
             return round < n_seg;
         } else {
             const int G = gridDim.x, b = blockIdx.x;
-            return pt_item<SHARES>(a, seg, n_seg, round * G + ((round & 1) ? G - 1 - b : b), it);
+            return pt_item<SHARES>(a, seg, n_seg, spread, round * G + ((round & 1) ? G - 1 - b : b), it);
         }
     };
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);

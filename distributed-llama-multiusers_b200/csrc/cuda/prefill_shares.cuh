@@ -3,6 +3,8 @@
 #pragma once
 
 #define PT_SHARE_SLOTS 160             // CTAs of such a launch at most, each with one share
+#define PT_LEAST_STEPS 4               // of 128 tokens, of a share; of an item that goes to two CTAs: 32
+#define PT_SHARE_TOKENS (3 * 128 * PT_LEAST_STEPS)      // no sequence below that has shares
 #define PT_SHARE_WARPS 8               // of a CTA, 32 rows each
 
 struct PtShares {
