@@ -1071,7 +1071,9 @@ extern "C" int dl_kv8_attention_prefill(const float* q, long long ldq, int n_hea
         int* meta16 = reinterpret_cast<int*>(scratch);
         const Kv8ExpandArgs x = {a, (__half*)k16, (__half*)v16, meta16};
         static SmemLimit none;
-        const dim3 grid(4 * dl_device_sm_count());
+        // a CTA for a page and head, as far as the tables hold them, and eight an SM (four: 130 rows of 32 heads behind 8000 tokens 66 us for 64, 512 behind 16000 156 for 153.5)
+        const long long pages = (long long)cache->n_kv_heads * max_pages * min(n_slots, a.n_seg), most = 8 * dl_device_sm_count();
+        const dim3 grid((unsigned)(pages < most ? pages : most));
         if (const int rc = hs == 128 ? ka_launch(who, kv8_expand_kernel<128>, none, grid, 1, 256, 0, pdl, stream, x) : ka_launch(who, kv8_expand_kernel<64>, none, grid, 1, 256, 0, pdl, stream, x)) return rc;
         // items that leave half of the SMs without one go to several CTAs each, where the tables may hold sequences that are long enough (PT_SHARE_TOKENS; 500 rows of 32
         // heads of 64 behind none 16.0 us, 17.4 by the instance that looks for shares)
