@@ -128,6 +128,6 @@ def test_required_memory_of_the_cache(tiny_model_path):
     h = read_header(tiny_model_path, 0)
     f16, q8 = (required_memory(h, 1, n_slots=3, seq_len=64, kv_cache=t)["kv_cache"] for t in ("f16", "q8"))
     assert f16 == 2 * 2 * 3 * 64 * 4 * 32 * 2 and q8 == 2 * 3 * 2 * K.kv8_page_bytes(4, 32)
-    wide = dataclasses.replace(h, dim=2048, n_heads=32, n_kv_heads=8)
+    wide = dataclasses.replace(h, dim=2048, n_heads=32, n_kv_heads=4)
     few, many = (required_memory(wide, 1, rows, n_slots=3, seq_len=64, kv_cache="q8")["kv_cache"] for rows in (64, 512))
-    assert few == 2 * 3 * 2 * K.kv8_page_bytes(8, 64) and many == few + 3 * 64 * 2 * 512 * 2        # and fp16 pages of one layer
+    assert few == 2 * 3 * 2 * K.kv8_page_bytes(4, 64) and many == few + 3 * 64 * 2 * 256 * 2        # and fp16 pages of one layer
