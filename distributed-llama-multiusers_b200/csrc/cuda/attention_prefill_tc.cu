@@ -134,11 +134,11 @@ template <bool LINES> DL_DEVINL uint32_t pt_pack2(float lo, float hi) {
 // exp2 on the FMA pipe (Cody-Waite split + degree-3 polynomial, relative error 8e-5 -- the result is rounded to fp16,
 // 5e-4, right after; LINES, whose other kernels form it in full: degree 5, 2e-7): the softmax is bound by the 16 MUFU results
 // per clock and SM (128 x 128 exp2 per step = 1024 clk, as long as the MMAs of the step), so every fourth element takes this
-// path instead
-template <bool LINES> DL_DEVINL pair_f pt_ex2_poly(pair_f x) {
-    float lo, hi;                                  // LINES: a NaN stays one, as in the mma.sync kernel
+// path instead.  LINES, CODES: a NaN stays one, as in the mma.sync kernels (an exponent that is added to its bits would make a number of it)
+template <bool LINES, bool CODES> DL_DEVINL pair_f pt_ex2_poly(pair_f x) {
+    float lo, hi;
     pair_get(x, lo, hi);
-    if (LINES) {
+    if (LINES || CODES) {
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-126.0f));
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-126.0f));
     } else {
@@ -150,24 +150,27 @@ template <bool LINES> DL_DEVINL pair_f pt_ex2_poly(pair_f x) {
     const pair_f f = fma2(add2(t, both(-12582912.0f)), both(-1.0f), xc);                // [-0.5, 0.5]
     float tl, th, pl, ph;
     pair_get(t, tl, th);
+    const auto power = [&] { return pair_of(__int_as_float((__float_as_int(tl) << 23) + 0x3f800000), __int_as_float((__float_as_int(th) << 23) + 0x3f800000)); };
     if (LINES) {
         const pair_f p = fma2(fma2(fma2(fma2(fma2(both(1.32764725e-3f), f, both(9.67554096e-3f)), f, both(0.0555071309f)), f, both(0.240221202f)), f, both(0.693146944f)), f, both(1.00000012f));
-        return mul2(p, pair_of(__int_as_float((__float_as_int(tl) << 23) + 0x3f800000), __int_as_float((__float_as_int(th) << 23) + 0x3f800000)));
+        return mul2(p, power());
     }
-    pair_get(fma2(fma2(fma2(both(0.0550886838f), f, both(0.242604051f)), f, both(0.693276242f)), f, both(0.99992894f)), pl, ph);
+    const pair_f p = fma2(fma2(fma2(both(0.0550886838f), f, both(0.242604051f)), f, both(0.693276242f)), f, both(0.99992894f));
+    if (CODES) return mul2(p, power());
+    pair_get(p, pl, ph);
     return pair_of(__int_as_float(__float_as_int(pl) + (__float_as_int(tl) << 23)), __int_as_float(__float_as_int(ph) + (__float_as_int(th) << 23)));
 }
 
 // 32 scores (masked ones are -inf) -> exp2(s * sc - ref) as 16 packed fp16 pairs; their sum is added to `sum`.  LINES: as bf16 and, in `lo`, the
 // bf16 remainder of each, 17 bits together
-template <bool LINES> DL_DEVINL void pt_probs(const uint32_t (&v)[32], float sc, float ref, uint32_t (&pk)[16], uint32_t (&lo)[LINES ? 16 : 1], pair_f& sum) {
+template <bool LINES, bool CODES> DL_DEVINL void pt_probs(const uint32_t (&v)[32], float sc, float ref, uint32_t (&pk)[16], uint32_t (&lo)[LINES ? 16 : 1], pair_f& sum) {
     const pair_f sc2 = pair_of(sc, sc), ref2 = pair_of(-ref, -ref);
 #pragma unroll
     for (int e = 0; e < 32; e += 2) {
         pair_f p = fma2(pair_of(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, ref2);
         float pa, pb;
         if ((e & 6) == 6) {
-            p = pt_ex2_poly<LINES>(p);
+            p = pt_ex2_poly<LINES, CODES>(p);
             pair_get(p, pa, pb);
         } else {
             pair_get(p, pa, pb);
@@ -449,8 +452,8 @@ DL_DEVINL void pt_load_rows(const float* mine, uint8_t* tile, int r0, Ready read
 }
 
 // HS: head size; 64 (LINES: not) takes the first half of every tile and accumulator.  SHARES (LINES: not): items may go to several CTAs (4001 rows, whose
-// items do not, take 1.2 % longer with it)
-template <bool LINES, int HS = PT_HS, bool SHARES = false>
+// items do not, take 1.2 % longer with it).  CODES (LINES: not): over the widened 8-bit cache, where a line may be a key of NaN
+template <bool LINES, int HS = PT_HS, bool SHARES = false, bool CODES = false>
 __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(const __grid_constant__ typename PtKernelArgs<LINES>::T a,
                                                                              const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -659,7 +662,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                 // LINES: formed ahead of the waits, in the scores' registers, as the place is free only when the other tile's have been multiplied
                 if constexpr (LINES) {
 #pragma unroll
-                    for (int c = 0; c < 4; c++) pt_probs<LINES>(v[c], sc, ref, pk[c], lo[c], sum);
+                    for (int c = 0; c < 4; c++) pt_probs<LINES, CODES>(v[c], sc, ref, pk[c], lo[c], sum);
                 }
                 // this tile's P V before is complete; LINES: and the other's, whose probabilities lie in this place.  Neither barrier can be more than the one
                 // phase ahead that a parity tells, as its next phase waits for the probabilities of this step (the phases of the other tile's o_full pass
@@ -680,7 +683,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                 }
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    if constexpr (!LINES) pt_probs<LINES>(v[c], sc, ref, pk[c], lo[c], sum);
+                    if constexpr (!LINES) pt_probs<LINES, CODES>(v[c], sc, ref, pk[c], lo[c], sum);
                     tmem_st_32x32b_x16(T_P + c * 16, pk[c]);
                     if constexpr (LINES) tmem_st_32x32b_x16(T_P + 64 + c * 16, lo[c]);
                 }
@@ -1022,11 +1025,12 @@ static int pt_make_map(CUtensorMap* m, const void* base, long long rows, int wid
 // CTAs of a launch that may leave shares
 int pt_share_ctas() { return dl_device_sm_count() < PT_SHARE_SLOTS ? dl_device_sm_count() : PT_SHARE_SLOTS; }
 
-// heads of 64 too; y_type other than f32: y_out aligned to 8 bytes; shares: NULL, or where a launch may leave shares of items to be joined
+// codes: over the widened 8-bit cache.  Heads of 64, y_type other than f32 (y_out aligned to 8 bytes) and shares (NULL, or where a launch may leave shares of
+// items to be joined): there alone
 int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_heads, int head_size, const void* k_cache, const void* v_cache, const int* pos,
                                   const int* slot, const int* block_table, int max_pages, int page_size, const int* meta, uint8_t* xq_out, uint8_t* xh_out,
-                                  int out_mcap, void* y_out, int y_type, const PtShares* shares, int n_cache_pages, int pdl, void* stream) {
-    if (page_size != 32 || (head_size != 128 && head_size != 64)) { dl_set_error("dl_attention_prefill_tc: page size 32 and head size 64 or 128 only"); return -1; }
+                                  int out_mcap, void* y_out, int y_type, bool codes, const PtShares* shares, int n_cache_pages, int pdl, void* stream) {
+    if (page_size != 32 || (head_size != 128 && !(head_size == 64 && codes))) { dl_set_error("dl_attention_prefill_tc: page size 32 and head size 64 or 128 only"); return -1; }
     if (n_heads % n_kv_heads != 0) { dl_set_error("dl_attention_prefill_tc: bad head grouping"); return -1; }
     if (n_cache_pages < 1) { dl_set_error("dl_attention_prefill_tc: n_cache_pages < 1"); return -1; }
     PtArgs a;
@@ -1040,9 +1044,10 @@ int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_h
     const long long rows = (long long)n_cache_pages * n_kv_heads * 32;
     if (pt_make_map(&kmap, k_cache, rows, head_size, false) != 0 || pt_make_map(&vmap, v_cache, rows, head_size, false) != 0) return -1;
     const size_t smem = PT_SMEM;
-    static SmemLimit given[4];
-    const int which = (head_size == 64) + 2 * (shares != nullptr);
-    auto* kernel = which == 0 ? attention_prefill_tc_kernel<false> : which == 1 ? attention_prefill_tc_kernel<false, 64> : which == 2 ? attention_prefill_tc_kernel<false, 128, true> : attention_prefill_tc_kernel<false, 64, true>;
+    static SmemLimit given[5];
+    const int which = !codes ? 0 : 1 + (head_size == 64) + 2 * (shares != nullptr);
+    auto* kernel = which == 0 ? attention_prefill_tc_kernel<false> : which == 1 ? attention_prefill_tc_kernel<false, 128, false, true> : which == 2 ? attention_prefill_tc_kernel<false, 64, false, true>
+                 : which == 3 ? attention_prefill_tc_kernel<false, 128, true, true> : attention_prefill_tc_kernel<false, 64, true, true>;
     if (const int rc = dl_smem_limit("attention_prefill_tc", kernel, smem, given[which])) return rc;
     cudaLaunchConfig_t cfg = {};
     const long long most = ((long long)(M + PT_ROWS - 1) / PT_ROWS + PT_MAX_SEG - 1) * n_heads;        // upper bound of the tiles of all segments
@@ -1068,7 +1073,7 @@ extern "C" int dl_attention_prefill_tc(const float* q, int M, int n_heads, int n
                                        int out_mcap, float* y_out, int n_cache_pages, int pdl, void* stream) {
     if (head_size != PT_HS) { dl_set_error("dl_attention_prefill_tc: page size 32 and head size 128 only"); return -1; }
     return dl_attention_prefill_tc_typed(q, M, n_heads, n_kv_heads, head_size, k_cache, v_cache, pos, slot, block_table, max_pages, page_size, meta, xq_out, xh_out,
-                                         out_mcap, y_out, DL_KV8_F32, nullptr, n_cache_pages, pdl, stream);
+                                         out_mcap, y_out, DL_KV8_F32, false, nullptr, n_cache_pages, pdl, stream);
 }
 
 // 0 if the kernel's LINES instance takes these sizes: bf16 lines of a key and a value of 128, full tiles of 64 stacked rows

@@ -1045,7 +1045,7 @@ static bool ka_widens(long long rows, int n_heads, int hs) { return (hs == 128 &
 
 extern int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_heads, int head_size, const void* k_cache, const void* v_cache, const int* pos,
                                          const int* slot, const int* block_table, int max_pages, int page_size, const int* meta, uint8_t* xq_out, uint8_t* xh_out,
-                                         int out_mcap, void* y_out, int y_type, const PtShares* shares, int n_cache_pages, int pdl, void* stream);
+                                         int out_mcap, void* y_out, int y_type, bool codes, const PtShares* shares, int n_cache_pages, int pdl, void* stream);
 extern int pt_share_ctas();
 
 #define KV8_META_BYTES 128             // of a workspace's scratch: the segments of the launch, then its shares
@@ -1085,7 +1085,7 @@ extern "C" int dl_kv8_attention_prefill(const float* q, long long ldq, int n_hea
             part.sums = reinterpret_cast<float4*>(part.norms + PT_SHARE_SLOTS * PT_SHARE_WARPS * 32);
         }
         return dl_attention_prefill_tc_typed(q, M, n_heads, cache->n_kv_heads, hs, k16, v16, pos, slot, block_table, max_pages, KV8_PAGE, meta16, xq_out, xh_out,
-                                             out_mcap, y_out, y_type, part.arrived != nullptr ? &part : nullptr, cache->n_pages, 1, stream);
+                                             out_mcap, y_out, y_type, true, part.arrived != nullptr ? &part : nullptr, cache->n_pages, 1, stream);
     }
     return hs == 128 ? ka_prompt<128>(a, pdl, stream) : hs == 64 ? ka_prompt<64>(a, pdl, stream) : ka_prompt<32>(a, pdl, stream);
 }

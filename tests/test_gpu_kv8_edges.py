@@ -1,0 +1,64 @@
+"""The 8-bit token cache where lines are not ordinary: NaN lines at every place of a step.
+
+Tolerances are those of test_gpu_kv8.py, which derives them.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_kv8 import K, PAGE, _attention, _cache, _dev, _i32, _table, _values
+
+pytestmark = pytest.mark.gpu
+
+
+class _Prompt:
+    """One segment of `rows` rows behind `context` tokens, `wide` pages more in the block table."""
+
+    def __init__(self, heads, kv, hs, rows, context, seed=0, wide=0):
+        rng = np.random.default_rng(seed + heads * 3 + hs + context)
+        self.heads, self.kv, self.hs, self.rows, self.context = heads, kv, hs, rows, context
+        bt, self.n_pages = _table(rng, [context + rows])
+        self.bt = np.concatenate((bt, np.full((1, wide), -7, dtype=np.int32)), 1) if wide else bt
+        self.host = _cache(rng, self.n_pages, kv, hs)
+        self.q = torch.from_numpy(rng.standard_normal((rows, heads * hs)).astype(np.float32))
+
+    def at(self, t):
+        """Page and place of token t."""
+        return int(self.bt[0, t // PAGE]), t % PAGE
+
+    def run(self, workspace, dtype=torch.float32):
+        k = K()
+        if workspace:
+            assert k.kv8_widens(self.rows, self.heads, self.hs)
+        cache = k.Kv8Cache(*_dev(*self.host))
+        where = (_i32(list(range(self.context, self.context + self.rows))), _i32([0] * self.rows), torch.from_numpy(self.bt).cuda())
+        work = k.kv8_prefill_workspace(self.n_pages, self.kv, self.hs, self.rows, "cuda") if workspace else None
+        y = torch.full((self.rows, self.heads * self.hs), 7.0, dtype=dtype, device="cuda")
+        k.kv8_attention_prefill(self.q.cuda(), self.rows, self.heads, *where, _i32([1, 0, self.rows]), cache, workspace=work, y_out=y)
+        return y.cpu().view(self.rows, self.heads, self.hs)
+
+    def ref(self, m):
+        """f64 [heads][hs] of row m."""
+        T = self.context + m + 1
+        return _attention(self.q[m].view(self.heads, self.hs), _values(self.host[0], self.host[2], self.bt[0], T), _values(self.host[1], self.host[3], self.bt[0], T))
+
+
+@pytest.mark.parametrize("workspace", [False, True])
+@pytest.mark.parametrize("heads,kv,hs,rows,context,wide,first", [
+    (16, 8, 128, 300, 200, 0, 8), (16, 8, 128, 300, 200, 0, 136), (16, 8, 128, 300, 200, 0, 304), (16, 8, 128, 300, 200, 0, 488),
+    (16, 8, 128, 300, 200, 60, 304),                                     # tables that may hold long sequences
+    (16, 8, 128, 260, 2600, 0, 1400), (16, 8, 128, 260, 2600, 0, 2736),    # steps that go to several CTAs
+    (8, 8, 128, 530, 0, 0, 264),                                         # heads that come alone: two tiles of rows side by side
+    (32, 8, 64, 300, 200, 0, 8), (32, 8, 64, 300, 200, 60, 304), (32, 8, 64, 240, 3000, 0, 1704), (8, 8, 64, 930, 100, 0, 520),
+])
+def test_a_nan_line_is_seen_wherever_it_stands(heads, kv, hs, rows, context, wide, first, workspace):
+    """Eight neighbouring tokens from `first` on, one for each key/value head: key of the even ones, value of the odd ones."""
+    p = _Prompt(heads, kv, hs, rows, context, wide=wide)
+    for h in range(kv):
+        page, place = p.at(first + h)
+        p.host[2 + h % 2][page, h, place] = math.nan
+    nan = torch.isnan(p.run(workspace))
+    sees = torch.tensor([[context + m >= first + h // (heads // kv) for h in range(heads)] for m in range(rows)])
+    assert torch.equal(nan.all(-1), sees) and torch.equal(nan.any(-1), sees)
