@@ -827,15 +827,19 @@ class LlamaEngine:
         return out
 
     def read_cache(self, layer: int, slot: int, n_tokens: int, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
-        """Keys and values of a sequence's first n_tokens, [n_tokens][this rank's key/value heads * head size]: to keep a conversation outside of its pages."""
-        assert 0 < n_tokens <= int(self.pages.n_used[slot]) * PAGE
+        """Keys and values of a sequence's first n_tokens, [n_tokens][this rank's key/value heads * head size]: to keep a conversation outside of its pages.
+        n_tokens: those that have been run (a place that is only reserved holds what its page held before).  Queued behind the steps of the current
+        stream; the slot may be freed at once."""
+        n_pages = (n_tokens + PAGE - 1) // PAGE
+        assert 0 < n_pages <= int(self.pages.n_used[slot])
         if not self.kv8:
-            pages = torch.from_numpy(self.pages.table[slot, :(n_tokens + PAGE - 1) // PAGE].astype(np.int64)).to(self.device)
+            pages = torch.from_numpy(self.pages.table[slot, :n_pages].astype(np.int64)).to(self.device)
             return tuple(c[layer][pages].transpose(1, 2).reshape(-1, self.kv_loc)[:n_tokens].to(dtype) for c in (self.k_cache, self.v_cache))
-        self._sync_block_table()
+        # a table of its own, in pinned memory that nothing writes again: the staged one belongs to the steps in the queue (set_batch)
+        table = torch.from_numpy(self.pages.table[slot:slot + 1, :n_pages]).pin_memory().to(self.device, non_blocking=True)
         k, v = (torch.empty(n_tokens, self.kv_loc, dtype=dtype, device=self.device) for _ in range(2))
         pos = torch.arange(n_tokens, dtype=torch.int32, device=self.device)
-        K.kv8_read(n_tokens, pos, torch.full_like(pos, slot), self.block_table, self.kv8_cache[layer], k, v)
+        K.kv8_read(n_tokens, pos, torch.zeros_like(pos), table, self.kv8_cache[layer], k, v)
         return k, v
 
     def current_step(self) -> int:

@@ -1,4 +1,4 @@
-"""The 8-bit token cache where lines are not ordinary: NaN lines at every place of a step.
+"""The 8-bit token cache where lines are not ordinary: NaN lines at every place of a step, lines read back beside queued work.
 
 Tolerances are those of test_gpu_kv8.py, which derives them.
 """
@@ -62,3 +62,51 @@ def test_a_nan_line_is_seen_wherever_it_stands(heads, kv, hs, rows, context, wid
     nan = torch.isnan(p.run(workspace))
     sees = torch.tensor([[context + m >= first + h // (heads // kv) for h in range(heads)] for m in range(rows)])
     assert torch.equal(nan.all(-1), sees) and torch.equal(nan.any(-1), sees)
+
+
+def _engine(path, **kw):
+    from dllama_b200.models.llama import LlamaEngine
+    return LlamaEngine(path, max_rows=64, n_slots=3, max_seq_len=512, kv_dtype=torch.int8, **kw)
+
+
+def test_read_cache_ahead_of_the_next_user(tiny_tp_model_path):
+    """A conversation is read out behind queued work, and its sequence and pages go to another user before the read has run."""
+    rng = np.random.default_rng(1)
+    e = _engine(tiny_tp_model_path)
+    a = e.alloc_slot()
+    e.prefill(a, rng.integers(1, 1024, 100).tolist(), 0)
+    e.forward(rng.integers(1, 1024, 64).tolist(), list(range(64)), [e.alloc_slot()] * 64)      # (the shape's graph is captured)
+    want = [t.clone() for t in e.read_cache(0, a, 100, torch.float32)]
+    e.ensure_capacity(a, 140)                                      # the table that the read needs is on its way
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    got = e.read_cache(0, a, 100, torch.float32)
+    e.free_slot(a)
+    b = e.alloc_slot()
+    assert a == b
+    e.forward(rng.integers(1, 1024, 64).tolist(), list(range(64)), [b] * 64)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    e.close()
+
+
+def test_read_cache_behind_a_queued_step(tiny_tp_model_path):
+    """A step waits with the table that it was given; a conversation is read out when its sequence has been given to another user."""
+    rng = np.random.default_rng(2)
+    e = _engine(tiny_tp_model_path)
+    a, b = e.alloc_slot(), e.alloc_slot()
+    e.prefill(a, rng.integers(1, 1024, 100).tolist(), 0)
+    e.prefill(b, rng.integers(1, 1024, 50).tolist(), 0)
+    want = e.forward([7], [100], [a]).clone()
+    held = [t.clone() for t in e.read_cache(1, b, 50, torch.float16)]
+    e.ensure_capacity(b, 70)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    got = e.forward([7], [100], [a])
+    e.free_slot(a)
+    assert e.alloc_slot() == a
+    e.ensure_capacity(a, 128)                                      # its pages in another order
+    again = e.read_cache(1, b, 50, torch.float16)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and all(torch.equal(x, y) for x, y in zip(again, held))
+    e.close()
