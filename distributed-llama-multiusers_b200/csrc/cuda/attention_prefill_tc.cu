@@ -434,9 +434,11 @@ DL_DEVINL void pt_run_item(const PtLineArgs& a, const int (&run)[4], PtItem& it)
     it.first_page = max(it.first_page, it.j0 * (PT_KV / 32));
 }
 
-// Queries of 32 rows into the tile's K-major, swizzled image: lane i holds the address of row r0 + i; all in flight, a row (two of heads of 64) a load
-template <bool LINES, int HS, typename Ready>
-DL_DEVINL void pt_load_rows(const float* mine, uint8_t* tile, int r0, Ready ready) {
+// Queries of 32 rows into the tile's K-major, swizzled image: lane i holds the address of row r0 + i; all in flight, a row (two of heads of 64) a load.
+// Returns what the scores of lane i's row are multiplied with.  CODES: a row beyond fp16's range goes in times a power of two that brings its largest value
+// below 2^15, one that is not finite as zeros times NaN (rare, and then each row again)
+template <bool LINES, int HS, bool CODES, typename Ready>
+DL_DEVINL float pt_load_rows(const float* mine, uint8_t* tile, int r0, Ready ready) {
     constexpr int PER = PT_HS / HS;
     const int lane = threadIdx.x & 31, in = lane * 4 / HS, col = lane * 4 % HS;
     uint8_t* qd = tile + (r0 + in) * 128 + (col >> 6) * 16384 + (lane & 1) * 8;
@@ -448,11 +450,38 @@ DL_DEVINL void pt_load_rows(const float* mine, uint8_t* tile, int r0, Ready read
     for (int u = 0; u < 32; u += PER)            // 16-byte piece c of a half row -> swizzled slot c ^ (row & 7)
         *reinterpret_cast<uint2*>(qd + u * 128 + ((((lane >> 1) & 7) ^ ((u + in) & 7)) << 4)) =
             make_uint2(pt_pack2<LINES>(x[u / PER].x, x[u / PER].y), pt_pack2<LINES>(x[u / PER].z, x[u / PER].w));
+    float factor = 1.f;
+    if constexpr (CODES) {
+        const auto size = [](float4 y) {           // as bits: an infinity or a NaN is above every number
+            return max(max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu), max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu));
+        };
+        unsigned top = 0;
+#pragma unroll
+        for (int u = 0; u < 32; u += PER) top = max(top, size(x[u / PER]));
+        if (__any_sync(0xffffffffu, top > 0x477fe000u)) {        // 65504
+#pragma unroll 1
+            for (int u = 0; u < 32; u += PER) {
+                float4 y = reinterpret_cast<const float4*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)mine, u + in))[col >> 2];
+                unsigned most = size(y);
+#pragma unroll
+                for (int o = HS / 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const bool finite = most < 0x7f800000u, down = finite && most > 0x477fe000u;
+                const float by = down ? __uint_as_float((268u - (most >> 23)) << 23) : 1.f;      // 2^(14 - exponent)
+                const float back = !finite ? __uint_as_float(0x7fffffffu) : down ? __uint_as_float(((most >> 23) - 14u) << 23) : 1.f;
+                y = finite ? make_float4(y.x * by, y.y * by, y.z * by, y.w * by) : make_float4(0.f, 0.f, 0.f, 0.f);
+                *reinterpret_cast<uint2*>(qd + u * 128 + ((((lane >> 1) & 7) ^ ((u + in) & 7)) << 4)) = make_uint2(pt_pack2<LINES>(y.x, y.y), pt_pack2<LINES>(y.z, y.w));
+                const float row = __shfl_sync(0xffffffffu, back, lane % PER * (HS / 4));         // of row u + lane % PER
+                if (lane / PER * PER == u) factor = row;
+            }
+        }
+    }
     fence_proxy_async_smem();
+    return factor;
 }
 
 // HS: head size; 64 (LINES: not) takes the first half of every tile and accumulator.  SHARES (LINES: not): items may go to several CTAs (4001 rows, whose
-// items do not, take 1.2 % longer with it).  CODES (LINES: not): over the widened 8-bit cache, where a line may be a key of NaN
+// items do not, take 1.2 % longer with it).  CODES (LINES: not): over the widened 8-bit cache, where a line may be a key of NaN, and queries
+// of any size meet keys of any size
 template <bool LINES, int HS = PT_HS, bool SHARES = false, bool CODES = false>
 __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(const __grid_constant__ typename PtKernelArgs<LINES>::T a,
                                                                              const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -569,11 +598,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16, T_S = tmem_base + lane_base, T_P = t_p(t) + lane_base, T_O = tmem_base + lane_base + 256 + t * 128;
         float* stage = out_s + (size_t)warp * 32 * PT_OUT_LD;
         uint32_t ns = 0, nq = 0;                                 // steps of this tile so far, items whose queries are loaded
+        float q_factor = 1.f;                                    // of this row's queries, as they were loaded last
         PtItem it, next;
         // the queries of the tile's next item: all rows in flight at once, ahead of this item's outputs
         auto load_queries = [&](const PtItem& of) {
             if (!(t ? of.jb[1] > of.ja[1] : of.jb[0] > of.ja[0])) return;
-            pt_load_rows<LINES, HS>(row_of(of, t, row), q_s + t * PT_TILE_BYTES, quarter * 32, [&] {
+            q_factor = pt_load_rows<LINES, HS, CODES>(row_of(of, t, row), q_s + t * PT_TILE_BYTES, quarter * 32, [&] {
                 if (nq > 0) wait(&q_empty[t], (nq - 1) & 1);      // the tile's last scores have read the queries before
             });
             nq++;
@@ -603,6 +633,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
             } else {
                 pos_r = it.p0 + r_abs;
                 sc = 1.4426950408889634f * rsqrtf((float)HS);        // scores in the log2 domain
+                if constexpr (CODES) sc *= q_factor;
             }
             float m_used = -INFINITY, l = 0.0f;
             for (int j = ja; j < jb; j++, ns++) {

@@ -426,7 +426,7 @@ def kv8_attention_prefill(q, M: int, n_heads: int, pos, slot, block_table, meta,
                           y_out=None, pdl: bool = False):
     """`attention_prefill` over an 8-bit cache: meta = [n_seg, begin0, end0, ...] (device int32), each range consecutive positions of one sequence, no row
     in two, eight at most (what is listed beyond that, or beyond the tensor's end, is not looked at); rows outside are not touched.  workspace: kv8_prefill_workspace(), for one launch at a time; with
-    it long prompts are multiplied in fp16 (queries, keys and values in its range)."""
+    it long prompts are multiplied in fp16 (keys and values within its range; queries are brought there)."""
     rows = _kv8_rows(M, pos, slot, block_table, cache)
     ldq, ldy, y_type = _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out)
     if meta.dtype is not torch.int32 or meta.get_device() != cache.index or not meta.is_contiguous() or meta.numel() < 3:

@@ -1,4 +1,5 @@
-"""The 8-bit token cache where lines are not ordinary: NaN lines at every place of a step, lines read back beside queued work.
+"""The 8-bit token cache where lines are not ordinary: NaN lines at every place of a step, queries beyond fp16, lines read back beside
+queued work.
 
 Tolerances are those of test_gpu_kv8.py, which derives them.
 """
@@ -8,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv8 import K, PAGE, _attention, _cache, _dev, _i32, _table, _values
+from test_gpu_kv8 import K, PAGE, PROMPT_REL, _attention, _cache, _dev, _i32, _near, _table, _values
 
 pytestmark = pytest.mark.gpu
 
@@ -62,6 +63,39 @@ def test_a_nan_line_is_seen_wherever_it_stands(heads, kv, hs, rows, context, wid
     nan = torch.isnan(p.run(workspace))
     sees = torch.tensor([[context + m >= first + h // (heads // kv) for h in range(heads)] for m in range(rows)])
     assert torch.equal(nan.all(-1), sees) and torch.equal(nan.any(-1), sees)
+
+
+@pytest.mark.parametrize("workspace", [False, True])
+@pytest.mark.parametrize("heads,kv,hs,rows,context", [(16, 4, 128, 300, 0), (16, 4, 128, 300, 90), (16, 8, 128, 260, 2600), (32, 8, 64, 240, 0), (32, 8, 64, 240, 3000), (8, 8, 64, 930, 0)])
+def test_prompt_queries_beyond_fp16(heads, kv, hs, rows, context, workspace):
+    """Finite ones count as they are, whatever their size beside the row's others; an infinity or a NaN makes the row of its head NaN, and no other."""
+    p = _Prompt(heads, kv, hs, rows, context)
+    p.host[0][..., 5] = 0                                          # a channel that no key has: queries may be large there
+    q = p.q.view(rows, heads, hs)
+    large = {0: 1e5, 1: -7e4, 33: 65519.0, 64: -3e6, 131: 4e5, rows - 1: 65536.0}
+    for m, x in large.items():
+        q[m, :, 5] = x
+    q[2, 0, 5], q[40, 3, 7], q[rows - 2, 1, hs - 1], q[130, 2, 0] = math.inf, math.nan, -math.inf, math.inf
+    y = p.run(workspace)
+    bad = torch.zeros(rows, heads, dtype=torch.bool)
+    bad[2, 0] = bad[40, 3] = bad[rows - 2, 1] = bad[130, 2] = True
+    nan = torch.isnan(y)
+    assert torch.equal(nan.all(-1), bad) and torch.equal(nan.any(-1), bad)
+    for m in sorted(set(large) | {3, 32, 41, 129, rows - 3}):
+        if workspace or m not in large:                            # (without one queries have 16 bits of the largest of them: the others are lost beside it here)
+            _near(y[m].reshape(1, -1), p.ref(m).reshape(1, -1), PROMPT_REL)
+
+
+@pytest.mark.parametrize("heads,kv,hs,rows", [(16, 4, 128, 300), (32, 8, 64, 240)])
+def test_first_rows_of_large_queries(heads, kv, hs, rows):
+    """One token is seen: its value, however far below zero its score is."""
+    p = _Prompt(heads, kv, hs, rows, 0)
+    q = p.q.view(rows, heads, hs)
+    page, place = p.at(0)
+    for h in range(heads):
+        q[0, h] = -2e5 * torch.sign(p.host[0][page, h // (heads // kv), place].float())
+    for workspace in (False, True):
+        _near(p.run(workspace)[0].reshape(1, -1), p.ref(0).reshape(1, -1), PROMPT_REL)
 
 
 def _engine(path, **kw):
