@@ -567,9 +567,10 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
 // ------------------------------------------------------------------------------------------------
 // Prompt chunks: eight (row, head) pairs of one key/value head, of two digits a query (16 bits), fill an int8 MMA, two of them make the 16 rows of a tile, whose
 // pages four warps share.  Two digits of a weight would not do: what is below 2^-16 of the largest weight is lost, however many tokens there are.  So
-// weights are fp16 here (2^-12 of themselves), values are widened in registers -- codes are exact in fp16 -- and sums are the f32 accumulators of m16n8k16.
-// p = 2^(s - ref) goes by a reference that moves only when a score is more than 2^8 above it, or a weight outgrows fp16: a vote of the warp, so that a page in the
-// steady state takes no exchange for a running maximum and no rescaling.
+// weights p s_v are fp16 here, in a unit by the row's largest one that still counts (2^-11 of themselves, below 2^-20 of the largest 2^-31 of that), values are widened
+// in registers -- codes are exact in fp16 -- and sums are the f32 accumulators of m16n8k16.
+// p = 2^(s - ref) goes by a reference that moves only when a score is more than 2^8 above it, the unit only then or when a weight outgrows fp16: a vote of the warp, so
+// that a page in the steady state takes no exchange for a running maximum and no rescaling.
 //
 // What bounds it: a warp's chain of latencies through a page, with two warps of 218 registers on each scheduler (64 MMAs a page, the tensor pipe is 14 % busy, a
 // third of the clocks issue).  100 rows of 32 heads on 8 of 128 behind 1000 tokens 18.8 us, 500 of 64 behind none 21.  32 stacked rows a CTA, which halves the
@@ -639,7 +640,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, HS == 128 ? 2 : 4) kv8_prompt_k
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
     uint32_t qf[2][KS][4];
-    float fl[2], ref[2], run_l[2], up[2];                      // reference of the weights, their sum (this lane's tokens), their unit's inverse
+    float fl[2], ref[2], run_l[2], run_w[2], up[2];            // reference of the weights, their sum and largest weight * scale (this lane's tokens), their unit's inverse
     int lim[2];                                                // tokens that the lane's rows see
 #pragma unroll
     for (int mt = 0; mt < 2; mt++) {
@@ -647,13 +648,13 @@ __global__ void __launch_bounds__(KA_WARPS * 32, HS == 128 ? 2 : 4) kv8_prompt_k
         fl[mt] = ka_digits<HS, false>(x[mt], s < n_live, true, qf[mt]);
         lim[mt] = s < n_live ? min(T, p0 + (s_lo + s) / G + 1) : 0;
         ref[mt] = -INFINITY;
-        run_l[mt] = 0.f;
-        up[mt] = 0x1p125f;
+        run_l[mt] = run_w[mt] = 0.f;
+        up[mt] = 0x1p109f;
     }
     float o[NT][4];                                            // rows g (0, 1) and g + 8 (2, 3)
 #pragma unroll
     for (int n = 0; n < NT; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    auto rescale = [&](float c0, float c1) {
+    const auto rescale = [&](float c0, float c1) {
 #pragma unroll
         for (int n = 0; n < NT; n++) { o[n][0] *= c0; o[n][1] *= c0; o[n][2] *= c1; o[n][3] *= c1; }
     };
@@ -696,8 +697,9 @@ __global__ void __launch_bounds__(KA_WARPS * 32, HS == 128 ? 2 : 4) kv8_prompt_k
             for (int e = 1; e < 8; e++) top[mt] = fmaxf(top[mt], s[mt][e]);
             move |= top[mt] > ref[mt] + AHEAD;
         }
-        if (__any_sync(0xffffffffu, move)) {                   // the references move to the maxima
-            float corr[2];
+        float corr[2] = {1.f, 1.f};
+        bool unit = __any_sync(0xffffffffu, move);
+        if (unit) {                                            // the references move to the maxima
 #pragma unroll
             for (int mt = 0; mt < 2; mt++) {
                 top[mt] = fmaxf(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 1));
@@ -706,8 +708,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, HS == 128 ? 2 : 4) kv8_prompt_k
                 corr[mt] = ref[mt] == -INFINITY ? 0.f : ka_exp2(ref[mt] - top[mt]);
                 ref[mt] = top[mt];
                 run_l[mt] *= corr[mt];
+                run_w[mt] *= corr[mt];
             }
-            rescale(corr[0], corr[1]);
         }
         bool grow = false;
 #pragma unroll
@@ -723,22 +725,23 @@ __global__ void __launch_bounds__(KA_WARPS * 32, HS == 128 ? 2 : 4) kv8_prompt_k
                 top[mt] = ka_max_nan(top[mt], w[mt][e]);
             }
             run_l[mt] += sum;
+            run_w[mt] = ka_max_nan(run_w[mt], top[mt]);
             grow |= !(top[mt] * up[mt] < MOST_W);
         }
-        if (__any_sync(0xffffffffu, grow)) {                   // a larger unit (or a NaN)
-            float wider[2] = {1.f, 1.f};
+        unit |= __any_sync(0xffffffffu, grow);
+        if (unit) {                                            // another unit: weights have grown, or the largest ones count less beside the new maxima (or a NaN)
 #pragma unroll
             for (int mt = 0; mt < 2; mt++) {
-                top[mt] = ka_max_nan(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 1));
-                top[mt] = ka_max_nan(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 2));
-                if (!(top[mt] < INFINITY)) run_l[mt] = __uint_as_float(0x7fffffffu);
-                else if (top[mt] * up[mt] >= MOST_W) {
-                    const float unit = __uint_as_float((uint32_t)(TOP + 254 - min(max((int)(__float_as_uint(top[mt]) >> 23), 24), 254)) << 23);
-                    wider[mt] = unit / up[mt];
-                    up[mt] = unit;
+                float big = ka_max_nan(run_w[mt], __shfl_xor_sync(0xffffffffu, run_w[mt], 1));
+                big = ka_max_nan(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                if (!(big < INFINITY)) run_l[mt] = __uint_as_float(0x7fffffffu);
+                else {
+                    const float now = __uint_as_float((uint32_t)(TOP + 254 - min(max((int)(__float_as_uint(big) >> 23), 24), 254)) << 23);
+                    corr[mt] = corr[mt] * (1.f / up[mt]) * now;      // (2 at most, as what counted before counts in `big`)
+                    up[mt] = now;
                 }
             }
-            rescale(wider[0], wider[1]);
+            rescale(corr[0], corr[1]);
         }
         // values of 8 tokens for each lane: k index 2 a, 2 a + 1, 8 + 2 a, 9 + 2 a of an MMA are tokens 8 a .. + 3, of the next one 8 a + 4 .. + 7
         uint32_t pa[2][4];

@@ -1,5 +1,5 @@
-"""The 8-bit token cache where lines are not ordinary: NaN lines at every place of a step, queries beyond fp16, lines read back beside
-queued work.
+"""The 8-bit token cache where lines are not ordinary: NaN lines at every place of a step, queries beyond fp16, weights of very
+unlike sizes, lines read back beside queued work.
 
 Tolerances are those of test_gpu_kv8.py, which derives them.
 """
@@ -96,6 +96,24 @@ def test_first_rows_of_large_queries(heads, kv, hs, rows):
         q[0, h] = -2e5 * torch.sign(p.host[0][page, h // (heads // kv), place].float())
     for workspace in (False, True):
         _near(p.run(workspace)[0].reshape(1, -1), p.ref(0).reshape(1, -1), PROMPT_REL)
+
+
+@pytest.mark.parametrize("heads,kv,hs", [(4, 1, 128), (8, 2, 64), (4, 2, 32)])
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 26, 2.0 ** 40, 2.0 ** 100])
+def test_prompt_values_of_very_unlike_sizes(heads, kv, hs, size):
+    """Early tokens whose values are huge and whose weights vanish beside those of later ones: what counts are the later ones' values, to the last digit."""
+    p = _Prompt(heads, kv, hs, 40, 500)
+    p.q = 1.0 + 0.1 * p.q                                          # queries of about one direction
+    low = -(math.log(size) + 45.0)                                 # scores: the early weights are size * e^low = e^-45 of the others
+    page = int(p.bt[0, 0])
+    p.host[0][page], p.host[2][page] = -127, -low / math.sqrt(hs) / 127
+    p.host[3][page] *= size
+    page = int(p.bt[0, 4])                                         # (this one too: less low, less huge)
+    p.host[0][page], p.host[2][page] = -127, 30.0 / math.sqrt(hs) / 127
+    p.host[3][page] *= 2.0 ** 10
+    y = p.run(False)
+    for m in (0, 1, 17, 39):
+        _near(y[m].reshape(1, -1), p.ref(m).reshape(1, -1), PROMPT_REL)
 
 
 def _engine(path, **kw):
