@@ -4,8 +4,8 @@
 // keys and values as the cache holds them; output f32 (or rounded once to 16 bits) and / or cast to Q80 in the slabs that the wo matmul consumes
 // (OP_CAST, src/llm.cpp:296-301).
 //
-// A row without tokens (a negative position) gives zeros; one whose sequence, position or page is not in the tables, or whose query is not finite,
-// gives NaN, and so does a token whose line holds a NaN to the rows that see it.
+// A row without tokens (a negative position) gives zeros; one whose sequence, position or page is not in the tables, whose query is not finite or whose
+// scores are all below what f32 holds gives NaN, and so does a token whose line holds a NaN to the rows that see it.
 #include <math.h>
 #include <type_traits>
 #include "epilogue.cuh"
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
             O.x = fmaf(x.x, e, O.x); O.y = fmaf(x.y, e, O.y); O.z = fmaf(x.z, e, O.z); O.w = fmaf(x.w, e, O.w);
         }
         if (single) {
-            const float inv = L == 0.f ? 0.f : 1.f / L;
+            const float inv = L == 0.f && T == 0 ? 0.f : 1.f / L;
             kv8_store4(a, m0, hd * HS + d, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv), live, lane);
         } else if (live) {
             const size_t pidx = ((size_t)m0 * a.heads + hd) * wk.n_splits + sp;
@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
             O.x += __shfl_xor_sync(0xffffffffu, O.x, w); O.y += __shfl_xor_sync(0xffffffffu, O.y, w);
             O.z += __shfl_xor_sync(0xffffffffu, O.z, w); O.w += __shfl_xor_sync(0xffffffffu, O.w, w);
         }
-        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const float inv = 1.f / L;
         kv8_store4(a, m0, hd * HS + lane % LPH * 4, make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv), lane < LPH, lane);
     }
 }
@@ -810,7 +810,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, HS == 128 ? 2 : 4) kv8_prompt_k
         float L = l * e;
         for (int w = 1; w < parts; w <<= 1) L += __shfl_xor_sync(0xffffffffu, L, w);
         if (j < mine) {
-            share[tid] = L == 0.f ? 0.f : e / L;
+            share[tid] = L == 0.f && T == 0 ? 0.f : e / L;
             if (z == 0) { place[j * 2] = row_of(s); place[j * 2 + 1] = head_of(s) * HS; }
         }
     }

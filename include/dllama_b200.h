@@ -220,7 +220,7 @@ typedef struct {
 } DlKv8Cache;
 /* The rows of a batch (device arrays): row m is position pos[m] of sequence slot[m], whose page i is block_table[slot * max_pages + i], of n_slots sequences.  A row
  * with a negative position has no token: nothing is written or read, attention gives zeros.  Sequences, positions and pages that are not in the tables are not
- * followed: nothing is written, what is read or attended to is NaN. */
+ * followed: nothing is written, what is read or attended to is NaN.  So is attention whose scores are all below what f32 holds.  In Q80 slabs a NaN is 0. */
 /* merged rows q | k | v (row stride ld_qkv): rotary positions on the n_heads query heads and the key heads (pairs of neighbouring values; freqs NULL: none),
  * queries to q_out (row stride ld_q), keys and values into their pages.  Keys are turned in 64 bits and rounded once, so that their codes do not depend on the
  * order of anything.  Rows of one place (slot, position) have to hold the same values (reference: OP_ROPE_LLAMA + OP_SHIFT, nn-cpu-ops.cpp:1090-1120,1253-1275) */

@@ -1,5 +1,5 @@
 """The 8-bit token cache where lines are not ordinary: NaN lines at every place of a step, queries beyond fp16, weights of very
-unlike sizes, lines read back beside queued work.
+unlike sizes, scores beyond f32, lines read back beside queued work.
 
 Tolerances are those of test_gpu_kv8.py, which derives them.
 """
@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv8 import K, PAGE, PROMPT_REL, _attention, _cache, _dev, _i32, _near, _table, _values
+from test_gpu_kv8 import ATT_REL, K, PAGE, PROMPT_REL, _attention, _cache, _dev, _i32, _near, _table, _values
 
 pytestmark = pytest.mark.gpu
 
@@ -114,6 +114,39 @@ def test_prompt_values_of_very_unlike_sizes(heads, kv, hs, size):
     y = p.run(False)
     for m in (0, 1, 17, 39):
         _near(y[m].reshape(1, -1), p.ref(m).reshape(1, -1), PROMPT_REL)
+
+
+@pytest.mark.parametrize("heads,kv,hs", [(4, 1, 128), (4, 1, 64), (4, 2, 32)])
+def test_scores_beyond_f32(heads, kv, hs):
+    """Where every score of a row is below what f32 holds, no weight can be formed: NaN, and not the zeros of a row without tokens."""
+    k = K()
+    positions, M = [900, 3, -1, 40], 4
+    rng = np.random.default_rng(hs)
+    bt, n_pages = _table(rng, [max(p, 0) + 1 for p in positions])
+    host = _cache(rng, n_pages, kv, hs)
+    q = torch.from_numpy(rng.standard_normal((M, heads * hs)).astype(np.float32))
+    for m in (0, 1):
+        host[0][bt[m, :positions[m] // PAGE + 1]], host[2][bt[m, :positions[m] // PAGE + 1]] = -127, 1e18
+        q[m] = 1e22
+    cache = k.Kv8Cache(*_dev(*host))
+    where = (_i32(positions), _i32(list(range(M))), torch.from_numpy(bt).cuda())
+    for splits in (1, 8):
+        scratch = torch.zeros(k.attention_scratch_bytes(M, heads, hs, splits), dtype=torch.uint8, device="cuda")
+        y = torch.full((M, heads * hs), 3.0, device="cuda")
+        k.kv8_attention(q.cuda(), M, heads, *where, cache, splits, scratch, y_out=y)
+        assert torch.isnan(y[:2]).all() and (y[2] == 0).all()
+        _near(y[3:], _attention(q[3].view(heads, hs), _values(host[0], host[2], bt[3], 41), _values(host[1], host[3], bt[3], 41)).reshape(1, -1), ATT_REL)
+
+
+@pytest.mark.parametrize("heads,kv,hs,rows,context,workspace", [
+    (16, 4, 128, 300, 40, True), (32, 8, 64, 240, 0, True), (16, 8, 128, 260, 2600, True), (32, 8, 64, 240, 3000, True), (4, 2, 32, 60, 10, False), (8, 1, 64, 33, 0, False), (4, 1, 128, 20, 700, False)])
+def test_prompt_scores_beyond_f32(heads, kv, hs, rows, context, workspace):
+    p = _Prompt(heads, kv, hs, rows, context)
+    p.host[0][:], p.host[2][:] = -127, 60000.0 / 127 if workspace else 1e18
+    q = p.q.view(rows, heads, hs)
+    q[3] = q[rows - 1] = 3e38 if workspace else 1e22
+    nan = torch.isnan(p.run(workspace))
+    assert nan[3].all() and nan[rows - 1].all() and not nan[:3].any() and not nan[4:rows - 1].any()
 
 
 def _engine(path, **kw):
