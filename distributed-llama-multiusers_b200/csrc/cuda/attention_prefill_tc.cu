@@ -122,6 +122,12 @@ DL_DEVINL float pt_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+template <bool NAN_TOO> DL_DEVINL float pt_max(float a, float b) {      // NAN_TOO: of a NaN and a number the NaN
+    if (!NAN_TOO) return fmaxf(a, b);
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
 template <bool LINES> DL_DEVINL uint32_t pt_pack2(float lo, float hi) {
     if (LINES) {
         __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -134,11 +140,11 @@ template <bool LINES> DL_DEVINL uint32_t pt_pack2(float lo, float hi) {
 // exp2 on the FMA pipe (Cody-Waite split + degree-3 polynomial, relative error 8e-5 -- the result is rounded to fp16,
 // 5e-4, right after; LINES, whose other kernels form it in full: degree 5, 2e-7): the softmax is bound by the 16 MUFU results
 // per clock and SM (128 x 128 exp2 per step = 1024 clk, as long as the MMAs of the step), so every fourth element takes this
-// path instead.  LINES, CODES: a NaN stays one, as in the mma.sync kernels (an exponent that is added to its bits would make a number of it)
-template <bool LINES, bool CODES> DL_DEVINL pair_f pt_ex2_poly(pair_f x) {
-    float lo, hi;
+// path instead
+template <bool LINES> DL_DEVINL pair_f pt_ex2_poly(pair_f x) {
+    float lo, hi;                                  // LINES: a NaN stays one, as in the mma.sync kernel
     pair_get(x, lo, hi);
-    if (LINES || CODES) {
+    if (LINES) {
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-126.0f));
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-126.0f));
     } else {
@@ -150,27 +156,24 @@ template <bool LINES, bool CODES> DL_DEVINL pair_f pt_ex2_poly(pair_f x) {
     const pair_f f = fma2(add2(t, both(-12582912.0f)), both(-1.0f), xc);                // [-0.5, 0.5]
     float tl, th, pl, ph;
     pair_get(t, tl, th);
-    const auto power = [&] { return pair_of(__int_as_float((__float_as_int(tl) << 23) + 0x3f800000), __int_as_float((__float_as_int(th) << 23) + 0x3f800000)); };
     if (LINES) {
         const pair_f p = fma2(fma2(fma2(fma2(fma2(both(1.32764725e-3f), f, both(9.67554096e-3f)), f, both(0.0555071309f)), f, both(0.240221202f)), f, both(0.693146944f)), f, both(1.00000012f));
-        return mul2(p, power());
+        return mul2(p, pair_of(__int_as_float((__float_as_int(tl) << 23) + 0x3f800000), __int_as_float((__float_as_int(th) << 23) + 0x3f800000)));
     }
-    const pair_f p = fma2(fma2(fma2(both(0.0550886838f), f, both(0.242604051f)), f, both(0.693276242f)), f, both(0.99992894f));
-    if (CODES) return mul2(p, power());
-    pair_get(p, pl, ph);
+    pair_get(fma2(fma2(fma2(both(0.0550886838f), f, both(0.242604051f)), f, both(0.693276242f)), f, both(0.99992894f)), pl, ph);
     return pair_of(__int_as_float(__float_as_int(pl) + (__float_as_int(tl) << 23)), __int_as_float(__float_as_int(ph) + (__float_as_int(th) << 23)));
 }
 
 // 32 scores (masked ones are -inf) -> exp2(s * sc - ref) as 16 packed fp16 pairs; their sum is added to `sum`.  LINES: as bf16 and, in `lo`, the
 // bf16 remainder of each, 17 bits together
-template <bool LINES, bool CODES> DL_DEVINL void pt_probs(const uint32_t (&v)[32], float sc, float ref, uint32_t (&pk)[16], uint32_t (&lo)[LINES ? 16 : 1], pair_f& sum) {
+template <bool LINES> DL_DEVINL void pt_probs(const uint32_t (&v)[32], float sc, float ref, uint32_t (&pk)[16], uint32_t (&lo)[LINES ? 16 : 1], pair_f& sum) {
     const pair_f sc2 = pair_of(sc, sc), ref2 = pair_of(-ref, -ref);
 #pragma unroll
     for (int e = 0; e < 32; e += 2) {
         pair_f p = fma2(pair_of(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, ref2);
         float pa, pb;
         if ((e & 6) == 6) {
-            p = pt_ex2_poly<LINES, CODES>(p);
+            p = pt_ex2_poly<LINES>(p);
             pair_get(p, pa, pb);
         } else {
             pair_get(p, pa, pb);
@@ -676,9 +679,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
 #pragma unroll
                 for (int e = 0; e < 32; e += 2)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) mx4[c] = fmaxf(mx4[c], fmaxf(__uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1])));
-                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
-                const bool need = mx > m_used + 8.0f;            // the reference may lag the maximum by 2^8
+                    for (int c = 0; c < 4; c++) mx4[c] = pt_max<CODES>(mx4[c], pt_max<CODES>(__uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1])));
+                const float mx = pt_max<CODES>(pt_max<CODES>(mx4[0], mx4[1]), pt_max<CODES>(mx4[2], mx4[3])) * sc;
+                // the reference may lag the maximum by 2^8.  (CODES: a score of NaN, which the polynomial in pt_probs would lose, makes it NaN, and with it
+                // the sum of the weights for good)
+                const bool need = CODES ? !(mx <= m_used + 8.0f) : mx > m_used + 8.0f;
                 const bool moved = __any_sync(0xffffffffu, need);
                 float alpha = 1.f;
                 if (moved) {
@@ -693,7 +698,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                 // LINES: formed ahead of the waits, in the scores' registers, as the place is free only when the other tile's have been multiplied
                 if constexpr (LINES) {
 #pragma unroll
-                    for (int c = 0; c < 4; c++) pt_probs<LINES, CODES>(v[c], sc, ref, pk[c], lo[c], sum);
+                    for (int c = 0; c < 4; c++) pt_probs<LINES>(v[c], sc, ref, pk[c], lo[c], sum);
                 }
                 // this tile's P V before is complete; LINES: and the other's, whose probabilities lie in this place.  Neither barrier can be more than the one
                 // phase ahead that a parity tells, as its next phase waits for the probabilities of this step (the phases of the other tile's o_full pass
@@ -714,7 +719,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                 }
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    if constexpr (!LINES) pt_probs<LINES, CODES>(v[c], sc, ref, pk[c], lo[c], sum);
+                    if constexpr (!LINES) pt_probs<LINES>(v[c], sc, ref, pk[c], lo[c], sum);
                     tmem_st_32x32b_x16(T_P + c * 16, pk[c]);
                     if constexpr (LINES) tmem_st_32x32b_x16(T_P + 64 + c * 16, lo[c]);
                 }
