@@ -1,5 +1,5 @@
 """The 8-bit token cache where lines are not ordinary: NaN lines at every place of a step, queries beyond fp16, weights of very
-unlike sizes, scores beyond f32, lines read back beside queued work.
+unlike sizes, scores beyond f32, pages beyond 2^32 bytes, lines read back beside queued work, users of unlike lengths.
 
 Tolerances are those of test_gpu_kv8.py, which derives them.
 """
@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv8 import ATT_REL, K, PAGE, PROMPT_REL, _attention, _cache, _dev, _i32, _near, _table, _values
+from test_gpu_kv8 import ATT_REL, K, PAGE, PROMPT_REL, _attention, _cache, _code, _dev, _i32, _near, _table, _values
 
 pytestmark = pytest.mark.gpu
 
@@ -149,6 +149,37 @@ def test_prompt_scores_beyond_f32(heads, kv, hs, rows, context, workspace):
     assert nan[3].all() and nan[rows - 1].all() and not nan[:3].any() and not nan[4:rows - 1].any()
 
 
+def test_far_pages_of_a_larger_cache():
+    """Pages beyond 2^32 bytes of codes, and of the fp16 pages of a workspace: written, read back, attended to by tokens and by prompts on both routes."""
+    k = K()
+    n_pages, kv, hs, heads, T, n = 135000, 8, 128, 8, 1200, 530    # 4.4 GB of codes of the keys, 8.8 GB of keys as fp16; as many of the values
+    if torch.cuda.mem_get_info()[0] < 36 << 30:
+        pytest.skip("36 GB of device memory")
+    rng = np.random.default_rng(4)
+    bt = np.concatenate([n_pages - 1 - 3 * rng.permutation(T // PAGE), [7]]).astype(np.int32)[None]
+    cache, table = k.alloc_kv8(n_pages, kv, hs, "cuda"), torch.from_numpy(bt).cuda()
+    pos, slot = torch.arange(T, dtype=torch.int32, device="cuda"), torch.zeros(T, dtype=torch.int32, device="cuda")
+    qkv, q = torch.from_numpy(rng.standard_normal((T, (heads + 2 * kv) * hs)).astype(np.float32)), torch.zeros(T, heads * hs, device="cuda")
+    k.kv8_write(qkv.cuda(), T, heads, None, pos, slot, table, q, cache)
+    codes, scales = _code(qkv.view(T, -1, hs)[:, heads:])
+    held = codes.double() * scales.double()[..., None]
+    kk, vv = (torch.zeros(T, kv * hs, device="cuda") for _ in range(2))
+    k.kv8_read(T, pos, slot, table, cache, kk, vv)
+    assert torch.equal(kk.cpu().view(T, kv, hs), held[:, :kv].float()) and torch.equal(vv.cpu().view(T, kv, hs), held[:, kv:].float())
+    ref = {m: _attention(q[m].cpu().view(heads, hs), held[:m + 1, :kv], held[:m + 1, kv:]).reshape(1, -1) for m in (T - n, T - n + 127, T - 300, T - 1)}
+    splits = k.kv8_attention_splits(1, heads, kv, bt.shape[1])
+    y = torch.zeros(1, heads * hs, device="cuda")
+    k.kv8_attention(q[T - 1:], 1, heads, pos[T - 1:], slot[:1], table, cache, splits, torch.zeros(k.attention_scratch_bytes(1, heads, hs, splits), dtype=torch.uint8, device="cuda"), y_out=y)
+    _near(y, ref[T - 1], ATT_REL)
+    assert k.kv8_widens(n, heads, hs)
+    for work in (k.kv8_prefill_workspace(n_pages, kv, hs, n, "cuda"), None):
+        y = torch.zeros(n, heads * hs, device="cuda")
+        k.kv8_attention_prefill(q[T - n:], n, heads, pos[T - n:], slot[:n], table, _i32([1, 0, n]), cache, work, y_out=y)
+        for m, r in ref.items():
+            _near(y[m - T + n:m - T + n + 1], r, PROMPT_REL)
+
+
+
 def _engine(path, **kw):
     from dllama_b200.models.llama import LlamaEngine
     return LlamaEngine(path, max_rows=64, n_slots=3, max_seq_len=512, kv_dtype=torch.int8, **kw)
@@ -194,4 +225,29 @@ def test_read_cache_behind_a_queued_step(tiny_tp_model_path):
     again = e.read_cache(1, b, 50, torch.float16)
     torch.cuda.synchronize()
     assert torch.equal(got, want) and all(torch.equal(x, y) for x, y in zip(again, held))
+    e.close()
+
+
+def test_users_of_unlike_lengths(tmp_path):
+    """One user deep in a conversation beside others at its beginning: steps of few users, and of more than 32, with shares for the long one."""
+    from dllama_b200.formats import mfile
+    from dllama_b200.models.llama import LlamaEngine
+    from dllama_b200.models.oracle import OracleLlama
+    from test_gpu_kv8_model import TOL, _rel_err
+    rng, path = np.random.default_rng(3), str(tmp_path / "m.m")
+    mfile.write_random_model(path, dict(dim=512, hidden_dim=512, n_layers=2, n_heads=8, n_kv_heads=2, vocab_size=1024, max_seq_len=1024, rope_theta=500000, rope=(32, 1, 4, 8192)), exact=True, seed=6)
+    e = LlamaEngine(path, max_rows=64, n_slots=40, max_seq_len=1024, kv_dtype=torch.int8)
+    prompts = [rng.integers(1, 1024, 950).tolist()] + [rng.integers(1, 1024, 1 + i % 50).tolist() for i in range(36)]
+    slots = [e.alloc_slot() for _ in prompts]
+    for s, p in zip(slots, prompts):
+        e.prefill(s, p[:-1], 0) if len(p) > 1 else None
+    want = {}
+    for i in (0, 1, 2, 17, 36):
+        o = OracleLlama(mfile.ModelFile(path), n_nodes=1, max_seq_len=1024)
+        want[i] = o.forward(prompts[i], 0).numpy()[-1]
+    for users in (range(3), range(37)):
+        order = list(rng.permutation(list(users)))
+        got = e.forward([prompts[i][-1] for i in order], [len(prompts[i]) - 1 for i in order], [slots[i] for i in order]).float().cpu().numpy()
+        for i in set(users) & set(want):
+            assert _rel_err(got[order.index(i)], want[i]) < TOL
     e.close()
