@@ -55,8 +55,8 @@
 #define PT_SHARE_STEPS 4
 
 struct PtArgs {
-    const float* q;            // [M][n_heads*128]
-    const __half* k_cache;     // [pages][n_kv][32][128]
+    const float* q;            // [M][n_heads * head size]
+    const __half* k_cache;     // [pages][n_kv][32][head size]
     const __half* v_cache;
     const int* pos;
     const int* slot;
@@ -66,7 +66,7 @@ struct PtArgs {
     uint8_t* xq_out;
     uint8_t* xh_out;
     int out_mcap;
-    void* y_out;               // [M][n_heads*128] of DL_KV8_F32 / BF16 / F16
+    void* y_out;               // [M][n_heads * head size] of DL_KV8_F32 / BF16 / F16
     int y_type;
     PtShares part;
     unsigned long long* tr;
@@ -327,8 +327,8 @@ struct PtWaits {
 // Llama path: the items of a batch are (128-row tile of a segment, query head), late tiles (long histories) first: two heads of one key/value head
 // side by side, or two tiles of one head where the heads come alone; single tiles while there are SMs for all of them.  With a place for shares the steps of
 // a long item go to as many CTAs as there are for each.  Two tiles in one CTA take 1.75 us a step, a single one 1.03, and the join 5 us more: 130 rows of 32 heads
-// behind 2000 tokens 37 us alike, behind 8000 92 without shares and 63 with them; 512 rows (two shares) behind none 21 / 27, behind 4000 62 / 61, behind 16000 182 / 159
-// (those of heads of 64 behind 16000 156 / 122).  Item `idx` of the order that all roles of all CTAs walk; false behind the last one.
+// behind 2000 tokens 37 us alike, behind 8000 92 without shares and 63 with them; 512 rows (two shares) behind none 21 / 27, behind 4000 62 / 61, behind 16000 182 / 147
+// (those of heads of 64 behind 16000 156 / 125).  Item `idx` of the order that all roles of all CTAs walk; false behind the last one.
 template <bool SHARES> DL_DEVINL bool pt_item(const PtArgs& a, const int (*seg)[4], int n_seg, int spread, int idx, PtItem& it) {
     const int rep = a.n_heads / a.n_kv_heads;
     const bool even = rep % 2 == 0;

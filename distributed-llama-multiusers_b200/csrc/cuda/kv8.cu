@@ -8,8 +8,8 @@
 // computed, keys are turned in 64 bits (angle, sine, cosine and both products) and rounded once to f32, and x * factor goes to the nearest integer in
 // one rounding, an fma with 1.5 2^23.  Queries take f32 products of the same sines and cosines.  The sines of a row are formed once for all heads.
 //
-// What bounds both: the bytes, for many rows, else one chain of latencies.  Written, 32 query heads and 8 key/value heads of 128: one row 3.1 us, 32 3.3, 4001 (172 MB) 37.6,
-// 4.6 TB/s; read as fp16: 4001 rows 8.3 us, 100003 (621 MB) 101.9, 6.1 TB/s, of which a copy reaches 6.45.
+// What bounds them: few rows, one chain of latencies; many rows read, the bytes; many rows written, still the chains (position, sines in 64 bits and a barrier come ahead of a
+// CTA's loads: DRAM is active 45 % of the time).  Written, 32 query heads and 8 key/value heads of 128: one row 3.1 us, 32 3.3, 4001 (172 MB) 37.6, 4.6 TB/s; read as fp16: 4001 rows 8.3 us, 100003 (621 MB) 101.9, 6.1 TB/s, of which a copy reaches 6.45.
 #include <type_traits>
 #include "epilogue.cuh"
 #include "kv8.cuh"

@@ -572,8 +572,9 @@ __global__ void __launch_bounds__(KA_WARPS * 32) kv8_attention_kernel(const __gr
 // p = 2^(s - ref) goes by a reference that moves only when a score is more than 2^8 above it, the unit only then or when a weight outgrows fp16: a vote of the warp, so
 // that a page in the steady state takes no exchange for a running maximum and no rescaling.
 //
-// What bounds it: a warp's chain of latencies through a page, with two warps of 218 registers on each scheduler (64 MMAs a page, the tensor pipe is 14 % busy, a
-// third of the clocks issue).  100 rows of 32 heads on 8 of 128 behind 1000 tokens 18.8 us, 500 of 64 behind none 21.  32 stacked rows a CTA, which halves the
+// What bounds it: a warp's chain of latencies through a page, with two warps of 221 registers on each scheduler (64 MMAs a page, the tensor pipe is active 21 % of
+// the SMs' time, a third of the clocks issue).  100 rows of 32 heads on 8 of 128 behind 1000 tokens 18.3 to 19.3 us, 200 of 64 behind 1000 21, 500 of 32 behind 500 24.6.
+// Against 64 bits 2.1e-4 of a row's size (f32 rows, 130 behind 1000).  32 stacked rows a CTA, which halves the
 // widening, takes 34 % more for 30 rows of heads of 64 behind 1000 tokens (there are half the CTAs) and as much for 200; the next page's scores ahead of this one's
 // products spill.
 // ------------------------------------------------------------------------------------------------
@@ -900,9 +901,10 @@ static int ka_prompt(const Kv8AttArgs& a, int pdl, void* stream) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// Long prompt chunks of heads of 64 and 128: the segments' pages widened once to fp16 (fp16(code * scale): 2^-12 of a value, the queries of that kernel are rounded alike),
+// Long prompt chunks of heads of 64 and 128: the segments' pages widened once to fp16 (fp16(code * scale): 2^-11 of a value at most, the queries of that kernel are rounded alike),
 // then the tcgen05 kernel of the fp16 cache on them, under the same page numbers.  Widening inside that kernel would be done again by every CTA that meets a page
-// (rows / 128 * heads / 2 of them).  4001 rows behind 77 tokens: 8 MB in and 17 MB out, beside 136 GFLOP; both kernels 150 us, 908 TFLOP/s (174 with inputs in turn).
+// (rows / 128 * heads / 2 of them).  4001 rows behind 77 tokens: 8 MB in and 17 MB out, beside 136 GFLOP; both kernels 144 to 150 us, 910 to 945 TFLOP/s (172 with inputs in turn).
+// Against 64 bits 5.4e-4 of a row's size (f32 rows, 130 behind 1000).
 // Eight lanes list a segment each: one thread after the other, and every CTA for pages that are not there, took 0.8 us more.
 //
 // A line with a NaN (of the key or the value) becomes a key of NaN and a value of zeros: the rows that see it give NaN, and the weights of 0 that others
@@ -1040,10 +1042,14 @@ extern "C" int dl_kv8_attention(const float* q, long long ldq, int n_heads, cons
     return hs == 128 ? ka_decode<128>(a, n_splits, scratch, pdl, stream) : hs == 64 ? ka_decode<64>(a, n_splits, scratch, pdl, stream) : ka_decode<32>(a, n_splits, scratch, pdl, stream);
 }
 
-// Rows times heads above which a prompt takes the tcgen05 kernel on widened pages, where there is a workspace (us on mma.sync / widened.  Heads of 128, 32
-// of them: 128 rows behind 1000 tokens 21 / 24, behind 8000 95 / 92, 256 behind 2000 63 / 36, 512 behind 4000 208 / 60; 8 heads: 512 rows behind none
-// 13.5 / 17.9, 1024 27 / 22.  Heads of 64, 32 of them: 200 rows behind 1000 21 / 22, 256 behind 2000 36 / 31, 512 behind 4000 103 / 52, 4001 behind none
-// 382 / 108; 8 heads: 520 behind none 10.4 / 16.6, 1024 19.1 / 19.9)
+// Rows times heads above which a prompt takes the tcgen05 kernel on widened pages, where there is a workspace.  By rows alone, as positions are on the device: right for
+// contexts of up to some 2000 tokens; far behind a conversation fewer rows would gain, too.  us on mma.sync / widened, 32 heads of 128:
+//   rows        behind 0     1000         2000         8000         16000
+//    16         8.1 / 13.4   11.7 / 20.5  13.8 / 33.1  28.6 / 54.3  47.7 / 78.3
+//    64         9.1 / 14.4   14.7 / 22.4  19.4 / 33.5  47.5 / 53.2  85.5 / 79.1
+//   128         8.5 / 14.3   18.5 / 22.9  27.8 / 33.9  85.1 / 55.4  162 / 79.1
+// 256 behind 2000 55.2 / 35.6, 512 behind 4000 184 / 55.3; 8 heads: 512 behind none 12 / 17, 1024 28.4 / 21.5.  Heads of 64, 32 of them: 128 behind 1000 17.1 / 20.2, 200
+// 20.6 / 21.5, 128 behind 8000 84 / 38.7, 256 behind 2000 34.7 / 27.3, 512 behind 4000 102 / 46.7, 4001 behind none 376 / 107; 8 heads: 520 behind none 10.1 / 15, 1024 18.6 / 18.7
 static bool ka_widens(long long rows, int n_heads, int hs) { return (hs == 128 && rows * n_heads > 4096) || (hs == 64 && rows * n_heads > 7168); }
 
 extern int dl_attention_prefill_tc_typed(const float* q, int M, int n_heads, int n_kv_heads, int head_size, const void* k_cache, const void* v_cache, const int* pos,

@@ -371,7 +371,7 @@ def _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out):
 
 
 def kv8_attention_splits(M: int, n_heads: int, n_kv_heads: int, max_pages: int) -> int:
-    """Shares of a row's context that kv8_attention is given room for: for few rows 32, each of eight pages or more, for more rows fewer, so that the
+    """Shares of a row's context that kv8_attention is given room for (M: all rows of the launch, skipped ones too): for few rows 32, each of eight pages or more, for more rows fewer, so that the
     scratch stays small, beyond 64 rows one (128 rows of 500 tokens take 23.4 us, and 28.1 where shares are looked for).  How many a row takes goes by its part of
     all rows' pages (ka_shares in csrc/cuda/kv8_attention.cu)."""
     return max(1, min(512 // max(1, M) if M <= 64 else 1, max_pages // 8, 32))
@@ -426,7 +426,8 @@ def kv8_attention_prefill(q, M: int, n_heads: int, pos, slot, block_table, meta,
                           y_out=None, pdl: bool = False):
     """`attention_prefill` over an 8-bit cache: meta = [n_seg, begin0, end0, ...] (device int32), each range consecutive positions of one sequence, no row
     in two, eight at most (what is listed beyond that, or beyond the tensor's end, is not looked at); rows outside are not touched.  workspace: kv8_prefill_workspace(), for one launch at a time; with
-    it long prompts are multiplied in fp16 (keys and values within its range; queries are brought there)."""
+    it long prompts are multiplied in fp16 (keys and values within its range; queries are brought there), without it queries have 16 bits of their
+    largest value and weights are fp16."""
     rows = _kv8_rows(M, pos, slot, block_table, cache)
     ldq, ldy, y_type = _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out)
     if meta.dtype is not torch.int32 or meta.get_device() != cache.index or not meta.is_contiguous() or meta.numel() < 3:
