@@ -373,8 +373,10 @@ def _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out):
 def kv8_attention_splits(M: int, n_heads: int, n_kv_heads: int, max_pages: int) -> int:
     """Shares of a row's context that kv8_attention is given room for (M: all rows of the launch, skipped ones too): for few rows 32, each of eight pages or more, for more rows fewer, so that the
     scratch stays small, beyond 64 rows one (128 rows of 500 tokens take 23.4 us, and 28.1 where shares are looked for).  How many a row takes goes by its part of
-    all rows' pages (ka_shares in csrc/cuda/kv8_attention.cu)."""
-    return max(1, min(512 // max(1, M) if M <= 64 else 1, max_pages // 8, 32))
+    all rows' pages (ka_shares in csrc/cuda/kv8_attention.cu).  One, too, where rows, key/value heads and groups of four query heads are
+    more than the scratch has counters."""
+    counters = M * n_kv_heads * ((n_heads // n_kv_heads + 3) // 4)
+    return max(1, min(512 // max(1, M) if M <= 64 and counters <= 16384 else 1, max_pages // 8, 32))
 
 
 @functools.lru_cache(maxsize=4096)
