@@ -255,8 +255,8 @@ _KV8_TYPES = {torch.float32: KV8_F32, torch.bfloat16: KV8_BF16, torch.float16: K
 
 
 class Kv8Cache:
-    """The pages of one layer's 8-bit token cache: k / v int8 [pages][kv heads][32][head size], k_scale / v_scale f32 [pages][kv heads][32].
-    Checked once, here; the tensors have to keep their memory."""
+    """The pages of one layer's 8-bit token cache: k / v int8 [pages][kv heads][32][head size], k_scale / v_scale f32 [pages][kv heads][32], no scale
+    below zero.  Checked once, here (their values not); the tensors have to keep their memory."""
     __slots__ = ("k", "v", "k_scale", "v_scale", "n_pages", "n_kv_heads", "head_size", "device", "index", "args", "ref")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
@@ -306,8 +306,10 @@ def _kv8_rows(M: int, pos: torch.Tensor, slot: torch.Tensor, block_table: torch.
     return pos.data_ptr(), slot.data_ptr(), block_table.data_ptr(), M, table[0], table[1]
 
 
-def _kv8_matrix(t: torch.Tensor, M: int, cols: int, cache: Kv8Cache, what: str) -> int:
+def _kv8_matrix(t: Optional[torch.Tensor], M: int, cols: int, cache: Kv8Cache, what: str) -> int:
     """Row stride of [>= M][cols] (neighbouring values of a row lie side by side)."""
+    if t is None:
+        raise ValueError(f"{what} is missing")
     shape = t.shape                                # (half the time of dim(), size() and stride() with an argument: 0.7 us of a wrapper's 5)
     if len(shape) == 2 and shape[0] >= M and shape[1] == cols and t.get_device() == cache.index:
         if t.is_contiguous():

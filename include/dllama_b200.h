@@ -214,7 +214,7 @@ enum { DL_KV8_F32 = 0, DL_KV8_BF16 = 1, DL_KV8_F16 = 2 };      /* types of outpu
 typedef struct {
     int8_t* k;                 /* [n_pages][n_kv_heads][32][head_size] */
     int8_t* v;
-    float* k_scale;            /* [n_pages][n_kv_heads][32] */
+    float* k_scale;            /* [n_pages][n_kv_heads][32], none below zero */
     float* v_scale;
     int n_pages, n_kv_heads, head_size;      /* head_size 32, 64 or 128 */
 } DlKv8Cache;
