@@ -237,7 +237,8 @@ int dl_kv8_attention(const float* q, long long ldq, int n_heads, const int* pos,
  * all of its rows; no row in two segments).  max_seg: segments that meta has room for, eight of which are looked at.  k16 / v16 / scratch16: NULL, or a workspace for one launch at a time, fp16 [n_pages][n_kv_heads][32][head_size] twice and dl_kv8_prefill_scratch_bytes()
  * zeroed once (all aligned to 16 bytes): pages of heads of 128 with more than 4096 rows times heads, of 64 with more than 7168, are then widened once, and multiplied on
  * tcgen05 (16-bit operands, as over the fp16 cache: keys and values beyond fp16's range
- * saturate, those below 2^-14 lose digits; a query beyond it goes in times a power of two). Queries that are not finite give NaN */
+ * saturate, those below 2^-14 lose digits; a query beyond it goes in times a power of two); without a workspace they count as the cache
+ * holds them, queries in 16 bits of their largest value. Queries that are not finite give NaN */
 long long dl_kv8_prefill_scratch_bytes(int head_size);
 int dl_kv8_attention_prefill(const float* q, long long ldq, int n_heads, const int* pos, const int* slot, const int* block_table, int M, int n_slots, int max_pages, const int* meta /*device*/, int max_seg, const DlKv8Cache* cache /*host*/,
                              void* k16, void* v16, void* scratch16, uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, int pdl,

@@ -1,5 +1,5 @@
 """The 8-bit token cache where lines are not ordinary: NaN lines at every place of a step, queries beyond fp16, weights of very
-unlike sizes, scores beyond f32, pages beyond 2^32 bytes, lines read back beside queued work, users of unlike lengths.
+unlike sizes, scores beyond f32, pages beyond 2^32 bytes, calls in graphs side by side, lines read back beside queued work, users of unlike lengths.
 
 Tolerances are those of test_gpu_kv8.py, which derives them.
 """
@@ -177,6 +177,55 @@ def test_far_pages_of_a_larger_cache():
         k.kv8_attention_prefill(q[T - n:], n, heads, pos[T - n:], slot[:n], table, _i32([1, 0, n]), cache, work, y_out=y)
         for m, r in ref.items():
             _near(y[m - T + n:m - T + n + 1], r, PROMPT_REL)
+
+
+
+@pytest.mark.parametrize("heads,kv,hs,rows,context", [(16, 8, 128, 260, 2600), (32, 8, 64, 240, 10), (32, 8, 64, 240, 3000), (16, 4, 128, 100, 900)])
+def test_prompts_captured_and_side_by_side(heads, kv, hs, rows, context):
+    """A layer's calls -- rows written, one row of another user, the prompt -- twice over in two graphs with buffers of their own, replayed on two streams at once and
+    again on new rows, each launch ahead of its predecessor's end where it may: what single calls give, bit for bit."""
+    k = K()
+    rng = np.random.default_rng(rows)
+    bt, n_pages = _table(rng, [context + rows, 900])
+    host, M = _cache(rng, n_pages, kv, hs), rows + 1
+    where = (_i32([899] + list(range(context, context + rows))), _i32([1] + [0] * rows), torch.from_numpy(bt).cuda())
+    meta, skip, splits = _i32([1, 1, M]), _i32([0] + [1] * rows), 3
+    freqs = torch.from_numpy((10000.0 ** (-np.arange(0, hs, 2) / hs)).astype(np.float32)).cuda()
+
+    class Side:
+        def __init__(self):
+            self.cache = k.Kv8Cache(*_dev(*host))
+            self.qkv, self.q, self.y = (torch.zeros(M, n * hs, device="cuda") for n in (heads + 2 * kv, heads, heads))
+            self.work = k.kv8_prefill_workspace(n_pages, kv, hs, M, "cuda")
+            self.scratch = torch.zeros(k.attention_scratch_bytes(M, heads, hs, splits), dtype=torch.uint8, device="cuda")
+
+        def run(self, pdl):
+            k.kv8_write(self.qkv, M, heads, freqs, *where, self.q, self.cache, pdl=pdl)
+            k.kv8_attention(self.q, M, heads, *where, self.cache, splits, self.scratch, y_out=self.y, row_skip=skip, pdl=pdl)
+            k.kv8_attention_prefill(self.q, M, heads, *where, meta, self.cache, self.work, y_out=self.y, pdl=pdl)
+
+    sides, plain, graphs, streams = [Side(), Side()], Side(), [], [torch.cuda.Stream() for _ in range(2)]
+    plain.run(False)                                               # (functions are loaded ahead of the captures)
+    torch.cuda.synchronize()
+    for st, side in zip(streams, sides):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=st):
+            for _ in range(2):
+                side.run(True)
+    for seed in (1, 2, 3):
+        x = torch.from_numpy(np.random.default_rng(seed).standard_normal((M, (heads + 2 * kv) * hs)).astype(np.float32)).cuda()
+        for s in sides + [plain]:
+            s.qkv.copy_(x)
+        plain.run(False)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for st, graph in zip(streams, graphs):
+                with torch.cuda.stream(st):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for s in sides:
+            assert torch.equal(s.y, plain.y) and torch.equal(s.cache.k, plain.cache.k) and torch.equal(s.cache.v_scale, plain.cache.v_scale)
+    assert not torch.isnan(plain.y).any() and not any(s.scratch[:65536].any() for s in sides)
 
 
 
