@@ -737,8 +737,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                 inv = it.shares > 1 ? 1.f : (a.w.gate ? 1.f / (1.f + expf(-a.w.gate[(size_t)m_row * a.w.ld_gate + h_row])) : 1.f) / l;
             } else {
                 inv = l > 0.0f ? 1.0f / l : 0.0f;
-                // the largest weight is 1 or more, but where all scores are below what f32 holds there is none (2^-126 for each of the polynomial's)
-                if (CODES && !(l >= 0.5f)) inv = __int_as_float(0x7fffffff);
+                // the largest weight is 1 or more, but for the rounding of a large reference (2^-4 at scores of 2^26 in the log2 domain, beyond fp16 from 2^28 on); where all scores
+                // are below what f32 holds there is none (2^-126 for each of the polynomial's)
+                if (CODES && !(l >= 0x1p-13f)) inv = __int_as_float(0x7fffffff);
             }
             float* out = nullptr;                                // this thread's row (of 16-bit values: y16); null: none
             bool vec = true;                                     // 16-byte rows
@@ -817,7 +818,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) attention_prefill_tc_kernel(con
                         const float2 n = __ldcg(norms + z * PT_SHARE_WARPS * 32);
                         if (!(n.y < 0.f)) l = fmaf(n.y, pt_ex2(n.x - top), l);
                     }
-                    inv = 1.f / l;
+                    inv = l >= 0x1p-13f ? 1.f / l : __int_as_float(0x7fffffff);      // (as above)
                 }
             }
             const int live = it.rows - (row0 + quarter * 32);      // rows of this warp that are there

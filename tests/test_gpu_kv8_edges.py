@@ -86,14 +86,15 @@ def test_prompt_queries_beyond_fp16(heads, kv, hs, rows, context, workspace):
             _near(y[m].reshape(1, -1), p.ref(m).reshape(1, -1), PROMPT_REL)
 
 
+@pytest.mark.parametrize("size", [2e5, 1e6, 4e6])                # scores of -3e6, -1.6e7, -6e7 in the log2 domain
 @pytest.mark.parametrize("heads,kv,hs,rows", [(16, 4, 128, 300), (32, 8, 64, 240)])
-def test_first_rows_of_large_queries(heads, kv, hs, rows):
+def test_first_rows_of_large_queries(heads, kv, hs, rows, size):
     """One token is seen: its value, however far below zero its score is."""
     p = _Prompt(heads, kv, hs, rows, 0)
     q = p.q.view(rows, heads, hs)
     page, place = p.at(0)
     for h in range(heads):
-        q[0, h] = -2e5 * torch.sign(p.host[0][page, h // (heads // kv), place].float())
+        q[0, h] = -size * torch.sign(p.host[0][page, h // (heads // kv), place].float())
     for workspace in (False, True):
         _near(p.run(workspace)[0].reshape(1, -1), p.ref(0).reshape(1, -1), PROMPT_REL)
 
