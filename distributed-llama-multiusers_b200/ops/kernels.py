@@ -489,6 +489,87 @@ def sample_rows(logits: torch.Tensor, temperature: torch.Tensor, topp: torch.Ten
     lib.count_launch()
 
 
+def _on_device(t: Optional[torch.Tensor], dtype, n: int, index: int, what: str):
+    """The pointer of a contiguous tensor of at least n values of that type on device `index`; of None, None."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.get_device() != index or t.numel() < n or not t.is_contiguous():
+        raise ValueError(f"{what}: {tuple(t.shape)} of {t.dtype} on {t.device}; at least {n} contiguous values of {dtype} beside the others are wanted")
+    return t.data_ptr()
+
+
+def _launching(t: torch.Tensor, what: str) -> int:
+    """The index of t's device, which has to be the current one."""
+    index = t.get_device()
+    if index < 0 or index != _current_device():
+        raise ValueError(f"{what} is on {t.device}: the current device launches")
+    return index
+
+
+def sample_tokens(logits: torch.Tensor, M: int, temperature: torch.Tensor, top_k: Optional[torch.Tensor], top_p: Optional[torch.Tensor], min_p: Optional[torch.Tensor],
+                  coin: torch.Tensor, tokens_out: torch.Tensor, prob_out: Optional[torch.Tensor] = None, pdl: bool = False):
+    """tokens_out[m] = a token of logits[m] (f32, bf16 or fp16; neighbouring values of a row side by side) drawn with coin[m] in [0, 1), for the first M rows; prob_out[m]: its probability
+    among those that top_k (int32), top_p and min_p (f32, each [M] or None) leave, in that order: k <= 0 or beyond the vocabulary, p outside of (0, 1) and min_p <= 0 are
+    off.  Of equal logits the lowest index is ahead.  temperature <= 0: the first of the largest logits.  A NaN counts as -inf; a row of -inf alone gives token 0 with probability 0."""
+    d = _launching(logits, "logits")
+    kind = _KV8_TYPES.get(logits.dtype)
+    if kind is None or logits.dim() != 2 or not 0 <= M <= logits.shape[0] or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError(f"logits {tuple(logits.shape)} of {logits.dtype}: at least {M} rows of f32, bf16 or fp16 values side by side are wanted")
+    vocab = logits.shape[1]
+    if not 1 <= vocab <= _max_vocab():
+        raise ValueError(f"{vocab} logits a row: 1 to {_max_vocab()} are wanted")
+    if M > 1 and logits.stride(0) < vocab:
+        raise ValueError("rows of logits overlap")
+    if temperature is None or coin is None or tokens_out is None:
+        raise ValueError("temperature, coin or tokens_out is missing")
+    rc = cuda_lib().dl_sample_tokens(logits.data_ptr(), kind, M, vocab, max(vocab, logits.stride(0)), _on_device(temperature, _F32, M, d, "temperature"), _on_device(top_k, _I32, M, d, "top_k"),
+                                     _on_device(top_p, _F32, M, d, "top_p"), _on_device(min_p, _F32, M, d, "min_p"), _on_device(coin, _F32, M, d, "coin"),
+                                     _on_device(tokens_out, _I32, M, d, "tokens_out"), _on_device(prob_out, _F32, M, d, "prob_out"), 1 if pdl else 0, torch._C._cuda_getCurrentRawStream(d))
+    if rc:
+        check(rc, "dl_sample_tokens")
+    lib.count_launch()
+
+
+@functools.lru_cache(maxsize=1)
+def _max_vocab() -> int:
+    return cuda_lib().dl_sample_tokens_max_vocab()
+
+
+TABLES_BAD_LENGTH, TABLES_BAD_SEQ, TABLES_BAD_LEAD, TABLES_NO_PAGES, TABLES_BAD_PAGE, TABLES_NO_ROWS = 1, 2, 4, 8, 16, 32      # bits of page_tables' status
+TABLES_MAX_REQUESTS, TABLES_MAX_SEQS = 8192, 131072
+
+
+def page_tables(n: int, held: torch.Tensor, new: torch.Tensor, seq: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, taken: torch.Tensor, n_pages: int, pos: torch.Tensor,
+                slot: torch.Tensor, status: torch.Tensor, line: Optional[torch.Tensor] = None, start: Optional[torch.Tensor] = None, held_out: Optional[torch.Tensor] = None,
+                taken_out: Optional[torch.Tensor] = None, lead_seq: Optional[torch.Tensor] = None, lead_pages: Optional[torch.Tensor] = None, pdl: bool = False):
+    """The next step's block table, positions, table rows (slot) and cache lines of n requests, from lengths on the device (int32 all): request i holds held[i] tokens in table row seq[i] and runs
+    new[i] more.  Pages are taken off free_pages from place `taken` on; the first lead_pages[i] pages of a request (whole ones, of the tokens held) are those of table row lead_seq[i].
+    pos, slot (and line = page * 32 + place) list the requests' new tokens one behind the other, start [n + 1] where each begins; the places behind the last one are -1, 0, -1.  held and
+    taken go on to held_out and taken_out (None: in place).  status: 0, or bits TABLES_*: then all rows are empty, nothing is taken and the table is as it was.  No row of the table in two
+    requests, no request's own row a lead while its first pages are another's (both are noticed)."""
+    d = _launching(block_table, "block_table")
+    if block_table.dim() != 2 or block_table.dtype is not _I32 or not block_table.is_contiguous() or not 1 <= block_table.shape[0] <= TABLES_MAX_SEQS or block_table.shape[1] < 1:
+        raise ValueError(f"block_table {tuple(block_table.shape)} of {block_table.dtype}: contiguous int32 [1 to {TABLES_MAX_SEQS} sequences][pages] is wanted")
+    if not 0 <= n <= TABLES_MAX_REQUESTS or not 1 <= n_pages <= 1 << 26:
+        raise ValueError(f"{n} requests, {n_pages} pages: at most {TABLES_MAX_REQUESTS} and {1 << 26}")
+    if (lead_seq is None) != (lead_pages is None):
+        raise ValueError("lead_seq and lead_pages come together")
+    if any(t is None for t in (held, new, seq, free_pages, taken, pos, slot, status)):
+        raise ValueError("a tensor is missing")
+    M = pos.numel()
+    if M >= 1 << 31 or free_pages.numel() >= 1 << 31:
+        raise ValueError(f"{M} rows, {free_pages.numel()} free pages")
+    rc = cuda_lib().dl_page_tables(n, _on_device(held, _I32, n, d, "held"), _on_device(new, _I32, n, d, "new"), _on_device(seq, _I32, n, d, "seq"), block_table.data_ptr(), *block_table.shape,
+                                   _on_device(free_pages, _I32, 0, d, "free_pages"), free_pages.numel(), _on_device(taken, _I32, 1, d, "taken"), n_pages, M, _on_device(pos, _I32, M, d, "pos"),
+                                   _on_device(slot, _I32, M, d, "slot"), _on_device(line, _I32, M, d, "line"), _on_device(start, _I32, n + 1, d, "start"),
+                                   _on_device(held if held_out is None else held_out, _I32, n, d, "held_out"), _on_device(taken if taken_out is None else taken_out, _I32, 1, d, "taken_out"),
+                                   _on_device(status, _I32, 1, d, "status"), _on_device(lead_seq, _I32, n, d, "lead_seq"), _on_device(lead_pages, _I32, n, d, "lead_pages"), 1 if pdl else 0,
+                                   torch._C._cuda_getCurrentRawStream(d))
+    if rc:
+        check(rc, "dl_page_tables")
+    lib.count_launch()
+
+
 def gemm_f32(w: torch.Tensor, x: torch.Tensor, out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
     """out[M][d] (+)= x[M][n] @ w[d][n]^T with plain f32 FMAs (the f32-weights path).  w may be a column
     slice of a wider matrix (row stride w.stride(0)); x and out are row-major."""

@@ -175,6 +175,11 @@ def cuda_lib():
     L.dl_quant_q80.argtypes = [vp, i32, i32, i32, vp, vp, vp]
     L.dl_embedding.argtypes = [vp, vp, vp, i32, i32, vp, vp]
     L.dl_sample_rows.argtypes = [vp, i32, i32, i32, vp, vp, vp, vp, vp]
+    L.dl_sample_tokens.argtypes = [vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, vp, vp, i32, vp]
+    L.dl_page_tables.argtypes = [i32, vp, vp, vp, vp, i32, i32, vp, i32, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, vp]
+    L.dl_sample_tokens_max_vocab.argtypes = []
+    for name in ("dl_sample_tokens", "dl_page_tables", "dl_sample_tokens_max_vocab"):
+        getattr(L, name).restype = i32
     L.dl_gemm_f32.argtypes = [vp, i32, i32, i64, vp, i32, i32, vp, i32, i32, vp]
     L.dl_gemv_q40.argtypes = [vp, i32, i32, vp, i32, i32, i32, i32, C.POINTER(DlNormProlog), C.POINTER(DlEpilogue), i32, vp]
     L.dl_gemv_q40_smem_bytes.restype = i64

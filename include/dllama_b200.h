@@ -132,6 +132,32 @@ int dl_embedding(const float* table, const int* tokens, float* x, int M, int dim
 int dl_sample_rows(const float* logits, int M, int vocab, int ld, const float* temperature, const float* topp,
                    const float* coin, int* tokens_out, void* stream);
 
+/* per-row sampling with top-k and min-p beside it: logits of DL_KV8_* (row stride ld), w_i = exp((x_i - max x) / temperature), tokens in order of their logits, of equal
+ * ones the lowest index first.  top_k (0 < k < vocab): a token stays if fewer than k are ahead of it; top_p (0 < p < 1): if the weight ahead of it is below p times the weight of
+ * what top_k leaves; min_p (> 0; above 1 as 1): if w_i >= min_p.  The token is the first one in the order of the vocabulary where the sum of the weights that
+ * stay is above coin[m] (in [0, 1)) times their total; prob_out (NULL or [M]): its weight / their total.  temperature <= 0 or NaN: the first of the largest
+ * logits, prob 1.  A NaN counts as -inf, weights below 2^-45 as none; of several +inf each has weight 1; a row of -inf alone gives token 0 and prob 0.  top_k, top_p, min_p: NULL or
+ * [M] on the device; values outside of those ranges: off.  vocab: at most dl_sample_tokens_max_vocab() */
+int dl_sample_tokens_max_vocab(void);
+int dl_sample_tokens(const void* logits, int type, int M, int vocab, long long ld, const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* coin,
+                     int* tokens_out, float* prob_out, int pdl, void* stream);
+
+/* Block tables and slot maps from the lengths of n requests (device arrays): request i holds held[i] tokens in the pages of table row seq[i] (table [n_seqs][max_pages], pages of 32
+ * tokens) and runs new_tokens[i] more.  With have = ceil(held / 32) and need = ceil((held + new) / 32), pages and rows of the requests ahead of it counted in P and R:
+ *   table[seq][k] = free_pages[*taken + P + k - have], have <= k < need
+ *   table[seq][k] = table[lead_seq[i]][k], k < lead_pages[i]: a shared prompt's pages, whole ones of the tokens held (32 lead_pages <= held); that row may be a request's, too, but none whose own
+ *                   first pages are another's; lead_seq and lead_pages: both NULL: none
+ *   pos[R + j] = held + j, slot[R + j] = seq, line[R + j] = 32 table[seq][pos / 32] + pos % 32 (-1 where that is no page); the other ones of the M rows: -1, 0, -1
+ *   start[i] = R (n + 1 of them), held_out = held + new, *taken_out = *taken + all pages taken.  held_out and taken_out may be held and taken.  line, start: NULL or wanted.
+ * *status: 0, or what was wrong, bits added: then all rows are empty, start is 0, nothing is taken and the table is as it was.
+ * At most 8192 requests, 131072 table rows. */
+enum { DL_TABLES_BAD_LENGTH = 1,   /* below zero, or more tokens than a table row has pages for */
+       DL_TABLES_BAD_SEQ = 2,      /* not a table row, or one of two requests */
+       DL_TABLES_BAD_LEAD = 4, DL_TABLES_NO_PAGES = 8 /* the list of n_free pages is too short */, DL_TABLES_BAD_PAGE = 16 /* not one of n_pages in the part of the list that is taken */, DL_TABLES_NO_ROWS = 32 /* more than M */ };
+int dl_page_tables(int n, const int* held, const int* new_tokens, const int* seq, int* table, int n_seqs, int max_pages, const int* free_pages, int n_free, const int* taken,
+                   int n_pages, int M, int* pos, int* slot, int* line, int* start, int* held_out, int* taken_out, int* status, const int* lead_seq, const int* lead_pages, int pdl,
+                   void* stream);
+
 /* F32 x F32 -> F32 matmul (f32-weights / f32-buffer path; reference: matmul_F32_F32_F32, nn-cpu-ops.cpp:182-220):
  * y[m][r] (+)= sum_k w[r*ldw + k] * x[m*ldx + k], plain f32 FMAs; n, ldw, ldx multiples of 4, w and x 16-byte aligned */
 int dl_gemm_f32(const float* w, int d, int n, long long ldw, const float* x, int M, int ldx, float* y, int ldy,
