@@ -450,6 +450,58 @@ def kv8_attention_prefill(q, M: int, n_heads: int, pos, slot, block_table, meta,
     lib.count_launch()
 
 
+# ---- attention of sequences that begin with the same pages ------------------------------------------
+class _Pages(NamedTuple):
+    """What the checks above want to know of a cache."""
+    index: int
+    device: torch.device
+    head_size: int
+
+
+@functools.lru_cache(maxsize=4096)
+def _shared_bytes(M: int, n_heads: int, n_kv_heads: int, head_size: int) -> int:
+    return int(cuda_lib().dl_shared_attention_scratch_bytes(M, n_heads, n_kv_heads, head_size))
+
+
+def shared_attention_workspace(max_rows: int, n_heads: int, n_kv_heads: int, head_size: int, device) -> torch.Tensor:
+    """What shared_attention wants beside its arguments for up to max_rows rows, for one launch at a time (one serves all layers of a model)."""
+    return torch.empty(_shared_bytes(max_rows, n_heads, n_kv_heads, head_size), dtype=torch.uint8, device=device)
+
+
+def shared_attention(q, M: int, n_heads: int, pos, slot, block_table, groups, k_cache: torch.Tensor, v_cache: torch.Tensor, workspace: torch.Tensor, xq_out=None, xh_out=None, out_mcap: int = 0,
+                     y_out=None, pdl: bool = False):
+    """`attention` over the fp16 cache where groups of rows begin with the same pages, which are read once for all of them: groups = [n, begin, end, pages, ...] (device int32), rows begin .. end - 1
+    naming the same pages in the first `pages` places of their block tables; eight groups at most, in the order of their rows (a row of two belongs to the first one), rows of no group by themselves.
+    What not all rows of a group see is not shared.  Heads of 64 and 128, up to 16 query heads for each key/value head.  Queries (times a power of two of the row) and weights are fp16; y_out is
+    f32, fp16 or bf16.  workspace: shared_attention_workspace(), for one launch at a time."""
+    if k_cache.dim() != 4 or k_cache.shape[2] != PAGE_SIZE or k_cache.shape[3] not in (64, 128) or k_cache.shape[0] < 1 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"keys {tuple(k_cache.shape)} and values {tuple(v_cache.shape)}: [pages][kv heads][{PAGE_SIZE}][64 or 128] is wanted")
+    if k_cache.dtype is not torch.float16 or v_cache.dtype is not torch.float16 or v_cache.get_device() != k_cache.get_device() or not k_cache.is_contiguous() or not v_cache.is_contiguous() \
+            or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+        raise ValueError("keys and values are contiguous fp16 tensors on one device, aligned to 16 bytes")
+    n_pages, n_kv, _, hs = k_cache.shape
+    if n_heads < 1 or n_heads % n_kv or n_heads // n_kv > 16:
+        raise ValueError(f"{n_heads} query heads on {n_kv} key/value heads")
+    cache = _Pages(k_cache.get_device(), k_cache.device, hs)
+    if n_pages * n_kv * PAGE_SIZE >= 1 << 31 or M > 65535:
+        raise ValueError(f"{M} rows over {n_pages} pages of {n_kv} heads")
+    rows = _kv8_rows(M, pos, slot, block_table, cache)
+    ldq, ldy, y_type = _kv8_attention_args(q, M, n_heads, cache, xq_out, xh_out, out_mcap, y_out)
+    if q.data_ptr() % 16 or ldq % 4:
+        raise ValueError("rows of q are aligned to 16 bytes")
+    if groups is None or groups.dtype is not _I32 or groups.get_device() != cache.index or not groups.is_contiguous() or groups.numel() < 1:
+        raise ValueError("groups is a contiguous int32 tensor [n, begin, end, pages, ...]")
+    need = _shared_bytes(M, n_heads, n_kv, hs)
+    if workspace is None or workspace.get_device() != cache.index or not workspace.is_contiguous() or workspace.nbytes < need or workspace.data_ptr() % 16:
+        raise ValueError(f"the workspace is not one of shared_attention_workspace() for {M} rows")
+    rc = cuda_lib().dl_shared_attention(q.data_ptr(), ldq, n_heads, n_kv, hs, k_cache.data_ptr(), v_cache.data_ptr(), n_pages, *rows, groups.data_ptr(), (groups.numel() - 1) // 3,
+                                        workspace.data_ptr(), workspace.nbytes, _p(xq_out), _p(xh_out), out_mcap, _p(y_out), ldy, y_type, 1 if pdl else 0,
+                                        torch._C._cuda_getCurrentRawStream(cache.index))
+    if rc:
+        check(rc, "dl_shared_attention")
+    lib.count_launch(2 if M else 0)
+
+
 def argmax(logits, M: int, vocab: int, ld: int, out: torch.Tensor, flags=None, n_flags=0, step_counter=None,
            flag_mul=0, flag_add=0, pos_inc=None, history=None, history_cap=0, scratch=None, pdl=False):
     lp = logits.data_ptr() if isinstance(logits, torch.Tensor) else logits

@@ -270,7 +270,20 @@ int dl_kv8_attention_prefill(const float* q, long long ldq, int n_heads, const i
                              void* k16, void* v16, void* scratch16, uint8_t* xq_out, uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, int pdl,
                              void* stream);
 
-/* Kernels that wait on copies inside a CTA (dl_attention_prefill_tc, dl_window_attention_tc's prompts, dl_attention on a ring of pages, dl_gemv_q40, dl_gemm_q40_tc,
+/* ---- attention of sequences that begin with the same pages ------------------------------------ */
+/* dl_attention over the fp16 cache (k_cache / v_cache [n_pages][n_kv_heads][32][head_size], heads of 64 and 128, at most 16 query heads for each key/value head) where groups of rows share their first
+ * pages: those are read once for the group.  groups (device) = [n, begin, end, pages, ...]: rows begin .. end - 1 name the same pages in the first `pages` places of their block tables (taken from
+ * the first row that has a token).  Eight groups are looked at, of max_groups that the array has room for; rows of two groups belong to the first one, groups come in the order of
+ * their rows; what not all rows of a group see is not shared; rows of no group are attended to by themselves.  q (row stride ldq, a multiple of 4) and what is aligned: 16 bytes.
+ * y_out (NULL or rows of stride ldy) of DL_KV8_*, xq_out / xh_out as of dl_attention.  Queries are taken in fp16 times a power of two of the row, weights in fp16: 2^-12 of a weight at random.
+ * pos, slot and pages that are not in the tables: as for the 8-bit cache below (zeros without a token, else NaN).  scratch: dl_shared_attention_scratch_bytes(), any contents; launches that may
+ * run at the same time need scratches of their own.  Two launches. */
+long long dl_shared_attention_scratch_bytes(int M, int n_heads, int n_kv_heads, int head_size);
+int dl_shared_attention(const float* q, long long ldq, int n_heads, int n_kv_heads, int head_size, const void* k_cache, const void* v_cache, int n_pages, const int* pos, const int* slot,
+                        const int* block_table, int M, int n_slots, int max_pages, const int* groups, int max_groups, void* scratch, long long scratch_bytes, uint8_t* xq_out,
+                        uint8_t* xh_out, int out_mcap, void* y_out, long long ldy, int y_type, int pdl, void* stream);
+
+/* Kernels that wait on copies inside a CTA (dl_attention_prefill_tc, dl_shared_attention, dl_window_attention_tc's prompts, dl_attention on a ring of pages, dl_gemv_q40, dl_gemm_q40_tc,
  * dl_dense's ring for one and two rows) wait for some seconds at most.  Where one gives up, the outputs of that launch are not valid (NaN, of
  * dl_gemm_q40_tc most) and this word (in host memory; each device has its own, this is the current one's) changes: read it behind a synchronisation
  * with the launch.  NULL: no device, or no memory for it. */

@@ -63,3 +63,37 @@ def test_the_c_entries_refuse():
                    {"free": None}, {"taken": None}, {"pos": None}, {"held_out": None}, {"status": None}, {"ls": p}, {"lp": p}):
         assert L.dl_page_tables(*{**ok, **change}.values(), 0, None) == -1
     assert b"null" in L.dl_last_error()
+
+
+def _shared(monkeypatch, **change):
+    monkeypatch.setattr(K, "_current_device", lambda: -1)
+    monkeypatch.setattr(K, "_kv8_rows", lambda *a: (0, 0, 0, a[0], 4, 3))
+    kv = torch.zeros(6, 2, 32, 64, dtype=torch.float16)
+    a = {"q": torch.zeros(4, 4 * 64), "M": 4, "n_heads": 4, "pos": i32(4), "slot": i32(4), "block_table": i32(4, 3), "groups": i32(4), "k_cache": kv, "v_cache": kv.clone(),
+         "workspace": torch.zeros(1 << 22, dtype=torch.uint8), "y_out": torch.zeros(4, 4 * 64)}
+    monkeypatch.setattr(K, "_shared_bytes", lambda *a: 1 << 22)
+    a.update(change)
+    K.shared_attention(**a)
+
+
+@pytest.mark.parametrize("change", [
+    {"k_cache": torch.zeros(6, 2, 32, 64)}, {"k_cache": torch.zeros(6, 2, 32, 32).half()}, {"k_cache": torch.zeros(6, 2, 16, 64).half()}, {"v_cache": torch.zeros(5, 2, 32, 64).half()},
+    {"v_cache": torch.zeros(6, 2, 32, 64)}, {"k_cache": torch.zeros(6, 32, 2, 64).half().transpose(1, 2)}, {"n_heads": 3}, {"n_heads": 0}, {"n_heads": 34, "q": torch.zeros(4, 34 * 64)},
+    {"q": torch.zeros(4, 255)}, {"q": torch.zeros(3, 256)}, {"q": torch.zeros(4, 256).half()}, {"q": torch.zeros(4, 258)[:, 2:]}, {"q": torch.zeros(4, 257)[:, :256]}, {"q": None}, {"groups": None},
+    {"groups": torch.zeros(4)}, {"groups": i32(0)}, {"groups": i32(8)[::2]}, {"workspace": None}, {"workspace": torch.zeros(100, dtype=torch.uint8)}, {"y_out": torch.zeros(4, 256).double()},
+    {"y_out": torch.zeros(4, 255)}, {"M": 65536}, {"xq_out": torch.zeros(10, dtype=torch.uint8), "out_mcap": 4}, {"xh_out": torch.zeros(1 << 20, dtype=torch.uint8), "out_mcap": 3}])
+def test_shared_attention_refuses(monkeypatch, change):
+    with pytest.raises(ValueError):
+        _shared(monkeypatch, **change)
+
+
+def test_the_c_entry_of_shared_attention_refuses():
+    L = lib.cuda_lib()
+    p = torch.zeros(1 << 16, dtype=torch.int32).data_ptr() // 16 * 16
+    ok = dict(q=p, ldq=256, H=4, kv=2, hs=64, k=p, v=p, n_pages=6, pos=p, slot=p, bt=p, M=2, n_slots=2, max_pages=4, groups=p, max_groups=1, scratch=p, bytes=1 << 40, xq=None, xh=None, mcap=0, y=p, ldy=256,
+              yt=0)
+    for change in ({"hs": 32}, {"H": 3}, {"kv": 0}, {"H": 34}, {"M": -1}, {"M": 65536}, {"n_slots": 0}, {"max_pages": 0}, {"max_pages": 1 << 26}, {"n_pages": 0}, {"n_pages": 1 << 26}, {"max_groups": -1},
+                   {"q": None}, {"k": None}, {"pos": None}, {"groups": None}, {"scratch": None}, {"bytes": 100}, {"ldq": 255}, {"ldq": 258}, {"q": p + 4}, {"k": p + 2}, {"ldy": 255}, {"yt": 3},
+                   {"max_pages": 1 << 25, "M": 60000}):
+        assert L.dl_shared_attention(*{**ok, **change}.values(), 0, None) == -1, change
+    assert L.dl_shared_attention(*{**ok, "M": 0}.values(), 0, None) == 0
