@@ -67,7 +67,7 @@ def settings(rng, n):
             (rng.uniform(0.001, 0.4, n) * on[2]).tolist(), rng.random(n).astype(np.float32).tolist())
 
 
-@pytest.mark.parametrize("vocab", [1, 2, 31, 33, 511, 4096, 4097, 8193, 32003, 50001, 128256, 327680])
+@pytest.mark.parametrize("vocab", [1, 2, 31, 33, 511, 4096, 4097, 8193, 32003, 50001, 128256, 327680, 524288])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_rows_of_every_size(vocab, dtype):
     rng = np.random.default_rng(vocab)

@@ -25,7 +25,7 @@ def _sample(**change):
 
 @pytest.mark.parametrize("change", [
     {"logits": torch.zeros(4, 50, dtype=torch.float64)}, {"logits": torch.zeros(4, 50, 2)}, {"logits": torch.zeros(50, 4).t()}, {"M": 5}, {"M": -1}, {"logits": torch.zeros(4, 0)},
-    {"logits": torch.zeros(1, 327681).expand(4, 327681)}, {"logits": torch.zeros(1, 50).expand(4, 50)}, {"temperature": None}, {"temperature": torch.ones(3)}, {"temperature": torch.ones(4).double()},
+    {"logits": torch.zeros(1, 524289).expand(4, 524289)}, {"logits": torch.zeros(1, 50).expand(4, 50)}, {"temperature": None}, {"temperature": torch.ones(3)}, {"temperature": torch.ones(4).double()},
     {"temperature": torch.ones(8)[::2]}, {"top_k": torch.zeros(4)}, {"top_k": i32(3)}, {"top_p": i32(4)}, {"min_p": torch.zeros(2)}, {"coin": None}, {"coin": torch.zeros(4).half()},
     {"tokens_out": None}, {"tokens_out": torch.zeros(4, dtype=torch.int64)}, {"tokens_out": i32(3)}, {"prob_out": torch.zeros(4).double()}, {"prob_out": torch.zeros(3)}])
 def test_sample_tokens_refuses(change):
@@ -53,7 +53,7 @@ def test_the_c_entries_refuse():
     L = lib.cuda_lib()
     p = torch.zeros(64, dtype=torch.int32).data_ptr()
     assert L.dl_sample_tokens(p, 0, 2, 0, 8, p, p, p, p, p, p, p, 0, None) == -1
-    assert L.dl_sample_tokens(p, 0, 2, 327681, 327681, p, p, p, p, p, p, p, 0, None) == -1
+    assert L.dl_sample_tokens(p, 0, 2, 524289, 524289, p, p, p, p, p, p, p, 0, None) == -1
     assert L.dl_sample_tokens(p, 0, 2, 8, 7, p, p, p, p, p, p, p, 0, None) == -1
     assert L.dl_sample_tokens(p, 3, 2, 8, 8, p, p, p, p, p, p, p, 0, None) == -1
     assert L.dl_sample_tokens(None, 0, 2, 8, 8, p, p, p, p, p, p, p, 0, None) == -1
