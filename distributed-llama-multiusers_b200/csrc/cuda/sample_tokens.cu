@@ -11,7 +11,7 @@
 // within the bin, of a few tokens, by comparing them with each other (StRow::select).  What takes part in that is a list in the first CTA's shared memory, in which the border has to lie:
 //   top-k   The least of as many maxima, each over tokens of its own, as k or more is not above the k-th largest logit.  The first pass leaves such maxima (of threads, or of warps); what is not
 //           below the least of them, some thousand tokens, goes into the list, and the rest of the row has no part: the first CTA does it all.
-//   top-p   A second pass counts the tokens in 2048 bins of their distance to the maximum.  A bin's weights differ by 1 %, so that the counts tell the sums to some 0.1 %, and the border to a few
+//   top-p   A second pass counts the tokens in 4096 bins of their distance to the maximum.  A bin's weights differ by 0.5 %, so that the counts tell the sums to some 0.02 %, and the border to a few
 //           bins.  A third pass adds up the weights: of the row, for the target, and of what lies ahead of those bins, for each warp's run of the row; the bins' tokens go into the list.
 //           The first CTA finds the border there, and the warp's run in which the token lies.
 //   else    as top-p, without a border.
@@ -26,7 +26,7 @@
 #include "smem_limit.cuh"
 
 #define ST_BINS 256
-#define ST_FINE 2048                   // bins of top-p's counts
+#define ST_FINE 4096                   // bins of top-p's counts
 #define ST_LIST 6144
 #define ST_FEW 128                     // tokens that are compared with each other
 #define ST_MAX_CTAS 16
@@ -54,7 +54,7 @@ struct StSums { u64 weight; u64 count; };
 // what the CTAs of a row leave for each other; in each CTA's shared memory
 struct alignas(16) StShared {
     union {
-        u64 list[ST_LIST];             // in CTA 0's: keys
+        u64 list[ST_LIST];             // keys: this CTA's from the front; in CTA 0's the other ones' from the back
         struct { unsigned fine[ST_FINE], fine_sum[ST_FINE]; } count;      // ahead of it: this CTA's counts, the cluster's
     };
     unsigned hist[4][ST_BINS];         // this CTA's counts, and weights in three parts of 15 bits
@@ -66,7 +66,7 @@ struct alignas(16) StShared {
     float top[ST_MAX_CTAS], low[4][ST_MAX_CTAS];      // each CTA's largest logit; the least of the largest ones of its threads, of 2, 8 and 32 of them
     StSums above, inside;              // of the bin found: what lies ahead of it and in it
     int bin, bin_from, bin_to;
-    unsigned listed, few, done, first;
+    unsigned listed, others, few, done, first;      // listed: this CTA's; others: in CTA 0's the other ones'
     u64 found, upto;                   // the order of the token found, the sum up to it
     u64 warp_sum[ST_MAX_WARPS];
     float warp_top[ST_MAX_WARPS], warp_low[3][ST_MAX_WARPS];
@@ -173,15 +173,21 @@ template <typename T, int THREADS> struct StRow {
         if (i + 2 < count) v.z = st_load1<T>(x + i + 2);
         return v;
     }
-    // f(four logits, the first one's place) for places from `from` on; whole warps, ST_AHEAD loads in flight for each thread
-    template <typename F> DL_DEVINL void quads(int from, int to, int stride, F f) const {
+    // f(ST_AHEAD times four logits, the first one's place): the next four are `stride` behind it; whole warps, all loads in flight for each thread
+    template <typename F> DL_DEVINL void batches(int from, int to, int stride, F f) const {
         for (int i = from; i < to; i += ST_AHEAD * stride) {
             float4 v[ST_AHEAD];
 #pragma unroll
             for (int u = 0; u < ST_AHEAD; u++) v[u] = load(i + u * stride + lane * 4);
-#pragma unroll
-            for (int u = 0; u < ST_AHEAD; u++) f(v[u], i + u * stride + lane * 4);
+            f(v, i + lane * 4);
         }
+    }
+    // f(four logits, the first one's place)
+    template <typename F> DL_DEVINL void quads(int from, int to, int stride, F f) const {
+        batches(from, to, stride, [&](const float4 (&v)[ST_AHEAD], int i) {
+#pragma unroll
+            for (int u = 0; u < ST_AHEAD; u++) f(v[u], i + u * stride);
+        });
     }
     template <typename F> DL_DEVINL void all(F f) const { quads(warp * 128, count, THREADS * 4, f); }
     // f(logit, place) for what is not below `cut`; four neighbours a thread, most of which are passed over at once
@@ -208,35 +214,30 @@ template <typename T, int THREADS> struct StRow {
         else cluster.sync();
     }
 
-    // The CTAs' bins added up, in every CTA's sh.merged.
-    DL_DEVINL void merge(bool local) {
+    // The bin in which the weights reach the target (bin 0 is ahead of the others), of the CTA's bins or of the cluster's: sh.bin, sh.above.weight, sh.inside.  The bins are left empty.
+    DL_DEVINL void locate(bool local, u64 ahead, u64 target) {
+        static_assert(ST_BINS / 32 <= THREADS / 32 && ST_BINS <= 1024, "a warp for 32 bins");
+        const bool mine = warp < ST_BINS / 32;
+        StSums s = {0, 0};
         sync(local);
         if (local) {
-            for (int b = tid; b < ST_BINS; b += THREADS) sh.merged[b] = StSums{(u64)sh.hist[1][b] + ((u64)sh.hist[2][b] << 15) + ((u64)sh.hist[3][b] << 30), sh.hist[0][b]};
+            if (mine) s = StSums{(u64)sh.hist[1][tid] + ((u64)sh.hist[2][tid] << 15) + ((u64)sh.hist[3][tid] << 30), sh.hist[0][tid]};
         } else {
             const int share = ST_BINS / ctas;
             for (int j = tid; j < share * 4; j += THREADS) {   // four lanes a bin, one of its numbers each (a warp's lanes are all in or all out)
                 const int part = j & 3, b = rank * share + (j >> 2);
-                u64 s = 0;
+                u64 x = 0;
 #pragma unroll 8
-                for (int r = 0; r < ctas; r++) s += at(r)->hist[part][b];
-                const u64 n = __shfl_sync(0xffffffffu, s, lane & ~3);
-                u64 w = part ? s << (15 * (part - 1)) : 0;
+                for (int r = 0; r < ctas; r++) x += at(r)->hist[part][b];
+                const u64 n = __shfl_sync(0xffffffffu, x, lane & ~3);
+                u64 w = part ? x << (15 * (part - 1)) : 0;
                 w += __shfl_xor_sync(0xffffffffu, w, 1);
                 w += __shfl_xor_sync(0xffffffffu, w, 2);
                 for (int r = part; r < ctas; r += 4) at(r)->merged[b] = StSums{w, n};
             }
+            cluster.sync();
+            if (mine) s = sh.merged[tid];
         }
-        if (tid == 0) sh.few = 0;
-        sync(local);
-    }
-
-    // The bin in which the weights reach the target (bin 0 is ahead of the others): sh.bin, sh.above, sh.inside; each CTA for itself.
-    DL_DEVINL void locate(u64 ahead, u64 target) {
-        static_assert(ST_BINS / 32 <= THREADS / 32 && ST_BINS <= 1024, "a warp for 32 bins");
-        const bool mine = warp < ST_BINS / 32;
-        StSums s = {0, 0};
-        if (mine) s = sh.merged[warp * 32 + lane];
         u64 incl = s.weight;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -244,27 +245,26 @@ template <typename T, int THREADS> struct StRow {
             if (lane >= o) incl += w;
         }
         if (lane == 31) sh.warp_sum[warp] = incl;
+        if (mine) sh.hist[0][tid] = sh.hist[1][tid] = sh.hist[2][tid] = sh.hist[3][tid] = 0;
+        if (tid == 0) sh.few = 0;
         __syncthreads();
         if (mine) {
             for (int w = 0; w < warp; w++) ahead += sh.warp_sum[w];
             const u64 to = ahead + incl, from = to - s.weight;
             if (from < target && to >= target) {
-                sh.bin = warp * 32 + lane;
+                sh.bin = tid;
                 sh.above.weight = from;
                 sh.inside = s;
             }
         }
-        __syncthreads();
+        sync(local);                                            // (the cluster: `few` is zero everywhere)
     }
 
     // The first token, in an order, with which the sum of the weights reaches the target: its place in the order in sh.found, the sum up to it in sh.upto.  each(f) calls
     // f(order, bin, weight()) for every token that counts: larger orders are ahead, and so are lower bins; no two tokens have the same order.
     template <typename Each> DL_DEVINL void select(bool local, Each each, u64 target) {
-        for (int b = tid; b < 4 * ST_BINS; b += THREADS) (&sh.hist[0][0])[b] = 0;
-        __syncthreads();
         each([&](u64, int b, auto w) { add(b, w()); });
-        merge(local);
-        locate(0, target);
+        locate(local, 0, target);
         u64 above = sh.above.weight, inside = sh.inside.count;
         const int bin = sh.bin;
         u64 lo = 0, hi = ~0ull;                                 // the orders in the bin
@@ -299,12 +299,8 @@ template <typename T, int THREADS> struct StRow {
             }
             const int bits = 64 - __clzll(hi - lo), shift = bits > 8 ? bits - 8 : 0;      // (hi > lo: more than one token)
             const u64 top = hi, end = lo;
-            __syncthreads();
-            for (int b = tid; b < 4 * ST_BINS; b += THREADS) (&sh.hist[0][0])[b] = 0;
-            __syncthreads();
             each([&](u64 k, int, auto w) { if (k <= top && k >= end) add((int)((top - k) >> shift), w()); });
-            merge(local);
-            locate(above, target);
+            locate(local, above, target);
             above = sh.above.weight;
             inside = sh.inside.count;
             hi = top - ((u64)sh.bin << shift);
@@ -333,27 +329,47 @@ template <typename T, int THREADS> struct StRow {
         __syncthreads();
     }
 
-    // the tokens of a quad whose bits are set in `mask` go into CTA 0's list (by whole warps)
-    DL_DEVINL void push(unsigned mask, const float (&v)[4], int i) {
+    // Tokens of ST_AHEAD quads go into this CTA's list (by whole warps): bit 4 u + e of `mask` is token e of the quad at place i + u * stride
+    DL_DEVINL void push(unsigned mask, const float4 (&v)[ST_AHEAD], int i, int stride) {
+        static_assert(ST_AHEAD <= 8, "a bit for each token");
         if (!__any_sync(0xffffffffu, mask)) return;
-        StShared* o = at(0);
         const unsigned n = __popc(mask);
         unsigned incl = n;
 #pragma unroll
-        for (int s = 1; s < 32; s <<= 1) {
-            const unsigned y = __shfl_up_sync(0xffffffffu, incl, s);
-            if (lane >= s) incl += y;
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
         }
         unsigned base = 0;
-        if (lane == 31) base = atomicAdd(&o->listed, incl);
+        if (lane == 31) base = atomicAdd(&sh.listed, incl);
         base = __shfl_sync(0xffffffffu, base, 31) + incl - n;
+        if (!mask) return;
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (mask >> e & 1) {
-                if (base < ST_LIST) o->list[base] = st_key(v[e], first + i + e);
-                base++;
-            }
+        for (int u = 0; u < ST_AHEAD; u++) {
+            if (!(mask >> (4 * u) & 15)) continue;
+            const float x4[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (mask >> (4 * u + e) & 1) {
+                    if (base < ST_LIST) sh.list[base] = st_key(x4[e], first + i + u * stride + e);
+                    base++;
+                }
+        }
     }
+    // the CTAs' lists into CTA 0's
+    DL_DEVINL void collect() {
+        __syncthreads();
+        if (rank != 0) {
+            StShared* o = at(0);
+            const unsigned n = min(sh.listed, (unsigned)ST_LIST);
+            if (tid == 0) sh.few = atomicAdd(&o->others, sh.listed);
+            __syncthreads();
+            const unsigned from = sh.few;
+            for (unsigned i = tid; i < n; i += THREADS)
+                if (from + i < ST_LIST) o->list[ST_LIST - 1 - from - i] = sh.list[i];
+        }
+    }
+    DL_DEVINL u64 listed(int i) const { return sh.list[i < (int)sh.listed ? i : ST_LIST - 1 - (i - (int)sh.listed)]; }
     // in which of n sums the target lies (sh.bin) and what the ones ahead of it add up to (sh.above.weight); n at most THREADS
     DL_DEVINL void locate_run(const u64* sums, int n, u64 target) {
         const u64 s = tid < n ? sums[tid] : 0;
@@ -421,7 +437,8 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
         const double p = exp2((double)tid / 64.0);
         sh.pow2[tid] = make_uint2((unsigned)__double2uint_rn(p * 2147483648.0), __float_as_uint((float)p));
     }
-    if (tid == 64) { sh.listed = 0; sh.first = 0xffffffffu; }
+    if (tid == 64) { sh.listed = 0; sh.others = 0; sh.few = 0; sh.first = 0xffffffffu; }
+    for (int b = tid; b < 4 * ST_BINS; b += THREADS) (&sh.hist[0][0])[b] = 0;
     pdl_wait();
     StAsk q;
     q.T = a.temperature[row];
@@ -556,19 +573,30 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
             for (int r = 1; r < ctas; r++) cut = fminf(cut, sh.low[groups][r]);
         }
         if (cut > -CUDART_INF_F || a.vocab <= ST_LIST)
-            z.all([&](const float4& v4, int i) {
-                const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+            z.batches(z.warp * 128, z.count, THREADS * 4, [&](const float4 (&v)[ST_AHEAD], int i) {
                 unsigned mask = 0;
-                if (st_max4(v4) >= cut) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) mask |= v[e] >= cut && i + e < z.count ? 1u << e : 0;
+                for (int u = 0; u < ST_AHEAD; u++) {
+                    const int b = 4 * u;
+                    mask |= (v[u].x >= cut ? 1u << b : 0) | (v[u].y >= cut ? 2u << b : 0) | (v[u].z >= cut ? 4u << b : 0) | (v[u].w >= cut ? 8u << b : 0);
                 }
-                z.push(mask, v, i);
+                if (!(cut > -CUDART_INF_F)) {                    // (behind the slice it is -inf)
+                    mask = 0;
+#pragma unroll
+                    for (int u = 0; u < ST_AHEAD; u++) {
+                        const float x4[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) mask |= x4[e] >= cut && i + u * THREADS * 4 + e < z.count ? 1u << (4 * u + e) : 0;
+                    }
+                }
+                z.push(mask, v, i, THREADS * 4);
             });
+        z.collect();
         cluster.sync();
         if (rank == 0) {
-            const int n = (int)sh.listed;
-            const bool ok = n <= ST_LIST && n >= q.k;
+            const unsigned found = sh.listed + sh.others;
+            const int n = (int)min(found, (unsigned)ST_LIST);
+            const bool ok = found <= ST_LIST && n >= q.k;
             if (tid < ctas) z.at(tid)->done = ok ? 1 : 0;       // (the others may leave)
             st_cluster_arrive();
             if (ok) {
@@ -576,7 +604,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
                 auto by_logit = [&](bool counts) {              // the list in the order of the logits, from the border on
                     return [&, counts](auto f) {
                         for (int i = tid; i < n; i += THREADS) {
-                            const u64 key = sh.list[i];
+                            const u64 key = z.listed(i);
                             const float v = st_logit(key);
                             if (key >= border) f(key, v == m ? 0 : (int)fminf((m - v) * per, (float)(ST_BINS - 1)), [&] { return counts ? 1 : st_weight(v, z.scale, sh.pow2); });
                         }
@@ -585,7 +613,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
                 auto left = [&](bool min_too) {                  // the weight of what stays
                     u64 s = 0;
                     for (int i = tid; i < n; i += THREADS) {
-                        const u64 key = sh.list[i];
+                        const u64 key = z.listed(i);
                         const float v = st_logit(key);
                         if (key >= border && (!min_too || q.min_ok(v))) s += st_weight(v, z.scale, sh.pow2);
                     }
@@ -601,14 +629,14 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
                 const int per_bin = (a.vocab + ST_BINS - 1) / ST_BINS;
                 z.select(true, [&](auto f) {                     // in the order of the vocabulary
                     for (int i = tid; i < n; i += THREADS) {
-                        const u64 key = sh.list[i];
+                        const u64 key = z.listed(i);
                         const float v = st_logit(key);
                         if (key >= border && q.min_ok(v)) f(key & ST_IDX_MASK, st_index(key) / per_bin, [&] { return st_weight(v, z.scale, sh.pow2); });
                     }
                 }, q.want(kept) + 1);
                 if (a.prob != nullptr)
                     for (int i = tid; i < n; i += THREADS)
-                        if ((sh.list[i] & ST_IDX_MASK) == sh.found) a.prob[row] = q.prob(st_logit(sh.list[i]), kept);
+                        if ((z.listed(i) & ST_IDX_MASK) == sh.found) a.prob[row] = q.prob(st_logit(z.listed(i)), kept);
                 if (tid == 0) a.tokens[row] = (int)(ST_IDX_MASK - sh.found);
             }
         } else {
@@ -640,7 +668,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
             }
             if (tid == 0) { sh.bin_from = 0; sh.bin_to = ST_FINE - 1; }
             cluster.sync();
-            // sums from the counts, each bin's tokens in its middle; off by a random part of a bin's width for each token
+            // sums from the counts, each bin's tokens in its middle; off by a random part of the width for each bin (16-bit logits: a bin's tokens have one value)
             constexpr int PER = (ST_FINE + THREADS - 1) / THREADS;
             const float width = ST_REACH / (ST_FINE - 1);
             float w[PER], part = 0.f, off = 0.f;
@@ -650,7 +678,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
                 const float n = b < ST_FINE ? (float)sh.count.fine_sum[b] : 0.f, mid = __expf(-((float)b + 0.5f) * width);
                 w[e] = n * mid;
                 part += w[e];
-                off += w[e] * mid;
+                off += w[e] * w[e];
             }
             float incl = part;
 #pragma unroll
@@ -668,8 +696,8 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
                 all += sh.warp_top[u];
                 off += sh.warp_low[0][u];
             }
-            // four standard deviations (width / sqrt 12 of a token's weight), and 2^-12 for the tail and the sums
-            const float room = 1.2f * width * sqrtf(off) + all * 0x1p-12f, lo = q.p * all - room, hi = q.p * all + room;
+            // four standard deviations (width / sqrt 12 of a bin's weight), e^-20 for each token of the tail, and the sums' roundings
+            const float room = 1.2f * width * sqrtf(off) + 2.1e-9f * (float)a.vocab + all * 0x1p-17f, lo = q.p * all - room, hi = q.p * all + room;
 #pragma unroll
             for (int e = 0; e < PER; e++) {
                 const int b = tid * PER + e;
@@ -685,53 +713,69 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
             cluster.sync();                                     // (the list takes the counts' place)
         }
         // ---- the weights: of all that is ahead of those bins, by runs, and of the row ----
-        u64 mine = 0, ahead = 0, rest = 0;
-        z.quads(r0, r1, 128, [&](const float4& v4, int i) {
-            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+        // (a run ends with a whole quad or with the slice, behind which logits are -inf)
+        u64 mine = 0, ahead = 0, all = 0;                        // what is drawn from, what is ahead of the border's bins, the row
+        const float from_t = (float)from, to_t = to == ST_FINE - 1 ? CUDART_INF_F : (float)(to + 1);
+        z.batches(r0, r1, 128, [&](const float4 (&v4)[ST_AHEAD], int i) {
             unsigned mask = 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const bool in = i + e < r1;
-                const u64 w = in ? st_weight(v[e], z.scale, sh.pow2) : 0;
-                const int b = to < 0 ? 0 : q.fine(v[e]);
-                if (b < from) ahead += w;
-                else rest += w;
-                if (b < from && v[e] >= lowest && q.min_ok(v[e])) mine += w;
-                mask |= b >= from && b <= to && in && v[e] > -CUDART_INF_F ? 1u << e : 0;
+            for (int u = 0; u < ST_AHEAD; u++) {
+                const float v[4] = {v4[u].x, v4[u].y, v4[u].z, v4[u].w};
+                if (i - z.lane * 4 + u * 128 >= r1) break;       // (uniform for the warp)
+                if (to < 0) {
+                    if (!(st_max4(v4[u]) >= lowest)) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (!q.by_min || (v[e] >= lowest && q.min_ok(v[e]))) mine += st_weight(v[e], z.scale, sh.pow2);
+                    continue;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const u64 w = st_weight_below(v[e], z.scale, sh.pow2);      // (of the maximum, too: it is finite)
+                    const float t = (m - v[e]) * q.per;          // (fine())
+                    const bool front = t < from_t;
+                    all += w;
+                    ahead += front ? w : 0;
+                    if (q.by_min) mine += front && v[e] >= lowest && q.min_ok(v[e]) ? w : 0;
+                    mask |= t >= from_t && t < to_t ? 1u << (4 * u + e) : 0;
+                }
             }
-            if (to >= 0) z.push(mask, v, i);
+            if (to >= 0) z.push(mask, v4, i, 128);
         });
+        if (to >= 0 && !q.by_min) mine = ahead;
+        if (to >= 0) z.collect();
         mine = st_sum_u64(mine);
         if (z.lane == 0) z.at(0)->run_sum[rank * WARPS + z.warp] = mine;
         if (to >= 0) {
             ahead = z.sum(ahead);
-            rest = z.sum(rest);
-            if (tid == 0) { z.at(0)->cta_sum[rank] = ahead; z.at(0)->lo[rank] = rest; }
+            all = z.sum(all);
+            if (tid == 0) { z.at(0)->cta_sum[rank] = ahead; z.at(0)->lo[rank] = all; }
         }
         cluster.sync();
         if (rank == 0) {
             bool ok = true;
             if (to >= 0) {
-                const int n = (int)min(sh.listed, (unsigned)ST_LIST);
+                const unsigned found = sh.listed + sh.others;
+                const int n = (int)min(found, (unsigned)ST_LIST);
                 u64 total = 0, near = 0;
                 ahead = 0;
-                for (int r = 0; r < ctas; r++) { ahead += sh.cta_sum[r]; total += sh.cta_sum[r] + sh.lo[r]; }
-                for (int i = tid; i < n; i += THREADS) near += st_weight(st_logit(sh.list[i]), z.scale, sh.pow2);
+                for (int r = 0; r < ctas; r++) { ahead += sh.cta_sum[r]; total += sh.lo[r]; }
+                for (int i = tid; i < n; i += THREADS) near += st_weight(st_logit(z.listed(i)), z.scale, sh.pow2);
                 near = z.sum(near);
                 const u64 target = q.part(total);
-                ok = sh.listed <= ST_LIST && ahead < target && target <= ahead + near;
+                ok = m < CUDART_INF_F && found <= ST_LIST && ahead < target && target <= ahead + near;
                 if (ok) {
                     const int wide = (to - from) / ST_BINS + 1;      // fine bins to one of select's
                     z.select(true, [&](auto f) {
                         for (int i = tid; i < n; i += THREADS) {
-                            const u64 key = sh.list[i];
+                            const u64 key = z.listed(i);
                             const float v = st_logit(key);
                             f(key, (q.fine(v) - from) / wide, [&] { return st_weight(v, z.scale, sh.pow2); });
                         }
                     }, target - ahead);
                     border = sh.found;
                     for (int i = tid; i < n; i += THREADS) {         // those of the list that stay, to their runs
-                        const u64 key = sh.list[i];
+                        const u64 key = z.listed(i);
                         const float v = st_logit(key);
                         const int at = st_index(key), r = at / a.slice;
                         if (key >= border && q.min_ok(v)) atomicAdd(&sh.run_sum[r * WARPS + (at - r * a.slice) / run], st_weight(v, z.scale, sh.pow2));
@@ -851,9 +895,14 @@ extern "C" int dl_sample_tokens(const void* logits, int type, int M, int vocab, 
     const bool wide = ((uintptr_t)logits % group) == 0 && (M == 1 || ld * (group / 4) % group == 0);
     const StArgs a = {logits, ld, temperature, top_p, min_p, coin, top_k, tokens_out, prob_out, vocab, slice, wide ? 1 : 0};
     cudaStream_t st = (cudaStream_t)stream;
-    // few rows: an SM for each CTA, and all of its threads
-    const bool few = (long long)M * ctas <= n_sms;
-    if (type == 0) return few ? st_launch<float, 1024, 1>(a, M, ctas, pdl, st) : st_launch<float, 384, 3>(a, M, ctas, pdl, st);
-    if (type == 1) return few ? st_launch<__nv_bfloat16, 1024, 1>(a, M, ctas, pdl, st) : st_launch<__nv_bfloat16, 384, 3>(a, M, ctas, pdl, st);
-    return few ? st_launch<__half, 1024, 1>(a, M, ctas, pdl, st) : st_launch<__half, 384, 3>(a, M, ctas, pdl, st);
+    // few rows: an SM for each CTA, and all of its threads; half of them where the cluster is so large that its barriers cost more (one row, top-p: 22.2 us with 512, 24.9 with 1024; eight rows,
+    // top-k and top-p, in clusters of eight: 23.7 and 19.6)
+    const int variant = (long long)M * ctas > n_sms ? 0 : ctas > 8 ? 1 : 2;
+    auto go = [&](auto zero) {
+        using T = decltype(zero);
+        return variant == 0 ? st_launch<T, 384, 3>(a, M, ctas, pdl, st) : variant == 1 ? st_launch<T, 512, 1>(a, M, ctas, pdl, st) : st_launch<T, 1024, 1>(a, M, ctas, pdl, st);
+    };
+    if (type == 0) return go(float());
+    if (type == 1) return go(__nv_bfloat16());
+    return go(__half());
 }
