@@ -28,7 +28,7 @@
 #define SH_MAX_GROUPS 8
 #define SH_PAIR_COST 7                 // of a step with two tiles
 #define SH_ONE_COST 4                  // ... with one
-#define SH_LEAST_STEPS 2               // of a CTA's share
+#define SH_LEAST_COST 8                // of a CTA's share: two steps of one tile
 #define SH_PLAN_BYTES 1024
 #define SH_OWN_WARPS 4
 #define SH_OWN_TOK 16                  // tokens of a warp's turn
@@ -73,15 +73,20 @@ DL_DEVINL int sh_tokens(const ShArgs& a, int m) {
     if (p < 0) return 0;
     return (unsigned)s < (unsigned)a.n_slots && p < a.max_pages * SH_PAGE ? p + 1 : -1;
 }
+// The list of groups, by the first threads of a CTA, into shared memory ([1 + 3 SH_MAX_GROUPS]; a barrier has to follow)
+DL_DEVINL void sh_fetch_groups(const ShArgs& a, int* list) {
+    const int i = threadIdx.x;
+    if (i <= 3 * SH_MAX_GROUPS) list[i] = i <= 3 * a.max_groups ? a.groups[i] : 0;
+}
 // the rows of group i as they are taken: in order, none in two groups
-DL_DEVINL void sh_group(const ShArgs& a, int i, int& at, int& begin, int& end, int& pages) {
-    begin = max(a.groups[1 + 3 * i], at);
-    end = min(a.groups[2 + 3 * i], a.M);
+DL_DEVINL void sh_group(const ShArgs& a, const int* list, int i, int& at, int& begin, int& end, int& pages) {
+    begin = max(list[1 + 3 * i], at);
+    end = min(list[2 + 3 * i], a.M);
     end = max(begin, end);
-    pages = max(0, min(a.groups[3 + 3 * i], a.max_pages));
+    pages = max(0, min(list[3 + 3 * i], a.max_pages));
     at = end;
 }
-DL_DEVINL int sh_n_groups(const ShArgs& a) { return max(0, min(min(a.groups[0], a.max_groups), SH_MAX_GROUPS)); }
+DL_DEVINL int sh_n_groups(const ShArgs& a, const int* list) { return max(0, min(min(list[0], a.max_groups), SH_MAX_GROUPS)); }
 
 DL_DEVINL int sh_tiles(const ShArgs& a, int rows) { return (rows * (a.n_heads / a.n_kv_heads) + SH_ROWS - 1) / SH_ROWS; }
 DL_DEVINL int sh_steps(int pages) { return (pages + SH_KV / SH_PAGE - 1) / (SH_KV / SH_PAGE); }
@@ -104,11 +109,22 @@ DL_DEVINL void sh_unit_at(const ShArgs& a, const ShPlan& p, int x, ShUnit& u) {
     const int tiles = sh_tiles(a, p.end[g] - p.begin[g]), steps = sh_steps(p.pages[g]), head = sh_head_cost(tiles, steps), rest = x - p.cost[g];
     sh_unit(a, p, g, rest / head, min(rest % head / (steps * SH_PAIR_COST), (tiles + 1) / 2 - 1), u);
 }
+// ... and the one behind it (there is one: the whole cost has not been reached)
+DL_DEVINL void sh_next_unit(const ShArgs& a, const ShPlan& p, ShUnit& u) {
+    int g = u.g, kvh = u.kvh, pair = u.pair + 1;
+    if (pair * 2 >= sh_tiles(a, p.end[g] - p.begin[g])) { pair = 0; kvh++; }
+    if (kvh == a.n_kv_heads) {
+        kvh = 0;
+        do g++; while (g + 1 < p.n && p.cost[g + 1] == p.cost[g]);      // (groups that cost nothing)
+    }
+    sh_unit(a, p, g, kvh, pair, u);
+}
+DL_DEVINL int sh_div(int x, int w) { return w == SH_PAIR_COST ? x / SH_PAIR_COST : x / SH_ONE_COST; }
 // the steps [j0, j1) of a unit that share b has
 DL_DEVINL void sh_share(const ShPlan& p, const ShUnit& u, int b, int& j0, int& j1) {
     const int lo = b * p.quota - u.c0, hi = lo + p.quota;
-    j0 = lo <= 0 ? 0 : min(u.steps, (lo + u.w - 1) / u.w);
-    j1 = hi <= 0 ? 0 : min(u.steps, (hi + u.w - 1) / u.w);
+    j0 = lo <= 0 ? 0 : min(u.steps, sh_div(lo + u.w - 1, u.w));
+    j1 = hi <= 0 ? 0 : min(u.steps, sh_div(hi + u.w - 1, u.w));
 }
 
 // the exponent field of the power of two that brings a row's largest value (its bits) to 2^8 .. 2^9; its inverse has 254 less that
@@ -118,8 +134,8 @@ struct ShItem {
     int kvh, row0, rows, begin, slot, pages, j0, J, tiles, piece;      // row0: first stacked row; rows: stacked rows of the group
 };
 
-// Queries of 32 stacked rows into a tile's K-major, swizzled image, each row times the power of two that brings its largest value to 2^8 .. 2^9; lane i holds the
-// address of row r0 + i and gets what the scores of that row are multiplied with (NaN: the row is not finite).
+// Queries of 32 stacked rows into a tile's K-major, swizzled image; where one of them is beyond what fp16 holds well, each row times the power of two that brings its largest value to 2^8 .. 2^9
+// (always, with a maximum over the warp for each row, the load took 5.3 us of a CTA's time).  Lane i holds the address of row r0 + i and gets what the scores of that row are multiplied with (NaN: the row is not finite).
 template <int HS, typename Ready>
 DL_DEVINL float sh_load_rows(const float* mine, uint8_t* tile, int r0, Ready ready) {
     constexpr int PER = 128 / HS;                              // rows a load
@@ -133,58 +149,77 @@ DL_DEVINL float sh_load_rows(const float* mine, uint8_t* tile, int r0, Ready rea
     }
     ready();
     float factor = 1.f;
+    // rows whose largest value is 2^-6 or more and below 2^15, as queries are, go in as they are
+    unsigned fits = 0, top = 0;
+    auto most_of = [](const float4& y) {
+        return max(max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu), max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu));
+    };
 #pragma unroll
     for (int u = 0; u < 32; u += PER) {
-        const float4 y = x[u / PER];
-        unsigned most = max(max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu), max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu));
+        const unsigned most = most_of(x[u / PER]), large = __ballot_sync(0xffffffffu, most >= 0x3c800000u);
+        top = max(top, most);
+        fits += (large & 0xffffu) && (large >> 16) ? 1u : PER == 1 && large ? 1u : 0u;
+    }
+    const bool plain = fits == 32 / PER && __reduce_max_sync(0xffffffffu, top) < 0x47000000u;
 #pragma unroll
-        for (int o = HS / 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-        const bool finite = most < 0x7f800000u;
-        const unsigned up = sh_up(most);
-        const float by = finite ? __uint_as_float(up << 23) : 0.f, back = finite ? __uint_as_float((254u - up) << 23) : __uint_as_float(0x7fffffffu);
-        // (an infinity or NaN times zero is a NaN, in its row alone)
-        *reinterpret_cast<uint2*>(qd + u * 128 + ((((lane >> 1) & 7) ^ ((u + in) & 7)) << 4)) = make_uint2(pt_pack2<false>(y.x * by, y.y * by), pt_pack2<false>(y.z * by, y.w * by));
-        const float row = __shfl_sync(0xffffffffu, back, lane % PER * (HS / 4));
-        if (lane / PER * PER == u) factor = row;
+    for (int u = 0; u < 32; u += PER)            // 16-byte piece c of a half row -> swizzled slot c ^ (row & 7)
+        *reinterpret_cast<uint2*>(qd + u * 128 + ((((lane >> 1) & 7) ^ ((u + in) & 7)) << 4)) =
+            make_uint2(pt_pack2<false>(x[u / PER].x, x[u / PER].y), pt_pack2<false>(x[u / PER].z, x[u / PER].w));
+    if (!plain) {
+#pragma unroll
+        for (int u = 0; u < 32; u += PER) {
+            const float4 y = x[u / PER];
+            unsigned most = most_of(y);
+#pragma unroll
+            for (int o = HS / 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const bool finite = most < 0x7f800000u;
+            const unsigned up = sh_up(most);
+            const float by = finite ? __uint_as_float(up << 23) : 0.f, back = finite ? __uint_as_float((254u - up) << 23) : __uint_as_float(0x7fffffffu);
+            // (an infinity or NaN times zero is a NaN, in its row alone)
+            *reinterpret_cast<uint2*>(qd + u * 128 + ((((lane >> 1) & 7) ^ ((u + in) & 7)) << 4)) = make_uint2(pt_pack2<false>(y.x * by, y.y * by), pt_pack2<false>(y.z * by, y.w * by));
+            const float row = __shfl_sync(0xffffffffu, back, lane % PER * (HS / 4));
+            if (lane / PER * PER == u) factor = row;
+        }
     }
     fence_proxy_async_smem();
     return factor;
 }
 
 // The plan, by all threads of a CTA (in shared memory).
-DL_DEVINL void sh_make_plan(const ShArgs& a, ShPlan& p, int* red) {
+DL_DEVINL void sh_make_plan(const ShArgs& a, ShPlan& p, int* list, int (*red)[2]) {
     const int tid = threadIdx.x;
-    const int n = sh_n_groups(a);
-    int at = 0;
-    if (tid == 0) { p.n = n; p.total = 0; }
-    int unit = 0;
-    long long cost = 0;
+    const int mine = tid < a.M ? sh_tokens(a, tid) : 0;          // (asked for together with the list)
+    sh_fetch_groups(a, list);
+    if (tid < 2 * SH_MAX_GROUPS) red[tid >> 1][tid & 1] = 0x7fffffff;
+    __syncthreads();
+    const int n = sh_n_groups(a, list);
+    int at = 0, b, e, pages;
     for (int g = 0; g < n; g++) {
-        int b, e, pages;
-        sh_group(a, g, at, b, e, pages);
-        __syncthreads();
-        if (tid < 2) red[tid] = 0x7fffffff;
-        __syncthreads();
+        sh_group(a, list, g, at, b, e, pages);
         int least = 0x7fffffff, first = 0x7fffffff;
-        for (int m = b + tid; m < e; m += blockDim.x) {
-            const int t = sh_tokens(a, m);
+        for (int m = tid < b ? b + (tid - b % (int)blockDim.x + (int)blockDim.x) % (int)blockDim.x : tid; m < e; m += blockDim.x) {      // rows tid, tid + blockDim.x .. that are the group's
+            const int t = m == tid ? mine : sh_tokens(a, m);
             if (t > 0) { least = min(least, t / SH_PAGE); first = min(first, m); }
         }
         least = __reduce_min_sync(0xffffffffu, least);
         first = __reduce_min_sync(0xffffffffu, first);
-        if ((tid & 31) == 0) { atomicMin(&red[0], least); atomicMin(&red[1], first); }
-        __syncthreads();
-        pages = red[1] == 0x7fffffff ? 0 : min(pages, red[0]);
-        const int tiles = sh_tiles(a, e - b);
-        if (tid == 0) {
-            p.begin[g] = b; p.end[g] = e; p.pages[g] = pages; p.first[g] = red[1]; p.cost[g] = (int)cost; p.unit[g] = unit;
-        }
-        cost += (long long)a.n_kv_heads * sh_head_cost(tiles, sh_steps(pages));
-        unit += a.n_kv_heads * ((tiles + 1) / 2);
+        if ((tid & 31) == 0 && first != 0x7fffffff) { atomicMin(&red[g][0], least); atomicMin(&red[g][1], first); }
     }
+    __syncthreads();
     if (tid == 0) {
-        p.total = (int)cost;
-        p.quota = max((int)((cost + gridDim.x - 1) / gridDim.x), SH_LEAST_STEPS * SH_PAIR_COST);
+        int unit = 0, cost = 0;
+        at = 0;
+        for (int g = 0; g < n; g++) {
+            sh_group(a, list, g, at, b, e, pages);
+            pages = red[g][1] == 0x7fffffff ? 0 : min(pages, red[g][0]);
+            const int tiles = sh_tiles(a, e - b);
+            p.begin[g] = b; p.end[g] = e; p.pages[g] = pages; p.first[g] = red[g][1]; p.cost[g] = cost; p.unit[g] = unit;
+            cost += a.n_kv_heads * sh_head_cost(tiles, sh_steps(pages));      // (the host has seen to it that all of it fits)
+            unit += a.n_kv_heads * ((tiles + 1) / 2);
+        }
+        p.n = n;
+        p.total = cost;
+        p.quota = max((cost + (int)gridDim.x - 1) / (int)gridDim.x, SH_LEAST_COST);
     }
     __syncthreads();
 }
@@ -194,7 +229,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
                                                                          const __grid_constant__ WaitLimit limit) {
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ ShPlan plan;
-    __shared__ int red[2], gave_up_s, bad_s;
+    __shared__ int list[1 + 3 * SH_MAX_GROUPS], red[SH_MAX_GROUPS][2], gave_up_s, bad_s;
     uint8_t* q_s = smem;                                        // [2] query tiles
     uint8_t* k_s = q_s + 2 * SH_TILE_BYTES;                     // [2] K tiles (tokens x head dim, K-major)
     uint8_t* v_s = k_s + SH_STAGES * SH_TILE_BYTES;             // [2] V tiles (tokens x head dim, MN-major for P V)
@@ -231,7 +266,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
     }
     pdl_wait();                                                  // q, the rows' places and the cache come from earlier kernels
     pdl_launch_dependents();                                     // ... and are complete for the second launch, too, when it starts
-    sh_make_plan(a, plan, red);
+    sh_make_plan(a, plan, list, red);
     if (blockIdx.x == 0)
         for (int i = tid; i < (int)(sizeof(ShPlan) / 4); i += SH_THREADS) reinterpret_cast<int*>(a.scratch)[i] = reinterpret_cast<const int*>(&plan)[i];
     const int b = blockIdx.x, x_end = min((int)min((long long)plan.total, (long long)(b + 1) * plan.quota), plan.total);
@@ -243,28 +278,31 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
     const PtWaits wait = {&gave_up_s, globaltimer_ns(), limit.ns};
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
     // this CTA's items, in the same order for every role: `x` goes from the start of its share to the end of the unit looked at
+    ShUnit u_at;
     auto next_item = [&](int& x, ShItem& it) {
         while (x < x_end) {
-            ShUnit u;
             int j0, j1;
-            sh_unit_at(a, plan, x, u);
-            sh_share(plan, u, b, j0, j1);
-            x = u.c0 + u.steps * u.w;
+            if (x == b * plan.quota) sh_unit_at(a, plan, x, u_at);
+            else sh_next_unit(a, plan, u_at);
+            sh_share(plan, u_at, b, j0, j1);
+            x = u_at.c0 + u_at.steps * u_at.w;
             if (j1 <= j0) continue;
-            it.kvh = u.kvh;
-            it.begin = plan.begin[u.g];
-            it.row0 = u.pair * 2 * SH_ROWS;
-            it.rows = (plan.end[u.g] - it.begin) * (a.n_heads / a.n_kv_heads);
-            it.slot = plan.first[u.g];
-            it.pages = plan.pages[u.g];
+            it.kvh = u_at.kvh;
+            it.begin = plan.begin[u_at.g];
+            it.row0 = u_at.pair * 2 * SH_ROWS;
+            it.rows = (plan.end[u_at.g] - it.begin) * (a.n_heads / a.n_kv_heads);
+            it.slot = plan.first[u_at.g];
+            it.pages = plan.pages[u_at.g];
             it.j0 = j0;
             it.J = j1 - j0;
-            it.tiles = u.tiles;
-            it.piece = u.index + b;
+            it.tiles = u_at.tiles;
+            it.piece = u_at.index + b;
             return true;
         }
         return false;
     };
+    // A single tile takes both places, too: its steps in turn, so that the softmax of one step runs beside the next one's (two pieces; a step took 1.9 us in one place, 1.6 for two tiles).  Step j of place t?
+    auto on = [](const ShItem& it, int t, int j) { return j < it.J && (it.tiles == 2 || (j & 1) == t); };
     // TMEM columns: one buffer of scores at 0, which the tiles take in turn; probabilities at 128, of 64 columns for each tile; outputs at 256 + 128 t
     if (warp < 8) {
         // ---------------- softmax: warps 0-3 tile 0, warps 4-7 tile 1; a thread per stacked row (= TMEM lane) ----------------
@@ -274,8 +312,8 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
         uint32_t ns = 0, nq = 0;                                 // steps of this tile so far, items whose queries are loaded
         float q_factor = 1.f;
         auto load_queries = [&](const ShItem& of) {
-            if (t >= of.tiles) return;
-            const int r = min(of.row0 + t * SH_ROWS + row, of.rows - 1);      // rows that are not there: the last one
+            if (of.tiles == 1 && of.J <= t) return;
+            const int r = min(of.row0 + (of.tiles == 2 ? t * SH_ROWS : 0) + row, of.rows - 1);      // rows that are not there: the last one
             q_factor = sh_load_rows<HS>(a.q + (long long)(of.begin + r / rep) * a.ldq + (of.kvh * rep + r % rep) * HS, q_s + t * SH_TILE_BYTES, quarter * 32, [&] {
                 if (nq > 0) wait(&q_empty[t], (nq - 1) & 1);      // the tile's last scores have read the queries before
             });
@@ -287,10 +325,10 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
         bool more = next_item(x, it);
         if (more) load_queries(it);
         for (; more; it = next) {
-            const bool on = t < it.tiles;
+            const int by = it.tiles == 2 ? 1 : 2, ja = it.tiles == 2 ? 0 : t;      // steps ja, ja + by .. are this place's
             const float sc = 1.4426950408889634f * rsqrtf((float)HS) * q_factor;      // scores in the log2 domain
             float m_used = -INFINITY, l = 0.f;
-            for (int j = 0; on && j < it.J; j++, ns++) {
+            for (int j = ja; j < it.J; j += by, ns++) {
                 uint32_t v[4][32];
                 wait(&s_full[t], ns & 1);
                 tc_fence_after();
@@ -327,9 +365,9 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
                 const float ref = (m_used == -INFINITY) ? 0.0f : m_used;
                 pair_f sum = 0;
                 uint32_t pk[4][16], none[1];
-                if (j > 0) wait(&o_full[t], (ns - 1) & 1);
+                if (j > ja) wait(&o_full[t], (ns - 1) & 1);
                 tc_fence_after();
-                if (moved && j > 0) {      // the accumulated output moves to the new reference (rare after the first steps)
+                if (moved && j > ja) {      // the accumulated output moves to the new reference (rare after the first steps)
                     uint32_t w[32];
 #pragma unroll 1
                     for (int ch = 0; ch < HS / 32; ch++) {
@@ -352,7 +390,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
             }
             more = next_item(x, next);
             if (more) load_queries(next);
-            if (!on) continue;
+            if (ja >= it.J) continue;
             wait(&o_full[t], (ns - 1) & 1);
             tc_fence_after();
             // the largest weight is 1 or more; where it is not, a score was no number.  No score at all above -inf: nothing to add
@@ -383,12 +421,13 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
             uint32_t g = 0, n_s = 0, ns[2] = {0, 0}, nq[2] = {0, 0};      // steps, scores, steps of a tile, items of a tile so far
             ShItem it;
             for (int x = b * plan.quota; next_item(x, it);) {
-                auto on = [&](int t, int j) { return t < it.tiles && j < it.J; };
-                auto scores = [&](int t, int j) {                // S = Q K^T of a step
-                    const int st = (g + j) & 1;
-                    if (!on(t, j)) return;
-                    wait(&k_full[st], ((g + j) >> 1) & 1);
-                    if (j == 0) wait(&q_full[t], nq[t]++ & 1);
+                // what is multiplied, in this order: (place, step) (0, 0), (1, 0), (0, 1) .. of two tiles, (0, 0), (1, 1), (0, 2) .. of one
+                const int two = it.tiles == 2 ? 1 : 0, E = it.J << two;
+                auto scores = [&](int e) {                       // S = Q K^T
+                    if (e >= E) return;
+                    const int t = e & 1, j = e >> two, st = (g + j) & 1;
+                    if (!two || t == 0) wait(&k_full[st], ((g + j) >> 1) & 1);
+                    if (j == (two ? 0 : t)) wait(&q_full[t], nq[t]++ & 1);
                     if (n_s > 0) wait(s_empty, (n_s - 1) & 1);
                     n_s++;
                     tc_fence_after();
@@ -396,40 +435,35 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
                     if constexpr (HS == 128) pt_mma_ss(tmem_base, q_lo + t * (SH_TILE_BYTES >> 4), k_lo + st * (SH_TILE_BYTES >> 4), desc_hi, idesc_s, 0);
                     else pt_mma_ss4(tmem_base, q_lo + t * (SH_TILE_BYTES >> 4), k_lo + st * (SH_TILE_BYTES >> 4), desc_hi, idesc_s, 0);
                     pt_commit(&s_full[t]);
-                    if (t + 1 == it.tiles) pt_commit(&k_empty[st]);
-                    if (j + 1 == it.J) pt_commit(&q_empty[t]);
+                    if (!two || t == 1) pt_commit(&k_empty[st]);
+                    if (!on(it, t, j + 2 - two)) pt_commit(&q_empty[t]);
                 };
-                auto outputs = [&](int t, int j) {               // O += P V of a step
-                    const int st = (g + j) & 1;
-                    if (on(t, j)) {
-                        wait(&p_full[t], ns[t]++ & 1);
-                        tc_fence_after();
-                        __syncwarp();
-                        pt_mma_ts(tmem_base + 256 + t * 128, tmem_base + 128 + t * 64, v_lo + st * (SH_TILE_BYTES >> 4), desc_hi, idesc_pv, j > 0 ? 1u : 0u);
-                        pt_commit(&o_full[t]);
-                    }
-                    if (t == 1) pt_commit(&v_empty[st]);
-                };
-                scores(0, 0);
-                scores(1, 0);
-                scores(0, 1);
-                for (int j = 0; j < it.J; j++) {
-                    const int st = (g + j) & 1, live = it.pages - (it.j0 + j) * (SH_KV / SH_PAGE);
-                    wait(&v_full[st], ((g + j) >> 1) & 1);
-                    if (live < SH_KV / SH_PAGE) {                // pages that were not copied: a weight of zero times what lies there may be a NaN
-                        uint8_t* vz = v_s + st * SH_TILE_BYTES;
-                        for (int i = live * SH_PAGE * (HS / 8) + lane; i < SH_KV * (HS / 8); i += 32) {      // 16-byte pieces of a token's row
-                            const int r = i / (HS / 8), c = i % (HS / 8);
-                            *reinterpret_cast<uint4*>(vz + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                scores(0);
+                scores(1);
+                scores(2);
+                for (int e = 0; e < E; e++) {                    // O += P V
+                    const int t = e & 1, j = e >> two, st = (g + j) & 1;
+                    if (!two || t == 0) {
+                        const int live = it.pages - (it.j0 + j) * (SH_KV / SH_PAGE);
+                        wait(&v_full[st], ((g + j) >> 1) & 1);
+                        if (live < SH_KV / SH_PAGE) {            // pages that were not copied: a weight of zero times what lies there may be a NaN
+                            uint8_t* vz = v_s + st * SH_TILE_BYTES;
+                            for (int i = live * SH_PAGE * (HS / 8) + lane; i < SH_KV * (HS / 8); i += 32) {      // 16-byte pieces of a token's row
+                                const int r = i / (HS / 8), c = i % (HS / 8);
+                                *reinterpret_cast<uint4*>(vz + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            }
+                            fence_proxy_async_smem();
+                            __syncwarp();
                         }
-                        fence_proxy_async_smem();
-                        __syncwarp();
                     }
+                    wait(&p_full[t], ns[t]++ & 1);
+                    tc_fence_after();
+                    __syncwarp();
+                    pt_mma_ts(tmem_base + 256 + t * 128, tmem_base + 128 + t * 64, v_lo + st * (SH_TILE_BYTES >> 4), desc_hi, idesc_pv, j > (two ? 0 : t) ? 1u : 0u);
+                    pt_commit(&o_full[t]);
+                    if (!two || t == 1) pt_commit(&v_empty[st]);
                     // the scores after next wait in the buffer when the softmax threads come for them
-                    outputs(0, j);
-                    scores(1, j + 1);
-                    outputs(1, j);
-                    scores(0, j + 2);
+                    scores(e + 3);
                 }
                 g += it.J;
             }
@@ -519,8 +553,7 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32) shared_own_kernel(const __g
     constexpr int KS = HS / 16, NT = HS / 8, LPH = HS / 4;                                     // MMA steps of a score, tiles of an output, threads of a head in the join
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ ShPlan plan;
-    __shared__ int red[1];
-    __shared__ int bad_s;
+    __shared__ int list[1 + 3 * SH_MAX_GROUPS], red[1], bad_s;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = blockIdx.x, n_cl = gridDim.x, kvh = blockIdx.y, m = blockIdx.z;           // (a row of the grid is one cluster)
@@ -530,16 +563,17 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32) shared_own_kernel(const __g
     float* c_acc = w_ml + SH_OWN_WARPS * G * 2;                 // [G][HS] of the CTA
     float* c_ml = c_acc + G * HS;                               // [G][2]
     pdl_launch_dependents();
-    if (tid == 0) { red[0] = 0x7fffffff; bad_s = 0; }
-    __syncthreads();
     const int T = sh_tokens(a, m);
+    if (tid == 0) { red[0] = 0x7fffffff; bad_s = 0; }
+    sh_fetch_groups(a, list);
+    __syncthreads();
     // the pages of this row's group that all of its rows see
     int shared = 0, g_of = -1;
     {
         int at = 0, b = 0, e = 0, pages = 0;
-        const int n = sh_n_groups(a);
+        const int n = sh_n_groups(a, list);
         for (int i = 0; i < n; i++) {
-            sh_group(a, i, at, b, e, pages);
+            sh_group(a, list, i, at, b, e, pages);
             if (m >= b && m < e) { g_of = i; break; }
         }
         if (g_of >= 0 && pages > 0) {
@@ -716,39 +750,69 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32) shared_own_kernel(const __g
     __syncthreads();
     // (a scratch that another launch writes meanwhile names other groups: no place of it is looked at that this launch has not)
     const bool planned = shared == 0 || (plan.n > g_of && plan.begin[g_of] <= m && m < plan.end[g_of] && plan.pages[g_of] == shared && plan.quota > 0);
-    // this CTA's pieces of the group's pages: every n_cl-th share
-    for (int h0 = 0; h0 < G; h0 += SH_OWN_WARPS * 32 / LPH) {
-        const int h = h0 + tid / LPH, d4 = tid % LPH;
-        if (h >= G) continue;                                    // (no barrier below)
+    // A warp joins a head, a lane four of its values (heads of 64: half a warp every other piece): the warps' own parts, then this CTA's pieces of the group's pages (those of every n_cl-th share),
+    // 32 maxima and sums at a time, and their values all in flight.
+    for (int h = warp; h < G; h += SH_OWN_WARPS) {
+        const int d4 = lane % LPH, half = lane / LPH;
         float M = -INFINITY, L = 0.f;
         float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto add = [&](float pm, float pl, const float4& x) {
-            if (pl == 0.f) return;                               // nothing was seen (not: a NaN)
-            const float mn = fmaxf(M, pm), mu = mn == -INFINITY ? 0.f : mn, c = pt_ex2(M - mu), e = pt_ex2(pm - mu);
-            L = fmaf(L, c, pl * e);
-            O = make_float4(fmaf(O.x, c, x.x * e), fmaf(O.y, c, x.y * e), fmaf(O.z, c, x.z * e), fmaf(O.w, c, x.w * e));
+        auto put = [&](const float4& x, float e) { O = make_float4(fmaf(x.x, e, O.x), fmaf(x.y, e, O.y), fmaf(x.z, e, O.z), fmaf(x.w, e, O.w)); };
+        // maxima and sums of 32 parts (sum 0: nothing was seen; a NaN is something), one a lane: this lane's factor
+        auto weigh = [&](float pm, float pl) {
+            const float mn = fmaxf(M, warp_max(pl != 0.f ? pm : -INFINITY)), mu = mn == -INFINITY ? 0.f : mn, c = pt_ex2(M - mu), e = pl != 0.f ? pt_ex2(pm - mu) : 0.f;
+            L = fmaf(L, c, warp_sum(pl * e));
+            O = make_float4(O.x * c, O.y * c, O.z * c, O.w * c);
             M = mn;
+            return e;
         };
+        {
+            const bool mine = lane < SH_OWN_WARPS;
+            const float e = weigh(mine ? w_ml[(lane * G + h) * 2] : -INFINITY, mine ? w_ml[(lane * G + h) * 2 + 1] : 0.f);
 #pragma unroll
-        for (int w = 0; w < SH_OWN_WARPS; ++w)
-            add(w_ml[(w * G + h) * 2], w_ml[(w * G + h) * 2 + 1], *reinterpret_cast<const float4*>(w_acc + (w * G + h) * HS + d4 * 4));
+            for (int w = 0; w < SH_OWN_WARPS; ++w) {
+                const float ew = __shfl_sync(0xffffffffu, e, w);
+                if (half == 0 && ew != 0.f) put(*reinterpret_cast<const float4*>(w_acc + (w * G + h) * HS + d4 * 4), ew);
+            }
+        }
         if (shared > 0 && planned) {
             const int r = (m - plan.begin[g_of]) * G + h, t = r / SH_ROWS;
             ShUnit unit;
             sh_unit(a, plan, g_of, kvh, t / 2, unit);
-            const int b0 = unit.c0 / plan.quota, b1 = (unit.c0 + unit.steps * unit.w - 1) / plan.quota + 1;
-#pragma unroll 4
-            for (int b = b0 + rank; b < b1; b += n_cl) {
-                int j0, j1;
-                sh_share(plan, unit, b, j0, j1);
-                const size_t at = (size_t)min((long long)(unit.index + b), a.n_pieces - 1) * 2 + (t & 1);
-                const float2 n = j1 > j0 ? __ldcg(sh_norms(a) + at * SH_ROWS + r % SH_ROWS) : make_float2(0.f, 0.f);
-                const float4 x = j1 > j0 ? __ldcg(sh_sums(a) + ((at * 4 + (r % SH_ROWS) / 32) * LPH + d4) * 32 + r % 32) : make_float4(0.f, 0.f, 0.f, 0.f);
-                add(n.x, n.y, x);
+            const int subs = unit.tiles == 2 ? 1 : 2;            // pieces of a share that hold this row
+            const int b0 = unit.c0 / plan.quota + rank, b1 = (unit.c0 + unit.steps * unit.w - 1) / plan.quota + 1, n = b1 > b0 ? (b1 - b0 + n_cl - 1) / n_cl * subs : 0;
+            const float2* norms = sh_norms(a) + r % SH_ROWS;
+            const float4* sums = sh_sums(a) + ((r % SH_ROWS) / 32 * LPH + d4) * 32 + r % 32;
+            for (int c0 = 0; c0 < n; c0 += 32) {
+                const int c = c0 + lane, b = b0 + c / subs * n_cl, sub = c % subs;
+                int j0 = 0, j1 = 0;
+                if (c < n) sh_share(plan, unit, b, j0, j1);
+                const unsigned at = (unsigned)min((long long)(unit.index + b), a.n_pieces - 1) * 2 + (subs == 1 ? t & 1 : sub);
+                const float2 x = j1 - j0 > (subs == 1 ? 0 : sub) ? __ldcg(norms + (size_t)at * SH_ROWS) : make_float2(-INFINITY, 0.f);
+                const float e = weigh(x.x, x.y);
+                const int live = min(32, n - c0);
+#pragma unroll 1
+                for (int i0 = 0; i0 < live; i0 += 8 * 32 / LPH) {
+                    float4 v[8];
+                    float f[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int from = i0 + i * (32 / LPH) + half;
+                        const unsigned where = __shfl_sync(0xffffffffu, at, from & 31);
+                        f[i] = __shfl_sync(0xffffffffu, e, from & 31);
+                        if (from >= live) f[i] = 0.f;
+                        v[i] = f[i] != 0.f ? __ldcg(sums + (size_t)where * 4 * LPH * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) put(v[i], f[i]);
+                }
             }
         }
-        *reinterpret_cast<float4*>(c_acc + h * HS + d4 * 4) = O;
-        if (d4 == 0) { c_ml[h * 2] = M; c_ml[h * 2 + 1] = bad_s || !planned ? __int_as_float(0x7fffffff) : L; }
+        if (HS == 64) {
+            O.x += __shfl_xor_sync(0xffffffffu, O.x, 16); O.y += __shfl_xor_sync(0xffffffffu, O.y, 16);
+            O.z += __shfl_xor_sync(0xffffffffu, O.z, 16); O.w += __shfl_xor_sync(0xffffffffu, O.w, 16);
+        }
+        if (half == 0) *reinterpret_cast<float4*>(c_acc + h * HS + d4 * 4) = O;
+        if (lane == 0) { c_ml[h * 2] = M; c_ml[h * 2 + 1] = bad_s || !planned ? __int_as_float(0x7fffffff) : L; }
     }
     if (n_cl > 1) cluster.sync();
     else __syncthreads();
