@@ -25,11 +25,11 @@
 #define SH_THREADS 384
 #define SH_TILE_BYTES 32768            // 128 x 128 fp16
 #define SH_STAGES 2
+#define SH_OUT_LD 20
 #define SH_MAX_GROUPS 8
 #define SH_PAIR_COST 7                 // of a step with two tiles
 #define SH_ONE_COST 4                  // ... with one
 #define SH_LEAST_COST 8                // of a CTA's share: two steps of one tile
-#define SH_PLAN_BYTES 1024
 #define SH_OWN_WARPS 4
 #define SH_OWN_TOK 16                  // tokens of a warp's turn
 #define SH_OWN_MAX_CTAS 8
@@ -42,8 +42,9 @@ struct ShArgs {
     long long ldq;
     const __half *k_cache, *v_cache;   // [pages][n_kv][32][head size]
     const int *pos, *slot, *block_table, *groups;
-    int M, n_heads, n_kv_heads, n_slots, max_pages, n_pages, max_groups;
-    uint8_t* scratch;                  // plan | norms | sums
+    int M, n_heads, n_kv_heads, rep, n_slots, max_pages, n_pages, max_groups;      // rep: query heads of a key/value head
+    uint8_t* scratch;                  // norms | sums
+    int shares;                        // CTAs of the first launch
     long long n_pieces;                // that the scratch has room for
     uint8_t *xq_out, *xh_out;
     int out_mcap;
@@ -52,7 +53,7 @@ struct ShArgs {
     int y_type;
 };
 
-// What the first launch works on; the second one reads it (in the scratch).
+// What the first launch works on.  Every CTA of both makes it for itself.
 struct ShPlan {
     int n, quota;                                              // groups; a CTA's share
     int total;
@@ -60,12 +61,11 @@ struct ShPlan {
     int pages[SH_MAX_GROUPS], first[SH_MAX_GROUPS];            // pages that all rows of the group see; a row whose table names them
     int cost[SH_MAX_GROUPS], unit[SH_MAX_GROUPS];              // cost and units (key/value head, two tiles) of the groups ahead
 };
-static_assert(sizeof(ShPlan) <= SH_PLAN_BYTES, "");
 
 struct ShUnit { int g, kvh, pair, tiles, steps, w, c0, index; };
 
-DL_DEVINL float2* sh_norms(const ShArgs& a) { return reinterpret_cast<float2*>(a.scratch + SH_PLAN_BYTES); }                 // [piece][2][128]
-DL_DEVINL float4* sh_sums(const ShArgs& a) { return reinterpret_cast<float4*>(sh_norms(a) + a.n_pieces * 2 * SH_ROWS); }     // [piece][2][4 warps][head size / 4][32]
+DL_DEVINL float2* sh_norms(const ShArgs& a) { return reinterpret_cast<float2*>(a.scratch); }                                 // [piece][2][128]
+DL_DEVINL float4* sh_sums(const ShArgs& a) { return reinterpret_cast<float4*>(sh_norms(a) + a.n_pieces * 2 * SH_ROWS); }     // [piece][2][128][head size / 4]
 
 // positions that a row sees; 0: it has no token, -1: its sequence or position is not in the table
 DL_DEVINL int sh_tokens(const ShArgs& a, int m) {
@@ -88,7 +88,7 @@ DL_DEVINL void sh_group(const ShArgs& a, const int* list, int i, int& at, int& b
 }
 DL_DEVINL int sh_n_groups(const ShArgs& a, const int* list) { return max(0, min(min(list[0], a.max_groups), SH_MAX_GROUPS)); }
 
-DL_DEVINL int sh_tiles(const ShArgs& a, int rows) { return (rows * (a.n_heads / a.n_kv_heads) + SH_ROWS - 1) / SH_ROWS; }
+DL_DEVINL int sh_tiles(const ShArgs& a, int rows) { return (rows * a.rep + SH_ROWS - 1) / SH_ROWS; }
 DL_DEVINL int sh_steps(int pages) { return (pages + SH_KV / SH_PAGE - 1) / (SH_KV / SH_PAGE); }
 // cost of a group's steps for one key/value head
 DL_DEVINL int sh_head_cost(int tiles, int steps) { return steps * (tiles / 2 * SH_PAIR_COST + (tiles & 1) * SH_ONE_COST); }
@@ -102,12 +102,20 @@ DL_DEVINL void sh_unit(const ShArgs& a, const ShPlan& p, int g, int kvh, int pai
     u.c0 = p.cost[g] + kvh * sh_head_cost(tiles, u.steps) + pair * u.steps * SH_PAIR_COST;
     u.index = p.unit[g] + kvh * pairs + pair;
 }
+// x / d of numbers that are not negative, without the compiler's sequence for it (2000 clk of a CTA's start went there)
+DL_DEVINL int sh_quot(int x, int d) {
+    int q = (int)__fdividef((float)x, (float)d);
+    while (q > 0 && (long long)q * d > x) q--;
+    while ((long long)(q + 1) * d <= x) q++;
+    return q;
+}
 // the unit in which place x of the whole cost lies
 DL_DEVINL void sh_unit_at(const ShArgs& a, const ShPlan& p, int x, ShUnit& u) {
     int g = 0;
     while (g + 1 < p.n && p.cost[g + 1] <= x) g++;
     const int tiles = sh_tiles(a, p.end[g] - p.begin[g]), steps = sh_steps(p.pages[g]), head = sh_head_cost(tiles, steps), rest = x - p.cost[g];
-    sh_unit(a, p, g, rest / head, min(rest % head / (steps * SH_PAIR_COST), (tiles + 1) / 2 - 1), u);
+    const int kvh = sh_quot(rest, head);
+    sh_unit(a, p, g, kvh, min(sh_quot(rest - kvh * head, steps * SH_PAIR_COST), (tiles + 1) / 2 - 1), u);
 }
 // ... and the one behind it (there is one: the whole cost has not been reached)
 DL_DEVINL void sh_next_unit(const ShArgs& a, const ShPlan& p, ShUnit& u) {
@@ -188,7 +196,8 @@ DL_DEVINL float sh_load_rows(const float* mine, uint8_t* tile, int r0, Ready rea
 // The plan, by all threads of a CTA (in shared memory).
 DL_DEVINL void sh_make_plan(const ShArgs& a, ShPlan& p, int* list, int (*red)[2]) {
     const int tid = threadIdx.x;
-    const int mine = tid < a.M ? sh_tokens(a, tid) : 0;          // (asked for together with the list)
+    const int n_thr = blockDim.x;
+    const int mine = tid < a.M ? sh_tokens(a, tid) : 0, mine2 = tid + n_thr < a.M ? sh_tokens(a, tid + n_thr) : 0;      // (asked for together with the list)
     sh_fetch_groups(a, list);
     if (tid < 2 * SH_MAX_GROUPS) red[tid >> 1][tid & 1] = 0x7fffffff;
     __syncthreads();
@@ -197,8 +206,9 @@ DL_DEVINL void sh_make_plan(const ShArgs& a, ShPlan& p, int* list, int (*red)[2]
     for (int g = 0; g < n; g++) {
         sh_group(a, list, g, at, b, e, pages);
         int least = 0x7fffffff, first = 0x7fffffff;
-        for (int m = tid < b ? b + (tid - b % (int)blockDim.x + (int)blockDim.x) % (int)blockDim.x : tid; m < e; m += blockDim.x) {      // rows tid, tid + blockDim.x .. that are the group's
-            const int t = m == tid ? mine : sh_tokens(a, m);
+        for (int m = tid; m < e; m += n_thr) {
+            if (m < b) continue;
+            const int t = m == tid ? mine : m == tid + n_thr ? mine2 : sh_tokens(a, m);
             if (t > 0) { least = min(least, t / SH_PAGE); first = min(first, m); }
         }
         least = __reduce_min_sync(0xffffffffu, least);
@@ -219,7 +229,7 @@ DL_DEVINL void sh_make_plan(const ShArgs& a, ShPlan& p, int* list, int (*red)[2]
         }
         p.n = n;
         p.total = cost;
-        p.quota = max((cost + (int)gridDim.x - 1) / (int)gridDim.x, SH_LEAST_COST);
+        p.quota = max(sh_quot(cost + a.shares - 1, a.shares), SH_LEAST_COST);
     }
     __syncthreads();
 }
@@ -233,7 +243,8 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
     uint8_t* q_s = smem;                                        // [2] query tiles
     uint8_t* k_s = q_s + 2 * SH_TILE_BYTES;                     // [2] K tiles (tokens x head dim, K-major)
     uint8_t* v_s = k_s + SH_STAGES * SH_TILE_BYTES;             // [2] V tiles (tokens x head dim, MN-major for P V)
-    uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + SH_STAGES * SH_TILE_BYTES);
+    float* out_s = reinterpret_cast<float*>(v_s + SH_STAGES * SH_TILE_BYTES);      // [8 warps][32][SH_OUT_LD] f32: sums on their way out
+    uint64_t* bars = reinterpret_cast<uint64_t*>(out_s + 8 * 32 * SH_OUT_LD);
     uint64_t* k_full = bars;             // [2] transaction bytes of the step's K copies
     uint64_t* k_empty = bars + 2;        // [2] the scores that read the stage are complete (both tiles')
     uint64_t* v_full = bars + 4;         // [2] transaction bytes of the step's V copies
@@ -264,17 +275,18 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
         mbar_init(s_empty, 128);
         mbar_fence_init();
     }
+    if (warp == 0) tmem_alloc(tmem_holder, 512);
     pdl_wait();                                                  // q, the rows' places and the cache come from earlier kernels
     pdl_launch_dependents();                                     // ... and are complete for the second launch, too, when it starts
     sh_make_plan(a, plan, list, red);
-    if (blockIdx.x == 0)
-        for (int i = tid; i < (int)(sizeof(ShPlan) / 4); i += SH_THREADS) reinterpret_cast<int*>(a.scratch)[i] = reinterpret_cast<const int*>(&plan)[i];
     const int b = blockIdx.x, x_end = min((int)min((long long)plan.total, (long long)(b + 1) * plan.quota), plan.total);
-    if ((long long)b * plan.quota >= plan.total) return;         // (uniform for the CTA)
-    if (warp == 0) tmem_alloc(tmem_holder, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if ((long long)b * plan.quota >= plan.total) {               // (uniform for the CTA)
+        if (warp == 0) tmem_dealloc(__shfl_sync(0xffffffffu, *tmem_holder, 0), 512);
+        return;
+    }
     const PtWaits wait = {&gave_up_s, globaltimer_ns(), limit.ns};
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
     // this CTA's items, in the same order for every role: `x` goes from the start of its share to the end of the unit looked at
@@ -290,7 +302,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
             it.kvh = u_at.kvh;
             it.begin = plan.begin[u_at.g];
             it.row0 = u_at.pair * 2 * SH_ROWS;
-            it.rows = (plan.end[u_at.g] - it.begin) * (a.n_heads / a.n_kv_heads);
+            it.rows = (plan.end[u_at.g] - it.begin) * a.rep;
             it.slot = plan.first[u_at.g];
             it.pages = plan.pages[u_at.g];
             it.j0 = j0;
@@ -307,14 +319,15 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
     if (warp < 8) {
         // ---------------- softmax: warps 0-3 tile 0, warps 4-7 tile 1; a thread per stacked row (= TMEM lane) ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, rep = a.n_heads / a.n_kv_heads;
+        const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, rep = a.rep;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16, T_S = tmem_base + lane_base, T_P = tmem_base + lane_base + 128 + t * 64, T_O = tmem_base + lane_base + 256 + t * 128;
         uint32_t ns = 0, nq = 0;                                 // steps of this tile so far, items whose queries are loaded
         float q_factor = 1.f;
         auto load_queries = [&](const ShItem& of) {
             if (of.tiles == 1 && of.J <= t) return;
             const int r = min(of.row0 + (of.tiles == 2 ? t * SH_ROWS : 0) + row, of.rows - 1);      // rows that are not there: the last one
-            q_factor = sh_load_rows<HS>(a.q + (long long)(of.begin + r / rep) * a.ldq + (of.kvh * rep + r % rep) * HS, q_s + t * SH_TILE_BYTES, quarter * 32, [&] {
+            const int of_row = sh_quot(r, rep);
+            q_factor = sh_load_rows<HS>(a.q + (long long)(of.begin + of_row) * a.ldq + (of.kvh * rep + r - of_row * rep) * HS, q_s + t * SH_TILE_BYTES, quarter * 32, [&] {
                 if (nq > 0) wait(&q_empty[t], (nq - 1) & 1);      // the tile's last scores have read the queries before
             });
             nq++;
@@ -398,15 +411,25 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
             if (bad_s || gave_up_s) l = __int_as_float(0x7fffffff);
             const size_t at = (size_t)it.piece * 2 + t;
             sh_norms(a)[at * SH_ROWS + row] = make_float2(m_used, l);
-            float4* out = sh_sums(a) + (at * 4 + quarter) * (HS / 4) * 32 + lane;
+            // 16 columns of the warp's rows at a time, then as many lanes along a row (a thread along its own row: 5 us for 128 of them)
+            float4* out = sh_sums(a) + (at * SH_ROWS + quarter * 32) * (HS / 4);
+            float* stage = out_s + (size_t)warp * 32 * SH_OUT_LD;
+            const int live = it.rows - (it.row0 + (it.tiles == 2 ? t * SH_ROWS : 0) + quarter * 32);      // rows of this warp that are there
 #pragma unroll 1
-            for (int ch = 0; ch < HS / 32; ch++) {
-                uint32_t o[32];
-                tmem_ld_32x32b_x32(T_O + ch * 32, o);
+            for (int ch = 0; ch < HS / 16; ch++) {
+                uint32_t o[16];
+                tmem_ld_32x32b_x16(T_O + ch * 16, o);
                 tmem_ld_wait();
+                __syncwarp();
 #pragma unroll
-                for (int e = 0; e < 32; e += 4)
-                    out[(ch * 8 + e / 4) * 32] = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<float4*>(stage + lane * SH_OUT_LD + e) = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                __syncwarp();
+#pragma unroll
+                for (int r0 = 0; r0 < 32; r0 += 8) {
+                    const int r = r0 + (lane >> 2);
+                    if (r < live) out[r * (HS / 4) + ch * 4 + (lane & 3)] = *reinterpret_cast<const float4*>(stage + r * SH_OUT_LD + (lane & 3) * 4);
+                }
             }
             tc_fence_before();                                   // the next item's P V may write the output (behind p_full)
         }
@@ -467,8 +490,8 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
                 }
                 g += it.J;
             }
-        } else if ((warp == 9 || warp == 10) && lane == 0) {
-            // ---------------- K producer (warp 9) / V producer (warp 10), one lane each ----------------
+        } else if (warp == 9 || warp == 10) {
+            // ---------------- K producer (warp 9) / V producer (warp 10): a lane for each of a step's four pages ----------------
             const bool is_k = warp == 9;
             const uint64_t map = is_k ? reinterpret_cast<uint64_t>(&kmap) : reinterpret_cast<uint64_t>(&vmap);
             uint64_t* full = is_k ? k_full : v_full;
@@ -478,39 +501,32 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
             ShItem it;
             for (int x = b * plan.quota; next_item(x, it);) {
                 const int* bt = a.block_table + (size_t)a.slot[it.slot] * a.max_pages;
-                auto page_of = [&](int p) { return p < it.pages ? bt[p] : 0; };
-                // the page ids of a step are fetched one step ahead, so the table reads (dependent global loads) overlap the
-                // wait for a free stage instead of delaying the copies
-                int pg[4], pg_next[4];
-#pragma unroll
-                for (int p4 = 0; p4 < 4; p4++) pg_next[p4] = page_of(4 * it.j0 + p4);
+                const int last = min(it.pages, 4 * (it.j0 + it.J));      // pages of this item end here
+                auto page_of = [&](int p) {                      // (not in the cache: the first one, and the piece is not valid)
+                    if (lane >= 4 || p >= last) return -1;
+                    const int page = bt[p];
+                    if ((unsigned)page < (unsigned)a.n_pages) return page;
+                    *(volatile int*)&bad_s = 1;                  // (seen by the softmax threads behind the barriers)
+                    return 0;
+                };
+                auto line_of = [&](int page) { return (page * a.n_kv_heads + it.kvh) * SH_PAGE; };      // first row of the page in the [rows][head size] view
+                int next = page_of(4 * it.j0 + lane);
                 for (int j = 0; j < it.J; j++, g++) {
-                    const int st = g & 1;
-#pragma unroll
-                    for (int p4 = 0; p4 < 4; p4++) {
-                        pg[p4] = pg_next[p4];
-                        pg_next[p4] = page_of(4 * (it.j0 + j + 1) + p4);
-                    }
+                    const int st = g & 1, page = next;
+                    next = page_of(4 * (it.j0 + j + 1) + lane);  // (a step ahead, so that the table's latency is not in the copies' way)
                     if (g >= SH_STAGES) wait(&empty[st], ((g >> 1) & 1) ^ 1);
-                    if (gave_up_s) break;                        // no more copies into a CTA that ends
-                    const int n_pg = min(4, it.pages - 4 * (it.j0 + j));
-                    bool bad = false;
-#pragma unroll
-                    for (int p4 = 0; p4 < 4; p4++)
-                        if ((unsigned)pg[p4] >= (unsigned)a.n_pages) { pg[p4] = 0; bad = true; }
-                    if (bad) *(volatile int*)&bad_s = 1;         // (seen by the softmax threads behind the barriers)
-                    mbar_arrive_expect_tx(&full[st], (uint32_t)n_pg * (HS / 64) * 4096u);
-                    const uint32_t dst = smem_u32(ring + st * SH_TILE_BYTES), bar = smem_u32(&full[st]);
-#pragma unroll
-                    for (int p4 = 0; p4 < 4; p4++) {
-                        if (p4 >= n_pg) break;
-                        const int y = (pg[p4] * a.n_kv_heads + it.kvh) * SH_PAGE;      // first row of the page in the [rows][head size] view
+                    if (__any_sync(0xffffffffu, gave_up_s)) break;      // no more copies into a CTA that ends
+                    if (lane == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)min(4, last - 4 * (it.j0 + j)) * (HS / 64) * 4096u);
+                    __syncwarp();
+                    if (page >= 0) {
+                        const uint32_t dst = smem_u32(ring + st * SH_TILE_BYTES) + lane * 4096, bar = smem_u32(&full[st]);
 #pragma unroll
                         for (int h = 0; h < HS / 64; h++)
-                            asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst + h * 16384 + p4 * 4096),
-                                         "l"(map), "r"(h * 64), "r"(y), "r"(bar)
+                            asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst + h * 16384), "l"(map), "r"(h * 64),
+                                         "r"(line_of(page)), "r"(bar)
                                          : "memory");
                     }
+                    __syncwarp();
                 }
             }
         }
@@ -548,54 +564,48 @@ DL_DEVINL void sh_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32
 // grid (CTAs of a row's cluster, key/value heads, rows).  Rows of the MMAs: the query heads of the key/value head (16 at most); tokens 16 at a time, a ring of stages for each
 // warp.  Then every thread joins four values of a head over the warps and this CTA's pieces, and the cluster's CTAs over each other's.
 template <int HS>
-__global__ void __launch_bounds__(SH_OWN_WARPS * 32) shared_own_kernel(const __grid_constant__ ShArgs a) {
+__global__ void __launch_bounds__(SH_OWN_WARPS * 32, 3) shared_own_kernel(const __grid_constant__ ShArgs a) {
     constexpr int ROWB = HS * 2, CH = ROWB / 16, HALF = SH_OWN_TOK * ROWB, ST = 256 / HS;      // bytes and 16-byte pieces of a line, bytes of a turn's K or V, stages
     constexpr int KS = HS / 16, NT = HS / 8, LPH = HS / 4;                                     // MMA steps of a score, tiles of an output, threads of a head in the join
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ ShPlan plan;
-    __shared__ int list[1 + 3 * SH_MAX_GROUPS], red[1], bad_s;
+    __shared__ int list[1 + 3 * SH_MAX_GROUPS], red[SH_MAX_GROUPS][2], bad_s;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = blockIdx.x, n_cl = gridDim.x, kvh = blockIdx.y, m = blockIdx.z;           // (a row of the grid is one cluster)
-    const int G = a.n_heads / a.n_kv_heads;
+    const int G = a.rep;
     float* w_acc = reinterpret_cast<float*>(smem);              // [warps][G][HS], after the ring is done with
     float* w_ml = w_acc + SH_OWN_WARPS * G * HS;                // [warps][G][2]
     float* c_acc = w_ml + SH_OWN_WARPS * G * 2;                 // [G][HS] of the CTA
     float* c_ml = c_acc + G * HS;                               // [G][2]
     pdl_launch_dependents();
-    const int T = sh_tokens(a, m);
-    if (tid == 0) { red[0] = 0x7fffffff; bad_s = 0; }
-    sh_fetch_groups(a, list);
-    __syncthreads();
-    // the pages of this row's group that all of its rows see
-    int shared = 0, g_of = -1;
-    {
-        int at = 0, b = 0, e = 0, pages = 0;
-        const int n = sh_n_groups(a, list);
-        for (int i = 0; i < n; i++) {
-            sh_group(a, list, i, at, b, e, pages);
-            if (m >= b && m < e) { g_of = i; break; }
+    if (tid == 0) bad_s = 0;
+    const int g = lane >> 2, qd = lane & 3;
+    // what needs no more than the row's number is asked for at once: its place, its queries (head g, and g + 8 where there are so many), and what the plan is made of
+    const int T = sh_tokens(a, m), slot = a.slot[m];
+    float2 qx[2][KS][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+        if (u * 8 < G) {
+            const int h = g + u * 8;
+            const float* q = a.q + (long long)m * a.ldq + (size_t)(kvh * G + (h < G ? h : 0)) * HS + qd * 2;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) qx[u][k][w] = *reinterpret_cast<const float2*>(q + k * 16 + w * 8);
         }
-        if (g_of >= 0 && pages > 0) {
-            int least = 0x7fffffff;
-            for (int r = b + tid; r < e; r += SH_OWN_WARPS * 32) {
-                const int t = sh_tokens(a, r);
-                if (t > 0) least = min(least, t / SH_PAGE);
-            }
-            least = __reduce_min_sync(0xffffffffu, least);
-            if (lane == 0) atomicMin(&red[0], least);
-            __syncthreads();
-            shared = min(pages, red[0]);
-        }
-    }
+    sh_make_plan(a, plan, list, red);
+    int g_of = -1;                                               // the row's group, and the pages that all of its rows see
+    for (int i = 0; i < plan.n; i++)
+        if (m >= plan.begin[i] && m < plan.end[i]) { g_of = i; break; }
+    const int shared = g_of >= 0 ? plan.pages[g_of] : 0;
     const int n_pages = T > 0 ? (T + SH_PAGE - 1) / SH_PAGE : 0;
     const int own = T > 0 ? n_pages - shared : 0, shares = max(1, min(n_cl, (own + 7) / 8)), per = (own + shares - 1) / shares;
     const int pg0 = shared + min(own, rank * per), pg1 = shared + (rank < shares ? min(own, rank * per + per) : 0);
     const int t_end = min(max(T, 0), pg1 * SH_PAGE);
     const int n_turns = pg1 > pg0 ? (t_end - pg0 * SH_PAGE + SH_OWN_TOK - 1) / SH_OWN_TOK : 0, n_my = (n_turns - warp + SH_OWN_WARPS - 1) / SH_OWN_WARPS;      // warp w takes turns w, w + 4, ...
-    const int* bt = a.block_table + (size_t)(T > 0 ? a.slot[m] : 0) * a.max_pages;
+    const int* bt = a.block_table + (size_t)(T > 0 ? slot : 0) * a.max_pages;
     const uint32_t ring = smem_u32(smem) + warp * (ST * 2 * HALF);
-    const int g = lane >> 2, qd = lane & 3;
     float run_m[2] = {-INFINITY, -INFINITY}, run_l[2] = {0.f, 0.f};      // of heads g and g + 8; run_l: this lane's own tokens
     float o[NT][4];
 #pragma unroll
@@ -637,20 +647,21 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32) shared_own_kernel(const __g
         float sc[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int h = g + u * 8;
-            const float* q = a.q + (long long)m * a.ldq + (size_t)(kvh * G + (h < G ? h : 0)) * HS + qd * 2;
-            float2 x[KS][2];
+            sc[u] = 0.f;
+            if (u * 8 >= G) {
+#pragma unroll
+                for (int k = 0; k < KS; ++k) qf[k][u] = qf[k][2 + u] = 0u;
+                continue;
+            }
             unsigned most = 0;
+            const float2 (&x)[KS][2] = qx[u];
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    x[k][w] = *reinterpret_cast<const float2*>(q + k * 16 + w * 8);
-                    most = max(most, max(__float_as_uint(x[k][w].x) & 0x7fffffffu, __float_as_uint(x[k][w].y) & 0x7fffffffu));
-                }
+                for (int w = 0; w < 2; ++w) most = max(most, max(__float_as_uint(x[k][w].x) & 0x7fffffffu, __float_as_uint(x[k][w].y) & 0x7fffffffu));
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const bool finite = most < 0x7f800000u, there = h < G;
+            const bool finite = most < 0x7f800000u, there = g + u * 8 < G;
             const unsigned up = sh_up(most);
             const float by = finite && there ? __uint_as_float(up << 23) : 0.f;
             sc[u] = (finite ? __uint_as_float((254u - up) << 23) : __uint_as_float(0x7fffffffu)) * (1.44269504088896341f * rsqrtf((float)HS));
@@ -746,10 +757,7 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32) shared_own_kernel(const __g
         if (qd == 0) { w_ml[(warp * G + h) * 2] = run_m[u]; w_ml[(warp * G + h) * 2 + 1] = run_l[u]; }
     }
     pdl_wait();                                                  // the pieces (and what follows this launch follows the first one, too)
-    for (int i = tid; i < (int)(sizeof(ShPlan) / 4); i += SH_OWN_WARPS * 32) reinterpret_cast<int*>(&plan)[i] = __ldcg(reinterpret_cast<const int*>(a.scratch) + i);
     __syncthreads();
-    // (a scratch that another launch writes meanwhile names other groups: no place of it is looked at that this launch has not)
-    const bool planned = shared == 0 || (plan.n > g_of && plan.begin[g_of] <= m && m < plan.end[g_of] && plan.pages[g_of] == shared && plan.quota > 0);
     // A warp joins a head, a lane four of its values (heads of 64: half a warp every other piece): the warps' own parts, then this CTA's pieces of the group's pages (those of every n_cl-th share),
     // 32 maxima and sums at a time, and their values all in flight.
     for (int h = warp; h < G; h += SH_OWN_WARPS) {
@@ -774,36 +782,44 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32) shared_own_kernel(const __g
                 if (half == 0 && ew != 0.f) put(*reinterpret_cast<const float4*>(w_acc + (w * G + h) * HS + d4 * 4), ew);
             }
         }
-        if (shared > 0 && planned) {
+        if (shared > 0) {
             const int r = (m - plan.begin[g_of]) * G + h, t = r / SH_ROWS;
             ShUnit unit;
             sh_unit(a, plan, g_of, kvh, t / 2, unit);
             const int subs = unit.tiles == 2 ? 1 : 2;            // pieces of a share that hold this row
-            const int b0 = unit.c0 / plan.quota + rank, b1 = (unit.c0 + unit.steps * unit.w - 1) / plan.quota + 1, n = b1 > b0 ? (b1 - b0 + n_cl - 1) / n_cl * subs : 0;
+            const int b0 = sh_quot(unit.c0, plan.quota) + rank, b1 = sh_quot(unit.c0 + unit.steps * unit.w - 1, plan.quota) + 1, n = b1 > b0 ? (b1 - b0 + n_cl - 1) / n_cl * subs : 0;
             const float2* norms = sh_norms(a) + r % SH_ROWS;
-            const float4* sums = sh_sums(a) + ((r % SH_ROWS) / 32 * LPH + d4) * 32 + r % 32;
+            const float4* sums = sh_sums(a) + r % SH_ROWS * LPH + d4;
             for (int c0 = 0; c0 < n; c0 += 32) {
                 const int c = c0 + lane, b = b0 + c / subs * n_cl, sub = c % subs;
                 int j0 = 0, j1 = 0;
                 if (c < n) sh_share(plan, unit, b, j0, j1);
-                const unsigned at = (unsigned)min((long long)(unit.index + b), a.n_pieces - 1) * 2 + (subs == 1 ? t & 1 : sub);
-                const float2 x = j1 - j0 > (subs == 1 ? 0 : sub) ? __ldcg(norms + (size_t)at * SH_ROWS) : make_float2(-INFINITY, 0.f);
-                const float e = weigh(x.x, x.y);
+                const unsigned at = (unsigned)(unit.index + b) * 2 + (subs == 1 ? t & 1 : sub);
+                const bool there = j1 - j0 > (subs == 1 ? 0 : sub);
+                const unsigned all = __ballot_sync(0xffffffffu, there);
+                const float2 x = there ? __ldcg(norms + (size_t)at * SH_ROWS) : make_float2(-INFINITY, 0.f);
                 const int live = min(32, n - c0);
-#pragma unroll 1
-                for (int i0 = 0; i0 < live; i0 += 8 * 32 / LPH) {
-                    float4 v[8];
-                    float f[8];
+                constexpr int BY = 32 / LPH, FLY = 16;           // pieces a load, loads in flight: the first ones together with the norms
+                float4 v[FLY];
+                auto fetch = [&](int i0) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int from = i0 + i * (32 / LPH) + half;
-                        const unsigned where = __shfl_sync(0xffffffffu, at, from & 31);
-                        f[i] = __shfl_sync(0xffffffffu, e, from & 31);
-                        if (from >= live) f[i] = 0.f;
-                        v[i] = f[i] != 0.f ? __ldcg(sums + (size_t)where * 4 * LPH * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int i = 0; i < FLY; i++) {
+                        const int from = (i0 + i * BY + half) & 31;
+                        const unsigned where = __shfl_sync(0xffffffffu, at, from);
+                        v[i] = all >> from & 1 && i0 + i * BY < live ? __ldcg(sums + (size_t)where * SH_ROWS * LPH) : make_float4(0.f, 0.f, 0.f, 0.f);
                     }
+                };
+                fetch(0);
+                const float e = weigh(x.x, x.y);
+#pragma unroll 1
+                for (int i0 = 0; i0 < live; i0 += FLY * BY) {
+                    if (i0 > 0) fetch(i0);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) put(v[i], f[i]);
+                    for (int i = 0; i < FLY; i++) {
+                        const int from = i0 + i * BY + half;
+                        const float f = __shfl_sync(0xffffffffu, e, from & 31);
+                        if (from < live && f != 0.f) put(v[i], f);      // (a piece in which nothing was seen may hold anything)
+                    }
                 }
             }
         }
@@ -812,7 +828,7 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32) shared_own_kernel(const __g
             O.z += __shfl_xor_sync(0xffffffffu, O.z, 16); O.w += __shfl_xor_sync(0xffffffffu, O.w, 16);
         }
         if (half == 0) *reinterpret_cast<float4*>(c_acc + h * HS + d4 * 4) = O;
-        if (lane == 0) { c_ml[h * 2] = M; c_ml[h * 2 + 1] = bad_s || !planned ? __int_as_float(0x7fffffff) : L; }
+        if (lane == 0) { c_ml[h * 2] = M; c_ml[h * 2 + 1] = bad_s ? __int_as_float(0x7fffffff) : L; }
     }
     if (n_cl > 1) cluster.sync();
     else __syncthreads();
@@ -845,7 +861,7 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32) shared_own_kernel(const __g
     if (n_cl > 1) cluster.sync();                                // nobody leaves while its sums are read
 }
 
-#define SH_SMEM ((2 + 2 * SH_STAGES) * SH_TILE_BYTES + 20 * 8)
+#define SH_SMEM ((2 + 2 * SH_STAGES) * SH_TILE_BYTES + 8 * 32 * SH_OUT_LD * 4 + 20 * 8)
 
 static size_t sh_own_smem(int head_size, int G) {
     const size_t ring = (size_t)SH_OWN_WARPS * (256 / head_size) * 2 * SH_OWN_TOK * head_size * 2;
@@ -861,7 +877,7 @@ static long long sh_pieces(long long M, int n_heads, int n_kv_heads) {
 
 extern "C" long long dl_shared_attention_scratch_bytes(int M, int n_heads, int n_kv_heads, int head_size) {
     if (M < 0 || n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads != 0 || head_size < 1) return 0;
-    return SH_PLAN_BYTES + sh_pieces(M, n_heads, n_kv_heads) * 2 * SH_ROWS * (8 + (long long)head_size * 4);
+    return sh_pieces(M, n_heads, n_kv_heads) * 2 * SH_ROWS * (8 + (long long)head_size * 4);
 }
 
 static int sh_map(CUtensorMap* map, const void* base, long long rows, int width) {
@@ -888,7 +904,7 @@ template <int HS> static int sh_launch(const ShArgs& a, int pdl, cudaStream_t st
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
-    cfg.gridDim = dim3(n_sms);
+    cfg.gridDim = dim3(a.shares);
     cfg.blockDim = dim3(SH_THREADS);
     cfg.dynamicSmemBytes = SH_SMEM;
     cfg.stream = stream;
@@ -929,7 +945,7 @@ extern "C" int dl_shared_attention(const float* q, long long ldq, int n_heads, i
     const long long cols = (long long)n_heads * head_size;
     if (ldq < cols || ldq % 4 != 0 || (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)scratch) & 15) != 0) { dl_set_error("dl_shared_attention: q, cache and scratch are aligned to 16 bytes, rows of q to 4 values"); return -1; }
     if (y_out != nullptr && (ldy < cols || (y_type != DL_KV8_F32 && y_type != DL_KV8_BF16 && y_type != DL_KV8_F16))) { dl_set_error("dl_shared_attention: y_out of type %d, row stride %lld", y_type, ldy); return -1; }
-    const ShArgs a = {q, ldq, (const __half*)k_cache, (const __half*)v_cache, pos, slot, block_table, groups, M, n_heads, n_kv_heads, n_slots, max_pages, n_pages, max_groups,
-                      (uint8_t*)scratch, sh_pieces(M, n_heads, n_kv_heads), xq_out, xh_out, out_mcap, y_out, ldy, y_type};
+    const ShArgs a = {q, ldq, (const __half*)k_cache, (const __half*)v_cache, pos, slot, block_table, groups, M, n_heads, n_kv_heads, n_heads / n_kv_heads, n_slots, max_pages, n_pages, max_groups,
+                      (uint8_t*)scratch, dl_device_sm_count(), sh_pieces(M, n_heads, n_kv_heads), xq_out, xh_out, out_mcap, y_out, ldy, y_type};
     return head_size == 128 ? sh_launch<128>(a, pdl, (cudaStream_t)stream) : sh_launch<64>(a, pdl, (cudaStream_t)stream);
 }
