@@ -52,6 +52,9 @@ class AppArgs:
     port: int = 9990
     temperature: float = 0.8
     topp: float = 0.9
+    topk: int = 0
+    minp: float = 0.0
+    samples: int = 1            # dllama inference: answers to the prompt, drawn on the GPU
     steps: int = 0
     seed: int = 0
     chat_template_type: int = T.CHAT_UNKNOWN
@@ -99,6 +102,9 @@ class AppArgs:
             elif name == "--steps": a.steps = int(value)
             elif name == "--temperature": a.temperature = float(value)
             elif name == "--topp": a.topp = float(value)
+            elif name == "--topk": a.topk = int(value)
+            elif name == "--minp": a.minp = float(value)
+            elif name == "--samples": a.samples = int(value)
             elif name == "--seed": a.seed = int(value)
             elif name == "--chat-template":
                 if value not in T.CHAT_NAMES:
@@ -147,6 +153,7 @@ Options:
   --model <path.m | model directory> --tokenizer <path.t> --prompt <text> --steps <n>
   --dtype {bfloat16,float32}   (model directories: config.json + model.safetensors)
   --buffer-float-type {f32,f16,q40,q80}   --max-seq-len <n>   --temperature <f> --topp <f> --seed <n>
+  --samples <n> --topk <n> --minp <f>   (inference, Q40 models on one GPU: n answers to the prompt, which is run and read once for all of them)
   --workers <host:port> ...   --port <n>   --chat-template {llama2,llama3,deepSeek3}
   --kv-cache {f16,q8}   (Q40 models on a GPU: tokens of a conversation in 16 or 8 bits)
   --max-batch <rows>  --n-slots <sequences>  --gpu-index <i>  --device {auto,cuda,cpu,cpu-oracle}

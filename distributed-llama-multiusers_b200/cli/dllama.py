@@ -86,6 +86,8 @@ def inference(ctx: InferenceContext):
         raise ValueError("The number of prompt tokens is greater than the sequence length")
     if n_in > a.steps:
         raise ValueError("The number of prompt tokens is greater than the number of steps")
+    if a.samples != 1 or a.topk > 0 or a.minp > 0:
+        return samples(ctx, input_tokens)
     inf = RootInference(ctx)
     chunk = min(a.n_batches, ctx.engine.max_rows)
     sent = recv = 0
@@ -143,6 +145,32 @@ def inference(ctx: InferenceContext):
     print("    nTokens: %d" % n_pred)
     if n_pred > 0 and pred_ms > 0:
         print("   tokens/s: %3.2f (%3.2f ms/tok)" % (n_pred * 1000 / pred_ms, pred_ms / n_pred))
+
+
+def samples(ctx: InferenceContext, prompt: List[int]):
+    """`inference --samples n`: n answers to the prompt, each up to its stop token (LlamaEngine.sample_many)."""
+    a, tok = ctx.args, ctx.tokenizer
+    if not hasattr(ctx.engine, "sample_many"):
+        raise ValueError("--samples, --topk and --minp need a Q40 model on a GPU")
+    if a.samples < 1:
+        raise ValueError("--samples: one or more are wanted")
+    count = min(ctx.header.seq_len, a.steps) - len(prompt)
+    if count < 1:
+        raise ValueError("The number of prompt tokens is not below the number of steps")
+    t0 = time.perf_counter()
+    drawn = ctx.engine.sample_many(prompt, a.samples, count, a.temperature, a.topk, a.topp, a.minp, a.seed)
+    ms = (time.perf_counter() - t0) * 1e3
+    for i, row in enumerate(drawn):
+        tok.reset_decoder()
+        text = ""
+        for t in row.tolist():
+            if t in tok.eos_token_ids:
+                break
+            text += tok.decode(t) or ""
+        print("🔶 Sample %d | %s%s" % (i, a.prompt, text), flush=True)
+    print("Prediction")
+    print("    nTokens: %d" % drawn.size)
+    print("   tokens/s: %3.2f (%3.2f ms/tok)" % (drawn.size * 1000 / ms, ms / drawn.size))
 
 
 def chat(ctx: InferenceContext):

@@ -115,7 +115,8 @@ struct Gen {
     void* sampler = nullptr;
     void* dec = nullptr;
     void* stops = nullptr;
-    float temperature = 0.f, topp = 0.f;
+    float temperature = 0.f, topp = 0.f, min_p = 0.f;
+    int top_k = 0;
     int n_prompt = 0, n_gen = 0;
     std::string text;               // non-streaming answers accumulate here
     const char* finish = nullptr;
@@ -132,6 +133,7 @@ struct Server {
     std::string chat_eos;
     int vocab = 0;
     float def_temp = 0.8f, def_topp = 0.9f;
+    bool filters = false;               // top_k and min_p can be served (dl_srv_set_filters)
     unsigned long long def_seed = 0;
     int max_default_tokens = 128;
     int max_waiting = 4096;             // admission queue bound (DLLAMA_MAX_WAITING): beyond it requests get 503
@@ -400,7 +402,8 @@ int parse_head(const std::string& in, HttpRequest& r) {
 struct Params {
     std::vector<std::string> roles, contents;
     int max_tokens = -1;
-    float temperature, topp;
+    float temperature, topp, min_p = 0.f;
+    int top_k = 0;
     unsigned long long seed;
     std::vector<std::string> stop;
     bool stream = false, include_usage = false;
@@ -442,6 +445,9 @@ bool parse_params(const Server* s, const Value& body, Params& p, std::string& er
     if (const Value* v = body.get("stream")) p.stream = v->truthy();
     if (num("temperature", d)) p.temperature = (float)d;
     if (num("top_p", d)) p.topp = (float)d;
+    if (num("top_k", d)) p.top_k = d >= 1.0 ? (int)std::min(d, 2147483647.0) : 0;
+    if (num("min_p", d)) p.min_p = (float)d;
+    if (err.empty() && (p.top_k > 0 || p.min_p > 0.f) && !s->filters) err = "`top_k` and `min_p` need the device sampler";
     if (const Value* v = body.get("seed")) {
         if (v->type == Value::NUM) p.seed = (unsigned long long)v->inum;
         else if (!v->is_null()) err = "`seed` must be a number";
@@ -520,6 +526,8 @@ void handle_completion(Server* s, Conn& c, const char* body, size_t n) {
     g.cid = new_completion_id(s);
     g.temperature = p.temperature;
     g.topp = p.topp;
+    g.top_k = p.top_k;
+    g.min_p = p.min_p;
     g.n_prompt = nt;
     g.t_submit = now_s();
     const unsigned long long seed = p.seed ? p.seed : (unsigned long long)g.id;
@@ -960,6 +968,23 @@ int dl_srv_next_batch(void* sv, int* tokens, int* pos, int* slots, int cap, int*
     }
     s->cancelled.resize(keep);
     return n;
+}
+
+// Whether requests may ask for top_k and min_p (the caller samples with dl_srv_batch_filters' settings); off until it is said.
+void dl_srv_set_filters(void* sv, int on) { ((Server*)sv)->filters = on != 0; }
+
+// top_k and min_p of the sampling rows of the batch last formed; returns how many rows have one of them on.
+int dl_srv_batch_filters(void* sv, int* top_k, float* min_p, int cap) {
+    auto* s = (Server*)sv;
+    std::lock_guard<std::mutex> g(s->mu);
+    int on = 0;
+    for (int i = 0; i < (int)s->batch_ids.size() && i < cap; i++) {
+        auto it = s->gens.find(s->batch_ids[i]);
+        top_k[i] = it == s->gens.end() ? 0 : it->second.top_k;
+        min_p[i] = it == s->gens.end() ? 0.f : it->second.min_p;
+        on += top_k[i] > 0 || min_p[i] > 0.f;
+    }
+    return on;
 }
 
 // CPU engines / DLLAMA_HOST_SAMPLER=1: sample the rows of the current batch on the host with each request's own

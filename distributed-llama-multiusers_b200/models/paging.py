@@ -36,6 +36,15 @@ class PageAllocator:
             self.free_pages.append(int(self.table[slot, i]))
         self.n_used[slot] = 0
 
+    def take(self, n: int) -> list:
+        """n pages out of the pool, of no sequence; give() returns them."""
+        if n > len(self.free_pages):
+            raise RuntimeError("KV cache exhausted")
+        return [self.free_pages.pop() for _ in range(n)]
+
+    def give(self, pages: list):
+        self.free_pages.extend(pages)
+
     def ensure(self, slot: int, n_tokens: int):
         need = (n_tokens + PAGE - 1) // PAGE
         if need > self.max_pages:

@@ -43,7 +43,7 @@ class ApiState:
         tokens = self.tok.encode(content, add_bos=True, add_special_tokens=True)
         max_tokens = p.max_tokens if p.max_tokens and p.max_tokens > 0 else self.max_default_tokens
         return GenerationRequest(prompt_tokens=tokens, max_tokens=max_tokens, temperature=p.temperature,
-                                 top_p=p.top_p, seed=p.seed, stop=p.stop)
+                                 top_p=p.top_p, seed=p.seed, stop=p.stop, top_k=p.top_k, min_p=p.min_p)
 
 
 def make_handler(state: ApiState):

@@ -17,6 +17,8 @@ class InferenceParams:
     stop: List[str] = field(default_factory=list)
     stream: bool = False
     seed: int = 0
+    top_k: int = 0                   # 0: off
+    min_p: float = 0.0               # 0: off
     include_usage: bool = False      # stream_options.include_usage: usage in the last SSE chunk (OpenAI)
 
 
@@ -44,6 +46,10 @@ def parse_inference_params(body: dict, defaults: InferenceParams) -> InferencePa
         p.temperature = float(body["temperature"])
     if body.get("top_p") is not None:
         p.top_p = float(body["top_p"])
+    if body.get("top_k") is not None:
+        p.top_k = max(0, min(int(body["top_k"]), (1 << 31) - 1))
+    if body.get("min_p") is not None:
+        p.min_p = float(body["min_p"])
     if body.get("seed") is not None:
         p.seed = int(body["seed"])
     if body.get("max_tokens") is not None:

@@ -35,6 +35,8 @@ class GenerationRequest:
     top_p: float = 0.9
     seed: int = 0
     stop: Sequence[str] = ()
+    top_k: int = 0                              # 0: off; with top_k or min_p the batch is drawn by ops.kernels.sample_tokens
+    min_p: float = 0.0                          # 0: off
     # filled by the engine
     id: int = -1
     out: "queue.Queue" = field(default_factory=queue.Queue)      # str deltas, then None
@@ -98,6 +100,8 @@ class BatchEngine:
             self._d_params = torch.zeros(3, R, dtype=torch.float32, device=dev)
             self._d_tok = torch.zeros(R, dtype=torch.int32, device=dev)
             self._h_tok = torch.zeros(R, dtype=torch.int32).pin_memory()
+            self._h_top_k, self._d_top_k = torch.zeros(R, dtype=torch.int32).pin_memory(), torch.zeros(R, dtype=torch.int32, device=dev)
+            self._h_min_p, self._d_min_p = torch.zeros(R, dtype=torch.float32).pin_memory(), torch.zeros(R, dtype=torch.float32, device=dev)
             self._logits_host = None
         else:
             self._logits_host = torch.empty(self.max_rows, engine.h.vocab_size, dtype=torch.float32)
@@ -106,6 +110,8 @@ class BatchEngine:
 
     # ---- client side (any thread) ------------------------------------------------------------------
     def submit(self, req: GenerationRequest) -> GenerationRequest:
+        if (req.top_k > 0 or req.min_p > 0) and not self._device_sampler:
+            raise ValueError("top_k and min_p need the device sampler")
         req.id = next(self._ids)
         req.t_submit = time.time()
         req._sampler = T.Sampler(self.engine.h.vocab_size, req.temperature, req.top_p, req.seed or req.id)
@@ -207,7 +213,15 @@ class BatchEngine:
                     hp[0, i], hp[1, i] = r.temperature, r.top_p
                     hp[2, i] = r._sampler.coin() if r.temperature != 0.0 else 0.0
             self._d_params.copy_(self._h_params, non_blocking=True)
-            self._sample_rows(logits[:n_s], self._d_params[0], self._d_params[1], self._d_params[2], self._d_tok)
+            if any(r is not None and (r.top_k > 0 or r.min_p > 0) for r in rows):
+                from ..ops import kernels as _K
+                for i, r in enumerate(rows):
+                    self._h_top_k[i], self._h_min_p[i] = (r.top_k, r.min_p) if r is not None else (0, 0.0)
+                self._d_top_k.copy_(self._h_top_k, non_blocking=True)
+                self._d_min_p.copy_(self._h_min_p, non_blocking=True)
+                _K.sample_tokens(logits, n_s, self._d_params[0], self._d_top_k, self._d_params[1], self._d_min_p, self._d_params[2], self._d_tok)
+            else:
+                self._sample_rows(logits[:n_s], self._d_params[0], self._d_params[1], self._d_params[2], self._d_tok)
             self._h_tok.copy_(self._d_tok, non_blocking=True)
             torch.cuda.current_stream().synchronize()
             self._check_waits()

@@ -69,6 +69,9 @@ class NativeApiServer:
                 self._sample_rows = _K.sample_rows
             self._d_params = torch.zeros(3, R, dtype=torch.float32, device=dev)
             self._d_tok = torch.zeros(R, dtype=torch.int32, device=dev)
+            self._h_top_k, self._d_top_k = pin(torch.zeros(R, dtype=torch.int32)), torch.zeros(R, dtype=torch.int32, device=dev)
+            self._h_min_p, self._d_min_p = pin(torch.zeros(R, dtype=torch.float32)), torch.zeros(R, dtype=torch.float32, device=dev)
+            self._L.dl_srv_set_filters(self._h, 1)
         else:
             self._logits_host = pin(torch.empty(R, engine.h.vocab_size, dtype=torch.float32))
         self._stop = threading.Event()
@@ -177,7 +180,13 @@ class NativeApiServer:
         elif self._device_sampler:
             logits = eng.forward(toks, pos, slots, logits_from=lf)
             self._d_params.copy_(self._h_params, non_blocking=True)
-            self._sample_rows(logits[:n_s], self._d_params[0], self._d_params[1], self._d_params[2], self._d_tok)
+            if L.dl_srv_batch_filters(h, self._h_top_k.data_ptr(), self._h_min_p.data_ptr(), R):
+                from ..ops import kernels as _K
+                self._d_top_k.copy_(self._h_top_k, non_blocking=True)
+                self._d_min_p.copy_(self._h_min_p, non_blocking=True)
+                _K.sample_tokens(logits, n_s, self._d_params[0], self._d_top_k, self._d_params[1], self._d_min_p, self._d_params[2], self._d_tok)
+            else:
+                self._sample_rows(logits[:n_s], self._d_params[0], self._d_params[1], self._d_params[2], self._d_tok)
             self._h_tok.copy_(self._d_tok, non_blocking=True)
             torch.cuda.current_stream().synchronize()
             self._check_waits()
