@@ -7,9 +7,9 @@
 // All of it happens or nothing: every CTA checks everything by itself (lengths are a few KB), and where something is wrong `status` says what, all
 // rows are left empty and nothing is taken.
 //
-// What bounds it: the chain of latencies (lengths, sums, free pages, table, rows), and for many requests the stores.  So one cluster does it all: each of its CTAs
-// forms all sums, for which a barrier in between would cost more, and writes its part; as all have read before one writes, lengths and the count
-// of taken pages may be updated in place.  A row finds its request by bisection over the sums in shared memory.
+// What bounds it: the chain of latencies (lengths, sums, free pages, table, rows), and for many requests the shared pages' copies.  So every CTA forms all sums, for which a barrier in between would cost
+// more, and writes its part of the results; a row finds its request by bisection over the sums in shared memory.  Where lengths and the count of taken pages are updated in place, one cluster does
+// it all: its CTAs have all read before one writes.  32 requests of a token each 5.4 us, 2001 requests with 22000 rows behind 250 shared pages 11.6 (27.8 by one cluster).
 #include "common.cuh"
 #include "smem_limit.cuh"
 
@@ -17,6 +17,7 @@
 #define PGT_PAGE 32
 #define PGT_MAX_REQUESTS 8192
 #define PGT_MAX_SEQS 131072
+#define PGT_MAX_CLUSTERS 8
 #define PGT_UNIT 128                   // shared pages that a warp copies at a time
 
 extern void dl_set_error(const char* fmt, ...);
@@ -46,7 +47,7 @@ __global__ void __launch_bounds__(PGT_THREADS) page_tables_kernel(const __grid_c
     extern __shared__ uint32_t sm[];
     __shared__ unsigned long long warp_sums[3][32];
     const int n = a.n, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int cta = blockIdx.x, ctas = gridDim.x;              // (the grid is one cluster)
+    const int cta = blockIdx.x, ctas = gridDim.x;              // (one cluster where results go in place)
     const int words = (a.n_seqs + 31) / 32;
     uint32_t* row_at = sm;                                     // [n + 1] rows, pages and units of shared pages ahead of a request
     uint32_t* page_at = row_at + n + 1;
@@ -186,11 +187,13 @@ extern "C" int dl_page_tables(int n, const int* held, const int* new_tokens, con
     static SmemLimit given;
     if (smem > 48 * 1024)
         if (const int rc = dl_smem_limit("dl_page_tables", page_tables_kernel, smem, given)) return rc;
-    // one CTA where a barrier among several would cost more than their stores gain
+    // one CTA where a barrier among several would cost more than their stores gain; clusters of eight for every 8192 rows (and requests with shared pages, each as so many) up to half of the SMs
     const long long work = (long long)M + (lead_seq ? 64ll * n : 0);
     const int ctas = work <= 2048 ? 1 : work <= 4096 ? 2 : work <= 8192 ? 4 : 8;
+    const bool in_place = held_out == held || taken_out == taken;
+    const int clusters = in_place || work <= 8192 ? 1 : (int)(work / 8192 < PGT_MAX_CLUSTERS ? work / 8192 : PGT_MAX_CLUSTERS);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
+    cfg.gridDim = dim3(ctas * clusters);
     cfg.blockDim = dim3(PGT_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t)stream;

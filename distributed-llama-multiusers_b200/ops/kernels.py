@@ -606,17 +606,26 @@ def page_tables(n: int, held: torch.Tensor, new: torch.Tensor, seq: torch.Tensor
         raise ValueError(f"{n} requests, {n_pages} pages: at most {TABLES_MAX_REQUESTS} and {1 << 26}")
     if (lead_seq is None) != (lead_pages is None):
         raise ValueError("lead_seq and lead_pages come together")
-    if any(t is None for t in (held, new, seq, free_pages, taken, pos, slot, status)):
-        raise ValueError("a tensor is missing")
-    M = pos.numel()
-    if M >= 1 << 31 or free_pages.numel() >= 1 << 31:
-        raise ValueError(f"{M} rows, {free_pages.numel()} free pages")
-    rc = cuda_lib().dl_page_tables(n, _on_device(held, _I32, n, d, "held"), _on_device(new, _I32, n, d, "new"), _on_device(seq, _I32, n, d, "seq"), block_table.data_ptr(), *block_table.shape,
-                                   _on_device(free_pages, _I32, 0, d, "free_pages"), free_pages.numel(), _on_device(taken, _I32, 1, d, "taken"), n_pages, M, _on_device(pos, _I32, M, d, "pos"),
-                                   _on_device(slot, _I32, M, d, "slot"), _on_device(line, _I32, M, d, "line"), _on_device(start, _I32, n + 1, d, "start"),
-                                   _on_device(held if held_out is None else held_out, _I32, n, d, "held_out"), _on_device(taken if taken_out is None else taken_out, _I32, 1, d, "taken_out"),
-                                   _on_device(status, _I32, 1, d, "status"), _on_device(lead_seq, _I32, n, d, "lead_seq"), _on_device(lead_pages, _I32, n, d, "lead_pages"), 1 if pdl else 0,
-                                   torch._C._cuda_getCurrentRawStream(d))
+    if held_out is None:
+        held_out = held
+    if taken_out is None:
+        taken_out = taken
+    try:                                          # (all that is wanted at once: one call for each tensor took 6 us of 12)
+        M, n_free = pos.numel(), free_pages.numel()
+        fits = (held.dtype is new.dtype is seq.dtype is free_pages.dtype is taken.dtype is pos.dtype is slot.dtype is status.dtype is held_out.dtype is taken_out.dtype is _I32
+                and held.get_device() == new.get_device() == seq.get_device() == free_pages.get_device() == taken.get_device() == pos.get_device() == slot.get_device()
+                == status.get_device() == held_out.get_device() == taken_out.get_device() == d
+                and held.numel() >= n and new.numel() >= n and seq.numel() >= n and held_out.numel() >= n and slot.numel() >= M and taken.numel() and taken_out.numel() and status.numel()
+                and held.is_contiguous() and new.is_contiguous() and seq.is_contiguous() and free_pages.is_contiguous() and pos.is_contiguous() and slot.is_contiguous()
+                and held_out.is_contiguous() and M < 1 << 31 and n_free < 1 << 31)
+    except AttributeError:
+        raise ValueError("a tensor is missing") from None
+    if not fits:
+        raise ValueError(f"{n} requests want contiguous int32 tensors beside the block table: held, new, seq and held_out of {n} values, slot of as many as pos, taken, taken_out and status of one")
+    rc = cuda_lib().dl_page_tables(n, held.data_ptr(), new.data_ptr(), seq.data_ptr(), block_table.data_ptr(), *block_table.shape, free_pages.data_ptr(), n_free, taken.data_ptr(), n_pages, M,
+                                   pos.data_ptr(), slot.data_ptr(), None if line is None else _on_device(line, _I32, M, d, "line"), None if start is None else _on_device(start, _I32, n + 1, d, "start"),
+                                   held_out.data_ptr(), taken_out.data_ptr(), status.data_ptr(), None if lead_seq is None else _on_device(lead_seq, _I32, n, d, "lead_seq"),
+                                   None if lead_pages is None else _on_device(lead_pages, _I32, n, d, "lead_pages"), 1 if pdl else 0, torch._C._cuda_getCurrentRawStream(d))
     if rc:
         check(rc, "dl_page_tables")
     lib.count_launch()
