@@ -190,7 +190,7 @@ extern "C" int dl_page_tables(int n, const int* held, const int* new_tokens, con
     // one CTA where a barrier among several would cost more than their stores gain; clusters of eight for every 8192 rows (and requests with shared pages, each as so many) up to half of the SMs
     const long long work = (long long)M + (lead_seq ? 64ll * n : 0);
     const int ctas = work <= 2048 ? 1 : work <= 4096 ? 2 : work <= 8192 ? 4 : 8;
-    const bool in_place = held_out == held || taken_out == taken;
+    const bool in_place = (held_out < held + n && held < held_out + n) || taken_out == taken;
     const int clusters = in_place || work <= 8192 ? 1 : (int)(work / 8192 < PGT_MAX_CLUSTERS ? work / 8192 : PGT_MAX_CLUSTERS);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas * clusters);

@@ -572,35 +572,28 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
             cut = sh.low[groups][0];
             for (int r = 1; r < ctas; r++) cut = fminf(cut, sh.low[groups][r]);
         }
-        if (cut > -CUDART_INF_F || a.vocab <= ST_LIST)
-            z.batches(z.warp * 128, z.count, THREADS * 4, [&](const float4 (&v)[ST_AHEAD], int i) {
-                unsigned mask = 0;
+        // (of rows with masked tokens, or of a k beyond the maxima: all that is not -inf, which has no weight, whatever k is)
+        const bool every = !(cut > -CUDART_INF_F);
+        const float least = every ? -3.402823466e38f : cut;
+        z.batches(z.warp * 128, z.count, THREADS * 4, [&](const float4 (&v)[ST_AHEAD], int i) {
+            unsigned mask = 0;
 #pragma unroll
-                for (int u = 0; u < ST_AHEAD; u++) {
-                    const int b = 4 * u;
-                    mask |= (v[u].x >= cut ? 1u << b : 0) | (v[u].y >= cut ? 2u << b : 0) | (v[u].z >= cut ? 4u << b : 0) | (v[u].w >= cut ? 8u << b : 0);
-                }
-                if (!(cut > -CUDART_INF_F)) {                    // (behind the slice it is -inf)
-                    mask = 0;
-#pragma unroll
-                    for (int u = 0; u < ST_AHEAD; u++) {
-                        const float x4[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-#pragma unroll
-                        for (int e = 0; e < 4; e++) mask |= x4[e] >= cut && i + u * THREADS * 4 + e < z.count ? 1u << (4 * u + e) : 0;
-                    }
-                }
-                z.push(mask, v, i, THREADS * 4);
-            });
+            for (int u = 0; u < ST_AHEAD; u++) {
+                const int b = 4 * u;
+                mask |= (v[u].x >= least ? 1u << b : 0) | (v[u].y >= least ? 2u << b : 0) | (v[u].z >= least ? 4u << b : 0) | (v[u].w >= least ? 8u << b : 0);
+            }
+            z.push(mask, v, i, THREADS * 4);
+        });
         z.collect();
         cluster.sync();
         if (rank == 0) {
             const unsigned found = sh.listed + sh.others;
             const int n = (int)min(found, (unsigned)ST_LIST);
-            const bool ok = found <= ST_LIST && n >= q.k;
+            const bool ok = found <= ST_LIST && (every || n >= q.k);
             if (tid < ctas) z.at(tid)->done = ok ? 1 : 0;       // (the others may leave)
             st_cluster_arrive();
             if (ok) {
-                const float per = cut > -CUDART_INF_F ? (float)(ST_BINS - 1) / (m - cut) : q.per / (ST_FINE / ST_BINS);      // (bins from the maximum to the least of the list; infinities: some bin, the same for equal ones)
+                const float per = !every ? (float)(ST_BINS - 1) / (m - cut) : q.per / (ST_FINE / ST_BINS);      // (bins from the maximum to the least of the list; infinities: some bin, the same for equal ones)
                 auto by_logit = [&](bool counts) {              // the list in the order of the logits, from the border on
                     return [&, counts](auto f) {
                         for (int i = tid; i < n; i += THREADS) {
@@ -619,8 +612,10 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
                     }
                     return z.sum(s);
                 };
-                z.select(true, by_logit(true), (u64)q.k);
-                border = sh.found;
+                if (q.k < n) {
+                    z.select(true, by_logit(true), (u64)q.k);
+                    border = sh.found;
+                }
                 if (q.by_p) {
                     z.select(true, by_logit(false), q.part(left(false)));
                     border = sh.found;

@@ -30,7 +30,6 @@
 #define SH_PAIR_COST 7                 // of a step with two tiles
 #define SH_ONE_COST 4                  // ... with one
 #define SH_LEAST_COST 8                // of a CTA's share: two steps of one tile
-#define SH_OWN_WARPS 4
 #define SH_OWN_TOK 16                  // tokens of a warp's turn
 #define SH_OWN_MAX_CTAS 8
 
@@ -197,7 +196,9 @@ DL_DEVINL float sh_load_rows(const float* mine, uint8_t* tile, int r0, Ready rea
 DL_DEVINL void sh_make_plan(const ShArgs& a, ShPlan& p, int* list, int (*red)[2]) {
     const int tid = threadIdx.x;
     const int n_thr = blockDim.x;
-    const int mine = tid < a.M ? sh_tokens(a, tid) : 0, mine2 = tid + n_thr < a.M ? sh_tokens(a, tid + n_thr) : 0;      // (asked for together with the list)
+    int mine[4];                                                 // (asked for together with the list)
+#pragma unroll
+    for (int i = 0; i < 4; i++) mine[i] = tid + i * n_thr < a.M ? sh_tokens(a, tid + i * n_thr) : 0;
     sh_fetch_groups(a, list);
     if (tid < 2 * SH_MAX_GROUPS) red[tid >> 1][tid & 1] = 0x7fffffff;
     __syncthreads();
@@ -206,11 +207,13 @@ DL_DEVINL void sh_make_plan(const ShArgs& a, ShPlan& p, int* list, int (*red)[2]
     for (int g = 0; g < n; g++) {
         sh_group(a, list, g, at, b, e, pages);
         int least = 0x7fffffff, first = 0x7fffffff;
-        for (int m = tid; m < e; m += n_thr) {
-            if (m < b) continue;
-            const int t = m == tid ? mine : m == tid + n_thr ? mine2 : sh_tokens(a, m);
-            if (t > 0) { least = min(least, t / SH_PAGE); first = min(first, m); }
-        }
+        auto see = [&](int m, int t) {
+            if (m >= b && m < e && t > 0) { least = min(least, t / SH_PAGE); first = min(first, m); }
+        };
+#pragma unroll
+        for (int i = 0; i < 4; i++) see(tid + i * n_thr, mine[i]);
+        for (int m = tid + 4 * n_thr; m < e; m += n_thr)
+            if (m >= b) see(m, sh_tokens(a, m));
         least = __reduce_min_sync(0xffffffffu, least);
         first = __reduce_min_sync(0xffffffffu, first);
         if ((tid & 31) == 0 && first != 0x7fffffff) { atomicMin(&red[g][0], least); atomicMin(&red[g][1], first); }
@@ -275,7 +278,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
         mbar_init(s_empty, 128);
         mbar_fence_init();
     }
-    if (warp == 0) tmem_alloc(tmem_holder, 512);
+    if (warp == 0) tmem_alloc(tmem_holder, 512);                 // (ahead of the wait: the block has the SM's registers, so that nothing it waits for can want tensor memory beside it)
     pdl_wait();                                                  // q, the rows' places and the cache come from earlier kernels
     pdl_launch_dependents();                                     // ... and are complete for the second launch, too, when it starts
     sh_make_plan(a, plan, list, red);
@@ -563,8 +566,8 @@ DL_DEVINL void sh_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32
 
 // grid (CTAs of a row's cluster, key/value heads, rows).  Rows of the MMAs: the query heads of the key/value head (16 at most); tokens 16 at a time, a ring of stages for each
 // warp.  Then every thread joins four values of a head over the warps and this CTA's pieces, and the cluster's CTAs over each other's.
-template <int HS>
-__global__ void __launch_bounds__(SH_OWN_WARPS * 32, 3) shared_own_kernel(const __grid_constant__ ShArgs a) {
+template <int HS, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 12 / WARPS) shared_own_kernel(const __grid_constant__ ShArgs a) {
     constexpr int ROWB = HS * 2, CH = ROWB / 16, HALF = SH_OWN_TOK * ROWB, ST = 256 / HS;      // bytes and 16-byte pieces of a line, bytes of a turn's K or V, stages
     constexpr int KS = HS / 16, NT = HS / 8, LPH = HS / 4;                                     // MMA steps of a score, tiles of an output, threads of a head in the join
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -575,8 +578,8 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32, 3) shared_own_kernel(const 
     const int rank = blockIdx.x, n_cl = gridDim.x, kvh = blockIdx.y, m = blockIdx.z;           // (a row of the grid is one cluster)
     const int G = a.rep;
     float* w_acc = reinterpret_cast<float*>(smem);              // [warps][G][HS], after the ring is done with
-    float* w_ml = w_acc + SH_OWN_WARPS * G * HS;                // [warps][G][2]
-    float* c_acc = w_ml + SH_OWN_WARPS * G * 2;                 // [G][HS] of the CTA
+    float* w_ml = w_acc + WARPS * G * HS;                // [warps][G][2]
+    float* c_acc = w_ml + WARPS * G * 2;                 // [G][HS] of the CTA
     float* c_ml = c_acc + G * HS;                               // [G][2]
     pdl_launch_dependents();
     if (tid == 0) bad_s = 0;
@@ -603,7 +606,7 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32, 3) shared_own_kernel(const 
     const int own = T > 0 ? n_pages - shared : 0, shares = max(1, min(n_cl, (own + 7) / 8)), per = (own + shares - 1) / shares;
     const int pg0 = shared + min(own, rank * per), pg1 = shared + (rank < shares ? min(own, rank * per + per) : 0);
     const int t_end = min(max(T, 0), pg1 * SH_PAGE);
-    const int n_turns = pg1 > pg0 ? (t_end - pg0 * SH_PAGE + SH_OWN_TOK - 1) / SH_OWN_TOK : 0, n_my = (n_turns - warp + SH_OWN_WARPS - 1) / SH_OWN_WARPS;      // warp w takes turns w, w + 4, ...
+    const int n_turns = pg1 > pg0 ? (t_end - pg0 * SH_PAGE + SH_OWN_TOK - 1) / SH_OWN_TOK : 0, n_my = (n_turns - warp + WARPS - 1) / WARPS;      // warp w takes turns w, w + 4, ...
     const int* bt = a.block_table + (size_t)(T > 0 ? slot : 0) * a.max_pages;
     const uint32_t ring = smem_u32(smem) + warp * (ST * 2 * HALF);
     float run_m[2] = {-INFINITY, -INFINITY}, run_l[2] = {0.f, 0.f};      // of heads g and g + 8; run_l: this lane's own tokens
@@ -616,7 +619,7 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32, 3) shared_own_kernel(const 
     if (n_my > 0) {
         auto page_at = [&](int i) {
             if (i >= n_my) return 0;
-            const int p = bt[pg0 + ((warp + SH_OWN_WARPS * i) >> 1)];
+            const int p = bt[pg0 + ((warp + WARPS * i) >> 1)];
             if ((unsigned)p < (unsigned)a.n_pages) return p;
             bad = true;
             return 0;
@@ -624,7 +627,7 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32, 3) shared_own_kernel(const 
         int my_page = page_at(lane);                             // the lanes hold the next 32 turns' page numbers
         const uint8_t *kc = reinterpret_cast<const uint8_t*>(a.k_cache), *vc = reinterpret_cast<const uint8_t*>(a.v_cache);
         auto load = [&](int i, int st, int page) {
-            const int turn = warp + SH_OWN_WARPS * i;
+            const int turn = warp + WARPS * i;
             const int left = t_end - pg0 * SH_PAGE - turn * SH_OWN_TOK;      // tokens from this turn on
             const size_t off = (((size_t)page * a.n_kv_heads + kvh) * SH_PAGE + (turn & 1) * SH_OWN_TOK) * (size_t)ROWB;
             const uint32_t dst = ring + st * (2 * HALF);
@@ -694,7 +697,7 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32, 3) shared_own_kernel(const 
                     sh_mma(c[1], qf[k], b[2], b[3]);
                 }
             }
-            const int left = t_end - pg0 * SH_PAGE - (warp + SH_OWN_WARPS * i) * SH_OWN_TOK;
+            const int left = t_end - pg0 * SH_PAGE - (warp + WARPS * i) * SH_OWN_TOK;
             uint32_t pa[4];
             float corr[2];
 #pragma unroll
@@ -760,7 +763,7 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32, 3) shared_own_kernel(const 
     __syncthreads();
     // A warp joins a head, a lane four of its values (heads of 64: half a warp every other piece): the warps' own parts, then this CTA's pieces of the group's pages (those of every n_cl-th share),
     // 32 maxima and sums at a time, and their values all in flight.
-    for (int h = warp; h < G; h += SH_OWN_WARPS) {
+    for (int h = warp; h < G; h += WARPS) {
         const int d4 = lane % LPH, half = lane / LPH;
         float M = -INFINITY, L = 0.f;
         float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -774,10 +777,10 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32, 3) shared_own_kernel(const 
             return e;
         };
         {
-            const bool mine = lane < SH_OWN_WARPS;
+            const bool mine = lane < WARPS;
             const float e = weigh(mine ? w_ml[(lane * G + h) * 2] : -INFINITY, mine ? w_ml[(lane * G + h) * 2 + 1] : 0.f);
 #pragma unroll
-            for (int w = 0; w < SH_OWN_WARPS; ++w) {
+            for (int w = 0; w < WARPS; ++w) {
                 const float ew = __shfl_sync(0xffffffffu, e, w);
                 if (half == 0 && ew != 0.f) put(*reinterpret_cast<const float4*>(w_acc + (w * G + h) * HS + d4 * 4), ew);
             }
@@ -833,7 +836,7 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32, 3) shared_own_kernel(const 
     if (n_cl > 1) cluster.sync();
     else __syncthreads();
     // blocks of 32 values, a warp each: over the CTAs of the cluster
-    for (int blk = rank * SH_OWN_WARPS + warp; blk < G * (HS / 32); blk += n_cl * SH_OWN_WARPS) {
+    for (int blk = rank * WARPS + warp; blk < G * (HS / 32); blk += n_cl * WARPS) {
         const int h = blk / (HS / 32), d = blk % (HS / 32) * 32 + lane;
         float M = -INFINITY, L = 0.f, O = 0.f;
         for (int r = 0; r < n_cl; r++) {
@@ -863,9 +866,9 @@ __global__ void __launch_bounds__(SH_OWN_WARPS * 32, 3) shared_own_kernel(const 
 
 #define SH_SMEM ((2 + 2 * SH_STAGES) * SH_TILE_BYTES + 8 * 32 * SH_OUT_LD * 4 + 20 * 8)
 
-static size_t sh_own_smem(int head_size, int G) {
-    const size_t ring = (size_t)SH_OWN_WARPS * (256 / head_size) * 2 * SH_OWN_TOK * head_size * 2;
-    const size_t join = (size_t)(SH_OWN_WARPS + 1) * G * (head_size + 2) * 4;
+static size_t sh_own_smem(int head_size, int G, int warps) {
+    const size_t ring = (size_t)warps * (256 / head_size) * 2 * SH_OWN_TOK * head_size * 2;
+    const size_t join = (size_t)(warps + 1) * G * (head_size + 2) * 4;
     return ring > join ? ring : join;
 }
 
@@ -894,10 +897,14 @@ template <int HS> static int sh_launch(const ShArgs& a, int pdl, cudaStream_t st
     WaitLimit limit;
     if (dl_wait_limit("dl_shared_attention", &limit) != 0) return -1;
     const int G = a.n_heads / a.n_kv_heads, n_sms = dl_device_sm_count();
-    static SmemLimit given, given_own;
-    const size_t own_smem = sh_own_smem(HS, G);
+    // Many rows: two warps for each, so that an SM has six of them at work: what bounds a row are its latencies, one behind the other
+    const bool many = (long long)a.M * a.n_kv_heads > 3ll * n_sms;
+    const int warps = many ? 2 : 4;
+    auto* own_kernel = many ? shared_own_kernel<HS, 2> : shared_own_kernel<HS, 4>;
+    static SmemLimit given, given_own[2];
+    const size_t own_smem = sh_own_smem(HS, G, warps);
     if (const int rc = dl_smem_limit("dl_shared_attention", shared_attention_kernel<HS>, SH_SMEM, given)) return rc;
-    if (const int rc = dl_smem_limit("dl_shared_attention", shared_own_kernel<HS>, own_smem, given_own)) return rc;
+    if (const int rc = dl_smem_limit("dl_shared_attention", own_kernel, own_smem, given_own[many])) return rc;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -918,9 +925,9 @@ template <int HS> static int sh_launch(const ShArgs& a, int pdl, cudaStream_t st
         attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
         cfg.numAttrs = 2;
         cfg.gridDim = dim3(ctas, a.n_kv_heads, a.M);
-        cfg.blockDim = dim3(SH_OWN_WARPS * 32);
+        cfg.blockDim = dim3(warps * 32);
         cfg.dynamicSmemBytes = own_smem;
-        e = cudaLaunchKernelEx(&cfg, shared_own_kernel<HS>, a);
+        e = cudaLaunchKernelEx(&cfg, own_kernel, a);
     }
     if (e != cudaSuccess) { dl_set_error("dl_shared_attention launch: %s", cudaGetErrorString(e)); return -(int)e; }
     return 0;

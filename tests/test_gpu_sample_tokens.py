@@ -184,3 +184,30 @@ def test_captured_and_replayed_and_beside_itself():
             cc = c.cpu().numpy()
             f = [v.cpu().numpy() for v in a]
             assert out.tolist() == [oracle(xs[m], f[0][m], f[1][m], f[2][m], f[3][m], cc[m])[0] for m in range(24)]
+
+
+@pytest.mark.parametrize("left", [3, 200, 5000, 9000])
+def test_rows_of_which_a_mask_leaves_few(left):
+    """A grammar's mask over a large vocabulary: as many tokens as the list takes, and more; k below, at and above what is left."""
+    rng = np.random.default_rng(left)
+    x = np.full((8, 50000), -np.inf)
+    for m in range(8):
+        x[m, rng.choice(50000, left, replace=False)] = rng.standard_normal(left) * 3
+    check(torch.from_numpy(x).float().cuda(), [0.8] * 8, [1, left - 1, left, left + 1, 40, 2000, 49999, 7], [0.0, 0.9, 0.5, 0.99, 0.0, 0.9, 0.3, 0.0], [0.0, 0.0, 0.1, 0.0] * 2, rng.random(8).astype(np.float32).tolist())
+
+
+@pytest.mark.parametrize("order", [1, -1])
+def test_sorted_rows(order):
+    """The best tokens all in one place: the partial maxima say little."""
+    rng = np.random.default_rng(21)
+    x = np.sort(rng.standard_normal((9, 128256)) * 3, 1)[:, ::order].copy()
+    check(torch.from_numpy(x).float().cuda(), [0.7, 1.0, 1.3] * 3, [50, 0, 300, 0, 1, 20, 0, 3000, 100000], [0.9, 0.95, 0.0, 0.5, 0.9, 0.99, 0.999, 0.9, 0.8], [0.0, 0.0, 0.05] * 3,
+          rng.random(9).astype(np.float32).tolist())
+
+
+def test_rows_with_large_nuclei_in_16_bits():
+    """Nuclei of tens of thousands of tokens, whose logits have a few hundred values."""
+    rng = np.random.default_rng(22)
+    x = torch.from_numpy(rng.standard_normal((12, 128256)) * np.array([[0.3], [1.0], [2.2]] * 4)).cuda()
+    for dtype in (torch.bfloat16, torch.float16):
+        check(x.to(dtype), [1.0, 1.3, 0.7] * 4, [0] * 12, [0.9, 0.99, 0.999, 0.5] * 3, [0.0] * 9 + [0.01] * 3, rng.random(12).astype(np.float32).tolist())
