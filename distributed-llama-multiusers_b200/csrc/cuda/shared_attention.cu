@@ -137,6 +137,9 @@ DL_DEVINL void sh_share(const ShPlan& p, const ShUnit& u, int b, int& j0, int& j
 // the exponent field of the power of two that brings a row's largest value (its bits) to 2^8 .. 2^9; its inverse has 254 less that
 DL_DEVINL unsigned sh_up(unsigned most) { return most == 0 ? 127u : min(262u - (most >> 23), 250u); }
 
+// a barrier of the eight softmax warps
+template <int ID> DL_DEVINL void sh_bar() { asm volatile("bar.sync %0, 256;" ::"n"(ID) : "memory"); }
+
 struct ShItem {
     int kvh, row0, rows, begin, slot, pages, j0, J, tiles, piece;      // row0: first stacked row; rows: stacked rows of the group
 };
@@ -246,6 +249,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
     uint8_t* q_s = smem;                                        // [2] query tiles
     uint8_t* k_s = q_s + 2 * SH_TILE_BYTES;                     // [2] K tiles (tokens x head dim, K-major)
     uint8_t* v_s = k_s + SH_STAGES * SH_TILE_BYTES;             // [2] V tiles (tokens x head dim, MN-major for P V)
+    __shared__ float2 ml_s[SH_ROWS];                            // maxima and sums of the second place
     float* out_s = reinterpret_cast<float*>(v_s + SH_STAGES * SH_TILE_BYTES);      // [8 warps][32][SH_OUT_LD] f32: sums on their way out
     uint64_t* bars = reinterpret_cast<uint64_t*>(out_s + 8 * 32 * SH_OUT_LD);
     uint64_t* k_full = bars;             // [2] transaction bytes of the step's K copies
@@ -316,7 +320,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
         }
         return false;
     };
-    // A single tile takes both places, too: its steps in turn, so that the softmax of one step runs beside the next one's (two pieces; a step took 1.9 us in one place, 1.6 for two tiles).  Step j of place t?
+    // A single tile takes both places, too: its steps in turn, so that the softmax of one step runs beside the next one's (a step took 1.9 us in one place, 1.6 for two tiles).  Step j of place t?
     auto on = [](const ShItem& it, int t, int j) { return j < it.J && (it.tiles == 2 || (j & 1) == t); };
     // TMEM columns: one buffer of scores at 0, which the tiles take in turn; probabilities at 128, of 64 columns for each tile; outputs at 256 + 128 t
     if (warp < 8) {
@@ -412,6 +416,26 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
             // the largest weight is 1 or more; where it is not, a score was no number.  No score at all above -inf: nothing to add
             l = m_used == -INFINITY ? 0.f : l >= 0x1p-13f && !bad_s && !gave_up_s ? l : __int_as_float(0x7fffffff);
             if (bad_s || gave_up_s) l = __int_as_float(0x7fffffff);
+            // the two places of one tile have seen different steps of the same rows: the first one joins them (both lie in the same lanes of tensor memory)
+            const bool pair = it.tiles == 1 && it.J > 1;
+            float e0 = 1.f, e1 = 0.f;
+            if (pair) {
+                if (t == 1) {
+                    ml_s[row] = make_float2(m_used, l);
+                    tc_fence_before();
+                    sh_bar<1>();                                 // place 1 is complete
+                    sh_bar<2>();                                 // ... and read
+                    continue;
+                }
+                sh_bar<1>();
+                tc_fence_after();
+                const float2 o1 = ml_s[row];
+                const float top = fmaxf(l != 0.f ? m_used : -INFINITY, o1.y != 0.f ? o1.x : -INFINITY), ref = top == -INFINITY ? 0.f : top;
+                e0 = l != 0.f ? pt_ex2(m_used - ref) : 0.f;
+                e1 = o1.y != 0.f ? pt_ex2(o1.x - ref) : 0.f;
+                l = l * e0 + o1.y * e1;
+                m_used = top;
+            }
             const size_t at = (size_t)it.piece * 2 + t;
             sh_norms(a)[at * SH_ROWS + row] = make_float2(m_used, l);
             // 16 columns of the warp's rows at a time, then as many lanes along a row (a thread along its own row: 5 us for 128 of them)
@@ -420,9 +444,17 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
             const int live = it.rows - (it.row0 + (it.tiles == 2 ? t * SH_ROWS : 0) + quarter * 32);      // rows of this warp that are there
 #pragma unroll 1
             for (int ch = 0; ch < HS / 16; ch++) {
-                uint32_t o[16];
+                uint32_t o[16], p[16];
                 tmem_ld_32x32b_x16(T_O + ch * 16, o);
+                if (pair) tmem_ld_32x32b_x16(T_O + 128 + ch * 16, p);
                 tmem_ld_wait();
+                if (pair) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {               // (a place in which nothing was seen may hold anything)
+                        const float x = e0 != 0.f ? __uint_as_float(o[e]) * e0 : 0.f;
+                        o[e] = __float_as_uint(e1 != 0.f ? fmaf(__uint_as_float(p[e]), e1, x) : x);
+                    }
+                }
                 __syncwarp();
 #pragma unroll
                 for (int e = 0; e < 16; e += 4)
@@ -435,6 +467,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
                 }
             }
             tc_fence_before();                                   // the next item's P V may write the output (behind p_full)
+            if (pair) sh_bar<2>();
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
@@ -789,16 +822,15 @@ __global__ void __launch_bounds__(WARPS * 32, 12 / WARPS) shared_own_kernel(cons
             const int r = (m - plan.begin[g_of]) * G + h, t = r / SH_ROWS;
             ShUnit unit;
             sh_unit(a, plan, g_of, kvh, t / 2, unit);
-            const int subs = unit.tiles == 2 ? 1 : 2;            // pieces of a share that hold this row
-            const int b0 = sh_quot(unit.c0, plan.quota) + rank, b1 = sh_quot(unit.c0 + unit.steps * unit.w - 1, plan.quota) + 1, n = b1 > b0 ? (b1 - b0 + n_cl - 1) / n_cl * subs : 0;
+            const int b0 = sh_quot(unit.c0, plan.quota) + rank, b1 = sh_quot(unit.c0 + unit.steps * unit.w - 1, plan.quota) + 1, n = b1 > b0 ? (b1 - b0 + n_cl - 1) / n_cl : 0;
             const float2* norms = sh_norms(a) + r % SH_ROWS;
             const float4* sums = sh_sums(a) + r % SH_ROWS * LPH + d4;
             for (int c0 = 0; c0 < n; c0 += 32) {
-                const int c = c0 + lane, b = b0 + c / subs * n_cl, sub = c % subs;
+                const int c = c0 + lane, b = b0 + c * n_cl;
                 int j0 = 0, j1 = 0;
                 if (c < n) sh_share(plan, unit, b, j0, j1);
-                const unsigned at = (unsigned)(unit.index + b) * 2 + (subs == 1 ? t & 1 : sub);
-                const bool there = j1 - j0 > (subs == 1 ? 0 : sub);
+                const unsigned at = (unsigned)(unit.index + b) * 2 + (t & 1);
+                const bool there = j1 > j0;
                 const unsigned all = __ballot_sync(0xffffffffu, there);
                 const float2 x = there ? __ldcg(norms + (size_t)at * SH_ROWS) : make_float2(-INFINITY, 0.f);
                 const int live = min(32, n - c0);
