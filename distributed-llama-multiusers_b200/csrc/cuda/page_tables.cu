@@ -10,6 +10,7 @@
 // What bounds it: the chain of latencies (lengths, sums, free pages, table, rows), and for many requests the shared pages' copies.  So every CTA forms all sums, for which a barrier in between would cost
 // more, and writes its part of the results; a row finds its request by bisection over the sums in shared memory.  Where lengths and the count of taken pages are updated in place, one cluster does
 // it all: its CTAs have all read before one writes.  32 requests of a token each 5.4 us, 2001 requests with 22000 rows behind 250 shared pages 11.6 (27.8 by one cluster).
+#include "../../../include/dllama_b200.h"
 #include "common.cuh"
 #include "smem_limit.cuh"
 
@@ -22,7 +23,6 @@
 
 extern void dl_set_error(const char* fmt, ...);
 
-enum { PGT_BAD_LENGTH = 1, PGT_BAD_SEQ = 2, PGT_BAD_LEAD = 4, PGT_NO_PAGES = 8, PGT_BAD_PAGE = 16, PGT_NO_ROWS = 32 };
 
 struct PgtArgs {
     const int *held, *new_tokens, *seq, *lead_seq, *lead_pages;
@@ -69,12 +69,12 @@ __global__ void __launch_bounds__(PGT_THREADS) page_tables_kernel(const __grid_c
         const int h = a.held[i], c = a.new_tokens[i], s = a.seq[i], l = leads ? a.lead_pages[i] : 0;
         held[i] = h;
         seq[i] = s;
-        if (h < 0 || c < 0 || (long long)h + c > (long long)a.max_pages * PGT_PAGE) { bad |= PGT_BAD_LENGTH; continue; }
+        if (h < 0 || c < 0 || (long long)h + c > (long long)a.max_pages * PGT_PAGE) { bad |= DL_TABLES_BAD_LENGTH; continue; }
         const bool lead_ok = l >= 0 && (long long)l * PGT_PAGE <= h && (l == 0 || (unsigned)a.lead_seq[i] < (unsigned)a.n_seqs);
-        if (!lead_ok) bad |= PGT_BAD_LEAD;
-        if ((unsigned)s >= (unsigned)a.n_seqs) bad |= PGT_BAD_SEQ;
+        if (!lead_ok) bad |= DL_TABLES_BAD_LEAD;
+        if ((unsigned)s >= (unsigned)a.n_seqs) bad |= DL_TABLES_BAD_SEQ;
         else {
-            if (atomicOr(&used[s >> 5], 1u << (s & 31)) >> (s & 31) & 1) bad |= PGT_BAD_SEQ;
+            if (atomicOr(&used[s >> 5], 1u << (s & 31)) >> (s & 31) & 1) bad |= DL_TABLES_BAD_SEQ;
             if (lead_ok && l > 0 && a.lead_seq[i] != s) atomicOr(&led[s >> 5], 1u << (s & 31));
         }
         sum[0] += c;
@@ -116,21 +116,21 @@ __global__ void __launch_bounds__(PGT_THREADS) page_tables_kernel(const __grid_c
         ahead[2] += l > 0 ? (l + PGT_UNIT - 1) / PGT_UNIT : 0;
         if (l > 0 && bad == 0) {                   // pages of a row that gets its own from another in this call
             const int t = a.lead_seq[i];
-            if (t != seq[i] && (led[t >> 5] >> (t & 31) & 1)) bad |= PGT_BAD_LEAD;
+            if (t != seq[i] && (led[t >> 5] >> (t & 31) & 1)) bad |= DL_TABLES_BAD_LEAD;
         }
     }
     if (tid == 0) {
         row_at[n] = (uint32_t)total[0];
         page_at[n] = (uint32_t)total[1];
         unit_at[n] = (uint32_t)total[2];
-        if (total[0] > (unsigned long long)a.M) bad |= PGT_NO_ROWS;
-        if (taken < 0 || (unsigned long long)taken + total[1] > (unsigned long long)a.n_free) bad |= PGT_NO_PAGES;
+        if (total[0] > (unsigned long long)a.M) bad |= DL_TABLES_NO_ROWS;
+        if (taken < 0 || (unsigned long long)taken + total[1] > (unsigned long long)a.n_free) bad |= DL_TABLES_NO_PAGES;
     }
     if (taken >= 0 && total[1] <= (unsigned long long)a.n_free && (unsigned long long)taken + total[1] <= (unsigned long long)a.n_free)
         for (int j = tid; j < (int)total[1]; j += PGT_THREADS)
-            if ((unsigned)a.free_pages[taken + j] >= (unsigned)a.n_pages) bad |= PGT_BAD_PAGE;
+            if ((unsigned)a.free_pages[taken + j] >= (unsigned)a.n_pages) bad |= DL_TABLES_BAD_PAGE;
 #pragma unroll
-    for (int b = 1; b <= PGT_NO_ROWS; b <<= 1) if (__syncthreads_or(bad & b)) bad |= b;
+    for (int b = 1; b <= DL_TABLES_NO_ROWS; b <<= 1) if (__syncthreads_or(bad & b)) bad |= b;
     // every CTA has read what one of them may write
     if (ctas > 1) { cg::this_cluster().sync(); }
     const int n_rows = bad ? 0 : (int)total[0], n_new = bad ? 0 : (int)total[1], n_units = bad ? 0 : (int)total[2];
@@ -208,4 +208,13 @@ extern "C" int dl_page_tables(int n, const int* held, const int* new_tokens, con
     const cudaError_t e = cudaLaunchKernelEx(&cfg, page_tables_kernel, a);
     if (e != cudaSuccess) { dl_set_error("dl_page_tables launch: %s", cudaGetErrorString(e)); return -(int)e; }
     return 0;
+}
+
+extern "C" int dl_page_tables_packed(const DlPageTables* a) {
+    if (!a) { dl_set_error("dl_page_tables: a null pointer"); return -1; }
+    const long long counts[] = {a->n, a->n_seqs, a->max_pages, a->n_free, a->n_pages, a->M};
+    for (long long c : counts)
+        if (c != (int)c) { dl_set_error("dl_page_tables: a count of %lld", c); return -1; }
+    return dl_page_tables((int)a->n, a->held, a->new_tokens, a->seq, a->table, (int)a->n_seqs, (int)a->max_pages, a->free_pages, (int)a->n_free, a->taken, (int)a->n_pages, (int)a->M, a->pos, a->slot, a->line,
+                          a->start, a->held_out, a->taken_out, a->status, a->lead_seq, a->lead_pages, a->pdl != 0, a->stream);
 }

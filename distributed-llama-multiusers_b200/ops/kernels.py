@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import struct
 from typing import List, NamedTuple, Optional, Sequence
 
 import torch
@@ -589,6 +590,7 @@ def _max_vocab() -> int:
 
 TABLES_BAD_LENGTH, TABLES_BAD_SEQ, TABLES_BAD_LEAD, TABLES_NO_PAGES, TABLES_BAD_PAGE, TABLES_NO_ROWS = 1, 2, 4, 8, 16, 32      # bits of page_tables' status
 TABLES_MAX_REQUESTS, TABLES_MAX_SEQS = 8192, 131072
+_TABLES_ARGS = struct.Struct("23q")                 # DlPageTables
 
 
 def page_tables(n: int, held: torch.Tensor, new: torch.Tensor, seq: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, taken: torch.Tensor, n_pages: int, pos: torch.Tensor,
@@ -599,33 +601,37 @@ def page_tables(n: int, held: torch.Tensor, new: torch.Tensor, seq: torch.Tensor
     pos, slot (and line = page * 32 + place) list the requests' new tokens one behind the other, start [n + 1] where each begins; the places behind the last one are -1, 0, -1.  held and
     taken go on to held_out and taken_out (None: in place).  status: 0, or bits TABLES_*: then all rows are empty, nothing is taken and the table is as it was.  No row of the table in two
     requests, no request's own row a lead while its first pages are another's (both are noticed)."""
-    d = _launching(block_table, "block_table")
-    if block_table.dim() != 2 or block_table.dtype is not _I32 or not block_table.is_contiguous() or not 1 <= block_table.shape[0] <= TABLES_MAX_SEQS or block_table.shape[1] < 1:
-        raise ValueError(f"block_table {tuple(block_table.shape)} of {block_table.dtype}: contiguous int32 [1 to {TABLES_MAX_SEQS} sequences][pages] is wanted")
-    if not 0 <= n <= TABLES_MAX_REQUESTS or not 1 <= n_pages <= 1 << 26:
-        raise ValueError(f"{n} requests, {n_pages} pages: at most {TABLES_MAX_REQUESTS} and {1 << 26}")
-    if (lead_seq is None) != (lead_pages is None):
-        raise ValueError("lead_seq and lead_pages come together")
-    if held_out is None:
-        held_out = held
-    if taken_out is None:
-        taken_out = taken
-    try:                                          # (all that is wanted at once: one call for each tensor took 6 us of 12)
+    # (all that is wanted at once, and the arguments in one piece: a call for each tensor and ctypes' conversions took 8 us of 12)
+    try:
+        d = _launching(block_table, "block_table")
+        n_seqs, max_pages = block_table.shape
         M, n_free = pos.numel(), free_pages.numel()
-        fits = (held.dtype is new.dtype is seq.dtype is free_pages.dtype is taken.dtype is pos.dtype is slot.dtype is status.dtype is held_out.dtype is taken_out.dtype is _I32
+        if held_out is None:
+            held_out = held
+        if taken_out is None:
+            taken_out = taken
+        fits = (block_table.dtype is held.dtype is new.dtype is seq.dtype is free_pages.dtype is taken.dtype is pos.dtype is slot.dtype is status.dtype is held_out.dtype is taken_out.dtype is _I32
                 and held.get_device() == new.get_device() == seq.get_device() == free_pages.get_device() == taken.get_device() == pos.get_device() == slot.get_device()
                 == status.get_device() == held_out.get_device() == taken_out.get_device() == d
                 and held.numel() >= n and new.numel() >= n and seq.numel() >= n and held_out.numel() >= n and slot.numel() >= M and taken.numel() and taken_out.numel() and status.numel()
-                and held.is_contiguous() and new.is_contiguous() and seq.is_contiguous() and free_pages.is_contiguous() and pos.is_contiguous() and slot.is_contiguous()
-                and held_out.is_contiguous() and M < 1 << 31 and n_free < 1 << 31)
-    except AttributeError:
+                and block_table.is_contiguous() and held.is_contiguous() and new.is_contiguous() and seq.is_contiguous() and free_pages.is_contiguous() and pos.is_contiguous()
+                and slot.is_contiguous() and held_out.is_contiguous() and 1 <= n_seqs <= TABLES_MAX_SEQS and max_pages >= 1 and 0 <= n <= TABLES_MAX_REQUESTS and 1 <= n_pages <= 1 << 26
+                and M < 1 << 31 and n_free < 1 << 31
+                and (line is None or line.dtype is _I32 and line.get_device() == d and line.numel() >= M and line.is_contiguous())
+                and (start is None or start.dtype is _I32 and start.get_device() == d and start.numel() > n and start.is_contiguous())
+                and ((lead_seq is None and lead_pages is None) or lead_seq.dtype is lead_pages.dtype is _I32 and lead_seq.get_device() == lead_pages.get_device() == d
+                     and lead_seq.numel() >= n and lead_pages.numel() >= n and lead_seq.is_contiguous() and lead_pages.is_contiguous()))
+    except (AttributeError, TypeError):
         raise ValueError("a tensor is missing") from None
     if not fits:
-        raise ValueError(f"{n} requests want contiguous int32 tensors beside the block table: held, new, seq and held_out of {n} values, slot of as many as pos, taken, taken_out and status of one")
-    rc = cuda_lib().dl_page_tables(n, held.data_ptr(), new.data_ptr(), seq.data_ptr(), block_table.data_ptr(), *block_table.shape, free_pages.data_ptr(), n_free, taken.data_ptr(), n_pages, M,
-                                   pos.data_ptr(), slot.data_ptr(), None if line is None else _on_device(line, _I32, M, d, "line"), None if start is None else _on_device(start, _I32, n + 1, d, "start"),
-                                   held_out.data_ptr(), taken_out.data_ptr(), status.data_ptr(), None if lead_seq is None else _on_device(lead_seq, _I32, n, d, "lead_seq"),
-                                   None if lead_pages is None else _on_device(lead_pages, _I32, n, d, "lead_pages"), 1 if pdl else 0, torch._C._cuda_getCurrentRawStream(d))
+        raise ValueError(f"{n} requests (at most {TABLES_MAX_REQUESTS}) over block_table {tuple(block_table.shape)} [1 to {TABLES_MAX_SEQS} sequences][pages] of {n_pages} pages (at most {1 << 26}): contiguous "
+                         f"int32 tensors on one device are wanted, held, new, seq and held_out of {n} values (lead_seq and lead_pages too, together), start of one more, slot and line of as many as pos, taken, "
+                         f"taken_out and status of one")
+    rc = cuda_lib().dl_page_tables_packed(_TABLES_ARGS.pack(
+        n, held.data_ptr(), new.data_ptr(), seq.data_ptr(), block_table.data_ptr(), n_seqs, max_pages, free_pages.data_ptr(), n_free, taken.data_ptr(), n_pages, M, pos.data_ptr(), slot.data_ptr(),
+        0 if line is None else line.data_ptr(), 0 if start is None else start.data_ptr(), held_out.data_ptr(), taken_out.data_ptr(), status.data_ptr(),
+        0 if lead_seq is None else lead_seq.data_ptr(), 0 if lead_pages is None else lead_pages.data_ptr(), 1 if pdl else 0,
+        torch._C._cuda_getCurrentRawStream(d)))
     if rc:
         check(rc, "dl_page_tables")
     lib.count_launch()

@@ -177,11 +177,12 @@ def cuda_lib():
     L.dl_sample_rows.argtypes = [vp, i32, i32, i32, vp, vp, vp, vp, vp]
     L.dl_sample_tokens.argtypes = [vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, vp, vp, i32, vp]
     L.dl_page_tables.argtypes = [i32, vp, vp, vp, vp, i32, i32, vp, i32, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, vp]
+    L.dl_page_tables_packed.argtypes = [C.c_char_p]
     L.dl_sample_tokens_max_vocab.argtypes = []
     L.dl_shared_attention.argtypes = [vp, i64, i32, i32, i32, vp, vp, i32, vp, vp, vp, i32, i32, i32, vp, i32, vp, i64, vp, vp, i32, vp, i64, i32, i32, vp]
     L.dl_shared_attention.restype = i32
     L.dl_shared_attention_scratch_bytes.argtypes, L.dl_shared_attention_scratch_bytes.restype = [i32, i32, i32, i32], i64
-    for name in ("dl_sample_tokens", "dl_page_tables", "dl_sample_tokens_max_vocab"):
+    for name in ("dl_sample_tokens", "dl_page_tables", "dl_page_tables_packed", "dl_sample_tokens_max_vocab"):
         getattr(L, name).restype = i32
     L.dl_gemm_f32.argtypes = [vp, i32, i32, i64, vp, i32, i32, vp, i32, i32, vp]
     L.dl_gemv_q40.argtypes = [vp, i32, i32, vp, i32, i32, i32, i32, C.POINTER(DlNormProlog), C.POINTER(DlEpilogue), i32, vp]

@@ -148,7 +148,8 @@ int dl_sample_tokens(const void* logits, int type, int M, int vocab, long long l
  *   table[seq][k] = table[lead_seq[i]][k], k < lead_pages[i]: a shared prompt's pages, whole ones of the tokens held (32 lead_pages <= held); that row may be a request's, too, but none whose own
  *                   first pages are another's; lead_seq and lead_pages: both NULL: none
  *   pos[R + j] = held + j, slot[R + j] = seq, line[R + j] = 32 table[seq][pos / 32] + pos % 32 (-1 where that is no page); the other ones of the M rows: -1, 0, -1
- *   start[i] = R (n + 1 of them), held_out = held + new, *taken_out = *taken + all pages taken.  held_out and taken_out may be held and taken.  line, start: NULL or wanted.
+ *   start[i] = R (n + 1 of them), held_out = held + new, *taken_out = *taken + all pages taken.  line, start: NULL or wanted.  What is written lies apart from what is read, but held_out and
+ *                   taken_out may be held and taken.
  * *status: 0, or what was wrong, bits added: then all rows are empty, start is 0, nothing is taken and the table is as it was.
  * At most 8192 requests, 131072 table rows. */
 enum { DL_TABLES_BAD_LENGTH = 1,   /* below zero, or more tokens than a table row has pages for */
@@ -157,6 +158,22 @@ enum { DL_TABLES_BAD_LENGTH = 1,   /* below zero, or more tokens than a table ro
 int dl_page_tables(int n, const int* held, const int* new_tokens, const int* seq, int* table, int n_seqs, int max_pages, const int* free_pages, int n_free, const int* taken,
                    int n_pages, int M, int* pos, int* slot, int* line, int* start, int* held_out, int* taken_out, int* status, const int* lead_seq, const int* lead_pages, int pdl,
                    void* stream);
+/* the same with all arguments in one piece, eight bytes each, for callers to whom an argument costs more than that */
+typedef struct {
+    long long n;
+    const int *held, *new_tokens, *seq;
+    int* table;
+    long long n_seqs, max_pages;
+    const int* free_pages;
+    long long n_free;
+    const int* taken;
+    long long n_pages, M;
+    int *pos, *slot, *line, *start, *held_out, *taken_out, *status;
+    const int *lead_seq, *lead_pages;
+    long long pdl;
+    void* stream;
+} DlPageTables;
+int dl_page_tables_packed(const DlPageTables* a /*host*/);
 
 /* F32 x F32 -> F32 matmul (f32-weights / f32-buffer path; reference: matmul_F32_F32_F32, nn-cpu-ops.cpp:182-220):
  * y[m][r] (+)= sum_k w[r*ldw + k] * x[m*ldx + k], plain f32 FMAs; n, ldw, ldx multiples of 4, w and x 16-byte aligned */

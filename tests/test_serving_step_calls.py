@@ -40,7 +40,7 @@ def _tables(**change):
 
 
 @pytest.mark.parametrize("change", [
-    {"n": -1}, {"n": 4}, {"n": 8193}, {"held": None}, {"new": None}, {"seq": i32(2)}, {"held": torch.zeros(3)}, {"new": torch.zeros(3, dtype=torch.int64)}, {"seq": i32(6)[::2]}, {"block_table": i32(35)},
+    {"n": -1}, {"n": 4}, {"n": 8193}, {"held": None}, {"new": None}, {"seq": i32(2)}, {"held": torch.zeros(3)}, {"new": torch.zeros(3, dtype=torch.int64)}, {"seq": i32(6)[::2]}, {"block_table": i32(35)}, {"block_table": None},
     {"block_table": torch.zeros(5, 7)}, {"block_table": i32(7, 5).t()}, {"block_table": i32(0, 7)}, {"block_table": i32(5, 0)}, {"block_table": i32(131073, 1)}, {"free_pages": None},
     {"free_pages": torch.zeros(9)}, {"taken": i32(0)}, {"n_pages": 0}, {"n_pages": (1 << 26) + 1}, {"pos": None}, {"slot": i32(7)}, {"line": i32(7)}, {"start": i32(3)}, {"held_out": i32(2)},
     {"taken_out": i32(0)}, {"status": None}, {"status": torch.zeros(1)}, {"lead_seq": i32(3)}, {"lead_pages": i32(3)}, {"lead_seq": i32(3), "lead_pages": i32(2)}])
@@ -63,6 +63,9 @@ def test_the_c_entries_refuse():
                    {"free": None}, {"taken": None}, {"pos": None}, {"held_out": None}, {"status": None}, {"ls": p}, {"lp": p}):
         assert L.dl_page_tables(*{**ok, **change}.values(), 0, None) == -1
     assert b"null" in L.dl_last_error()
+    assert L.dl_page_tables_packed(None) == -1
+    packed = lambda **kw: K._TABLES_ARGS.pack(*[v or 0 for v in {**ok, **kw}.values()], 0, 0)
+    assert L.dl_page_tables_packed(packed(n=1 << 40)) == -1 and L.dl_page_tables_packed(packed(n=8193)) == -1 and L.dl_page_tables_packed(packed(table=None)) == -1
 
 
 def _shared(monkeypatch, **change):
