@@ -9,7 +9,7 @@
 //
 // What bounds it: the chain of latencies (lengths, sums, free pages, table, rows), and for many requests the shared pages' copies.  So every CTA forms all sums, for which a barrier in between would cost
 // more, and writes its part of the results; a row finds its request by bisection over the sums in shared memory.  Where lengths and the count of taken pages are updated in place, one cluster does
-// it all: its CTAs have all read before one writes.  32 requests of a token each 5.4 us, 2001 requests with 22000 rows behind 250 shared pages 11.6 (27.8 by one cluster).
+// it all: its CTAs have all read before one writes.  32 requests of a token each 5.2 us, 2001 requests with 22000 rows behind 250 shared pages 11.6 (27.8 by one cluster).
 #include "../../../include/dllama_b200.h"
 #include "common.cuh"
 #include "smem_limit.cuh"
@@ -56,8 +56,9 @@ __global__ void __launch_bounds__(PGT_THREADS) page_tables_kernel(const __grid_c
     int* seq = held + n;                                       // [n]
     uint32_t* used = reinterpret_cast<uint32_t*>(seq + n);     // [words] table rows of requests
     uint32_t* led = used + words;                              // [words] ... whose first pages are another's
+    uint32_t* grown = led + words;                             // [words] ... that get pages in this call
     pdl_launch_dependents();
-    for (int i = tid; i < 2 * words; i += PGT_THREADS) used[i] = 0;
+    for (int i = tid; i < 3 * words; i += PGT_THREADS) used[i] = 0;
     __syncthreads();
     pdl_wait();
     const int taken = *a.taken;
@@ -71,14 +72,16 @@ __global__ void __launch_bounds__(PGT_THREADS) page_tables_kernel(const __grid_c
         seq[i] = s;
         if (h < 0 || c < 0 || (long long)h + c > (long long)a.max_pages * PGT_PAGE) { bad |= DL_TABLES_BAD_LENGTH; continue; }
         const bool lead_ok = l >= 0 && (long long)l * PGT_PAGE <= h && (l == 0 || (unsigned)a.lead_seq[i] < (unsigned)a.n_seqs);
+        const int more = (h + c + PGT_PAGE - 1) / PGT_PAGE - (h + PGT_PAGE - 1) / PGT_PAGE;
         if (!lead_ok) bad |= DL_TABLES_BAD_LEAD;
         if ((unsigned)s >= (unsigned)a.n_seqs) bad |= DL_TABLES_BAD_SEQ;
         else {
             if (atomicOr(&used[s >> 5], 1u << (s & 31)) >> (s & 31) & 1) bad |= DL_TABLES_BAD_SEQ;
             if (lead_ok && l > 0 && a.lead_seq[i] != s) atomicOr(&led[s >> 5], 1u << (s & 31));
+            if (leads && more > 0) atomicOr(&grown[s >> 5], 1u << (s & 31));
         }
         sum[0] += c;
-        sum[1] += (h + c + PGT_PAGE - 1) / PGT_PAGE - (h + PGT_PAGE - 1) / PGT_PAGE;
+        sum[1] += more;
         sum[2] += lead_ok ? (l + PGT_UNIT - 1) / PGT_UNIT : 0;
     }
     unsigned long long incl[3];
@@ -106,6 +109,7 @@ __global__ void __launch_bounds__(PGT_THREADS) page_tables_kernel(const __grid_c
         const unsigned long long before = __shfl_sync(0xffffffffu, x, max(warp - 1, 0));
         ahead[q] = (warp ? before : 0) + incl[q] - sum[q];
     }
+    int grown_lead = -1, grown_have = 0;                       // a table row that gets pages in this call, and how many it has
     for (int i = i0; i < i1; i++) {
         row_at[i] = (uint32_t)ahead[0];
         page_at[i] = (uint32_t)ahead[1];
@@ -114,9 +118,15 @@ __global__ void __launch_bounds__(PGT_THREADS) page_tables_kernel(const __grid_c
         ahead[0] += c;
         ahead[1] += ((long long)h + c + PGT_PAGE - 1) / PGT_PAGE - ((long long)h + PGT_PAGE - 1) / PGT_PAGE;
         ahead[2] += l > 0 ? (l + PGT_UNIT - 1) / PGT_UNIT : 0;
-        if (l > 0 && bad == 0) {                   // pages of a row that gets its own from another in this call
+        if (l > 0 && bad == 0) {                   // pages of a row that gets its own from another in this call, or that this call takes for it
             const int t = a.lead_seq[i];
             if (t != seq[i] && (led[t >> 5] >> (t & 31) & 1)) bad |= DL_TABLES_BAD_LEAD;
+            if (t != seq[i] && (grown[t >> 5] >> (t & 31) & 1)) {
+                if (t != grown_lead)               // (seldom: whose request it is, nobody has noted)
+                    for (int j = 0; j < n; j++)
+                        if (seq[j] == t) { grown_lead = t; grown_have = (held[j] + PGT_PAGE - 1) / PGT_PAGE; }
+                if (l > grown_have) bad |= DL_TABLES_BAD_LEAD;
+            }
         }
     }
     if (tid == 0) {
@@ -177,13 +187,13 @@ extern "C" int dl_page_tables(int n, const int* held, const int* new_tokens, con
                               int n_pages, int M, int* pos, int* slot, int* line, int* start, int* held_out, int* taken_out, int* status, const int* lead_seq, const int* lead_pages, int pdl,
                               void* stream) {
     if (n < 0 || n > PGT_MAX_REQUESTS || n_seqs < 1 || n_seqs > PGT_MAX_SEQS) { dl_set_error("dl_page_tables: %d requests (at most %d), %d table rows (1 to %d)", n, PGT_MAX_REQUESTS, n_seqs, PGT_MAX_SEQS); return -1; }
-    if (max_pages < 1 || max_pages > 1 << 25 || n_free < 0 || n_pages < 1 || n_pages > 1 << 26 || M < 0) { dl_set_error("dl_page_tables: tables of %d pages, %d free of %d pages, %d rows", max_pages, n_free, n_pages, M); return -1; }
+    if (max_pages < 1 || max_pages > 1 << 25 || n_free < 0 || n_free > 1 << 30 || n_pages < 1 || n_pages > 1 << 26 || M < 0 || M > 1 << 30) { dl_set_error("dl_page_tables: tables of %d pages, %d free of %d pages, %d rows", max_pages, n_free, n_pages, M); return -1; }
     if (!table || !taken || !taken_out || !status || (n > 0 && (!held || !new_tokens || !seq || !held_out)) || (n_free > 0 && !free_pages) || (M > 0 && (!pos || !slot)) || !lead_seq != !lead_pages) {
         dl_set_error("dl_page_tables: a null pointer");
         return -1;
     }
     const PgtArgs a = {held, new_tokens, seq, lead_seq, lead_pages, table, free_pages, taken, pos, slot, line, start, held_out, taken_out, status, n, n_seqs, max_pages, n_free, n_pages, M};
-    const size_t smem = ((size_t)3 * (n + 1) + 2 * (size_t)n + 2 * (size_t)((n_seqs + 31) / 32)) * 4;
+    const size_t smem = ((size_t)3 * (n + 1) + 2 * (size_t)n + 3 * (size_t)((n_seqs + 31) / 32)) * 4;
     static SmemLimit given;
     if (smem > 48 * 1024)
         if (const int rc = dl_smem_limit("dl_page_tables", page_tables_kernel, smem, given)) return rc;

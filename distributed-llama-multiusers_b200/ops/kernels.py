@@ -600,7 +600,7 @@ def page_tables(n: int, held: torch.Tensor, new: torch.Tensor, seq: torch.Tensor
     new[i] more.  Pages are taken off free_pages from place `taken` on; the first lead_pages[i] pages of a request (whole ones, of the tokens held) are those of table row lead_seq[i].
     pos, slot (and line = page * 32 + place) list the requests' new tokens one behind the other, start [n + 1] where each begins; the places behind the last one are -1, 0, -1.  held and
     taken go on to held_out and taken_out (None: in place).  status: 0, or bits TABLES_*: then all rows are empty, nothing is taken and the table is as it was.  No row of the table in two
-    requests, no request's own row a lead while its first pages are another's (both are noticed)."""
+    requests, no request's own row a lead while its first pages are another's or for pages that it gets in this call (all of it is noticed)."""
     # (all that is wanted at once, and the arguments in one piece: a call for each tensor and ctypes' conversions took 8 us of 12)
     try:
         d = _launching(block_table, "block_table")
@@ -616,7 +616,7 @@ def page_tables(n: int, held: torch.Tensor, new: torch.Tensor, seq: torch.Tensor
                 and held.numel() >= n and new.numel() >= n and seq.numel() >= n and held_out.numel() >= n and slot.numel() >= M and taken.numel() and taken_out.numel() and status.numel()
                 and block_table.is_contiguous() and held.is_contiguous() and new.is_contiguous() and seq.is_contiguous() and free_pages.is_contiguous() and pos.is_contiguous()
                 and slot.is_contiguous() and held_out.is_contiguous() and 1 <= n_seqs <= TABLES_MAX_SEQS and max_pages >= 1 and 0 <= n <= TABLES_MAX_REQUESTS and 1 <= n_pages <= 1 << 26
-                and M < 1 << 31 and n_free < 1 << 31
+                and M <= 1 << 30 and n_free <= 1 << 30 and max_pages <= 1 << 25
                 and (line is None or line.dtype is _I32 and line.get_device() == d and line.numel() >= M and line.is_contiguous())
                 and (start is None or start.dtype is _I32 and start.get_device() == d and start.numel() > n and start.is_contiguous())
                 and ((lead_seq is None and lead_pages is None) or lead_seq.dtype is lead_pages.dtype is _I32 and lead_seq.get_device() == lead_pages.get_device() == d

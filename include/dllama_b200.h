@@ -146,12 +146,12 @@ int dl_sample_tokens(const void* logits, int type, int M, int vocab, long long l
  * tokens) and runs new_tokens[i] more.  With have = ceil(held / 32) and need = ceil((held + new) / 32), pages and rows of the requests ahead of it counted in P and R:
  *   table[seq][k] = free_pages[*taken + P + k - have], have <= k < need
  *   table[seq][k] = table[lead_seq[i]][k], k < lead_pages[i]: a shared prompt's pages, whole ones of the tokens held (32 lead_pages <= held); that row may be a request's, too, but none whose own
- *                   first pages are another's; lead_seq and lead_pages: both NULL: none
+ *                   first pages are another's, and for pages that it holds ahead of the call; lead_seq and lead_pages: both NULL: none
  *   pos[R + j] = held + j, slot[R + j] = seq, line[R + j] = 32 table[seq][pos / 32] + pos % 32 (-1 where that is no page); the other ones of the M rows: -1, 0, -1
  *   start[i] = R (n + 1 of them), held_out = held + new, *taken_out = *taken + all pages taken.  line, start: NULL or wanted.  What is written lies apart from what is read, but held_out and
  *                   taken_out may be held and taken.
  * *status: 0, or what was wrong, bits added: then all rows are empty, start is 0, nothing is taken and the table is as it was.
- * At most 8192 requests, 131072 table rows. */
+ * At most 8192 requests, 131072 table rows, 2^30 rows and free pages. */
 enum { DL_TABLES_BAD_LENGTH = 1,   /* below zero, or more tokens than a table row has pages for */
        DL_TABLES_BAD_SEQ = 2,      /* not a table row, or one of two requests */
        DL_TABLES_BAD_LEAD = 4, DL_TABLES_NO_PAGES = 8 /* the list of n_free pages is too short */, DL_TABLES_BAD_PAGE = 16 /* not one of n_pages in the part of the list that is taken */, DL_TABLES_NO_ROWS = 32 /* more than M */ };

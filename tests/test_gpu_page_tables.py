@@ -19,6 +19,7 @@ def oracle(c):
     lead = c.get("lead")
     bad, seen, rows = 0, set(), 0
     need = [-(-(int(h) + int(x)) // PAGE) - -(-int(h) // PAGE) for h, x in zip(c["held"], c["new"])]
+    has = {s: -(-int(h) // PAGE) for s, h, x in zip(c["seq"], c["held"], need) if x > 0}      # of rows that get pages
     led = {s for s, (t, l) in zip(c["seq"], lead) if l > 0 and t != s} if lead else set()
     for i, (h, x, s) in enumerate(zip(c["held"], c["new"], c["seq"])):
         if h < 0 or x < 0 or int(h) + int(x) > table.shape[1] * PAGE:
@@ -29,7 +30,7 @@ def oracle(c):
         seen.add(s)
         if lead:
             t, l = lead[i]
-            if l < 0 or l * PAGE > h or (l > 0 and (not 0 <= t < table.shape[0] or (t != s and t in led))):
+            if l < 0 or l * PAGE > h or (l > 0 and (not 0 <= t < table.shape[0] or (t != s and (t in led or l > has.get(t, l))))):
                 bad |= k.TABLES_BAD_LEAD
     ok_lengths = not bad & k.TABLES_BAD_LENGTH
     if ok_lengths:
@@ -140,6 +141,22 @@ def test_a_lead_may_be_a_request_and_a_row_its_own():
     c["free"] = list(range(500000, 501000))
     c["lead"] = [(c["seq"][0], 10)] * 6                        # the first one's own
     assert check(c)["status"] == 0
+
+
+@pytest.mark.parametrize("n", [6, 2500])
+def test_a_lead_that_gets_pages_leads_with_those_it_held(n):
+    """Pages that a call takes for one request are no lead for another one: nothing says which of the two comes first."""
+    rng = np.random.default_rng(6)
+    for held, status in ((320, 0), (289, 0), (288, K().TABLES_BAD_LEAD), (0, K().TABLES_BAD_LEAD)):      # 10, 10, 9 and no pages
+        c = case(rng, n, 300, 50)
+        c["held"] = [max(h, 10 * PAGE) for h in c["held"]]
+        i = n // 2
+        c["held"][i], c["new"][i] = held, 350
+        c["table"] = np.arange(c["table"].shape[0] * 24).reshape(-1, 24)
+        c["n_pages"], c["free"], c["M"] = 10 ** 6, list(range(500000, 520000)), n * 50 + 400
+        c["lead"] = [(c["seq"][i], 10 if j != i else 0) for j in range(n)]
+        assert check(c)["status"] == status
+        check(c, in_place=True)
 
 
 def test_no_requests_and_no_rows():

@@ -59,7 +59,7 @@ def test_the_c_entries_refuse():
     assert L.dl_sample_tokens(None, 0, 2, 8, 8, p, p, p, p, p, p, p, 0, None) == -1
     assert L.dl_sample_tokens(p, 0, 0, 8, 8, p, p, p, p, p, p, p, 0, None) == 0      # no rows: nothing to do
     ok = dict(n=1, held=p, new=p, seq=p, table=p, n_seqs=1, max_pages=1, free=p, n_free=1, taken=p, n_pages=1, M=1, pos=p, slot=p, line=p, start=p, held_out=p, taken_out=p, status=p, ls=None, lp=None)
-    for change in ({"n": -1}, {"n": 8193}, {"n_seqs": 0}, {"n_seqs": 131073}, {"max_pages": 0}, {"max_pages": (1 << 25) + 1}, {"n_free": -1}, {"n_pages": 0}, {"M": -1}, {"held": None}, {"table": None},
+    for change in ({"n": -1}, {"n": 8193}, {"n_seqs": 0}, {"n_seqs": 131073}, {"max_pages": 0}, {"max_pages": (1 << 25) + 1}, {"n_free": -1}, {"n_free": (1 << 30) + 1}, {"n_pages": 0}, {"M": -1}, {"M": (1 << 30) + 1}, {"held": None}, {"table": None},
                    {"free": None}, {"taken": None}, {"pos": None}, {"held_out": None}, {"status": None}, {"ls": p}, {"lp": p}):
         assert L.dl_page_tables(*{**ok, **change}.values(), 0, None) == -1
     assert b"null" in L.dl_last_error()
