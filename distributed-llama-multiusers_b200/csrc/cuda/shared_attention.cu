@@ -30,6 +30,7 @@
 #define SH_PAIR_COST 7                 // of a step with two tiles
 #define SH_ONE_COST 4                  // ... with one
 #define SH_LEAST_COST 8                // of a CTA's share: two steps of one tile
+#define SH_BAD 8                       // items of a CTA that can be at work at once, and more
 #define SH_OWN_TOK 16                  // tokens of a warp's turn
 #define SH_OWN_MAX_CTAS 8
 
@@ -142,6 +143,7 @@ template <int ID> DL_DEVINL void sh_bar() { asm volatile("bar.sync %0, 256;" ::"
 
 struct ShItem {
     int kvh, row0, rows, begin, slot, pages, j0, J, tiles, piece;      // row0: first stacked row; rows: stacked rows of the group
+    int number;                        // 1, 2, .. of the CTA's items
 };
 
 // Queries of 32 stacked rows into a tile's K-major, swizzled image; where one of them is beyond what fp16 holds well, each row times the power of two that brings its largest value to 2^8 .. 2^9
@@ -245,7 +247,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
                                                                          const __grid_constant__ WaitLimit limit) {
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ ShPlan plan;
-    __shared__ int list[1 + 3 * SH_MAX_GROUPS], red[SH_MAX_GROUPS][2], gave_up_s, bad_s;
+    __shared__ int list[1 + 3 * SH_MAX_GROUPS], red[SH_MAX_GROUPS][2], gave_up_s, bad_s[SH_BAD];      // bad_s: the number of an item with a page that is none, at its place modulo SH_BAD
     uint8_t* q_s = smem;                                        // [2] query tiles
     uint8_t* k_s = q_s + 2 * SH_TILE_BYTES;                     // [2] K tiles (tokens x head dim, K-major)
     uint8_t* v_s = k_s + SH_STAGES * SH_TILE_BYTES;             // [2] V tiles (tokens x head dim, MN-major for P V)
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         gave_up_s = limit.ns == 0;
-        bad_s = 0;
+        for (int i = 0; i < SH_BAD; i++) bad_s[i] = 0;
         for (int s = 0; s < 2; s++) {
             mbar_init(&k_full[s], 1);
             mbar_init(&k_empty[s], 1);
@@ -298,6 +300,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
     // this CTA's items, in the same order for every role: `x` goes from the start of its share to the end of the unit looked at
     ShUnit u_at;
+    int n_items = 0;
     auto next_item = [&](int& x, ShItem& it) {
         while (x < x_end) {
             int j0, j1;
@@ -316,6 +319,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
             it.J = j1 - j0;
             it.tiles = u_at.tiles;
             it.piece = u_at.index + b;
+            it.number = ++n_items;
             return true;
         }
         return false;
@@ -414,8 +418,8 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
             wait(&o_full[t], (ns - 1) & 1);
             tc_fence_after();
             // the largest weight is 1 or more; where it is not, a score was no number.  No score at all above -inf: nothing to add
-            l = m_used == -INFINITY ? 0.f : l >= 0x1p-13f && !bad_s && !gave_up_s ? l : __int_as_float(0x7fffffff);
-            if (bad_s || gave_up_s) l = __int_as_float(0x7fffffff);
+            l = m_used == -INFINITY ? 0.f : l >= 0x1p-13f ? l : __int_as_float(0x7fffffff);
+            if (*(volatile int*)&bad_s[it.number % SH_BAD] == it.number || gave_up_s) l = __int_as_float(0x7fffffff);
             // the two places of one tile have seen different steps of the same rows: the first one joins them (both lie in the same lanes of tensor memory)
             const bool pair = it.tiles == 1 && it.J > 1;
             float e0 = 1.f, e1 = 0.f;
@@ -542,7 +546,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
                     if (lane >= 4 || p >= last) return -1;
                     const int page = bt[p];
                     if ((unsigned)page < (unsigned)a.n_pages) return page;
-                    *(volatile int*)&bad_s = 1;                  // (seen by the softmax threads behind the barriers)
+                    *(volatile int*)&bad_s[it.number % SH_BAD] = it.number;      // (seen by the softmax threads behind the barriers; another item's rows keep their values)
                     return 0;
                 };
                 auto line_of = [&](int page) { return (page * a.n_kv_heads + it.kvh) * SH_PAGE; };      // first row of the page in the [rows][head size] view

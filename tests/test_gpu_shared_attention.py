@@ -224,6 +224,20 @@ def test_what_is_not_in_the_tables_is_not_followed(what):
     b.check(y, rows=[m for m in range(b.M) if m not in hit])
 
 
+@pytest.mark.parametrize("pages", [5, 9, 13, 21])
+def test_a_page_that_is_none_stays_in_its_group(pages):
+    """Shares of the work that end in one group and begin the next one: what is wrong in one reaches no row of another."""
+    for which in range(3):
+        b = Batch(18, [(3, pages, 50), (4, 12, 40), (2, pages, 30)], 8, 1, 128)
+        first = sum((3, 4, 2)[:which])
+        hit = range(first, first + (3, 4, 2)[which])
+        for m in hit:
+            b.table[b.slot[m], 4] = b.n_pages
+        y = b.run()
+        assert torch.isnan(y[list(hit)]).all()
+        b.check(y, rows=[m for m in range(9) if m not in hit])
+
+
 def test_strides_and_rows_behind():
     b = Batch(19, [(6, 8, 40)], 16, 4, 128)
     wide = torch.zeros(9, 16 * 128 + 12, device="cuda")
