@@ -22,6 +22,7 @@ import torch
 
 from ..parallel.control import OP_FORWARD, OP_STOP, OP_WARMUP, ControlChannel
 from ..text import native as T
+from .filters import Filters
 
 
 PAGE_TOKENS = 32          # tokens per KV page (ops.kernels.PAGE_SIZE)
@@ -35,7 +36,7 @@ class GenerationRequest:
     top_p: float = 0.9
     seed: int = 0
     stop: Sequence[str] = ()
-    top_k: int = 0                              # 0: off; with top_k or min_p the batch is drawn by ops.kernels.sample_tokens
+    top_k: int = 0                              # 0: off; a row with top_k or min_p is drawn by ops.kernels.sample_tokens
     min_p: float = 0.0                          # 0: off
     # filled by the engine
     id: int = -1
@@ -100,8 +101,7 @@ class BatchEngine:
             self._d_params = torch.zeros(3, R, dtype=torch.float32, device=dev)
             self._d_tok = torch.zeros(R, dtype=torch.int32, device=dev)
             self._h_tok = torch.zeros(R, dtype=torch.int32).pin_memory()
-            self._h_top_k, self._d_top_k = torch.zeros(R, dtype=torch.int32).pin_memory(), torch.zeros(R, dtype=torch.int32, device=dev)
-            self._h_min_p, self._d_min_p = torch.zeros(R, dtype=torch.float32).pin_memory(), torch.zeros(R, dtype=torch.float32, device=dev)
+            self._filters = Filters(R, dev)
             self._logits_host = None
         else:
             self._logits_host = torch.empty(self.max_rows, engine.h.vocab_size, dtype=torch.float32)
@@ -213,13 +213,12 @@ class BatchEngine:
                     hp[0, i], hp[1, i] = r.temperature, r.top_p
                     hp[2, i] = r._sampler.coin() if r.temperature != 0.0 else 0.0
             self._d_params.copy_(self._h_params, non_blocking=True)
-            if any(r is not None and (r.top_k > 0 or r.min_p > 0) for r in rows):
-                from ..ops import kernels as _K
+            n_on = sum(r is not None and (r.top_k > 0 or r.min_p > 0) for r in rows)
+            if n_on:
+                f = self._filters
                 for i, r in enumerate(rows):
-                    self._h_top_k[i], self._h_min_p[i] = (r.top_k, r.min_p) if r is not None else (0, 0.0)
-                self._d_top_k.copy_(self._h_top_k, non_blocking=True)
-                self._d_min_p.copy_(self._h_min_p, non_blocking=True)
-                _K.sample_tokens(logits, n_s, self._d_params[0], self._d_top_k, self._d_params[1], self._d_min_p, self._d_params[2], self._d_tok)
+                    f.top_k[i], f.min_p[i] = (r.top_k, r.min_p) if r is not None else (0, 0.0)
+                f.draw(logits, n_s, n_on, self._d_params, self._sample_rows, self._d_tok)
             else:
                 self._sample_rows(logits[:n_s], self._d_params[0], self._d_params[1], self._d_params[2], self._d_tok)
             self._h_tok.copy_(self._d_tok, non_blocking=True)

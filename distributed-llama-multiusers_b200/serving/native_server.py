@@ -22,6 +22,7 @@ import torch
 from ..parallel.control import OP_FORWARD, OP_STOP, OP_WARMUP, ControlChannel
 from ..text import native as T
 from . import api_types as A
+from .filters import Filters
 
 
 class NativeApiServer:
@@ -69,8 +70,7 @@ class NativeApiServer:
                 self._sample_rows = _K.sample_rows
             self._d_params = torch.zeros(3, R, dtype=torch.float32, device=dev)
             self._d_tok = torch.zeros(R, dtype=torch.int32, device=dev)
-            self._h_top_k, self._d_top_k = pin(torch.zeros(R, dtype=torch.int32)), torch.zeros(R, dtype=torch.int32, device=dev)
-            self._h_min_p, self._d_min_p = pin(torch.zeros(R, dtype=torch.float32)), torch.zeros(R, dtype=torch.float32, device=dev)
+            self._filters = Filters(R, dev)
             self._L.dl_srv_set_filters(self._h, 1)
         else:
             self._logits_host = pin(torch.empty(R, engine.h.vocab_size, dtype=torch.float32))
@@ -180,11 +180,10 @@ class NativeApiServer:
         elif self._device_sampler:
             logits = eng.forward(toks, pos, slots, logits_from=lf)
             self._d_params.copy_(self._h_params, non_blocking=True)
-            if L.dl_srv_batch_filters(h, self._h_top_k.data_ptr(), self._h_min_p.data_ptr(), R):
-                from ..ops import kernels as _K
-                self._d_top_k.copy_(self._h_top_k, non_blocking=True)
-                self._d_min_p.copy_(self._h_min_p, non_blocking=True)
-                _K.sample_tokens(logits, n_s, self._d_params[0], self._d_top_k, self._d_params[1], self._d_min_p, self._d_params[2], self._d_tok)
+            f = self._filters
+            n_on = L.dl_srv_batch_filters(h, f.top_k.data_ptr(), f.min_p.data_ptr(), R)
+            if n_on:
+                f.draw(logits, n_s, n_on, self._d_params, self._sample_rows, self._d_tok)
             else:
                 self._sample_rows(logits[:n_s], self._d_params[0], self._d_params[1], self._d_params[2], self._d_tok)
             self._h_tok.copy_(self._d_tok, non_blocking=True)

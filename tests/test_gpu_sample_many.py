@@ -134,3 +134,35 @@ def test_top_k_and_min_p_through_the_serving_loop(tiny_model_path, tmp_path):
         answers[name] = [r.tokens for r in reqs]
     assert answers["greedy"] == answers["top_k"] == answers["min_p"]
     e.close()
+
+
+def test_neighbours_with_top_k_change_no_answer():
+    """Rows without top_k and min_p are drawn as in a batch where nobody has them: by the sampler that they had before."""
+    from dllama_b200.ops import kernels as K
+    from dllama_b200.serving.filters import Filters
+    g = torch.Generator(device="cuda").manual_seed(3)
+    n, vocab = 24, 1024
+    logits = torch.zeros(32, vocab, device="cuda")
+    logits[:n] = 2 * torch.randn(n, vocab, generator=g, device="cuda")
+    logits[5] = 0.0                                                # all tokens alike: both samplers agree on none of top_p's
+    params = torch.stack([torch.full((32,), 0.9), torch.full((32,), 0.8), torch.rand(32, generator=torch.Generator().manual_seed(4))]).cuda()
+    alone = torch.zeros(32, dtype=torch.int32, device="cuda")
+    K.sample_rows(logits[:n], params[0], params[1], params[2], alone)
+    f = Filters(32, logits.device)
+    seen = []
+
+    def rows(*a):
+        seen.append(len(a[0]))
+        K.sample_rows(*a)
+    for on in ([], [0], [3, 17], list(range(n))):
+        f.top_k.zero_()
+        f.min_p.zero_()
+        f.top_k[on[::2]], f.min_p[on[1::2]] = 7, 0.2
+        f.top_k[n:] = 5                                            # (places behind the batch's rows)
+        want = torch.full((32,), -9, dtype=torch.int32, device="cuda")
+        K.sample_tokens(logits, n, params[0], f.top_k.cuda(), params[1], f.min_p.cuda(), params[2], want)
+        got = torch.full((32,), -9, dtype=torch.int32, device="cuda")
+        f.draw(logits, n, len(on), params, rows, got)
+        for m in range(32):
+            assert got[m] == (-9 if m >= n else want[m] if m in on else alone[m])
+    assert seen == [n] * 3
