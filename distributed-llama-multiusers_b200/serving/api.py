@@ -121,7 +121,7 @@ def make_handler(state: ApiState):
                     return self._json(400, {"error": {"message": "Prompt is empty.", "type": "invalid_request_error"}})
                 req = state.build_request(params)
                 state.batch.submit(req)
-            except (ValueError, KeyError, TypeError, json.JSONDecodeError) as e:
+            except (ValueError, KeyError, TypeError, OverflowError, json.JSONDecodeError) as e:
                 with state.lock:
                     state.n_errors += 1
                 return self._json(400, {"error": {"message": str(e), "type": "invalid_request_error"}})

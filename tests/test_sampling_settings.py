@@ -31,6 +31,9 @@ def test_api_parameters():
     assert p.top_k == 40 and p.min_p == 0.05
     assert A.parse_inference_params({**body, "top_k": -1}, d).top_k == 0
     assert A.parse_inference_params({**body, "top_k": 10 ** 12}, d).top_k == (1 << 31) - 1
+    for bad in (float("nan"), float("inf")):                     # (json.loads takes both; answered with 400)
+        with pytest.raises((ValueError, OverflowError)):
+            A.parse_inference_params({**body, "top_k": bad}, d)
 
 
 def test_cli_options():
