@@ -324,8 +324,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
         }
         return false;
     };
-    // A single tile takes both places, too: its steps in turn, so that the softmax of one step runs beside the next one's (a step took 1.9 us in one place, 1.6 for two tiles).  Step j of place t?
-    auto on = [](const ShItem& it, int t, int j) { return j < it.J && (it.tiles == 2 || (j & 1) == t); };
+    // A single tile takes both places, too: its steps in turn, so that the softmax of one step runs beside the next one's (a step took 1.9 us in one place, 1.6 for two tiles).
     // TMEM columns: one buffer of scores at 0, which the tiles take in turn; probabilities at 128, of 64 columns for each tile; outputs at 256 + 128 t
     if (warp < 8) {
         // ---------------- softmax: warps 0-3 tile 0, warps 4-7 tile 1; a thread per stacked row (= TMEM lane) ----------------
@@ -476,59 +475,72 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         const uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+        // The two products have a warp each: what one of them waits for does not hold up the other's (by one warp, scores behind the weights two steps ahead of them, a step of two tiles took 2.2 us).
+        // What is multiplied, in this order: (place, step) (0, 0), (1, 0), (0, 1) .. of two tiles, (0, 0), (1, 1), (0, 2) .. of one
         if (warp == 8) {
-            // ---------------- MMAs, all by one thread: what it issues runs in that order ----------------
-            const uint32_t idesc_s = pt_idesc(SH_ROWS, SH_KV, 0, false), idesc_pv = pt_idesc(SH_ROWS, HS, 1, false);
+            // ---------------- S = Q K^T ----------------
+            const uint32_t idesc_s = pt_idesc(SH_ROWS, SH_KV, 0, false);
             const uint32_t q_lo = ((smem_u32(q_s) & 0x3FFFFu) >> 4) | (1u << 16), k_lo = ((smem_u32(k_s) & 0x3FFFFu) >> 4) | (1u << 16);
-            const uint32_t v_lo = ((smem_u32(v_s) & 0x3FFFFu) >> 4) | ((16384u >> 4) << 16);
-            uint32_t g = 0, n_s = 0, ns[2] = {0, 0}, nq[2] = {0, 0};      // steps, scores, steps of a tile, items of a tile so far
+            uint32_t g = 0, q_phase = 0, s_phase = 1;            // steps so far; parities of q_full (a bit for each place) and s_empty (which is free at first)
             ShItem it;
             for (int x = b * plan.quota; next_item(x, it);) {
-                // what is multiplied, in this order: (place, step) (0, 0), (1, 0), (0, 1) .. of two tiles, (0, 0), (1, 1), (0, 2) .. of one
-                const int two = it.tiles == 2 ? 1 : 0, E = it.J << two;
-                auto scores = [&](int e) {                       // S = Q K^T
-                    if (e >= E) return;
-                    const int t = e & 1, j = e >> two, st = (g + j) & 1;
-                    if (!two || t == 0) wait(&k_full[st], ((g + j) >> 1) & 1);
-                    if (j == (two ? 0 : t)) wait(&q_full[t], nq[t]++ & 1);
-                    if (n_s > 0) wait(s_empty, (n_s - 1) & 1);
-                    n_s++;
+                auto scores = [&](int t, int st, bool first, bool last) {
+                    if (first) {
+                        wait(&q_full[t], q_phase >> t & 1);
+                        q_phase ^= 1u << t;
+                    }
+                    wait(s_empty, s_phase);
+                    s_phase ^= 1;
                     tc_fence_after();
                     __syncwarp();
                     if constexpr (HS == 128) pt_mma_ss(tmem_base, q_lo + t * (SH_TILE_BYTES >> 4), k_lo + st * (SH_TILE_BYTES >> 4), desc_hi, idesc_s, 0);
                     else pt_mma_ss4(tmem_base, q_lo + t * (SH_TILE_BYTES >> 4), k_lo + st * (SH_TILE_BYTES >> 4), desc_hi, idesc_s, 0);
                     pt_commit(&s_full[t]);
-                    if (!two || t == 1) pt_commit(&k_empty[st]);
-                    if (!on(it, t, j + 2 - two)) pt_commit(&q_empty[t]);
+                    if (last) pt_commit(&q_empty[t]);
                 };
-                scores(0);
-                scores(1);
-                scores(2);
-                for (int e = 0; e < E; e++) {                    // O += P V
-                    const int t = e & 1, j = e >> two, st = (g + j) & 1;
-                    if (!two || t == 0) {
-                        const int live = it.pages - (it.j0 + j) * (SH_KV / SH_PAGE);
-                        wait(&v_full[st], ((g + j) >> 1) & 1);
-                        if (live < SH_KV / SH_PAGE) {            // pages that were not copied: a weight of zero times what lies there may be a NaN
-                            uint8_t* vz = v_s + st * SH_TILE_BYTES;
-                            for (int i = live * SH_PAGE * (HS / 8) + lane; i < SH_KV * (HS / 8); i += 32) {      // 16-byte pieces of a token's row
-                                const int r = i / (HS / 8), c = i % (HS / 8);
-                                *reinterpret_cast<uint4*>(vz + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-                            }
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                        }
-                    }
-                    wait(&p_full[t], ns[t]++ & 1);
+                for (int j = 0; j < it.J; j++, g++) {
+                    const int st = g & 1;
+                    wait(&k_full[st], (g >> 1) & 1);
+                    if (it.tiles == 2) {
+                        scores(0, st, j == 0, j + 1 == it.J);
+                        scores(1, st, j == 0, j + 1 == it.J);
+                    } else scores(j & 1, st, j < 2, j + 2 >= it.J);
+                    pt_commit(&k_empty[st]);
+                }
+            }
+        } else if (warp == 11) {
+            // ---------------- O += P V ----------------
+            const uint32_t idesc_pv = pt_idesc(SH_ROWS, HS, 1, false);
+            const uint32_t v_lo = ((smem_u32(v_s) & 0x3FFFFu) >> 4) | ((16384u >> 4) << 16);
+            uint32_t g = 0, p_phase = 0;                         // steps so far, parities of p_full
+            ShItem it;
+            for (int x = b * plan.quota; next_item(x, it);) {
+                auto weigh = [&](int t, int st, bool first) {
+                    wait(&p_full[t], p_phase >> t & 1);
+                    p_phase ^= 1u << t;
                     tc_fence_after();
                     __syncwarp();
-                    pt_mma_ts(tmem_base + 256 + t * 128, tmem_base + 128 + t * 64, v_lo + st * (SH_TILE_BYTES >> 4), desc_hi, idesc_pv, j > (two ? 0 : t) ? 1u : 0u);
+                    pt_mma_ts(tmem_base + 256 + t * 128, tmem_base + 128 + t * 64, v_lo + st * (SH_TILE_BYTES >> 4), desc_hi, idesc_pv, first ? 0u : 1u);
                     pt_commit(&o_full[t]);
-                    if (!two || t == 1) pt_commit(&v_empty[st]);
-                    // the scores after next wait in the buffer when the softmax threads come for them
-                    scores(e + 3);
+                };
+                for (int j = 0; j < it.J; j++, g++) {
+                    const int st = g & 1, live = it.pages - (it.j0 + j) * (SH_KV / SH_PAGE);
+                    wait(&v_full[st], (g >> 1) & 1);
+                    if (live < SH_KV / SH_PAGE) {                // pages that were not copied: a weight of zero times what lies there may be a NaN
+                        uint8_t* vz = v_s + st * SH_TILE_BYTES;
+                        for (int i = live * SH_PAGE * (HS / 8) + lane; i < SH_KV * (HS / 8); i += 32) {      // 16-byte pieces of a token's row
+                            const int r = i / (HS / 8), c = i % (HS / 8);
+                            *reinterpret_cast<uint4*>(vz + (c >> 3) * 16384 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (it.tiles == 2) {
+                        weigh(0, st, j == 0);
+                        weigh(1, st, j == 0);
+                    } else weigh(j & 1, st, j < 2);
+                    pt_commit(&v_empty[st]);
                 }
-                g += it.J;
             }
         } else if (warp == 9 || warp == 10) {
             // ---------------- K producer (warp 9) / V producer (warp 10): a lane for each of a step's four pages ----------------
