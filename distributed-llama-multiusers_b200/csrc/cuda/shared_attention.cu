@@ -12,6 +12,11 @@
 //
 // Both have queries and weights in fp16 (queries times a power of two of their row, so that any size goes in; weights at most 2^8), sums and maxima in f32: 2^-12 of a weight is
 // what a result is off by, at random, an eighth of the half step of a bf16 output.
+//
+// What bounds it (us of both launches, 32 heads of 128 on 8): 3 rows behind 16 pages 16 and 32 behind 250 with up to 300 tokens of their own 31 (the bytes 8): latencies one behind the other, of which the first
+// launch has 6 us ahead of its first scores (places, plan, queries), a step's 1.0 to 1.8, 3 for sums on their way out, and the second one 5 for the join behind it.  200 behind 1000 with up to 400 of their own 151 (the
+// products 66): a step of two tiles takes 1.8 us, of which the MMAs run 0.6: the chain scores, maximum, exponentials, weights of one tile is hidden by the other one's alone (more of the exponentials as
+// polynomials: 154 to 158); the second launch reads the rows' own pages at 3.5 TB/s for 50 us, its CTAs of 200 tokens being starts and ends for the greater part.
 #define WAIT_UNIT 5u
 #include "attention_tc.cuh"
 #include "epilogue.cuh"
@@ -153,35 +158,36 @@ DL_DEVINL float sh_load_rows(const float* mine, uint8_t* tile, int r0, Ready rea
     constexpr int PER = 128 / HS;                              // rows a load
     const int lane = threadIdx.x & 31, in = lane * 4 / HS, col = lane * 4 % HS;
     uint8_t* qd = tile + (r0 + in) * 128 + (col >> 6) * 16384 + (lane & 1) * 8;
-    float4 x[32 / PER];
-#pragma unroll
-    for (int u = 0; u < 32; u += PER) {
-        const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)mine, u + in)) + col;
-        x[u / PER] = *reinterpret_cast<const float4*>(src);
-    }
-    ready();
+    constexpr int BATCH = 16;                                    // (a loop: all 32 rows side by side are code that every launch reads anew, 11 rows behind a book 44.2 us instead of 42.3)
     float factor = 1.f;
-    // rows whose largest value is 2^-6 or more and below 2^15, as queries are, go in as they are
-    unsigned fits = 0, top = 0;
-    auto most_of = [](const float4& y) {
-        return max(max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu), max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu));
-    };
+    // rows whose largest value is 2^-6 or more and below 2^15, as queries are, go in as they are (a NaN, too: its row's scores are NaN)
+    unsigned large = 0;                                          // a bit for each row of which this lane has such a value
+    float top = 0.f;
+#pragma unroll 1
+    for (int u0 = 0; u0 < 32; u0 += BATCH) {
+        float4 x[BATCH / PER];
 #pragma unroll
-    for (int u = 0; u < 32; u += PER) {
-        const unsigned most = most_of(x[u / PER]), large = __ballot_sync(0xffffffffu, most >= 0x3c800000u);
-        top = max(top, most);
-        fits += (large & 0xffffu) && (large >> 16) ? 1u : PER == 1 && large ? 1u : 0u;
+        for (int u = 0; u < BATCH; u += PER) {
+            const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)mine, u0 + u + in)) + col;
+            x[u / PER] = *reinterpret_cast<const float4*>(src);
+        }
+        if (u0 == 0) ready();
+#pragma unroll
+        for (int u = 0; u < BATCH; u += PER) {                    // 16-byte piece c of a half row -> swizzled slot c ^ (row & 7)
+            const float4& y = x[u / PER];
+            const float most = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
+            top = fmaxf(top, most);
+            large |= most >= 0x1p-6f ? 1u << (u0 + u) : 0u;
+            *reinterpret_cast<uint2*>(qd + (u0 + u) * 128 + ((((lane >> 1) & 7) ^ ((u + in) & 7)) << 4)) = make_uint2(pt_pack2<false>(y.x, y.y), pt_pack2<false>(y.z, y.w));
+        }
     }
-    const bool plain = fits == 32 / PER && __reduce_max_sync(0xffffffffu, top) < 0x47000000u;
-#pragma unroll
-    for (int u = 0; u < 32; u += PER)            // 16-byte piece c of a half row -> swizzled slot c ^ (row & 7)
-        *reinterpret_cast<uint2*>(qd + u * 128 + ((((lane >> 1) & 7) ^ ((u + in) & 7)) << 4)) =
-            make_uint2(pt_pack2<false>(x[u / PER].x, x[u / PER].y), pt_pack2<false>(x[u / PER].z, x[u / PER].w));
+    large <<= in;
+    const bool plain = __reduce_or_sync(0xffffffffu, large) == 0xffffffffu && __reduce_max_sync(0xffffffffu, __float_as_uint(top)) < 0x47000000u;
     if (!plain) {
-#pragma unroll
+#pragma unroll 1
         for (int u = 0; u < 32; u += PER) {
-            const float4 y = x[u / PER];
-            unsigned most = most_of(y);
+            const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)mine, u + in)) + col);
+            unsigned most = max(max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu), max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu));
 #pragma unroll
             for (int o = HS / 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
             const bool finite = most < 0x7f800000u;
