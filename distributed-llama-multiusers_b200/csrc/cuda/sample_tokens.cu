@@ -11,8 +11,8 @@
 // within the bin, of a few tokens, by comparing them with each other (StRow::select).  What takes part in that is a list in the first CTA's shared memory, in which the border has to lie:
 //   top-k   The least of as many maxima, each over tokens of its own, as k or more is not above the k-th largest logit.  The first pass leaves such maxima (of threads, or of warps); what is not
 //           below the least of them, some thousand tokens, goes into the list, and the rest of the row has no part: the first CTA does it all.
-//   top-p   A second pass counts the tokens in 4096 bins of their distance to the maximum.  A bin's weights differ by 0.5 %, so that the counts tell the sums to some 0.02 %, and the border to a few
-//           bins.  A third pass adds up the weights: of the row, for the target, and of what lies ahead of those bins, for each warp's run of the row; the bins' tokens go into the list.
+//   top-p   A second pass counts the tokens in 4096 bins of their distance to the maximum.  A bin's weights differ by 0.5 %, so that the counts tell the sums to some 0.02 % (of heavy tokens, which
+//           would be most of that, their weights count: without it the list was too short for one row in a hundred, 200 rows 347 us instead of 152), and the border to a few bins.  A third pass adds up the weights: of the row, for the target, and of what lies ahead of those bins, for each warp's run of the row; the bins' tokens go into the list.
 //           The first CTA finds the border there, and the warp's run in which the token lies.
 //   else    as top-p, without a border.
 // Where the list does not do -- more tokens than it takes, a border that is not in it -- all CTAs select over the whole row, by bins that are divided until few tokens are left.
@@ -20,6 +20,9 @@
 // Weights are whole numbers of 2^-44, so that sums do not depend on their order; they are exact to 2^-29 of themselves (a table of 64 powers of two and a
 // polynomial, after P. T. P. Tang's table-driven exponential, on the difference and the factor as pairs of f32 numbers): with sums of f32 results a
 // coin next to a border between two tokens would fall on the other side once in some thousand rows.
+//
+// What bounds it: for few rows some 25 phases, one behind the other, each a barrier of the cluster or a chain through shared memory, and code that is read once (one row of 128256 logits, us: top-p 23.5,
+// top-k and top-p 15, neither 11.5, min-p alone 8.3; the bytes 0.08); for many rows the instructions, 50 a token that is weighed (200 rows: 152, 74, 102, 46; the bytes 16).
 #include <math_constants.h>
 #include <cuda_bf16.h>
 #include "common.cuh"
@@ -27,6 +30,7 @@
 
 #define ST_BINS 256
 #define ST_FINE 4096                   // bins of top-p's counts
+#define ST_HEAVY 1024                  // ... of which the first ones' tokens count by their weights
 #define ST_LIST 6144
 #define ST_FEW 128                     // tokens that are compared with each other
 #define ST_MAX_CTAS 16
@@ -643,6 +647,8 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
         // ---- top-p: the bins in which the border has to lie; where there is none, no bin ----
         int from = ST_FINE, to = -1;
         if (q.by_p) {
+            const float width = ST_REACH / (ST_FINE - 1);
+            float more = 0.f;                                   // what the tokens of the heavy bins weigh beyond the middle of their bin, in widths of a bin
             for (int b = tid; b < ST_FINE; b += THREADS) sh.count.fine[b] = 0;
             __syncthreads();
             z.all([&](const float4& v4, int i) {
@@ -651,9 +657,16 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
                 for (int e = 0; e < 4; e++) {
                     const float t = (m - v[e]) * q.per;
                     if (t < (float)(ST_FINE - 1)) atomicAdd(&sh.count.fine[(int)t], 1u);      // (what is farther, or no number, has next to no weight)
+                    if (t < (float)ST_HEAVY) more = fmaf(__expf(-width * t), 0.5f - (t - truncf(t)), more);
                 }
             });
+            more = warp_sum(more);
+            if (z.lane == 0) sh.warp_low[1][z.warp] = more;
             cluster.sync();
+            if (z.warp == WARPS - 1) {
+                more = warp_sum(z.lane < WARPS ? sh.warp_low[1][z.lane] : 0.f);
+                if (z.lane < ctas) z.at(z.lane)->low[0][rank] = more;
+            }
             const int share = ST_FINE / ctas;
             for (int j = tid; j < share; j += THREADS) {
                 unsigned s = 0;
@@ -663,10 +676,10 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
             }
             if (tid == 0) { sh.bin_from = 0; sh.bin_to = ST_FINE - 1; }
             cluster.sync();
-            // sums from the counts, each bin's tokens in its middle; off by a random part of the width for each bin (16-bit logits: a bin's tokens have one value)
+            // sums from the counts, each bin's tokens in its middle; off by a random part of the width for each bin (16-bit logits: a bin's tokens have one value).  A few heavy tokens would make most of
+            // that: behind the heavy bins theirs are known
             constexpr int PER = (ST_FINE + THREADS - 1) / THREADS;
-            const float width = ST_REACH / (ST_FINE - 1);
-            float w[PER], part = 0.f, off = 0.f;
+            float w[PER], part = 0.f, off = 0.f, off_light = 0.f;
 #pragma unroll
             for (int e = 0; e < PER; e++) {
                 const int b = tid * PER + e;
@@ -674,6 +687,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
                 w[e] = n * mid;
                 part += w[e];
                 off += w[e] * w[e];
+                off_light += b >= ST_HEAVY ? w[e] * w[e] : 0.f;
             }
             float incl = part;
 #pragma unroll
@@ -682,26 +696,37 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
                 if (z.lane >= o) incl += y;
             }
             off = warp_sum(off);
-            if (z.lane == 31) { sh.warp_top[z.warp] = incl; sh.warp_low[0][z.warp] = off; }
+            off_light = warp_sum(off_light);
+            if (z.lane == 31) { sh.warp_top[z.warp] = incl; sh.warp_low[0][z.warp] = off; sh.warp_low[2][z.warp] = off_light; }
             __syncthreads();
             float ahead = incl - part, all = 0.f;
-            off = 0.f;
+            off = off_light = more = 0.f;
             for (int u = 0; u < WARPS; u++) {
                 if (u < z.warp) ahead += sh.warp_top[u];
                 all += sh.warp_top[u];
                 off += sh.warp_low[0][u];
+                off_light += sh.warp_low[2][u];
             }
+            for (int r = 0; r < ctas; r++) more += sh.low[0][r];
+            more *= width;
+            all += more;
             // four standard deviations (width / sqrt 12 of a bin's weight), e^-20 for each token of the tail, and the sums' roundings
-            const float room = 1.2f * width * sqrtf(off) + 2.1e-9f * (float)a.vocab + all * 0x1p-17f, lo = q.p * all - room, hi = q.p * all + room;
+            const float tail = 2.1e-9f * (float)a.vocab + all * 0x1p-17f, room = 1.2f * width * sqrtf(off) + tail, room_light = 1.2f * width * sqrtf(off_light) + tail, goal = q.p * all;
+            // the last bin that begins ahead of the target for sure, the first one that ends behind it
+            int f_b = 0, t_b = ST_FINE - 1;
 #pragma unroll
             for (int e = 0; e < PER; e++) {
                 const int b = tid * PER + e;
                 if (b < ST_FINE) {
-                    if (ahead < lo && ahead + w[e] >= lo) sh.bin_from = b;
-                    if (ahead < hi && ahead + w[e] >= hi) sh.bin_to = b;
+                    if (b < ST_HEAVY ? ahead + room < goal : ahead + more + room_light < goal) f_b = b;
+                    const float end = ahead + w[e];
+                    if (b < t_b && (b + 1 < ST_HEAVY ? end - room >= goal : end + more - room_light >= goal)) t_b = b;
                 }
                 ahead += w[e];
             }
+            f_b = __reduce_max_sync(0xffffffffu, f_b);
+            t_b = __reduce_min_sync(0xffffffffu, t_b);
+            if (z.lane == 0) { atomicMax(&sh.bin_from, f_b); atomicMin(&sh.bin_to, t_b); }
             __syncthreads();
             from = sh.bin_from;
             to = max(from, sh.bin_to);

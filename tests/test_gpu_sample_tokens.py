@@ -211,3 +211,17 @@ def test_rows_with_large_nuclei_in_16_bits():
     x = torch.from_numpy(rng.standard_normal((12, 128256)) * np.array([[0.3], [1.0], [2.2]] * 4)).cuda()
     for dtype in (torch.bfloat16, torch.float16):
         check(x.to(dtype), [1.0, 1.3, 0.7] * 4, [0] * 12, [0.9, 0.99, 0.999, 0.5] * 3, [0.0] * 9 + [0.01] * 3, rng.random(12).astype(np.float32).tolist())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_some_heavy_tokens_ahead_of_a_long_tail(dtype):
+    """Borders among the heavy tokens, at the weight from which they count as such, and far behind them; rows in which all tokens are heavy."""
+    rng = np.random.default_rng(31)
+    x = rng.standard_normal((48, 128256)) * 2.2
+    for m in range(48):
+        x[m, rng.integers(0, 128256, 64)] += 6 + 8 * rng.random(64) ** 3
+    x[:4] *= 0.2
+    t = np.concatenate([[1.0, 5.0, 20.0, 0.3], rng.uniform(0.5, 1.4, 44)]).tolist()
+    p = np.concatenate([[0.9, 0.5, 0.99, 0.95], 1 - 10 ** rng.uniform(-4, -0.3, 44)]).tolist()
+    check(torch.from_numpy(x).to(dtype).cuda(), t, None, p, None, rng.random(48).astype(np.float32).tolist())
+    check(torch.from_numpy(x[:5]).to(dtype).cuda(), t[:5], None, p[:5], [0.0, 0.01, 0.0, 0.0, 1e-4], rng.random(5).astype(np.float32).tolist())
