@@ -21,7 +21,7 @@
 // polynomial, after P. T. P. Tang's table-driven exponential, on the difference and the factor as pairs of f32 numbers): with sums of f32 results a
 // coin next to a border between two tokens would fall on the other side once in some thousand rows.
 //
-// What bounds it: for few rows some 25 phases, one behind the other, each a barrier of the cluster or a chain through shared memory, and code that is read once (one row of 128256 logits, us: top-p 23.5,
+// What bounds it: for few rows some 25 phases, one behind the other, each a barrier of the cluster or a chain through shared memory, and code that is read once (one row of 128256 logits, us: top-p 22,
 // top-k and top-p 15, neither 11.5, min-p alone 8.3; the bytes 0.08); for many rows the instructions, 50 a token that is weighed (200 rows: 152, 74, 102, 46; the bytes 16).
 #include <math_constants.h>
 #include <cuda_bf16.h>
@@ -177,26 +177,38 @@ template <typename T, int THREADS> struct StRow {
         if (i + 2 < count) v.z = st_load1<T>(x + i + 2);
         return v;
     }
-    // f(ST_AHEAD times four logits, the first one's place): the next four are `stride` behind it; whole warps, all loads in flight for each thread
-    template <typename F> DL_DEVINL void batches(int from, int to, int stride, F f) const {
-        for (int i = from; i < to; i += ST_AHEAD * stride) {
-            float4 v[ST_AHEAD];
+    // f(AH times four logits, the first one's place): the next four are `stride` behind it; whole warps, some loads in flight for each thread.  AH of one: a loop of one body
+    template <int AH, typename F> DL_DEVINL void batches(int from, int to, int stride, F f) const {
+        if constexpr (AH == 1) {
+            float4 a{}, b{}, c{};
+#pragma unroll 1
+            for (int i = from - 3 * stride; i < to; i += stride) {
+                const float4 v[1] = {a};
+                a = b;
+                b = c;
+                c = load(i + 3 * stride + lane * 4);
+                if (i >= from) f(v, i + lane * 4);
+            }
+        } else {
+            for (int i = from; i < to; i += AH * stride) {
+                float4 v[AH];
 #pragma unroll
-            for (int u = 0; u < ST_AHEAD; u++) v[u] = load(i + u * stride + lane * 4);
-            f(v, i + lane * 4);
+                for (int u = 0; u < AH; u++) v[u] = load(i + u * stride + lane * 4);
+                f(v, i + lane * 4);
+            }
         }
     }
     // f(four logits, the first one's place)
-    template <typename F> DL_DEVINL void quads(int from, int to, int stride, F f) const {
-        batches(from, to, stride, [&](const float4 (&v)[ST_AHEAD], int i) {
+    template <int AH, typename F> DL_DEVINL void quads(int from, int to, int stride, F f) const {
+        batches<AH>(from, to, stride, [&](const float4 (&v)[AH], int i) {
 #pragma unroll
-            for (int u = 0; u < ST_AHEAD; u++) f(v[u], i + u * stride);
+            for (int u = 0; u < AH; u++) f(v[u], i + u * stride);
         });
     }
-    template <typename F> DL_DEVINL void all(F f) const { quads(warp * 128, count, THREADS * 4, f); }
+    template <int AH, typename F> DL_DEVINL void all(F f) const { quads<AH>(warp * 128, count, THREADS * 4, f); }
     // f(logit, place) for what is not below `cut`; four neighbours a thread, most of which are passed over at once
     template <typename F> DL_DEVINL void each(float cut, F f) const {
-        all([&](const float4& v, int i) {
+        all<ST_AHEAD>([&](const float4& v, int i) {
             if (!(st_max4(v) >= cut) && cut > -CUDART_INF_F) return;
             const float e4[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -333,9 +345,9 @@ template <typename T, int THREADS> struct StRow {
         __syncthreads();
     }
 
-    // Tokens of ST_AHEAD quads go into this CTA's list (by whole warps): bit 4 u + e of `mask` is token e of the quad at place i + u * stride
-    DL_DEVINL void push(unsigned mask, const float4 (&v)[ST_AHEAD], int i, int stride) {
-        static_assert(ST_AHEAD <= 8, "a bit for each token");
+    // Tokens of AH quads go into this CTA's list (by whole warps): bit 4 u + e of `mask` is token e of the quad at place i + u * stride
+    template <int AH> DL_DEVINL void push(unsigned mask, const float4 (&v)[AH], int i, int stride) {
+        static_assert(AH <= 8, "a bit for each token");
         if (!__any_sync(0xffffffffu, mask)) return;
         const unsigned n = __popc(mask);
         unsigned incl = n;
@@ -349,7 +361,7 @@ template <typename T, int THREADS> struct StRow {
         base = __shfl_sync(0xffffffffu, base, 31) + incl - n;
         if (!mask) return;
 #pragma unroll
-        for (int u = 0; u < ST_AHEAD; u++) {
+        for (int u = 0; u < AH; u++) {
             if (!(mask >> (4 * u) & 15)) continue;
             const float x4[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
@@ -452,7 +464,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
     q.coin = a.coin[row];
     // ---- the maximum ----
     float top = -CUDART_INF_F;
-    z.all([&](const float4& v, int) { top = fmaxf(top, st_max4(v)); });      // (no NaN)
+    z.template all<ST_AHEAD>([&](const float4& v, int) { top = fmaxf(top, st_max4(v)); });      // (no NaN)
     {
         float t = top;
 #pragma unroll
@@ -501,7 +513,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
     q.least = q.by_min ? (double)q.T * log((double)fminf(q.min_p, 1.f)) : 0.;
     const float lowest = q.by_min ? fminf(m, __double2float_rd((double)m + q.least)) : -CUDART_INF_F;      // what is below, min-p takes out
     u64 border = 0;                                             // smallest key that stays
-    constexpr int WARPS = THREADS / 32;
+    constexpr int WARPS = THREADS / 32, AH = THREADS == 512 ? 1 : ST_AHEAD;      // quads a turn of top-p's passes (a row on sixteen CTAs: a turn or two, for which a long body is mostly code to be read: 23.7 and 22.0 us)
     const int run = ((a.slice + WARPS - 1) / WARPS + 127) / 128 * 128, r0 = z.warp * run, r1 = min(z.count, r0 + run);      // a warp's run of the slice
 
     // the weights of four neighbours that stay: not below the border, nor min-p's
@@ -579,7 +591,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
         // (of rows with masked tokens, or of a k beyond the maxima: all that is not -inf, which has no weight, whatever k is)
         const bool every = !(cut > -CUDART_INF_F);
         const float least = every ? -3.402823466e38f : cut;
-        z.batches(z.warp * 128, z.count, THREADS * 4, [&](const float4 (&v)[ST_AHEAD], int i) {
+        z.template batches<ST_AHEAD>(z.warp * 128, z.count, THREADS * 4, [&](const float4 (&v)[ST_AHEAD], int i) {
             unsigned mask = 0;
 #pragma unroll
             for (int u = 0; u < ST_AHEAD; u++) {
@@ -651,7 +663,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
             float more = 0.f;                                   // what the tokens of the heavy bins weigh beyond the middle of their bin, in widths of a bin
             for (int b = tid; b < ST_FINE; b += THREADS) sh.count.fine[b] = 0;
             __syncthreads();
-            z.all([&](const float4& v4, int i) {
+            z.template all<AH>([&](const float4& v4, int i) {
                 const float v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -736,10 +748,10 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
         // (a run ends with a whole quad or with the slice, behind which logits are -inf)
         u64 mine = 0, ahead = 0, all = 0;                        // what is drawn from, what is ahead of the border's bins, the row
         const float from_t = (float)from, to_t = to == ST_FINE - 1 ? CUDART_INF_F : (float)(to + 1);
-        z.batches(r0, r1, 128, [&](const float4 (&v4)[ST_AHEAD], int i) {
+        z.template batches<AH>(r0, r1, 128, [&](const float4 (&v4)[AH], int i) {
             unsigned mask = 0;
 #pragma unroll
-            for (int u = 0; u < ST_AHEAD; u++) {
+            for (int u = 0; u < AH; u++) {
                 const float v[4] = {v4[u].x, v4[u].y, v4[u].z, v4[u].w};
                 if (i - z.lane * 4 + u * 128 >= r1) break;       // (uniform for the warp)
                 if (to < 0) {
@@ -842,7 +854,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
         border = sh.found;
     }
     u64 mine = 0;
-    z.quads(r0, r1, 128, [&](const float4& v, int i) {
+    z.template quads<ST_AHEAD>(r0, r1, 128, [&](const float4& v, int i) {
         u64 w[4];
         weights(fmaxf(border ? st_logit(border) : -CUDART_INF_F, lowest), v, i, r1, w);
         mine += (w[0] + w[1]) + (w[2] + w[3]);
