@@ -349,11 +349,9 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
             nq++;
             mbar_arrive(&q_full[t]);
         };
-        ShItem it, next;
+        ShItem it{}, next{};                                     // (first an item without steps, so that the code for the next one's queries stands here once)
         int x = b * plan.quota;
-        bool more = next_item(x, it);
-        if (more) load_queries(it);
-        for (; more; it = next) {
+        for (bool more = true; more; it = next) {
             const int by = it.tiles == 2 ? 1 : 2, ja = it.tiles == 2 ? 0 : t;      // steps ja, ja + by .. are this place's
             const float sc = 1.4426950408889634f * rsqrtf((float)HS) * q_factor;      // scores in the log2 domain
             float m_used = -INFINITY, l = 0.f;
