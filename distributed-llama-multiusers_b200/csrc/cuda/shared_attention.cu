@@ -619,7 +619,7 @@ DL_DEVINL void sh_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32
 
 // grid (CTAs of a row's cluster, key/value heads, rows).  Rows of the MMAs: the query heads of the key/value head (16 at most); tokens 16 at a time, a ring of stages for each
 // warp.  Then every thread joins four values of a head over the warps and this CTA's pieces, and the cluster's CTAs over each other's.
-template <int HS, int WARPS>
+template <int HS, int WARPS, int HALVES>
 __global__ void __launch_bounds__(WARPS * 32, 12 / WARPS) shared_own_kernel(const __grid_constant__ ShArgs a) {
     constexpr int ROWB = HS * 2, CH = ROWB / 16, HALF = SH_OWN_TOK * ROWB, ST = 256 / HS;      // bytes and 16-byte pieces of a line, bytes of a turn's K or V, stages
     constexpr int KS = HS / 16, NT = HS / 8, LPH = HS / 4;                                     // MMA steps of a score, tiles of an output, threads of a head in the join
@@ -639,17 +639,16 @@ __global__ void __launch_bounds__(WARPS * 32, 12 / WARPS) shared_own_kernel(cons
     const int g = lane >> 2, qd = lane & 3;
     // what needs no more than the row's number is asked for at once: its place, its queries (head g, and g + 8 where there are so many), and what the plan is made of
     const int T = sh_tokens(a, m), slot = a.slot[m];
-    float2 qx[2][KS][2];
+    float2 qx[HALVES][KS][2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-        if (u * 8 < G) {
-            const int h = g + u * 8;
-            const float* q = a.q + (long long)m * a.ldq + (size_t)(kvh * G + (h < G ? h : 0)) * HS + qd * 2;
+    for (int u = 0; u < HALVES; ++u) {
+        const int h = g + u * 8;
+        const float* q = a.q + (long long)m * a.ldq + (size_t)(kvh * G + (h < G ? h : 0)) * HS + qd * 2;
 #pragma unroll
-            for (int k = 0; k < KS; ++k)
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-                for (int w = 0; w < 2; ++w) qx[u][k][w] = *reinterpret_cast<const float2*>(q + k * 16 + w * 8);
-        }
+            for (int w = 0; w < 2; ++w) qx[u][k][w] = *reinterpret_cast<const float2*>(q + k * 16 + w * 8);
+    }
     sh_make_plan(a, plan, list, red);
     int g_of = -1;                                               // the row's group, and the pages that all of its rows see
     for (int i = 0; i < plan.n; i++)
@@ -662,7 +661,9 @@ __global__ void __launch_bounds__(WARPS * 32, 12 / WARPS) shared_own_kernel(cons
     const int n_turns = pg1 > pg0 ? (t_end - pg0 * SH_PAGE + SH_OWN_TOK - 1) / SH_OWN_TOK : 0, n_my = (n_turns - warp + WARPS - 1) / WARPS;      // warp w takes turns w, w + 4, ...
     const int* bt = a.block_table + (size_t)(T > 0 ? slot : 0) * a.max_pages;
     const uint32_t ring = smem_u32(smem) + warp * (ST * 2 * HALF);
-    float run_m[2] = {-INFINITY, -INFINITY}, run_l[2] = {0.f, 0.f};      // of heads g and g + 8; run_l: this lane's own tokens
+    float run_m[HALVES], run_l[HALVES];                          // of heads g and g + 8; run_l: this lane's own tokens
+#pragma unroll
+    for (int u = 0; u < HALVES; ++u) { run_m[u] = -INFINITY; run_l[u] = 0.f; }
     float o[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -700,15 +701,13 @@ __global__ void __launch_bounds__(WARPS * 32, 12 / WARPS) shared_own_kernel(cons
         }
         // queries in the A fragments: head g in rows g, head g + 8 in rows g + 8; times a power of two of the head
         uint32_t qf[KS][4];
-        float sc[2];
+        float sc[HALVES];
+        if (HALVES == 1)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+            for (int k = 0; k < KS; ++k) qf[k][1] = qf[k][3] = 0u;
+#pragma unroll
+        for (int u = 0; u < HALVES; ++u) {
             sc[u] = 0.f;
-            if (u * 8 >= G) {
-#pragma unroll
-                for (int k = 0; k < KS; ++k) qf[k][u] = qf[k][2 + u] = 0u;
-                continue;
-            }
             unsigned most = 0;
             const float2 (&x)[KS][2] = qx[u];
 #pragma unroll
@@ -751,10 +750,10 @@ __global__ void __launch_bounds__(WARPS * 32, 12 / WARPS) shared_own_kernel(cons
                 }
             }
             const int left = t_end - pg0 * SH_PAGE - (warp + WARPS * i) * SH_OWN_TOK;
-            uint32_t pa[4];
-            float corr[2];
+            uint32_t pa[4] = {0u, 0u, 0u, 0u};
+            float corr[HALVES];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < HALVES; ++u) {
                 float mx = -INFINITY, s[2][2];
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
@@ -786,7 +785,7 @@ __global__ void __launch_bounds__(WARPS * 32, 12 / WARPS) shared_own_kernel(cons
                     uint32_t b[4];
                     sh_ldm_trans(b, base + (((n + c1) ^ (t & 7)) << 4));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) { o[n][e] *= corr[e >> 1]; o[n + 1][e] *= corr[e >> 1]; }
+                    for (int e = 0; e < 2 * HALVES; ++e) { o[n][e] *= corr[e >> 1]; o[n + 1][e] *= corr[e >> 1]; }
                     sh_mma(o[n], pa, b[0], b[1]);
                     sh_mma(o[n + 1], pa, b[2], b[3]);
                 }
@@ -797,14 +796,14 @@ __global__ void __launch_bounds__(WARPS * 32, 12 / WARPS) shared_own_kernel(cons
         asm volatile("cp.async.wait_all;" ::: "memory");
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < HALVES; ++u) {
         run_l[u] += __shfl_xor_sync(0xffffffffu, run_l[u], 1);
         run_l[u] += __shfl_xor_sync(0xffffffffu, run_l[u], 2);
     }
     if (bad) bad_s = 1;
     __syncthreads();                                             // the rings are done with
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < HALVES; ++u) {
         const int h = g + u * 8;
         if (h >= G) continue;
         float* w = w_acc + (warp * G + h) * HS + qd * 2;
@@ -952,11 +951,12 @@ template <int HS> static int sh_launch(const ShArgs& a, int pdl, cudaStream_t st
     // Many rows: two warps for each, so that an SM has six of them at work: what bounds a row are its latencies, one behind the other
     const bool many = (long long)a.M * a.n_kv_heads > 3ll * n_sms;
     const int warps = many ? 2 : 4;
-    auto* own_kernel = many ? shared_own_kernel<HS, 2> : shared_own_kernel<HS, 4>;
-    static SmemLimit given, given_own[2];
+    // (rows 8 to 15 of the MMAs and what belongs to them only where there are so many heads)
+    auto* own_kernel = G > 8 ? (many ? shared_own_kernel<HS, 2, 2> : shared_own_kernel<HS, 4, 2>) : many ? shared_own_kernel<HS, 2, 1> : shared_own_kernel<HS, 4, 1>;
+    static SmemLimit given, given_own[2][2];
     const size_t own_smem = sh_own_smem(HS, G, warps);
     if (const int rc = dl_smem_limit("dl_shared_attention", shared_attention_kernel<HS>, SH_SMEM, given)) return rc;
-    if (const int rc = dl_smem_limit("dl_shared_attention", own_kernel, own_smem, given_own[many])) return rc;
+    if (const int rc = dl_smem_limit("dl_shared_attention", own_kernel, own_smem, given_own[many][G > 8])) return rc;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -95,6 +95,7 @@ class Batch:
 CASES = [
     ([(3, 16, 60)], 32, 8, 128), ([(1, 5, 40)], 32, 8, 128), ([(2, 1, 1)], 4, 4, 128), ([(7, 3, 33), (5, 4, 70)], 32, 8, 64), ([(32, 25, 100)], 32, 8, 128), ([(33, 130, 40)], 32, 8, 128),
     ([(70, 9, 50)], 64, 8, 64), ([(4, 40, 900), (1, 0, 500), (9, 6, 20)], 16, 8, 128), ([(11, 300, 300)], 8, 2, 128), ([(40, 17, 64)], 16, 1, 128), ([(40, 17, 64)], 16, 1, 64), ([(5, 7, 10)], 6, 2, 64),
+    ([(70, 9, 50)], 128, 8, 64), ([(60, 5, 40)], 128, 8, 128), ([(23, 4, 40)], 18, 2, 128), ([(230, 4, 40)], 18, 2, 64),
     ([(130, 30, 45)], 8, 1, 128), ([(2, 2, 5)] * 8, 8, 4, 64), ([(9, 0, 200)], 32, 8, 128), ([(20, 64, 32), (20, 65, 32), (20, 66, 32), (20, 67, 32)], 16, 8, 64), ([(300, 12, 40)], 32, 8, 128),
 ]
 
