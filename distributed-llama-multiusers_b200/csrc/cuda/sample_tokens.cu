@@ -9,8 +9,8 @@
 //
 // A cluster of CTAs reads a row, from memory for its maximum, from the L2 then.  Nothing is sorted: "with which token does a sum, taken in some order, reach a target" is answered by bins and,
 // within the bin, of a few tokens, by comparing them with each other (StRow::select).  What takes part in that is a list in the first CTA's shared memory, in which the border has to lie:
-//   top-k   The least of as many maxima, each over tokens of its own, as k or more is not above the k-th largest logit.  The first pass leaves such maxima (of threads, or of warps); what is not
-//           below the least of them, some thousand tokens, goes into the list, and the rest of the row has no part: the first CTA does it all.
+//   top-k   The least of as many maxima, each over tokens of its own, as k or more is not above the k-th largest logit.  The first pass leaves such maxima (of threads, of 2, 4, .. 32
+//           threads: by steps of 4, of more than one row in a thousand more was left than the list takes); what is not below the least of them, some thousand tokens, goes into the list, and the rest of the row has no part: the first CTA does it all.
 //   top-p   A second pass counts the tokens in 4096 bins of their distance to the maximum.  A bin's weights differ by 0.5 %, so that the counts tell the sums to some 0.02 % (of heavy tokens, which
 //           would be most of that, their weights count: without it the list was too short for one row in a hundred, 200 rows 347 us instead of 152), and the border to a few bins.  A third pass adds up the weights: of the row, for the target, and of what lies ahead of those bins, for each warp's run of the row; the bins' tokens go into the list.
 //           The first CTA finds the border there, and the warp's run in which the token lies.
@@ -22,7 +22,7 @@
 // coin next to a border between two tokens would fall on the other side once in some thousand rows.
 //
 // What bounds it: for few rows some 25 phases, one behind the other, each a barrier of the cluster or a chain through shared memory, and code that is read once (one row of 128256 logits, us: top-p 22,
-// top-k and top-p 15, neither 11.5, min-p alone 8.3; the bytes 0.08); for many rows the instructions, 50 a token that is weighed (200 rows: 152, 74, 102, 46; the bytes 16).
+// top-k and top-p 15, neither 11.5, min-p alone 8.3; the bytes 0.08); for many rows the instructions, 50 a token that is weighed (200 rows: 152, 65, 102, 46; the bytes 16).
 #include <math_constants.h>
 #include <cuda_bf16.h>
 #include "common.cuh"
@@ -32,6 +32,7 @@
 #define ST_FINE 4096                   // bins of top-p's counts
 #define ST_HEAVY 1024                  // ... of which the first ones' tokens count by their weights
 #define ST_LIST 6144
+#define ST_LEVELS 6                    // sizes of the groups of threads whose maxima bound top-k
 #define ST_FEW 128                     // tokens that are compared with each other
 #define ST_MAX_CTAS 16
 #define ST_MAX_WARPS 32
@@ -67,13 +68,13 @@ struct alignas(16) StShared {
     u64 few_order[ST_FEW], few_weight[ST_FEW];
     u64 lo[ST_MAX_CTAS], hi[ST_MAX_CTAS];
     u64 cta_sum[ST_MAX_CTAS];
-    float top[ST_MAX_CTAS], low[4][ST_MAX_CTAS];      // each CTA's largest logit; the least of the largest ones of its threads, of 2, 8 and 32 of them
+    float top[ST_MAX_CTAS], low[ST_LEVELS][ST_MAX_CTAS];      // each CTA's largest logit; the least of the largest ones of its threads, of 2, 4, .. 32 of them
     StSums above, inside;              // of the bin found: what lies ahead of it and in it
     int bin, bin_from, bin_to;
     unsigned listed, others, few, done, first;      // listed: this CTA's; others: in CTA 0's the other ones'
     u64 found, upto;                   // the order of the token found, the sum up to it
     u64 warp_sum[ST_MAX_WARPS];
-    float warp_top[ST_MAX_WARPS], warp_low[3][ST_MAX_WARPS];
+    float warp_top[ST_MAX_WARPS], warp_low[ST_LEVELS - 1][ST_MAX_WARPS];
     StSums red[ST_MAX_WARPS];
     uint2 pow2[64];                    // 2^(j / 64): times 2^31, and as f32
 };
@@ -468,18 +469,19 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
     {
         float t = top;
 #pragma unroll
-        for (int g = 0; g < 3; g++) {
-            const float l = -warp_max(-t);
-            if (z.lane == 0) sh.warp_low[g][z.warp] = l;
+        for (int g = 0; g < ST_LEVELS - 1; g++) {
+            float l = t;
 #pragma unroll
-            for (int o = g == 0 ? 1 : g == 1 ? 4 : 16; o >= (g == 0 ? 1 : g == 1 ? 2 : 8); o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+            for (int o = 1 << g; o < 32; o <<= 1) l = fminf(l, __shfl_xor_sync(0xffffffffu, l, o));
+            if (z.lane == 0) sh.warp_low[g][z.warp] = l;
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1 << g));
         }
         if (z.lane == 0) sh.warp_top[z.warp] = t;
     }
     __syncthreads();
-    if (tid < ctas * 4) {
-        const int g = tid & 3, r = tid >> 2;
-        const float* from = g < 3 ? sh.warp_low[g] : sh.warp_top;
+    if (tid < ctas * 8 && (tid & 7) < ST_LEVELS) {
+        const int g = tid & 7, r = tid >> 3;
+        const float* from = g < ST_LEVELS - 1 ? sh.warp_low[g] : sh.warp_top;
         float t = sh.warp_top[0], l = from[0];
         for (int w = 1; w < THREADS / 32; w++) {
             t = fmaxf(t, sh.warp_top[w]);
@@ -582,7 +584,8 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
 
     if (q.by_k) {
         // ---- top-k: the list has all that can stay ----
-        const int groups = q.k <= ctas * WARPS ? 3 : q.k <= ctas * WARPS * 4 ? 2 : q.k <= ctas * WARPS * 16 ? 1 : q.k <= ctas * THREADS ? 0 : -1;
+        int groups = ST_LEVELS - 1;                             // the largest groups of which there are k
+        while (groups >= 0 && q.k > ctas * THREADS >> groups) groups--;
         float cut = -CUDART_INF_F;
         if (groups >= 0) {
             cut = sh.low[groups][0];

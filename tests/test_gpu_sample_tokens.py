@@ -225,3 +225,16 @@ def test_some_heavy_tokens_ahead_of_a_long_tail(dtype):
     p = np.concatenate([[0.9, 0.5, 0.99, 0.95], 1 - 10 ** rng.uniform(-4, -0.3, 44)]).tolist()
     check(torch.from_numpy(x).to(dtype).cuda(), t, None, p, None, rng.random(48).astype(np.float32).tolist())
     check(torch.from_numpy(x[:5]).to(dtype).cuda(), t[:5], None, p[:5], [0.0, 0.01, 0.0, 0.0, 1e-4], rng.random(5).astype(np.float32).tolist())
+
+
+@pytest.mark.parametrize("rows", [1, 3, 40, 160])
+def test_as_many_tokens_as_there_are_partial_maxima(rows):
+    """k at the numbers of groups whose maxima bound the list, and beside them, for clusters of every size."""
+    rng = np.random.default_rng(rows)
+    ks = sorted({b + d for n in (1, 3) for b in (n * 2 ** e for e in range(3, 13)) for d in (-1, 0, 1)})
+    x = rng.standard_normal((rows, 33000)) * 2
+    x[:, ::50] += 4
+    logits = torch.from_numpy(x).to(torch.bfloat16).cuda()
+    for i in range(0, len(ks), rows) if rows < 40 else [0]:
+        k = (ks[i:] + ks)[:rows] if rows < 40 else (ks * (rows // len(ks) + 1))[:rows]
+        check(logits, [0.9] * rows, k, [0.95] * rows, None, rng.random(rows).astype(np.float32).tolist())
