@@ -854,8 +854,8 @@ class LlamaEngine:
     # ------------------------------------------------------------------------------------------------
     def shares_prompt(self, n: int, n_pages: int) -> bool:
         """Whether n sequences that begin with the same n_pages pages read them once for all (K.shared_attention): over the fp16 cache, and where every sequence by itself would take longer.
-        Measured on 32 heads of 128 on 8, a layer's attention by itself / shared in us, own parts of 50 tokens: 2 sequences behind 1000 pages 40 / 45, 4 behind 64 11.5 / 19, behind 250 24 / 22,
-        8 behind 64 16 / 18, behind 250 42 / 22, 16 behind 64 22 / 19, 32 behind 16 11 / 16, behind 64 30 / 20, behind 1000 395 / 50, 64 behind 16 21 / 22, behind 64 60 / 28, 128 behind 16 34 / 35."""
+        Measured on 32 heads of 128 on 8, a layer's attention by itself / shared in us, own parts of 50 tokens: 4 sequences behind 1000 pages 79 / 39, 8 behind 64
+        16 / 18, behind 250 42 / 22, 16 behind 64 22 / 19, 32 behind 16 11 / 15, behind 64 30 / 19, behind 1000 395 / 43, 64 behind 16 21 / 21, behind 64 60 / 27, 128 behind 16 34 / 34."""
         fits = self.prefill_attention and not self.kv8 and self.n_heads_loc // self.n_kv_loc <= 16 and not self._mega_usable(n, False)
         return fits and n >= SHARE_MIN_ROWS and n_pages >= SHARE_MIN_PAGES and n * n_pages >= SHARE_MIN_WORK
 
