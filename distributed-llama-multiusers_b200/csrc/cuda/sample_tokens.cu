@@ -449,6 +449,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
     const int first = rank * a.slice;
     StRow<T, THREADS> z{sh, reinterpret_cast<const T*>(a.logits) + (long long)row * a.ld + first, first, max(0, min(a.vocab - first, a.slice)), a.wide != 0,
                         rank, ctas, tid, tid >> 5, tid & 31, cluster, {0.f, 0.f, 0.f}};
+    cluster_arrive_relaxed();                                   // (a CTA's shared memory is there once it has started: cluster_wait() ahead of the first store into another one's)
     pdl_launch_dependents();
     if (tid < 64) {
         const double p = exp2((double)tid / 64.0);
@@ -479,6 +480,7 @@ __global__ void __launch_bounds__(THREADS, PER_SM) sample_tokens_kernel(const __
         if (z.lane == 0) sh.warp_top[z.warp] = t;
     }
     __syncthreads();
+    cluster_wait();
     if (tid < ctas * 8 && (tid & 7) < ST_LEVELS) {
         const int g = tid & 7, r = tid >> 3;
         const float* from = g < ST_LEVELS - 1 ? sh.warp_low[g] : sh.warp_top;
