@@ -36,6 +36,7 @@
 #define SH_ONE_COST 4                  // ... with one
 #define SH_LEAST_COST 8                // of a CTA's share: two steps of one tile
 #define SH_BAD 8                       // items of a CTA that can be at work at once, and more
+#define SH_FAR 0x1p20f                 // references in the log2 domain whose rounding shows in the weights
 #define SH_OWN_TOK 16                  // tokens of a warp's turn
 #define SH_OWN_MAX_CTAS 8
 
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
                     for (int c = 0; c < 4; c++) mx4[c] = pt_max<true>(mx4[c], pt_max<true>(__uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1])));
                 const float mx = pt_max<true>(pt_max<true>(mx4[0], mx4[1]), pt_max<true>(mx4[2], mx4[3])) * sc;
                 // the reference may lag the maximum by 2^8; a NaN makes it NaN, and with it the sum of the weights for good
-                const bool need = !(mx <= m_used + 8.0f);
+                const bool need = !(mx <= m_used || mx - m_used <= 8.0f);
                 const bool moved = __any_sync(0xffffffffu, need);
                 float alpha = 1.f;
                 if (moved) {
@@ -390,6 +391,17 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
                     m_used = m_new;
                 }
                 const float ref = (m_used == -INFINITY) ? 0.0f : m_used;
+                float by = sc, from = ref;
+                if (__any_sync(0xffffffffu, fabsf(ref) >= SH_FAR)) {
+                    // the exact product less a rounded one leaves the largest score that rounding for an exponent (from 2^28 on up to 16 either way: a weight beyond fp16, or next to
+                    // none): the rounded products, as the maximum was formed
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int e = 0; e < 32; e++) v[c][e] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(v[c][e]), sc), ref));
+                    by = 1.f;
+                    from = 0.f;
+                }
                 pair_f sum = 0;
                 uint32_t pk[4][16], none[1];
                 if (j > ja) wait(&o_full[t], (ns - 1) & 1);
@@ -407,7 +419,7 @@ __global__ void __launch_bounds__(SH_THREADS, 1) shared_attention_kernel(const _
                 }
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    pt_probs<false>(v[c], sc, ref, pk[c], none, sum);
+                    pt_probs<false>(v[c], by, from, pk[c], none, sum);
                     tmem_st_32x32b_x16(T_P + c * 16, pk[c]);
                 }
                 l += pair_sum(sum);
