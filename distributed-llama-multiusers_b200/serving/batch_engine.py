@@ -22,7 +22,7 @@ import torch
 
 from ..parallel.control import OP_FORWARD, OP_STOP, OP_WARMUP, ControlChannel
 from ..text import native as T
-from .filters import Filters
+from .filters import Filters, settings
 
 
 PAGE_TOKENS = 32          # tokens per KV page (ops.kernels.PAGE_SIZE)
@@ -48,6 +48,7 @@ class GenerationRequest:
     t_submit: float = 0.0
     t_first_token: Optional[float] = None
     t_done: Optional[float] = None
+    _filters: tuple = (0, 0.0)                  # top_k and min_p as they are drawn with
     _sampler: Optional[T.Sampler] = None
     _decoder: Optional[T.StreamDecoder] = None
     _stops: Optional[T.EosDetector] = None
@@ -112,6 +113,7 @@ class BatchEngine:
     def submit(self, req: GenerationRequest) -> GenerationRequest:
         if (req.top_k > 0 or req.min_p > 0) and not self._device_sampler:
             raise ValueError("top_k and min_p need the device sampler")
+        req._filters = settings(req.top_k, req.min_p, self.engine.h.vocab_size)
         req.id = next(self._ids)
         req.t_submit = time.time()
         req._sampler = T.Sampler(self.engine.h.vocab_size, req.temperature, req.top_p, req.seed or req.id)
@@ -213,11 +215,11 @@ class BatchEngine:
                     hp[0, i], hp[1, i] = r.temperature, r.top_p
                     hp[2, i] = r._sampler.coin() if r.temperature != 0.0 else 0.0
             self._d_params.copy_(self._h_params, non_blocking=True)
-            n_on = sum(r is not None and (r.top_k > 0 or r.min_p > 0) for r in rows)
+            n_on = sum(r is not None and any(r._filters) for r in rows)
             if n_on:
                 f = self._filters
                 for i, r in enumerate(rows):
-                    f.top_k[i], f.min_p[i] = (r.top_k, r.min_p) if r is not None else (0, 0.0)
+                    f.top_k[i], f.min_p[i] = r._filters if r is not None else (0, 0.0)
                 f.draw(logits, n_s, n_on, self._d_params, self._sample_rows, self._d_tok)
             else:
                 self._sample_rows(logits[:n_s], self._d_params[0], self._d_params[1], self._d_params[2], self._d_tok)

@@ -4,6 +4,11 @@ from __future__ import annotations
 import torch
 
 
+def settings(top_k, min_p, vocab: int) -> tuple:
+    """top_k and min_p of a request as the kernel takes them: 0 where they take nothing out (a top_k below 1, or of the vocabulary or more; a min_p not above 0), a min_p of 1 at most."""
+    return int(top_k) if 0 < top_k < vocab else 0, min(float(min_p), 1.0) if min_p > 0 else 0.0
+
+
 class Filters:
     """Settings of up to `rows` rows: written into top_k (int32, 0: off) and min_p (f32, 0: off) on the host, pinned, and read by draw()."""
 
