@@ -445,7 +445,7 @@ bool parse_params(const Server* s, const Value& body, Params& p, std::string& er
     if (const Value* v = body.get("stream")) p.stream = v->truthy();
     if (num("temperature", d)) p.temperature = (float)d;
     if (num("top_p", d)) p.topp = (float)d;
-    if (num("top_k", d)) p.top_k = d >= 1.0 ? (int)std::min(d, 2147483647.0) : 0;
+    if (num("top_k", d)) p.top_k = d >= 1.0 && d < (double)s->vocab ? (int)d : 0;      // (of the vocabulary or more: it takes nothing out)
     if (num("min_p", d)) p.min_p = (float)d;
     if (err.empty() && (p.top_k > 0 || p.min_p > 0.f) && !s->filters) err = "`top_k` and `min_p` need the device sampler";
     if (const Value* v = body.get("seed")) {

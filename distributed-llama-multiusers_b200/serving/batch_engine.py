@@ -111,9 +111,9 @@ class BatchEngine:
 
     # ---- client side (any thread) ------------------------------------------------------------------
     def submit(self, req: GenerationRequest) -> GenerationRequest:
-        if (req.top_k > 0 or req.min_p > 0) and not self._device_sampler:
-            raise ValueError("top_k and min_p need the device sampler")
         req._filters = settings(req.top_k, req.min_p, self.engine.h.vocab_size)
+        if any(req._filters) and not self._device_sampler:
+            raise ValueError("top_k and min_p need the device sampler")
         req.id = next(self._ids)
         req.t_submit = time.time()
         req._sampler = T.Sampler(self.engine.h.vocab_size, req.temperature, req.top_p, req.seed or req.id)
