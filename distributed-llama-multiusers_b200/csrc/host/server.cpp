@@ -133,7 +133,7 @@ struct Server {
     std::string chat_eos;
     int vocab = 0;
     float def_temp = 0.8f, def_topp = 0.9f;
-    bool filters = false;               // top_k and min_p can be served (dl_srv_set_filters)
+    int filters = 0;                    // top_k and min_p: 0 refused, 1 served, 2 not looked at (dl_srv_set_filters)
     unsigned long long def_seed = 0;
     int max_default_tokens = 128;
     int max_waiting = 4096;             // admission queue bound (DLLAMA_MAX_WAITING): beyond it requests get 503
@@ -445,9 +445,11 @@ bool parse_params(const Server* s, const Value& body, Params& p, std::string& er
     if (const Value* v = body.get("stream")) p.stream = v->truthy();
     if (num("temperature", d)) p.temperature = (float)d;
     if (num("top_p", d)) p.topp = (float)d;
-    if (num("top_k", d)) p.top_k = d >= 1.0 && d < (double)s->vocab ? (int)d : 0;      // (of the vocabulary or more: it takes nothing out)
-    if (num("min_p", d)) p.min_p = (float)d;
-    if (err.empty() && (p.top_k > 0 || p.min_p > 0.f) && !s->filters) err = "`top_k` and `min_p` need the device sampler";
+    if (s->filters != 2) {
+        if (num("top_k", d)) p.top_k = d >= 1.0 && d < (double)s->vocab ? (int)d : 0;      // (of the vocabulary or more: it takes nothing out)
+        if (num("min_p", d)) p.min_p = (float)d;
+        if (err.empty() && (p.top_k > 0 || p.min_p > 0.f) && s->filters == 0) err = "`top_k` and `min_p` need the device sampler";
+    }
     if (const Value* v = body.get("seed")) {
         if (v->type == Value::NUM) p.seed = (unsigned long long)v->inum;
         else if (!v->is_null()) err = "`seed` must be a number";
@@ -970,8 +972,8 @@ int dl_srv_next_batch(void* sv, int* tokens, int* pos, int* slots, int cap, int*
     return n;
 }
 
-// Whether requests may ask for top_k and min_p (the caller samples with dl_srv_batch_filters' settings); off until it is said.
-void dl_srv_set_filters(void* sv, int on) { ((Server*)sv)->filters = on != 0; }
+// Requests with top_k or min_p: 0 (until it is said) refused, 1 served (the caller samples with dl_srv_batch_filters' settings), 2 served as without them.
+void dl_srv_set_filters(void* sv, int how) { ((Server*)sv)->filters = how; }
 
 // top_k and min_p of the sampling rows of the batch last formed; returns how many rows have one of them on.
 int dl_srv_batch_filters(void* sv, int* top_k, float* min_p, int cap) {

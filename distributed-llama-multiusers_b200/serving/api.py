@@ -116,6 +116,8 @@ def make_handler(state: ApiState):
             try:
                 n = int(self.headers.get("Content-Length", "0"))
                 body = json.loads(self.rfile.read(n).decode("utf-8")) if n > 0 else {}
+                if state.batch.ignores_filters and isinstance(body, dict):
+                    body = {k: v for k, v in body.items() if k not in ("top_k", "min_p")}
                 params = A.parse_inference_params(body, state.defaults)
                 if not params.messages:
                     return self._json(400, {"error": {"message": "Prompt is empty.", "type": "invalid_request_error"}})

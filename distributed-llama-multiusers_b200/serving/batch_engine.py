@@ -22,7 +22,7 @@ import torch
 
 from ..parallel.control import OP_FORWARD, OP_STOP, OP_WARMUP, ControlChannel
 from ..text import native as T
-from .filters import Filters, settings
+from .filters import Filters, host_ignores, settings
 
 
 PAGE_TOKENS = 32          # tokens per KV page (ops.kernels.PAGE_SIZE)
@@ -91,6 +91,7 @@ class BatchEngine:
         # the host sampler (reference-exact arithmetic) serves CPU engines and DLLAMA_HOST_SAMPLER=1
         dev = getattr(engine, "device", torch.device("cpu"))
         self._device_sampler = dev.type == "cuda" and os.environ.get("DLLAMA_HOST_SAMPLER", "0") != "1"
+        self.ignores_filters = not self._device_sampler and host_ignores()
         if self._device_sampler:
             # an engine with a kernel library of its own brings its binding of the sampler
             self._sample_rows = getattr(engine, "sample_rows", None)
@@ -111,7 +112,7 @@ class BatchEngine:
 
     # ---- client side (any thread) ------------------------------------------------------------------
     def submit(self, req: GenerationRequest) -> GenerationRequest:
-        req._filters = settings(req.top_k, req.min_p, self.engine.h.vocab_size)
+        req._filters = (0, 0.0) if self.ignores_filters else settings(req.top_k, req.min_p, self.engine.h.vocab_size)
         if any(req._filters) and not self._device_sampler:
             raise ValueError("top_k and min_p need the device sampler")
         req.id = next(self._ids)

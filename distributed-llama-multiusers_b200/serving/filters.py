@@ -1,7 +1,14 @@
 """top_k and min_p of a batch's rows, for the loops that draw on the GPU."""
 from __future__ import annotations
 
+import os
+
 import torch
+
+
+def host_ignores() -> bool:
+    """DLLAMA_HOST_FILTERS=ignore: loops that sample on the host leave top_k and min_p out of account, as they do with fields that they do not know."""
+    return os.environ.get("DLLAMA_HOST_FILTERS", "refuse") == "ignore"
 
 
 def settings(top_k, min_p, vocab: int) -> tuple:

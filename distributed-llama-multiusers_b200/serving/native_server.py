@@ -22,7 +22,7 @@ import torch
 from ..parallel.control import OP_FORWARD, OP_STOP, OP_WARMUP, ControlChannel
 from ..text import native as T
 from . import api_types as A
-from .filters import Filters
+from .filters import Filters, host_ignores
 
 
 class NativeApiServer:
@@ -74,6 +74,8 @@ class NativeApiServer:
             self._L.dl_srv_set_filters(self._h, 1)
         else:
             self._logits_host = pin(torch.empty(R, engine.h.vocab_size, dtype=torch.float32))
+            if host_ignores():
+                self._L.dl_srv_set_filters(self._h, 2)
         self._stop = threading.Event()
         self._thread: Optional[threading.Thread] = None
         self.n_errors = 0

@@ -25,6 +25,7 @@ ENV_VARS = {
     "DLLAMA_LAYERS_TC_MIN_ROWS": ("32", "layer-list models: batch size from which matrix products run on the tcgen05 GEMM"),
     # serving / tensor-parallel control
     "DLLAMA_HOST_SAMPLER": ("0", "1 = sample on the host (reference-exact sampler) instead of the device kernel"),
+    "DLLAMA_HOST_FILTERS": ("refuse", "requests with top_k or min_p where the host samples: refuse (400) or ignore (served as without them)"),
     "DLLAMA_MAX_WAITING": ("4096", "requests the native server queues before it answers 503"),
     "DLLAMA_CTL_TIMEOUT_S": ("120", "how long the root waits for a worker's acknowledgement of a batch"),
     "DLLAMA_RUN_NONCE": ("derived", "run identifier of the control mailbox (stale files of earlier runs are ignored)"),

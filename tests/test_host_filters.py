@@ -69,3 +69,41 @@ def test_what_takes_nothing_out_is_served(tiny_model_path, tok):
             with pytest.raises(urllib.error.HTTPError) as err:
                 s.post(**kw)
             assert err.value.code == 400
+
+
+def test_requests_are_served_without_them_where_that_is_said(tiny_model_path, tok, monkeypatch):
+    """DLLAMA_HOST_FILTERS=ignore: clients that send top_k with every request keep their server, whatever its value's type."""
+    e = _engine(tiny_model_path)
+    monkeypatch.setenv("DLLAMA_HOST_FILTERS", "ignore")
+    be = BatchEngine(e, tok)
+    plain = _loop(be)
+    for kw in ({"top_k": 5}, {"min_p": 0.1}, {"top_k": 40, "min_p": 0.5}):
+        assert _loop(be, **kw) == plain
+    with _Server(e, tok) as s:
+        plain = s.post()
+        for kw in ({"top_k": 5}, {"min_p": 0.1}, {"top_k": 40, "min_p": 0.5}, {"top_k": "many"}, {"min_p": [1]}):
+            assert s.post(**kw) == plain
+
+
+def test_the_python_front_end_leaves_them_out_as_well(tiny_model_path, tok, monkeypatch):
+    import threading
+    from http.server import ThreadingHTTPServer
+    from dllama_b200.serving.api import ApiState, make_handler
+    monkeypatch.setenv("DLLAMA_HOST_FILTERS", "ignore")
+    be = BatchEngine(_engine(tiny_model_path), tok)
+    be.start()
+    state = ApiState(be, tok, "tiny.m", A.InferenceParams(messages=[], temperature=0.8, top_p=0.9, seed=1))
+    srv = ThreadingHTTPServer(("127.0.0.1", 0), make_handler(state))
+    threading.Thread(target=srv.serve_forever, daemon=True).start()
+    try:
+        def post(**kw):
+            body = {"messages": [{"role": "user", "content": "hello"}], "max_tokens": 4, "seed": 5, **kw}
+            req = urllib.request.Request(f"http://127.0.0.1:{srv.server_address[1]}/v1/chat/completions", data=json.dumps(body).encode(), method="POST")
+            with urllib.request.urlopen(req, timeout=60) as r:
+                return json.load(r)["choices"][0]["message"]["content"]
+        plain = post()
+        for kw in ({"top_k": 5}, {"min_p": 0.1}, {"top_k": "many"}):
+            assert post(**kw) == plain
+    finally:
+        srv.shutdown()
+        be.stop()
