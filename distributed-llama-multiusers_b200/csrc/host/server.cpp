@@ -448,7 +448,7 @@ bool parse_params(const Server* s, const Value& body, Params& p, std::string& er
     if (s->filters != 2) {
         if (num("top_k", d)) p.top_k = d >= 1.0 && d < (double)s->vocab ? (int)d : 0;      // (of the vocabulary or more: it takes nothing out)
         if (num("min_p", d)) p.min_p = (float)d;
-        if (err.empty() && (p.top_k > 0 || p.min_p > 0.f) && s->filters == 0) err = "`top_k` and `min_p` need the device sampler";
+        if (err.empty() && (p.top_k > 0 || p.min_p > 0.f) && s->filters == 0) err = "`top_k` and `min_p` need the device sampler and a vocabulary that it takes";
     }
     if (const Value* v = body.get("seed")) {
         if (v->type == Value::NUM) p.seed = (unsigned long long)v->inum;

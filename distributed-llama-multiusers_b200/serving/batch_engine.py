@@ -22,7 +22,7 @@ import torch
 
 from ..parallel.control import OP_FORWARD, OP_STOP, OP_WARMUP, ControlChannel
 from ..text import native as T
-from .filters import Filters, host_ignores, settings
+from .filters import MAX_VOCAB, Filters, host_ignores, settings
 
 
 PAGE_TOKENS = 32          # tokens per KV page (ops.kernels.PAGE_SIZE)
@@ -91,7 +91,8 @@ class BatchEngine:
         # the host sampler (reference-exact arithmetic) serves CPU engines and DLLAMA_HOST_SAMPLER=1
         dev = getattr(engine, "device", torch.device("cpu"))
         self._device_sampler = dev.type == "cuda" and os.environ.get("DLLAMA_HOST_SAMPLER", "0") != "1"
-        self.ignores_filters = not self._device_sampler and host_ignores()
+        self._serves_filters = self._device_sampler and engine.h.vocab_size <= MAX_VOCAB
+        self.ignores_filters = not self._serves_filters and host_ignores()
         if self._device_sampler:
             # an engine with a kernel library of its own brings its binding of the sampler
             self._sample_rows = getattr(engine, "sample_rows", None)
@@ -113,8 +114,8 @@ class BatchEngine:
     # ---- client side (any thread) ------------------------------------------------------------------
     def submit(self, req: GenerationRequest) -> GenerationRequest:
         req._filters = (0, 0.0) if self.ignores_filters else settings(req.top_k, req.min_p, self.engine.h.vocab_size)
-        if any(req._filters) and not self._device_sampler:
-            raise ValueError("top_k and min_p need the device sampler")
+        if any(req._filters) and not self._serves_filters:
+            raise ValueError(f"top_k and min_p need the device sampler and a vocabulary of at most {MAX_VOCAB} tokens")
         req.id = next(self._ids)
         req.t_submit = time.time()
         req._sampler = T.Sampler(self.engine.h.vocab_size, req.temperature, req.top_p, req.seed or req.id)

@@ -5,6 +5,8 @@ import os
 
 import torch
 
+MAX_VOCAB = 1 << 19          # of sample_tokens (dl_sample_tokens_max_vocab)
+
 
 def host_ignores() -> bool:
     """DLLAMA_HOST_FILTERS=ignore: loops that sample on the host leave top_k and min_p out of account, as they do with fields that they do not know."""

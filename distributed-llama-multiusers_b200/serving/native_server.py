@@ -22,7 +22,7 @@ import torch
 from ..parallel.control import OP_FORWARD, OP_STOP, OP_WARMUP, ControlChannel
 from ..text import native as T
 from . import api_types as A
-from .filters import Filters, host_ignores
+from .filters import MAX_VOCAB, Filters, host_ignores
 
 
 class NativeApiServer:
@@ -71,11 +71,9 @@ class NativeApiServer:
             self._d_params = torch.zeros(3, R, dtype=torch.float32, device=dev)
             self._d_tok = torch.zeros(R, dtype=torch.int32, device=dev)
             self._filters = Filters(R, dev)
-            self._L.dl_srv_set_filters(self._h, 1)
         else:
             self._logits_host = pin(torch.empty(R, engine.h.vocab_size, dtype=torch.float32))
-            if host_ignores():
-                self._L.dl_srv_set_filters(self._h, 2)
+        self._L.dl_srv_set_filters(self._h, 1 if self._device_sampler and engine.h.vocab_size <= MAX_VOCAB else 2 if host_ignores() else 0)
         self._stop = threading.Event()
         self._thread: Optional[threading.Thread] = None
         self.n_errors = 0
