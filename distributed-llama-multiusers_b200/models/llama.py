@@ -483,7 +483,7 @@ class LlamaEngine:
         """Enqueue one forward over rows 0..M-1 of the descriptor; logits for rows row0..M-1.  groups: rows whose sequences begin with the same pages
         (K.shared_attention; fp16 cache, no prompt chunks)."""
         h, N, pdl = self.h, self.world, self.use_pdl
-        if self._mega_usable(M, chunk):
+        if groups is None and self._mega_usable(M, chunk):
             K.decode_mega(self._mega_args(M, row0, greedy, device_loop), self.mega_grid)
             if not greedy and N > 1:
                 K.wait_flags(self.flags_log_local, N, self.step_counter, 1, 0)
