@@ -580,7 +580,7 @@ def sample_tokens(logits: torch.Tensor, M: int, temperature: torch.Tensor, top_k
                                      _on_device(tokens_out, _I32, M, d, "tokens_out"), _on_device(prob_out, _F32, M, d, "prob_out"), 1 if pdl else 0, torch._C._cuda_getCurrentRawStream(d))
     if rc:
         check(rc, "dl_sample_tokens")
-    lib.count_launch()
+    lib.count_launch(1 if M else 0)
 
 
 @functools.lru_cache(maxsize=1)
