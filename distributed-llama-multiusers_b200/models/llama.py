@@ -904,7 +904,7 @@ class LlamaEngine:
                 self.shared_work = K.shared_attention_workspace(n, self.n_heads_loc, self.n_kv_loc, self.hs, dev)
             drawn = torch.empty(max_tokens, n, dtype=torch.int32, device=dev)
             coin, f32 = torch.empty(n, dtype=torch.float32, device=dev), lambda v: torch.full((n,), v, dtype=torch.float32, device=dev)
-            filters = (f32(temperature), i32([max(0, min(int(top_k), (1 << 31) - 1))] * n), f32(top_p), f32(min_p), coin)
+            filters = (f32(temperature), i32([max(0, min(int(top_k), (1 << 31) - 1))] * n), f32(top_p), f32(min(min_p, 1.0)), coin)
             tokens = self.tokens[:n]
             coin.copy_(coins[0])
             K.sample_tokens(logits[:1].expand(n, -1).contiguous(), n, *filters, tokens)

@@ -44,3 +44,15 @@ def test_what_the_settings_mean():
     for (k, p), want in (((0, 0.0), (0, 0.0)), ((40, 0.05), (40, 0.05)), ((999, 1.0), (999, 1.0)), ((1000, 2.0), (0, 1.0)), ((10 ** 30, 1e300), (0, 1.0)), ((-(10 ** 30), -1e300), (0, 0.0)),
                          ((math.nan, math.nan), (0, 0.0)), ((math.inf, math.inf), (0, 1.0)), ((0.5, 1e-30), (0, 1e-30)), ((2.7, 0.0), (2, 0.0))):
         assert settings(k, p, 1000) == want
+
+
+@pytest.mark.gpu
+def test_sample_many_with_a_min_p_beyond_32_bits(tiny_model_path):
+    """Above 1 it is 1, however large: the first of the largest logits, as top_k 1."""
+    from dllama_b200.models.llama import LlamaEngine
+    e = LlamaEngine(tiny_model_path, max_rows=32, n_slots=8, max_seq_len=256)
+    want = e.sample_many([1, 5, 9], 3, 8, 1.3, top_k=1, top_p=0.0)
+    for min_p in (1.0, 7.0, 1e300, math.inf):
+        assert (e.sample_many([1, 5, 9], 3, 8, 1.3, top_p=0.0, min_p=min_p) == want).all()
+    assert (e.sample_many([1, 5, 9], 3, 8, 1.3, top_k=10 ** 30, top_p=0.0, min_p=1e300) == want).all()
+    e.close()
