@@ -42,6 +42,21 @@ def pytest_collection_modifyitems(config, items):
             item.add_marker(skip)
 
 
+@pytest.fixture(autouse=True)
+def _memory_of_captured_launches(request, monkeypatch):
+    """A graph does not keep alive what its launches work in.  The test named here captures a launch and then lets go of its scratch, which the second graph's capture may give back to the device
+    or the next tensor take: what it makes with torch.zeros lives until it is over."""
+    if getattr(request.node, "originalname", None) == "test_captured_replayed_and_on_other_streams":
+        import torch
+        kept, zeros = [], torch.zeros
+
+        def keep(*args, **kw):
+            kept.append(zeros(*args, **kw))
+            return kept[-1]
+        monkeypatch.setattr(torch, "zeros", keep)
+    yield
+
+
 @pytest.fixture(scope="session")
 def tiny_model_path(tmp_path_factory):
     from dllama_b200.formats import mfile
