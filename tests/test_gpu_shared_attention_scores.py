@@ -92,3 +92,18 @@ def test_scores_that_grow_from_small_to_very_large():
         t = 60 * PAGE - 1 if order > 0 else 0
         want = b.v[lead[t // PAGE], :, t % PAGE].double()
         assert ((y - want[None, :, None]).abs() <= OFF * want[None, :, None].abs()).all()
+
+
+@pytest.mark.parametrize("hs", [64, 128])
+def test_scores_beyond_f32(hs):
+    """A row with a score that f32 does not hold is NaN, whichever part of the positions has it and whatever its sign is where there are no others; its neighbours keep their values."""
+    b = Batch(31, [(6, 12, 60), (2, 0, 40)], 8, 2, hs)
+    q = b.q.view(b.M, 8, hs)
+    q[2], q[7] = torch.sign(q[2]) * 3e38, torch.sign(q[7]) * 3e38
+    y = b.run().view(b.M, 8, hs)
+    for m in range(b.M):
+        page, place = _lines(b, m)
+        s = torch.matmul(q[m].double().view(2, 4, hs), b.k[page, :, place].double().permute(1, 2, 0)) * 1.4426950408889634 / hs ** 0.5
+        beyond = (s > 3.5e38).any(-1).flatten() | (s < -3.5e38).all(-1).flatten()
+        assert beyond.all() == (m in (2, 7)) and torch.isnan(y[m]).all(-1)[beyond].all()
+    b.check(y.reshape(b.M, -1), rows=[0, 1, 3, 4, 5, 6])
