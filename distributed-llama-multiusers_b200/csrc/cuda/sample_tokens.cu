@@ -17,12 +17,14 @@
 //   else    as top-p, without a border.
 // Where the list does not do -- more tokens than it takes, a border that is not in it -- all CTAs select over the whole row, by bins that are divided until few tokens are left.
 //
-// Weights are whole numbers of 2^-44, so that sums do not depend on their order; they are exact to 2^-29 of themselves (a table of 64 powers of two and a
-// polynomial, after P. T. P. Tang's table-driven exponential, on the difference and the factor as pairs of f32 numbers): with sums of f32 results a
-// coin next to a border between two tokens would fall on the other side once in some thousand rows.
+// Weights are whole numbers of 2^-44, so that sums do not depend on their order; they are off by 2^-29 of themselves (a table of 64 powers of two and a
+// polynomial, after P. T. P. Tang's table-driven exponential, on the difference and the factor as pairs of f32 numbers) and half a unit, 2^-45 of the largest one's: a sum over V tokens by 2^-29 of
+// itself and V 2^-45 at most, 2^-26 for the largest vocabulary.  With sums of f32 results a coin next to a border between two tokens would fall on the other side once in some thousand rows.
 //
-// What bounds it: for few rows some 25 phases, one behind the other, each a barrier of the cluster or a chain through shared memory, and code that is read once (one row of 128256 logits, us: top-p 22,
-// top-k and top-p 15, neither 11.5, min-p alone 8.3; the bytes 0.08); for many rows the instructions, 50 a token that is weighed (200 rows: 152, 65, 102, 46; the bytes 16).
+// What bounds it: for few rows some 25 phases, one behind the other, each a barrier of the cluster or a chain through shared memory, and code that is read once (one row of 128256 logits, us: top-p 22.6,
+// top-k and top-p 16, neither 12, min-p alone 9; the bytes 0.08).  200 rows take 153, 64, 102 and 47 us (the bytes 16): 100, 24, 72 and 15 instructions a token, which alone would take 70, 17, 50 and 11 us.
+// With seven warps a scheduler (56 registers) they issue in 54, 37, 57 and 27 % of its cycles; what the warps wait for in the others are loads, of rows that come from the L2 the second time and in part
+// from memory (136 to 206 MB for 103), first, then what the instruction ahead has to leave.
 #include <math_constants.h>
 #include <cuda_bf16.h>
 #include "common.cuh"

@@ -10,13 +10,14 @@
 // key/value head and begin the next).  It leaves m, l and o of each piece.  The second launch takes the rows' own pages, a CTA (a cluster, where rows are few) for each row and
 // key/value head, 16 tokens at a time on mma.sync, and joins them with the pieces; it is launched while the first one runs and waits for it ahead of the join.
 //
-// Both have queries and weights in fp16 (queries times a power of two of their row, so that any size goes in; weights at most 2^8), sums and maxima in f32: 2^-12 of a weight is
-// what a result is off by, at random, an eighth of the half step of a bf16 output.
+// Both have queries and weights in fp16 (queries times a power of two of their row, so that any size goes in; weights at most 2^8), sums and maxima in f32: 2^-12 of a weight (of one below 2^-14 of
+// the largest 2^-25 of that one's) is what a result is off by, at random, an eighth of the half step of a bf16 output.  Scores are f32 in the log2 domain: beyond its range, 2^128, a row is NaN.
 //
-// What bounds it (us of both launches, 32 heads of 128 on 8): 3 rows behind 16 pages 15.4 and 32 behind 250 with up to 300 tokens of their own 31 (the bytes 8): latencies one behind the other, of which the first
-// launch has 6 us ahead of its first scores (places, plan, queries), a step's 1.0 to 1.8, 3 for sums on their way out, and the second one 5 for the join behind it.  200 behind 1000 with up to 400 of their own 143 (the
-// products 66): a step of two tiles takes 1.8 us, of which the MMAs run 0.6: the chain scores, maximum, exponentials, weights of one tile is hidden by the other one's alone (more of the exponentials as
-// polynomials: 154 to 158); the second launch reads the rows' own pages at 3.5 TB/s for 50 us, its CTAs of 200 tokens being starts and ends for the greater part.
+// What bounds it (us of both launches, 32 heads of 128 on 8): 3 rows behind 16 pages 16 and 32 behind 250 with up to 300 tokens of their own 32 (the bytes 8): latencies one behind the other, of which the first
+// launch has 6 us ahead of its first scores (places, plan, queries), a step's 1.0 to 1.8, 3 for sums on their way out, and the second one 5 for the join behind it.  200 behind 1000 with up to 400 of their own 147 (the
+// products 66), and 174 once the card is at its power limit, after some 50 ms of nothing else (1545 MHz instead of 1965): a step of two tiles takes 1.8 us, of which the MMAs run 0.6: the chain scores,
+// maximum, exponentials, weights of one tile is hidden by the other one's alone (more of the exponentials as polynomials: 154 to 158); the second launch reads the rows' own pages at 3.5 TB/s for 50 us, its
+// CTAs of 200 tokens being starts and ends for the greater part.
 #define WAIT_UNIT 5u
 #include "attention_tc.cuh"
 #include "epilogue.cuh"

@@ -854,8 +854,13 @@ class LlamaEngine:
     # ------------------------------------------------------------------------------------------------
     def shares_prompt(self, n: int, n_pages: int) -> bool:
         """Whether n sequences that begin with the same n_pages pages read them once for all (K.shared_attention): over the fp16 cache, and where every sequence by itself would take longer.
-        Measured on 32 heads of 128 on 8, a layer's attention by itself / shared in us, own parts of 50 tokens: 4 sequences behind 1000 pages 79 / 39, 8 behind 64
-        16 / 18, behind 250 42 / 22, 16 behind 64 22 / 19, 32 behind 16 11 / 15, behind 64 30 / 19, behind 1000 395 / 43, 64 behind 16 21 / 21, behind 64 60 / 27, 128 behind 16 34 / 34."""
+        Measured, a layer's attention by itself / shared in us, sequences x pages, own parts of 50 to 100 tokens:
+
+        * 32 heads of 128 on 8: 4 x 1000 79 / 42, 8 x 64 16 / 19, 8 x 128 25 / 21, 4 x 256 26 / 25 (own parts of 600 27 / 28), 16 x 64 22 / 19, 32 x 16 12 / 16, 32 x 32 18 / 16, 32 x 1000 395 / 46, 64 x 16
+          21 / 22, 64 x 64 60 / 29, 128 x 16 35 / 36.  Heads of 64, or 8 to 32 heads on as many: the same borders.  2 x 1000 40 / 42 and 3 x 1000 56 / 42: few gain below four sequences.
+        * more than four heads on a key/value head: sharing takes less from 2 x 16 on (64 heads of 128 on 8: 25 / 17, 32 x 32 83 / 23; 8 on 1: 16 x 64 21 / 18, 32 x 32 19 / 21), here with the others' border.
+        * up to four on each of fewer than eight key/value heads, which leave less to read: it takes more up to some 8192 / key/value heads sequences x pages (8 heads of 128 on 2: 16 x 64 12 / 16, 32 x 32
+          12 / 15, 64 x 32 13 / 19, 32 x 64 16 / 16, 64 x 64 22 / 20, 32 x 1000 150 / 27), 2 to 5 us a layer that this border does not keep out."""
         fits = self.prefill_attention and not self.kv8 and self.n_heads_loc // self.n_kv_loc <= 16 and not self._mega_usable(n, False)
         return fits and n >= SHARE_MIN_ROWS and n_pages >= SHARE_MIN_PAGES and n * n_pages >= SHARE_MIN_WORK
 

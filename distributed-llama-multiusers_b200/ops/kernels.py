@@ -473,8 +473,8 @@ def shared_attention(q, M: int, n_heads: int, pos, slot, block_table, groups, k_
                      y_out=None, pdl: bool = False):
     """`attention` over the fp16 cache where groups of rows begin with the same pages, which are read once for all of them: groups = [n, begin, end, pages, ...] (device int32), rows begin .. end - 1
     naming the same pages in the first `pages` places of their block tables; eight groups at most, in the order of their rows (a row of two belongs to the first one), rows of no group by themselves.
-    What not all rows of a group see is not shared.  Heads of 64 and 128, up to 16 query heads for each key/value head.  Queries (times a power of two of the row) and weights are fp16; y_out is
-    f32, fp16 or bf16.  workspace: shared_attention_workspace(), for one launch at a time."""
+    What not all rows of a group see is not shared.  Heads of 64 and 128, up to 16 query heads for each key/value head.  Queries (times a power of two of the row) and weights are fp16, scores
+    f32 (beyond its range: NaN); y_out is f32, fp16 or bf16.  workspace: shared_attention_workspace(), for one launch at a time."""
     if k_cache.dim() != 4 or k_cache.shape[2] != PAGE_SIZE or k_cache.shape[3] not in (64, 128) or k_cache.shape[0] < 1 or v_cache.shape != k_cache.shape:
         raise ValueError(f"keys {tuple(k_cache.shape)} and values {tuple(v_cache.shape)}: [pages][kv heads][{PAGE_SIZE}][64 or 128] is wanted")
     if k_cache.dtype is not torch.float16 or v_cache.dtype is not torch.float16 or v_cache.get_device() != k_cache.get_device() or not k_cache.is_contiguous() or not v_cache.is_contiguous() \

@@ -292,7 +292,8 @@ int dl_kv8_attention_prefill(const float* q, long long ldq, int n_heads, const i
  * pages: those are read once for the group.  groups (device) = [n, begin, end, pages, ...]: rows begin .. end - 1 name the same pages in the first `pages` places of their block tables (taken from
  * the first row that has a token).  Eight groups are looked at, of max_groups that the array has room for; rows of two groups belong to the first one, groups come in the order of
  * their rows; what not all rows of a group see is not shared; rows of no group are attended to by themselves.  q (row stride ldq, a multiple of 4) and what is aligned: 16 bytes.
- * y_out (NULL or rows of stride ldy) of DL_KV8_*, xq_out / xh_out as of dl_attention.  Queries are taken in fp16 times a power of two of the row, weights in fp16: 2^-12 of a weight at random.
+ * y_out (NULL or rows of stride ldy) of DL_KV8_*, xq_out / xh_out as of dl_attention.  Queries are taken in fp16 times a power of two of the row, weights in fp16: 2^-12 of a weight at random.  Scores
+ * times log2 e are f32: a row with one beyond its range is NaN.
  * pos, slot and pages that are not in the tables: as for the 8-bit cache below (zeros without a token, else NaN).  scratch: dl_shared_attention_scratch_bytes(), any contents; launches that may
  * run at the same time need scratches of their own.  Two launches. */
 long long dl_shared_attention_scratch_bytes(int M, int n_heads, int n_kv_heads, int head_size);
