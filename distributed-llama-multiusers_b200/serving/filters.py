@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import os
 
+import numpy as np
 import torch
 
 MAX_VOCAB = 1 << 19          # of sample_tokens (dl_sample_tokens_max_vocab)
@@ -14,8 +15,8 @@ def host_ignores() -> bool:
 
 
 def settings(top_k, min_p, vocab: int) -> tuple:
-    """top_k and min_p of a request as the kernel takes them: 0 where they take nothing out (a top_k below 1, or of the vocabulary or more; a min_p not above 0), a min_p of 1 at most."""
-    return int(top_k) if 0 < top_k < vocab else 0, min(float(min_p), 1.0) if min_p > 0 else 0.0
+    """top_k and min_p of a request as the kernel takes them: 0 where they take nothing out (a top_k below 1, or of the vocabulary or more; a min_p that is not above 0 in f32), a min_p of 1 at most."""
+    return int(top_k) if 0 < top_k < vocab else 0, float(np.float32(min(min_p, 1.0))) if min_p > 0 else 0.0
 
 
 class Filters:

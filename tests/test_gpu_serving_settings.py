@@ -41,8 +41,8 @@ def test_settings_beyond_32_bits(tiny_model_path, tmp_path):
 
 def test_what_the_settings_mean():
     from dllama_b200.serving.filters import settings
-    for (k, p), want in (((0, 0.0), (0, 0.0)), ((40, 0.05), (40, 0.05)), ((999, 1.0), (999, 1.0)), ((1000, 2.0), (0, 1.0)), ((10 ** 30, 1e300), (0, 1.0)), ((-(10 ** 30), -1e300), (0, 0.0)),
-                         ((math.nan, math.nan), (0, 0.0)), ((math.inf, math.inf), (0, 1.0)), ((0.5, 1e-30), (0, 1e-30)), ((2.7, 0.0), (2, 0.0))):
+    for (k, p), want in (((0, 0.0), (0, 0.0)), ((40, 0.0625), (40, 0.0625)), ((999, 1.0), (999, 1.0)), ((1000, 2.0), (0, 1.0)), ((10 ** 30, 1e300), (0, 1.0)), ((-(10 ** 30), -1e300), (0, 0.0)),
+                         ((math.nan, math.nan), (0, 0.0)), ((math.inf, math.inf), (0, 1.0)), ((0.5, 2.0 ** -100), (0, 2.0 ** -100)), ((2.7, 0.0), (2, 0.0)), ((0, 1e-60), (0, 0.0))):
         assert settings(k, p, 1000) == want
 
 
